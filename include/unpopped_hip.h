@@ -120,9 +120,12 @@ enum unp_form_kind {
   UNP_FORM_DEQUANT_GEMM = 6, /* the dequantizing GEMM (tests/support/dequant.rs:104-181): U4/I4
                                weights, I32 zero and scale per group, I32 or I8 activations,
                                I32 out, all wrapping */
-  UNP_FORM_ELEMENTWISE = 7  /* Access::Elementwise, launched (kernel_lift.rs:96-153): a body over
+  UNP_FORM_ELEMENTWISE = 7, /* Access::Elementwise, launched (kernel_lift.rs:96-153): a body over
                                n inputs read at the output coordinate, each optionally through an
                                axis permutation; its body comes only through unp_hip_lower_kernel */
+  /* The forms of the rotary and cache descriptors below; unp_hip_lower_form refuses them. */
+  UNP_FORM_ROPE_TABLE = 8, UNP_FORM_ROPE = 9, UNP_FORM_CACHE4_APPEND = 10, UNP_FORM_CACHE4_READ = 11,
+  UNP_FORM_CACHE4_ATTENTION = 12
 };
 /* ReduceOp subset (crates/unpopped/src/ir.rs:1700-1735).  And/Or/Xor fold integers bitwise;
  * MaxNum/MinNum ignore NaN (a run of only NaN gives NaN); the reference lifts these five as
@@ -286,6 +289,120 @@ int32_t unp_lift_row_reduce(const char* name, int32_t dtype, int32_t rank, int32
                             uint32_t grid, char** json, unp_error* err);
 
 /* ---------------------------------------------------------------------------------------
+ * Rotary positions and the 4-bit paged key/value cache.  No reference lift: forms this backend
+ * authors beside its int4 dequant (the same (q - z) * s of a 4-bit code, an f16 scale and a 4-bit
+ * zero point).  They come from a descriptor instead of a KernelFn, because their loops are bounded
+ * by lengths that only the device holds; the unp_generated they give is compiled and launched as
+ * every other (unp_hip_exec_create, unp_hip_exec_launch; unp_hip_exec_launch_views is refused: they
+ * take their strides as scalars).
+ *
+ * Arguments are listed at each form in launch order.  Strides count elements; the elements of a head
+ * are adjacent; strides are not negative.  Scalars are read as 64-bit integers.  Sequence lengths,
+ * page numbers, slots and positions are device data: none of them, whatever its value, makes a kernel
+ * read or write outside the buffers that the scalars describe.  No form keeps anything between
+ * launches or allocates, so launches on several streams and in several captured graphs are
+ * independent as long as their buffers (a workspace among them) are.
+ * ------------------------------------------------------------------------------------- */
+
+/* How the frequency base^(-2i / rot) of pair i is stretched for long contexts. */
+enum unp_rope_scaling {
+  UNP_ROPE_NONE = 0,
+  UNP_ROPE_LINEAR = 1, /* frequency / factor: positions interpolated */
+  UNP_ROPE_RAMP = 2    /* r = original * frequency / (2 pi) turns over the original context; b = clamp((r - low)
+                          / (high - low), 0, 1): frequency * (b + (1 - b) / factor) */
+};
+typedef struct unp_rope_table {
+  int32_t rot;       /* rotated elements of a head: even, 2..4096 */
+  int32_t scaling;   /* unp_rope_scaling */
+  double base;       /* > 0 */
+  double factor;     /* > 0; LINEAR and RAMP */
+  double low, high;  /* RAMP: low < high */
+  double original;   /* RAMP: > 0, the context length that the frequencies were made for */
+  double amplitude;  /* multiplies the cosines and sines */
+} unp_rope_table;
+/* Launch: table (F32 [count][rot / 2][2]: cosine, sine); first, count.  Row r holds position first + r
+ * (|first| + count <= 2^52).  Angles, cosines and sines are computed in 64 bits and rounded once. */
+int32_t unp_hip_lower_rope_table(const unp_rope_table* t, unp_generated** out, unp_error* err);
+
+enum unp_rope_layout {
+  UNP_ROPE_HALVES = 0, /* pair i is elements i and i + rot / 2 */
+  UNP_ROPE_PAIRS = 1   /* pair i is elements 2i and 2i + 1 */
+};
+typedef struct unp_rope {
+  int32_t dtype;       /* F32, Bf16 or F16 */
+  int32_t head_dim;    /* 2..4096 */
+  int32_t rot;         /* even, 2..head_dim: the first rot elements rotate, the others are copied */
+  int32_t layout;      /* unp_rope_layout */
+  int32_t index_dtype; /* positions: I32 or I64 */
+  int32_t inverse;     /* 1: by the negative angle, which is the rotation's gradient */
+} unp_rope;
+/* (x0, x1) -> (x0 cos - x1 sin, x1 cos + x0 sin) in 32 bits, rounded once to the type.
+ * Launch: x, positions [tokens], table (F32 [table_rows][rot / 2][2]), out; tokens, heads, x_token, x_head,
+ * out_token, out_head (strides), table_first, table_rows.  Position p reads table row p - table_first; a token
+ * whose position is outside the table is skipped: nothing of it is written.  out is x with x's strides
+ * (in place), or shares no element with x; an out that names an element twice is refused. */
+int32_t unp_hip_lower_rope(const unp_rope* r, unp_generated** out, unp_error* err);
+
+/* The cache: an array of pages, each of `page` tokens for every key/value head.  A page is kv_heads records of
+ * unp_cache4_record_bytes bytes; with D = head_dim and G = D / group a record holds, in this order,
+ *   key codes     page x D / 2 bytes: token t's D / 8 words of 8 codes (low nibble first); the word of elements
+ *                 8w .. 8w + 7 is the token's word (w % 4) * (D / 32) + w / 4, so that the 16 bytes (D = 128) that
+ *                 one lane of a matrix instruction multiplies lie together;
+ *   value codes   page x D / 2 bytes: that word of token t is word ((t / 4) * (D / 8) + w) * 4 + t % 4: a lane reads
+ *                 four tokens' codes of 8 elements at once;
+ *   key words     G x page words of 32 bits: an f16 scale in the low half, the zero point (0..15) in the high half;
+ *   value words   the same.
+ * A code n stands for (n - zero) * scale.  The cache is 16-byte aligned. */
+typedef struct unp_cache4 {
+  int32_t dtype;       /* Bf16 or F16: the type of keys, values, queries and outputs */
+  int32_t kv_heads;    /* 1..1024 */
+  int32_t head_dim;    /* a multiple of 32, 32..256 */
+  int32_t group;       /* elements per scale: 32, 64, 128 or head_dim, dividing head_dim */
+  int32_t page;        /* tokens of a page: 16, 32, 64, 128 or 256 */
+  int32_t index_dtype; /* slots and positions: I32 or I64 (append and read) */
+} unp_cache4;
+int32_t unp_cache4_record_bytes(const unp_cache4* c, uint64_t* bytes, unp_error* err);
+
+/* Quantise a step's keys and values into their slots (page number * page + place).  With rot > 0 the first rot
+ * elements of each key are rotated on the way (layout as above): in 64 bits from the 32-bit table, then rounded
+ * once to the keys' type.  Each group of a head then takes lo = min(0, smallest), hi = max(0, largest),
+ * scale = f16((hi - lo) / 15), zero = clamp(round(-lo / scale), 0, 15) and n = clamp(round(y / scale) + zero, 0, 15),
+ * the quotients in 32 bits and rounded to even (scale 0 divides as 1); a group that holds a NaN or an infinity, or whose
+ * scale overflows f16, takes a NaN scale.
+ * Launch: k, v, slots [tokens], cache, and with rot > 0 positions [tokens], table; tokens, pages, k_token, k_head,
+ * v_token, v_head (strides), and with rot > 0 table_first, table_rows.  A token whose slot is outside the cache
+ * (negative: a padded row), or whose position is outside the table, is skipped.  Two tokens of one call must not
+ * name one slot: it would hold words of both. */
+int32_t unp_hip_lower_cache4_append(const unp_cache4* c, int32_t rot, int32_t layout, unp_generated** out,
+                                    unp_error* err);
+
+/* The values that slots hold, (n - zero) * scale rounded once to the type; a slot outside the cache reads as 0.
+ * Launch: slots [tokens], cache, k, v; tokens, pages, k_token, k_head, v_token, v_head (strides). */
+int32_t unp_hip_lower_cache4_read(const unp_cache4* c, unp_generated** out, unp_error* err);
+
+typedef struct unp_attention {
+  int32_t heads;   /* query heads: kv_heads times 1..128; query head h reads key/value head h / (heads / kv_heads) */
+  int32_t causal;  /* 1: row i of n of a sequence of length L sees keys 0 .. L - n + i; 0: every row sees all L */
+  int32_t lse;     /* 1: also write each row's log of the sum of exponentials */
+  int32_t pad;
+  double scale;    /* of the scores; 0: 1 / sqrt(head_dim) */
+} unp_attention;
+/* Attention of a ragged batch's rows over their sequences' pages.
+ * Launch: q (rows of heads x head_dim), cache, page_table (I32 [batch][width]), starts (I32 [batch + 1]: sequence b's
+ * rows are starts[b] .. starts[b + 1] - 1), lengths (I32 [batch]: its keys, its own rows' last), out, with lse
+ * lse (F32 [tokens][heads], natural log; -inf for an empty row), workspace; tokens, batch, width, pages, q_token, q_head,
+ * out_token, out_head (strides), window, workspace_bytes.
+ *   window > 0 (causal only): a row sees its last `window` keys.  A row that sees no key gives 0.
+ *   Keys that no row may see do not count, whatever they hold: keys past a sequence's length, keys of a page number
+ *   outside the cache, keys past width pages.  Rows that no sequence names are left as they were.  starts do not
+ *   decrease; in a list that does, which sequence takes a row, if any, is not said.
+ *   The scores, the softmax's statistics and the sums are held in 32 bits.  The workspace (16-byte aligned) holds the parts
+ *   of a context that is split over blocks; one smaller than unp_hip_exec_workspace says, 0 among them, lowers the
+ *   split.  The sums' order follows from the scalars and lengths alone: the same call gives the same bits. */
+int32_t unp_hip_lower_cache4_attention(const unp_cache4* c, const unp_attention* a, unp_generated** out,
+                                       unp_error* err);
+
+/* ---------------------------------------------------------------------------------------
  * Compiler seam (trait Compiler, jit.rs:271-285), through hipRTC for gfx950.
  * ------------------------------------------------------------------------------------- */
 
@@ -416,6 +533,10 @@ int32_t unp_hip_exec_set_timing(unp_exec* e, unp_event* start, unp_event* stop);
  * UNP_OK. */
 int32_t unp_hip_exec_set_wait_limit(unp_exec* e, uint32_t wait_us);
 int32_t unp_hip_exec_check(unp_exec* e, unp_error* err);
+/* The bytes of workspace with which a cache attention launch of these scalars (tokens, batch, width, pages)
+ * splits as far as it would; 0 where it splits nothing. */
+int32_t unp_hip_exec_workspace(const unp_exec* e, const int64_t* scalars, size_t nscalars, uint64_t* bytes,
+                               unp_error* err);
 /* The last launch's geometry and chosen entry point (for reports). */
 int32_t unp_hip_exec_last_launch(const unp_exec* e, uint32_t grid[3], uint32_t block[3],
                                  char* entry, size_t entry_len);

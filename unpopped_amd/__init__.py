@@ -38,6 +38,8 @@ SCHEDULES = {"device": 0, "serial": 1, "fixed": 2}
 FIDELITIES = ["BitIdentical", "DeterministicallyDivergent", "Nondeterministic", "MorePrecise"]
 FORMS = {"reduction": 0, "scan": 1, "gather": 2, "dequant4": 3, "row_reduce2": 4, "row_reduce": 5, "dequant_gemm": 6}
 DTYPE_SUPPORT = {0: "Supported", 1: "Unsupported", 2: "NotExpressible"}
+ROPE_SCALINGS = {"none": 0, "linear": 1, "ramp": 2}
+ROPE_LAYOUTS = {"halves": 0, "pairs": 1}
 ARTIFACT_KINDS = {0: "Ptx", 1: "Cubin", 2: "HipCodeObject", 3: "SpirV", 4: "Stub"}
 
 
@@ -139,6 +141,53 @@ class HipBackend:
         text = kernel if isinstance(kernel, str) else json.dumps(kernel)
         return self._wrap(lambda out, err: _lib.lib().unp_hip_lower_kernel(text.encode(), out, err))
 
+    def lower_rope_table(self, rot: int, base: float = 10000.0, scaling: str = "none", factor: float = 1.0,
+                         low: float = 1.0, high: float = 4.0, original: float = 8192, amplitude: float = 1.0) -> GeneratedKernel:
+        """A table of the cosines and sines of positions (``unp_hip_lower_rope_table``).  ``scaling``
+        stretches the frequencies for long contexts: ``"none"``, ``"linear"`` (divided by ``factor``) or
+        ``"ramp"`` (between the two, by each frequency's turns over ``original`` positions: kept from
+        ``high`` turns on, divided by ``factor`` up to ``low``).  Launch: table (F32 [count][rot / 2][2]);
+        first, count."""
+        t = _lib.RopeTable(rot, ROPE_SCALINGS[scaling], base, factor, low, high, original, amplitude)
+        return self._wrap(lambda out, err: _lib.lib().unp_hip_lower_rope_table(C.byref(t), out, err))
+
+    def lower_rope(self, dtype: str, head_dim: int, rot: int | None = None, layout: str = "halves",
+                   index_dtype: str = "I32", inverse: bool = False) -> GeneratedKernel:
+        """The rotation of heads by their tokens' positions, or with ``inverse`` its gradient
+        (``unp_hip_lower_rope``).  Launch: x, positions, table, out; tokens, heads, x_token, x_head,
+        out_token, out_head (strides in elements), table_first, table_rows."""
+        r = _lib.Rope(ELEMENT_KINDS[dtype], head_dim, head_dim if rot is None else rot, ROPE_LAYOUTS[layout],
+                      ELEMENT_KINDS[index_dtype], int(inverse))
+        return self._wrap(lambda out, err: _lib.lib().unp_hip_lower_rope(C.byref(r), out, err))
+
+    def lower_cache4_append(self, dtype: str, kv_heads: int, head_dim: int, group: int | None = None, page: int = 16,
+                            rot: int = 0, layout: str = "halves", index_dtype: str = "I32") -> GeneratedKernel:
+        """The append of a step's keys and values to a 4-bit paged cache, the keys' first ``rot`` elements
+        rotated on the way (``unp_hip_lower_cache4_append``).  Launch: k, v, slots, cache, with ``rot`` > 0
+        positions, table; tokens, pages, k_token, k_head, v_token, v_head, with ``rot`` > 0 table_first,
+        table_rows."""
+        c = _cache4(dtype, kv_heads, head_dim, group, page, index_dtype)
+        return self._wrap(lambda out, err: _lib.lib().unp_hip_lower_cache4_append(
+            C.byref(c), rot, ROPE_LAYOUTS[layout], out, err))
+
+    def lower_cache4_read(self, dtype: str, kv_heads: int, head_dim: int, group: int | None = None, page: int = 16,
+                          index_dtype: str = "I32") -> GeneratedKernel:
+        """The values that a 4-bit cache's slots hold (``unp_hip_lower_cache4_read``).  Launch: slots, cache,
+        k, v; tokens, pages, k_token, k_head, v_token, v_head."""
+        c = _cache4(dtype, kv_heads, head_dim, group, page, index_dtype)
+        return self._wrap(lambda out, err: _lib.lib().unp_hip_lower_cache4_read(C.byref(c), out, err))
+
+    def lower_cache4_attention(self, dtype: str, heads: int, kv_heads: int, head_dim: int, group: int | None = None,
+                               page: int = 16, causal: bool = True, lse: bool = False,
+                               scale: float = 0.0) -> GeneratedKernel:
+        """Attention of a ragged batch's rows over a 4-bit paged cache (``unp_hip_lower_cache4_attention``).
+        Launch: q, cache, page_table, starts, lengths, out, with ``lse`` lse, workspace; tokens, batch, width,
+        pages, q_token, q_head, out_token, out_head, window, workspace_bytes
+        (:meth:`Executor.workspace_bytes` says how many)."""
+        c = _cache4(dtype, kv_heads, head_dim, group, page, "I32")
+        a = _lib.Attention(heads, int(causal), int(lse), 0, scale)
+        return self._wrap(lambda out, err: _lib.lib().unp_hip_lower_cache4_attention(C.byref(c), C.byref(a), out, err))
+
     @staticmethod
     def _wrap(call) -> GeneratedKernel:
         L = _lib.lib()
@@ -151,6 +200,20 @@ class HipBackend:
             interface=json.loads(L.unp_generated_interface_json(out).decode()),
             _handle=out,
         )
+
+
+def _cache4(dtype: str, kv_heads: int, head_dim: int, group: int | None, page: int, index_dtype: str) -> "_lib.Cache4":
+    return _lib.Cache4(ELEMENT_KINDS[dtype], kv_heads, head_dim, head_dim if group is None else group, page,
+                       ELEMENT_KINDS[index_dtype])
+
+
+def cache4_page_bytes(dtype: str, kv_heads: int, head_dim: int, group: int | None = None, page: int = 16) -> int:
+    """The bytes of one page of a 4-bit cache: a record per key/value head (``unp_cache4_record_bytes``)."""
+    n = C.c_uint64()
+    err = _lib.Error()
+    c = _cache4(dtype, kv_heads, head_dim, group, page, "I32")
+    check(_lib.lib().unp_cache4_record_bytes(C.byref(c), C.byref(n), C.byref(err)), err)
+    return kv_heads * int(n.value)
 
 
 def _lifted(call) -> dict:
@@ -338,6 +401,14 @@ class DeviceBuffer:
         b.upload(a)
         return b
 
+    @classmethod
+    def held(cls, ptr: int, nbytes: int, owner) -> "DeviceBuffer":
+        """Device memory that ``owner`` owns (a tensor of another library) as a launch argument; the
+        buffer keeps ``owner`` alive."""
+        b = cls.__new__(cls)
+        b.nbytes, b.ptr, b._owner = int(nbytes), int(ptr), owner
+        return b
+
     def upload(self, a: np.ndarray) -> None:
         a = np.ascontiguousarray(a)
         assert a.nbytes <= self.nbytes
@@ -431,6 +502,14 @@ class Executor:
         rc = self._launch(self._h, _ARG_WORDS[len(args)](*words), len(args), stream, err)
         if rc:
             check(rc, err._obj)
+
+    def workspace_bytes(self, tokens: int, batch: int, width: int, pages: int) -> int:
+        """The workspace with which a cache attention launch of these scalars splits as far as it would."""
+        sc = (C.c_int64 * 4)(tokens, batch, width, pages)
+        n = C.c_uint64()
+        err = _lib.Error()
+        check(_lib.lib().unp_hip_exec_workspace(self._h, sc, 4, C.byref(n), C.byref(err)), err)
+        return int(n.value)
 
     def launch_static(self, *args, stream: int = 0) -> None:
         """``launch`` with every workspace in the library's static device scratch

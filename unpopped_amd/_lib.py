@@ -65,6 +65,27 @@ class View(C.Structure):
                 ("stride", C.c_int64 * MAX_RANK), ("base", C.c_int64)]
 
 
+class RopeTable(C.Structure):
+    """unp_rope_table: the frequencies of a position table."""
+    _fields_ = [("rot", C.c_int32), ("scaling", C.c_int32)] + [(n, C.c_double) for n in (
+        "base", "factor", "low", "high", "original", "amplitude")]
+
+
+class Rope(C.Structure):
+    """unp_rope: a rotation of heads."""
+    _fields_ = [(n, C.c_int32) for n in ("dtype", "head_dim", "rot", "layout", "index_dtype", "inverse")]
+
+
+class Cache4(C.Structure):
+    """unp_cache4: a 4-bit paged key/value cache."""
+    _fields_ = [(n, C.c_int32) for n in ("dtype", "kv_heads", "head_dim", "group", "page", "index_dtype")]
+
+
+class Attention(C.Structure):
+    """unp_attention: attention over a cache."""
+    _fields_ = [(n, C.c_int32) for n in ("heads", "causal", "lse", "pad")] + [("scale", C.c_double)]
+
+
 _lib = None
 
 
@@ -109,6 +130,13 @@ def lib() -> C.CDLL:
         "unp_kernel_dequant_gemm": (i32, [C.c_char_p, i32, i32, i32, u32, u32, C.POINTER(C.c_void_p), E]),
         "unp_lift_row_reduce": (i32, [C.c_char_p, i32, i32, i32, C.c_char_p, C.c_char_p, u32, u32,
                                       C.POINTER(C.c_void_p), E]),
+        "unp_hip_lower_rope_table": (i32, [C.POINTER(RopeTable), C.POINTER(P), E]),
+        "unp_hip_lower_rope": (i32, [C.POINTER(Rope), C.POINTER(P), E]),
+        "unp_cache4_record_bytes": (i32, [C.POINTER(Cache4), C.POINTER(u64), E]),
+        "unp_hip_lower_cache4_append": (i32, [C.POINTER(Cache4), i32, i32, C.POINTER(P), E]),
+        "unp_hip_lower_cache4_read": (i32, [C.POINTER(Cache4), C.POINTER(P), E]),
+        "unp_hip_lower_cache4_attention": (i32, [C.POINTER(Cache4), C.POINTER(Attention), C.POINTER(P), E]),
+        "unp_hip_exec_workspace": (i32, [P, C.POINTER(C.c_int64), sz, C.POINTER(u64), E]),
         "unp_hip_compile": (i32, [C.c_char_p, C.c_char_p, u32, C.POINTER(C.POINTER(C.c_uint8)),
                                   C.POINTER(sz), C.POINTER(C.c_void_p)]),
         "unp_hip_artifact_kind": (i32, []),

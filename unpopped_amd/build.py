@@ -22,7 +22,7 @@ LIB = HERE / "libunpopped_hip.so"
 SYNTH_LIB = HERE / "libunpopped_synth.so"
 ROCM = Path(os.environ.get("ROCM_PATH", "/opt/rocm"))
 
-HOST_SOURCES = ["emit_hip.cpp", "compile_rtc.cpp", "runtime.cpp", "kernel_ir.cpp", "lifts.cpp"]
+HOST_SOURCES = ["emit_hip.cpp", "emit_cache4.cpp", "compile_rtc.cpp", "runtime.cpp", "kernel_ir.cpp", "lifts.cpp"]
 
 HIPCC_DEVICE_FLAGS = [
     "--offload-arch=gfx950", "-O3", "-std=c++17", "-ffp-contract=off",
@@ -37,26 +37,27 @@ def _run(cmd: list[str]) -> None:
         raise RuntimeError(f"build step failed: {' '.join(cmd[:3])} ...")
 
 
-def embed_device_library() -> Path:
-    """Write the device library as a C++ string constant."""
+def embed_device_library(source: str, name: str) -> Path:
+    """Write a device library as a C++ string constant `name`."""
     BUILD.mkdir(exist_ok=True)
-    text = (CSRC / "kernels" / "unp_device.hip").read_bytes()
-    out = BUILD / "embedded_device.cpp"
+    text = (CSRC / "kernels" / source).read_bytes()
+    out = BUILD / f"embedded_{Path(source).stem.removeprefix('unp_')}.cpp"
     parts = ", ".join(str(b) for b in text)
     out.write_text(
-        "// generated by unpopped_amd/build.py from csrc/kernels/unp_device.hip\n"
+        f"// generated by unpopped_amd/build.py from csrc/kernels/{source}\n"
         "namespace unp {\n"
-        f"static const char kDeviceLibraryBytes[] = {{{parts}, 0}};\n"
-        "extern const char* const kDeviceLibrary = kDeviceLibraryBytes;\n"
+        f"static const char {name}Bytes[] = {{{parts}, 0}};\n"
+        f"extern const char* const {name} = {name}Bytes;\n"
         "}\n"
     )
     return out
 
 
 def build_host() -> Path:
-    embedded = embed_device_library()
+    embedded = [embed_device_library("unp_device.hip", "kDeviceLibrary"),
+                embed_device_library("unp_cache4.hip", "kCache4Library")]
     objs = []
-    for src in HOST_SOURCES + [str(embedded)]:
+    for src in HOST_SOURCES + [str(e) for e in embedded]:
         path = Path(src) if os.path.isabs(src) else CSRC / src
         obj = BUILD / (path.stem + ".o")
         _run([

@@ -21,6 +21,7 @@
 #include <cmath>
 #include <cstdlib>
 #include <cstring>
+#include <memory>
 
 #include "kernel_ir.hpp"
 #include "unp_internal.hpp"
@@ -156,6 +157,8 @@ size_t split_bytes(const unp_exec* x) {
   return split_counter_bytes(x) + split_items(x) * values * 16;
 }
 
+int32_t attention_workspace(const unp_exec* x, const int64_t* sc, size_t n, uint64_t& bytes, unp_error* err);
+
 bool splits(const unp_exec* x) {
   if (x->l.form.kind == UNP_FORM_ROW_REDUCE) return true;
   return x->l.form.kind == UNP_FORM_REDUCTION && (x->l.red_schedule == 'g' || x->l.red_schedule == 'm');
@@ -215,6 +218,68 @@ int32_t unp_hip_lower_form(const unp_form* form, unp_generated** out, unp_error*
   set_error(err, UNP_OK, "");
   *out = g;
   return UNP_OK;
+}
+
+}  // extern "C"
+
+namespace {
+
+// One of the descriptor forms lowered into a new handle; no exception leaves it.
+template <class F>
+int32_t lower_into(bool args_ok, unp_generated** out, unp_error* err, F lower) {
+  if (out) *out = nullptr;
+  if (!args_ok || !out) {
+    set_error(err, UNP_INVALID_ARGUMENT, "null descriptor or output");
+    return UNP_INVALID_ARGUMENT;
+  }
+  try {
+    std::unique_ptr<unp_generated> g(new unp_generated());
+    std::string why;
+    const int32_t rc = lower(g->l, why);
+    set_error(err, rc, why);
+    if (rc == UNP_OK) *out = g.release();
+    return rc;
+  } catch (const std::exception& e) {
+    set_error(err, UNP_COMPILE_ERROR, e.what());
+    return UNP_COMPILE_ERROR;
+  }
+}
+
+}  // namespace
+
+extern "C" {
+
+int32_t unp_hip_lower_rope_table(const unp_rope_table* t, unp_generated** out, unp_error* err) {
+  return lower_into(t, out, err, [&](unp::Lowered& l, std::string& why) { return unp::lower_rope_table(*t, l, why); });
+}
+int32_t unp_hip_lower_rope(const unp_rope* r, unp_generated** out, unp_error* err) {
+  return lower_into(r, out, err, [&](unp::Lowered& l, std::string& why) { return unp::lower_rope(*r, l, why); });
+}
+int32_t unp_cache4_record_bytes(const unp_cache4* c, uint64_t* bytes, unp_error* err) {
+  if (!c || !bytes) {
+    set_error(err, UNP_INVALID_ARGUMENT, "null descriptor or output");
+    return UNP_INVALID_ARGUMENT;
+  }
+  std::string why;
+  const int32_t rc = unp::check_cache4(*c, why);
+  *bytes = rc == UNP_OK ? unp::cache4_record_bytes(*c) : 0;
+  set_error(err, rc, why);
+  return rc;
+}
+int32_t unp_hip_lower_cache4_append(const unp_cache4* c, int32_t rot, int32_t layout, unp_generated** out,
+                                    unp_error* err) {
+  return lower_into(c, out, err, [&](unp::Lowered& l, std::string& why) {
+    return unp::lower_cache4_append(*c, rot, layout, l, why);
+  });
+}
+int32_t unp_hip_lower_cache4_read(const unp_cache4* c, unp_generated** out, unp_error* err) {
+  return lower_into(c, out, err, [&](unp::Lowered& l, std::string& why) { return unp::lower_cache4_read(*c, l, why); });
+}
+int32_t unp_hip_lower_cache4_attention(const unp_cache4* c, const unp_attention* a, unp_generated** out,
+                                       unp_error* err) {
+  return lower_into(c && a, out, err, [&](unp::Lowered& l, std::string& why) {
+    return unp::lower_cache4_attention(*c, *a, l, why);
+  });
 }
 
 int32_t unp_hip_form_variants(const unp_form* form, unp_variant* out, size_t cap, size_t* count, unp_error* err) {
@@ -569,6 +634,17 @@ int32_t unp_hip_exec_last_chunks(const unp_exec* x, int64_t* chunks, int32_t* sh
   if (chunks) *chunks = x->chunks;
   if (shared) *shared = x->shared ? 1 : 0;
   return UNP_OK;
+}
+
+int32_t unp_hip_exec_workspace(const unp_exec* x, const int64_t* scalars, size_t nscalars, uint64_t* bytes,
+                               unp_error* err) {
+  if (!x || !bytes || (nscalars && !scalars)) {
+    set_error(err, UNP_INVALID_ARGUMENT, "null executor, scalars or output");
+    return UNP_INVALID_ARGUMENT;
+  }
+  *bytes = 0;
+  set_error(err, UNP_OK, "");
+  return attention_workspace(x, scalars, nscalars, *bytes, err);
 }
 
 int32_t unp_hip_exec_last_launch(const unp_exec* x, uint32_t grid[3], uint32_t block[3], char* entry,
@@ -926,6 +1002,8 @@ static_assert(sizeof(unp::scan_view_host) == 29 * 8, "scan_view_host mirrors the
 static_assert(sizeof(unp::ew_tile_view_host) == 114 * 8, "ew_tile_view_host mirrors the device's ew_tile_view");
 static_assert(sizeof(unp::gather_view_host) == 35 * 8, "gather_view_host mirrors the device's gather_view");
 static_assert(sizeof(unp::red_axes_host) == 61 * 8, "red_axes_host mirrors the device's red_axes");
+
+int32_t invalid(unp_error* err, const std::string& what);
 
 int32_t launch(unp_exec* x, size_t entry, uint32_t grid, void** params, hipStream_t s, unp_error* err) {
   const uint32_t threads = (uint32_t)(x->l.entries[entry].threads ? x->l.entries[entry].threads : x->l.threads);
@@ -1777,6 +1855,227 @@ int32_t run_dequant_gemm(unp_exec* x, const unp_arg* a, size_t n, hipStream_t s,
   return launch(x, entry, grid, params, s, err);
 }
 
+// ---------------------------------------------------------------------------------------
+// The rotary and 4-bit cache forms.  Their scalars are 64-bit; every buffer's reach that the scalars
+// describe stays below 2^60 elements, so that the kernels' 64-bit offsets cannot wrap.
+// ---------------------------------------------------------------------------------------
+
+// Host images of the kernels' argument structs (passed by value).
+struct stretch_host {
+  int32_t kind, pad;
+  double log_base, factor, low, high, original, amplitude;
+};
+struct rope_args_host {
+  int64_t tokens, x_token, x_head, out_token, out_head, first, rows;
+  int32_t heads, units;
+};
+struct cache_args_host {
+  int64_t tokens, slots, k_token, k_head, v_token, v_head, first, rows;
+};
+struct attention_args_host {
+  int64_t tokens, batch, width, pages, q_token, q_head, out_token, out_head, window;
+};
+
+constexpr int64_t kMostOffset = (int64_t)1 << 60;
+
+// The elements that `tokens` rows of `heads` heads of `dim` reach, or -1 past kMostOffset.
+int64_t reach(int64_t tokens, int64_t token, int64_t heads, int64_t head, int64_t dim) {
+  if (tokens == 0 || heads == 0) return 0;
+  const __int128 n = (__int128)(tokens - 1) * token + (__int128)(heads - 1) * head + dim;
+  return n > kMostOffset ? -1 : (int64_t)n;
+}
+
+// A tensor of heads by its strides: none negative, in reach; one that is written names each element once.
+int32_t check_heads(const char* what, int64_t tokens, int64_t token, int64_t heads, int64_t head, int64_t dim, bool written,
+                    unp_error* err) {
+  if (token < 0 || head < 0) return invalid(err, std::string(what) + ": a negative stride");
+  if (reach(tokens, token, heads, head, dim) < 0) return invalid(err, std::string(what) + ": more than 2^60 elements");
+  if (!written || tokens == 0 || heads == 0) return UNP_OK;
+  // The axis with the smaller stride keeps heads apart, the other one whole runs of them.
+  const bool head_inner = heads > 1 && (tokens == 1 || head <= token);
+  const int64_t in = head_inner ? head : token, in_n = head_inner ? heads : tokens;
+  const int64_t out = head_inner ? token : head, out_n = head_inner ? tokens : heads;
+  const __int128 run = (__int128)(in_n - 1) * in + dim;
+  if ((in_n > 1 && in < dim) || (out_n > 1 && out < run))
+    return invalid(err, std::string(what) + ": the strides name an element twice");
+  return UNP_OK;
+}
+
+bool whole_vectors(uint64_t p, int64_t token, int64_t head, int v) {
+  return aligned16(p) && token % v == 0 && head % v == 0;
+}
+
+// Blocks of a device-class grid, no more than the work fills.
+uint32_t grid_for(const unp_exec* x, int64_t blocks) {
+  return (uint32_t)std::min<int64_t>((int64_t)x->cu_count * 8, blocks);
+}
+
+int32_t run_rope_table(unp_exec* x, const unp_arg* a, size_t n, hipStream_t s, unp_error* err) {
+  Args A;
+  int32_t rc = take_args(a, n, 1, 2, A, err);
+  if (rc != UNP_OK) return rc;
+  long long first = A.ext[0], count = A.ext[1];
+  const int64_t most = (int64_t)1 << 52;
+  if (count < 0 || count > most || first < -most || first > most || first + count > most)
+    return invalid(err, "first and count name positions outside -2^52..2^52");
+  if (count == 0) return UNP_OK;
+  if ((rc = need_buffers(A, true, err)) != UNP_OK) return rc;
+  const unp_rope_table& t = x->l.rope_table;
+  if (A.buf[0] % 8 != 0) return invalid(err, "the table is 8-byte aligned");
+  if (count > kMostOffset / t.rot) return invalid(err, "table: more than 2^60 elements");
+  stretch_host st{t.scaling, 0, std::log(t.base), t.factor, t.low, t.high, t.original, t.amplitude};
+  uint64_t out = A.buf[0];
+  void* params[] = {&out, &first, &count, &st};
+  return launch(x, 0, grid_for(x, (count * (t.rot / 2) + 255) / 256), params, s, err);
+}
+
+int32_t check_rows(int64_t first, int64_t rows, unp_error* err) {
+  const int64_t most = (int64_t)1 << 52;
+  if (rows < 0 || rows > most || first < -most || first > most) return invalid(err, "table: rows outside 0..2^52 or a first position outside -2^52..2^52");
+  return UNP_OK;
+}
+
+int32_t run_rope(unp_exec* x, const unp_arg* a, size_t n, hipStream_t s, unp_error* err) {
+  Args A;
+  int32_t rc = take_args(a, n, 4, 8, A, err);
+  if (rc != UNP_OK) return rc;
+  const unp_rope& r = x->l.rope;
+  const int64_t tokens = A.ext[0], heads = A.ext[1];
+  if (tokens < 0 || heads < 0 || heads > 65536 || tokens > kMostOffset)
+    return invalid(err, "tokens is 0..2^60 and heads 0..65536");
+  if ((rc = check_heads("x", tokens, A.ext[2], heads, A.ext[3], r.head_dim, false, err)) != UNP_OK) return rc;
+  if ((rc = check_heads("out", tokens, A.ext[4], heads, A.ext[5], r.head_dim, true, err)) != UNP_OK) return rc;
+  if ((rc = check_rows(A.ext[6], A.ext[7], err)) != UNP_OK) return rc;
+  if (tokens == 0 || heads == 0 || A.ext[7] == 0) return UNP_OK;
+  if ((rc = need_buffers(A, true, err)) != UNP_OK) return rc;
+  const uint64_t size = unp::kind_bytes(r.dtype);
+  if (A.buf[0] % size || A.buf[3] % size || A.buf[1] % unp::kind_bytes(r.index_dtype) || A.buf[2] % 16)
+    return invalid(err, "x, positions and out are aligned to their elements, the table to 16 bytes");
+  const bool same = A.buf[0] == A.buf[3];
+  if (same && ((tokens > 1 && A.ext[2] != A.ext[4]) || (heads > 1 && A.ext[3] != A.ext[5])))
+    return invalid(err, "in place, out has x's strides");
+  const int v = r.dtype == UNP_F32 ? 4 : 8;
+  const bool fast = x->l.entries[0].fast && r.rot % 4 == 0 && whole_vectors(A.buf[0], A.ext[2], A.ext[3], v) &&
+                    whole_vectors(A.buf[3], A.ext[4], A.ext[5], v);
+  const size_t entry = fast ? 0 : x->l.entries.size() - 1;
+  // In place the elements behind rot stay where they are.
+  const int unit = fast ? 2 * v : 1;
+  rope_args_host args{tokens, A.ext[2], A.ext[3], A.ext[4], A.ext[5], A.ext[6], A.ext[7], (int32_t)heads,
+                      r.rot / 2 / (fast ? v : 1) + (same ? 0 : (r.head_dim - r.rot) / unit)};
+  const __int128 items = (__int128)tokens * heads * args.units;
+  if (items > kMostOffset) return invalid(err, "x: more than 2^60 elements");
+  uint64_t xp = A.buf[0], pos = A.buf[1], tab = A.buf[2], out = A.buf[3];
+  void* params[] = {&xp, &pos, &tab, &out, &args};
+  return launch(x, entry, grid_for(x, ((int64_t)items + 255) / 256), params, s, err);
+}
+
+// The scalars that append and read share: tokens, pages and the strides of keys and values.
+int32_t cache_scalars(const unp_exec* x, const Args& A, bool written, cache_args_host& out, unp_error* err) {
+  const unp_cache4& c = x->l.cache4;
+  const int64_t tokens = A.ext[0], pages = A.ext[1];
+  if (tokens < 0 || tokens > kMostOffset || pages < 0 || pages > 0x7FFFFFFFLL)
+    return invalid(err, "tokens is 0..2^60 and pages 0..2^31 - 1");
+  int32_t rc = check_heads("k", tokens, A.ext[2], c.kv_heads, A.ext[3], c.head_dim, written, err);
+  if (rc == UNP_OK) rc = check_heads("v", tokens, A.ext[4], c.kv_heads, A.ext[5], c.head_dim, written, err);
+  if (rc != UNP_OK) return rc;
+  if ((__int128)tokens * c.kv_heads * c.head_dim > kMostOffset) return invalid(err, "k: more than 2^60 elements");
+  out = cache_args_host{tokens, pages * c.page, A.ext[2], A.ext[3], A.ext[4], A.ext[5], 0, 0};
+  return UNP_OK;
+}
+
+int32_t run_cache4_append(unp_exec* x, const unp_arg* a, size_t n, hipStream_t s, unp_error* err) {
+  Args A;
+  const bool rot = x->l.rope.rot > 0;
+  int32_t rc = take_args(a, n, rot ? 6 : 4, rot ? 8 : 6, A, err);
+  if (rc != UNP_OK) return rc;
+  const unp_cache4& c = x->l.cache4;
+  cache_args_host args;
+  if ((rc = cache_scalars(x, A, false, args, err)) != UNP_OK) return rc;
+  if (rot) {
+    if ((rc = check_rows(A.ext[6], A.ext[7], err)) != UNP_OK) return rc;
+    args.first = A.ext[6];
+    args.rows = A.ext[7];
+  }
+  if (args.tokens == 0 || args.slots == 0 || (rot && args.rows == 0)) return UNP_OK;
+  if ((rc = need_buffers(A, true, err)) != UNP_OK) return rc;
+  const uint64_t ib = unp::kind_bytes(c.index_dtype);
+  if (A.buf[0] % 2 || A.buf[1] % 2 || A.buf[2] % ib || !aligned16(A.buf[3]) ||
+      (rot && (A.buf[4] % ib || !aligned16(A.buf[5]))))
+    return invalid(err, "k, v, slots and positions are aligned to their elements, the cache and the table to 16 bytes");
+  const bool fast = whole_vectors(A.buf[0], A.ext[2], A.ext[3], 8) && whole_vectors(A.buf[1], A.ext[4], A.ext[5], 8);
+  int lanes = 1;
+  while (lanes < c.head_dim / 8) lanes *= 2;
+  const int64_t items = args.tokens * 2 * c.kv_heads, per = 256 / lanes;
+  uint64_t k = A.buf[0], v = A.buf[1], slots = A.buf[2], cache = A.buf[3], pos = rot ? A.buf[4] : 0, tab = rot ? A.buf[5] : 0;
+  void* params[] = {&k, &v, &slots, &cache, &pos, &tab, &args};
+  return launch(x, fast ? 0 : 1, grid_for(x, (items + per - 1) / per), params, s, err);
+}
+
+int32_t run_cache4_read(unp_exec* x, const unp_arg* a, size_t n, hipStream_t s, unp_error* err) {
+  Args A;
+  int32_t rc = take_args(a, n, 4, 6, A, err);
+  if (rc != UNP_OK) return rc;
+  const unp_cache4& c = x->l.cache4;
+  cache_args_host args;
+  if ((rc = cache_scalars(x, A, true, args, err)) != UNP_OK) return rc;
+  if (args.tokens == 0) return UNP_OK;
+  // An empty cache reads as zeros.
+  if (A.buf[0] == 0 || A.buf[2] == 0 || A.buf[3] == 0 || (args.slots > 0 && A.buf[1] == 0))
+    return invalid(err, "a null buffer");
+  if (A.buf[2] % 2 || A.buf[3] % 2 || A.buf[0] % unp::kind_bytes(c.index_dtype) || !aligned16(A.buf[1]))
+    return invalid(err, "slots, k and v are aligned to their elements, the cache to 16 bytes");
+  const bool fast = whole_vectors(A.buf[2], A.ext[2], A.ext[3], 8) && whole_vectors(A.buf[3], A.ext[4], A.ext[5], 8);
+  const int64_t lanes = args.tokens * 2 * c.kv_heads * (c.head_dim / 8);
+  uint64_t slots = A.buf[0], cache = A.buf[1], k = A.buf[2], v = A.buf[3];
+  void* params[] = {&slots, &cache, &k, &v, &args};
+  return launch(x, fast ? 0 : 1, grid_for(x, (lanes + 255) / 256), params, s, err);
+}
+
+int32_t check_attention(int64_t tokens, int64_t batch, int64_t width, int64_t pages, unp_error* err) {
+  const int64_t most = 0x7FFFFFFFLL;
+  if (tokens < 0 || tokens > most || batch < 0 || batch > most || width < 0 || width > most || pages < 0 || pages > most)
+    return invalid(err, "tokens, batch, width and pages are 0..2^31 - 1");
+  return UNP_OK;
+}
+
+int32_t attention_workspace(const unp_exec* x, const int64_t* sc, size_t n, uint64_t& bytes, unp_error* err) {
+  if (x->l.form.kind != UNP_FORM_CACHE4_ATTENTION) return invalid(err, "only a cache attention takes a workspace");
+  if (n != 4) return invalid(err, "expected tokens, batch, width and pages");
+  bytes = 0;
+  return check_attention(sc[0], sc[1], sc[2], sc[3], err);
+}
+
+int32_t run_cache4_attention(unp_exec* x, const unp_arg* a, size_t n, hipStream_t s, unp_error* err) {
+  Args A;
+  const unp_cache4& c = x->l.cache4;
+  const unp_attention& at = x->l.attention;
+  const size_t nb = at.lse ? 8 : 7;
+  int32_t rc = take_args(a, n, nb, 10, A, err);
+  if (rc != UNP_OK) return rc;
+  const int64_t tokens = A.ext[0], batch = A.ext[1];
+  if ((rc = check_attention(tokens, batch, A.ext[2], A.ext[3], err)) != UNP_OK) return rc;
+  if ((rc = check_heads("q", tokens, A.ext[4], at.heads, A.ext[5], c.head_dim, false, err)) != UNP_OK) return rc;
+  if ((rc = check_heads("out", tokens, A.ext[6], at.heads, A.ext[7], c.head_dim, true, err)) != UNP_OK) return rc;
+  if (A.ext[8] < 0) return invalid(err, "the window is negative");
+  if (A.ext[8] > 0 && !at.causal) return invalid(err, "a window needs a causal form");
+  if (A.ext[9] < 0) return invalid(err, "workspace_bytes is negative");
+  if (tokens == 0 || batch == 0) return UNP_OK;
+  const bool keys = A.ext[2] > 0 && A.ext[3] > 0;
+  for (size_t i = 0; i < nb; ++i) {
+    const bool may_be_null = (!keys && (i == 1 || i == 2)) || (i == nb - 1 && A.ext[9] == 0);
+    if (A.buf[i] == 0 && !may_be_null) return invalid(err, "buffer argument " + std::to_string(i) + " is null");
+  }
+  if (A.buf[0] % 2 || A.buf[5] % 2 || A.buf[2] % 4 || A.buf[3] % 4 || A.buf[4] % 4 || !aligned16(A.buf[1]) ||
+      (at.lse && A.buf[6] % 4) || !aligned16(A.buf[nb - 1]))
+    return invalid(err, "buffers are aligned to their elements, the cache and the workspace to 16 bytes");
+  attention_args_host args{tokens, batch, keys ? A.ext[2] : 0, A.ext[3], A.ext[4], A.ext[5], A.ext[6], A.ext[7], A.ext[8]};
+  uint64_t q = A.buf[0], cache = A.buf[1], table = A.buf[2], starts = A.buf[3], lengths = A.buf[4], out = A.buf[5];
+  uint64_t lse = at.lse ? A.buf[6] : 0;
+  float scale = (float)at.scale;
+  void* params[] = {&q, &cache, &table, &starts, &lengths, &out, &lse, &scale, &args};
+  return launch(x, 0, grid_for(x, tokens * at.heads), params, s, err);
+}
+
 }  // namespace
 
 // Element bits of buffer parameter b of a form: the element kinds of its storage images.
@@ -2252,6 +2551,8 @@ extern "C" int32_t unp_hip_exec_launch_views(unp_exec* x, const unp_view* views,
   if (!x) return invalid(err, "null executor");
   if ((nviews && !views) || (nscalars && !scalars)) return invalid(err, "null views or scalars");
   const unp_form& f = x->l.form;
+  if (f.kind >= UNP_FORM_ROPE_TABLE)
+    return invalid(err, "a rotary or cache form takes its strides as scalars (unp_hip_exec_launch)");
   size_t nbuf = 0, nscal = 0;
   param_counts(x, nbuf, nscal);
   if (nviews != nbuf || nscalars != nscal)
@@ -2343,6 +2644,16 @@ extern "C" int32_t unp_hip_exec_launch(unp_exec* x, const unp_arg* args, size_t 
       return run_dequant_gemm(x, args, nargs, s, err);
     case UNP_FORM_ELEMENTWISE:
       return run_elementwise(x, args, nargs, s, err);
+    case UNP_FORM_ROPE_TABLE:
+      return run_rope_table(x, args, nargs, s, err);
+    case UNP_FORM_ROPE:
+      return run_rope(x, args, nargs, s, err);
+    case UNP_FORM_CACHE4_APPEND:
+      return run_cache4_append(x, args, nargs, s, err);
+    case UNP_FORM_CACHE4_READ:
+      return run_cache4_read(x, args, nargs, s, err);
+    case UNP_FORM_CACHE4_ATTENTION:
+      return run_cache4_attention(x, args, nargs, s, err);
     default:
       set_error(err, UNP_UNSUPPORTED_KERNEL, "unknown form");
       return UNP_UNSUPPORTED_KERNEL;

@@ -179,6 +179,10 @@ struct Lowered {
   ReductionExpr rx;  // UNP_FORM_REDUCTION and UNP_FORM_SCAN: the pre-map body and the post
   GatherExpr gx;     // UNP_FORM_GATHER: the inputs and body
   ElementwiseExpr ew;  // UNP_FORM_ELEMENTWISE: the inputs, their permutations and the body
+  unp_rope_table rope_table{};  // UNP_FORM_ROPE_TABLE
+  unp_rope rope{};              // UNP_FORM_ROPE; UNP_FORM_CACHE4_APPEND: its rot
+  unp_cache4 cache4{};          // the UNP_FORM_CACHE4_* forms
+  unp_attention attention{};    // UNP_FORM_CACHE4_ATTENTION, its scale resolved
 };
 
 // Emit the HIP source and interface for `f`; on refusal returns a nonzero unp_status and
@@ -195,6 +199,17 @@ int32_t lower_gather_x(const unp_form& f, const GatherExpr& gx, Lowered& out, st
 int32_t lower_row_reduce(const RowReduceSpec& spec, Lowered& out, std::string& detail);
 // A recognised Access::Elementwise (its body comes only with the KernelFn).
 int32_t lower_elementwise(const unp_form& f, const ElementwiseExpr& ew, Lowered& out, std::string& detail);
+
+// The rotary and 4-bit cache forms (emit_cache4.cpp).
+int32_t lower_rope_table(const unp_rope_table& t, Lowered& out, std::string& why);
+int32_t lower_rope(const unp_rope& r, Lowered& out, std::string& why);
+int32_t lower_cache4_append(const unp_cache4& c, int32_t rot, int32_t layout, Lowered& out, std::string& why);
+int32_t lower_cache4_read(const unp_cache4& c, Lowered& out, std::string& why);
+int32_t lower_cache4_attention(const unp_cache4& c, const unp_attention& a, Lowered& out, std::string& why);
+int32_t check_cache4(const unp_cache4& c, std::string& why);  // a nonzero unp_status where no cache form takes it
+inline uint64_t cache4_record_bytes(const unp_cache4& c) {
+  return (uint64_t)c.page * (uint64_t)(c.head_dim + 8 * (c.head_dim / c.group));
+}
 
 // Backend::lower_kernel's recognizer (lifts.cpp): the form a KernelFn's JSON is, or a refusal.
 // A recognised kernel: the form to lower, the lift it matched, and the kernel's name, declared
