@@ -385,7 +385,7 @@ typedef struct unp_attention {
   int32_t causal;  /* 1: row i of n of a sequence of length L sees keys 0 .. L - n + i; 0: every row sees all L */
   int32_t lse;     /* 1: also write each row's log of the sum of exponentials */
   int32_t pad;
-  double scale;    /* of the scores; 0: 1 / sqrt(head_dim) */
+  double scale;    /* of the scores, 2^-24..2^24; 0: 1 / sqrt(head_dim) */
 } unp_attention;
 /* Attention of a ragged batch's rows over their sequences' pages.
  * Launch: q (rows of heads x head_dim), cache, page_table (I32 [batch][width]), starts (I32 [batch + 1]: sequence b's
@@ -396,7 +396,8 @@ typedef struct unp_attention {
  *   Keys that no row may see do not count, whatever they hold: keys past a sequence's length, keys of a page number
  *   outside the cache, keys past width pages.  Rows that no sequence names are left as they were.  starts do not
  *   decrease; in a list that does, which sequence takes a row, if any, is not said.
- *   The scores, the softmax's statistics and the sums are held in 32 bits.  The workspace (16-byte aligned) holds the parts
+ *   The scores, the softmax's statistics and the sums are held in 32 bits; in the products a probability and a value
+ *   are f16 numbers (values past 65504 overflow).  The workspace (16-byte aligned) holds the parts
  *   of a context that is split over blocks; one smaller than unp_hip_exec_workspace says, 0 among them, lowers the
  *   split.  The sums' order follows from the scalars and lengths alone: the same call gives the same bits. */
 int32_t unp_hip_lower_cache4_attention(const unp_cache4* c, const unp_attention* a, unp_generated** out,

@@ -264,8 +264,8 @@ int32_t lower_cache4_attention(const unp_cache4& c, const unp_attention& a, Lowe
     return why = "heads is kv_heads times 1..128", UNP_UNSUPPORTED_KERNEL;
   if ((a.causal != 0 && a.causal != 1) || (a.lse != 0 && a.lse != 1))
     return why = "causal and lse are 0 or 1", UNP_UNSUPPORTED_KERNEL;
-  if (!std::isfinite(a.scale) || a.scale < 0.0 || (a.scale != 0.0 && !((float)a.scale >= 0x1p-100f && (float)a.scale <= 0x1p100f)))
-    return why = "the scale is 0 (1 / sqrt(head_dim)) or a positive number in 2^-100..2^100", UNP_UNSUPPORTED_KERNEL;
+  if (a.scale != 0.0 && !(a.scale >= 0x1p-24 && a.scale <= 0x1p24))
+    return why = "the scale is 0 (1 / sqrt(head_dim)) or lies in 2^-24..2^24", UNP_UNSUPPORTED_KERNEL;
   L.form.kind = UNP_FORM_CACHE4_ATTENTION;
   L.form.dtype = c.dtype;
   L.cache4 = c;
@@ -274,17 +274,32 @@ int32_t lower_cache4_attention(const unp_cache4& c, const unp_attention& a, Lowe
   const char* T = device_type(c.dtype);
   L.name = "unp_cache4_attention_" + cache_name(c) + "_q" + std::to_string(a.heads) + (a.causal ? "_causal" : "_full") +
            (a.lse ? "_lse" : "");
-  L.threads = 64;
   std::ostringstream src;
   src << source_head(L.name);
+  const std::string same = std::string(T) + ", " + std::to_string(c.kv_heads) + ", " + std::to_string(a.heads) + ", " +
+                           std::to_string(c.head_dim);
+  const char* lse = a.lse ? "true" : "false";
+  auto add = [&](const char* tail, int qt, int wr, int wk) {
+    Entry e;
+    e.symbol = L.name + tail;
+    e.threads = 64 * wr * wk;
+    e.vec = 16 * qt * wr;  // rows of a block
+    e.k = wk;              // waves that share them
+    L.entries.push_back(e);
+    src << "extern \"C\" __global__ void __launch_bounds__(" << e.threads << ") " << e.symbol << "(const " << T
+        << "* q, const unsigned* cache, const int* table, const int* starts, const int* lengths, " << T
+        << "* out, float* lse, float* ws, float scale, unp4::attention_args a) {\n  unp4::attend<" << same << ", " << c.group
+        << ", " << c.page << ", " << (a.causal ? "true" : "false") << ", " << lse << ", " << qt << ", " << wr << ", " << wk
+        << ">(q, cache, table, starts, lengths, out, lse, ws, scale, a);\n}\n";
+  };
+  add("_few", 1, 1, 8);
+  add("_many", 2, 4, 1);
   Entry e;
-  e.symbol = L.name + "_a";
+  e.symbol = L.name + "_join";
   L.entries.push_back(e);
-  src << "extern \"C\" __global__ void __launch_bounds__(64) " << e.symbol << "(const " << T
-      << "* q, const unsigned* cache, const int* table, const int* starts, const int* lengths, " << T
-      << "* out, float* lse, float scale, unp4::attention_args a) {\n  unp4::attend<" << T << ", " << c.kv_heads << ", "
-      << a.heads << ", " << c.head_dim << ", " << c.group << ", " << c.page << ", " << (a.causal ? "true" : "false") << ", "
-      << (a.lse ? "true" : "false") << ">(q, cache, table, starts, lengths, out, lse, scale, a);\n}\n";
+  src << kBounds256 << e.symbol << "(const int* starts, " << T
+      << "* out, float* lse, float* ws, unp4::attention_args a) {\n  unp4::join<" << same << ", " << lse
+      << ">(starts, out, lse, ws, a);\n}\n";
   L.source = src.str();
   const char* dt = kind_name(c.dtype);
   std::vector<Param> ps = {{"q", "Read", dt}, {"cache", "Read", "U8"}, {"page_table", "Read", "I32"},
@@ -296,8 +311,10 @@ int32_t lower_cache4_attention(const unp_cache4& c, const unp_attention& a, Lowe
     ps.push_back({s, nullptr, "I64"});
   L.interface_json =
       interface(L, "cache4_attention", cache_fields(c) + ",\"heads\":" + std::to_string(a.heads), ps,
-                "a wave per row and head, striding over the grid", {"always"}, "the caller's, by unp_hip_exec_workspace",
-                "scores, softmax statistics and sums in f32; each output rounded once");
+                "a block per row tile, part of a context and key/value head",
+                {"at most 16 rows of a key/value head per sequence on average", "otherwise", "after either, where a context is split"},
+                "the caller's, by unp_hip_exec_workspace",
+                "scores, softmax statistics and sums in f32, probabilities and values as f16 in the products; each output rounded once");
   return UNP_OK;
 }
 

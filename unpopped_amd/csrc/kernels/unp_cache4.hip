@@ -303,98 +303,554 @@ UNP4_DEV void read(const I* slots, const u32* cache, T* k, T* v, const cache_arg
 
 // ---------------------------------------------------------------------------------------
 // Attention over the cache.
+//
+// A wave holds QT x 16 rows of a sequence (its tokens times the query heads of one key/value head) and
+// walks the keys 32 at a time, all in registers:
+//   * S' = K Q' by mfma 16x16x32 f16, keys as rows and query rows as columns.  A key word's nibbles are used
+//     as they lie: masked to bits 0..3 or 4..7 of a 16-bit half they are the subnormal f16 numbers n 2^-24
+//     and n 2^-20, so 8 codes cost 5 operations, and the queries carry the powers of two (exactly: each row is
+//     scaled to f16's range, bf16's 8 bits fit in f16's 11).  The group's scale and zero point are applied to the
+//     f32 result: s (sum q n - zero sum q).
+//   * softmax over the columns: a lane holds 8 keys of one row, so the row's maximum needs two exchanges, and
+//     only when some score passes the running one by 2^0.9 (below that p stays in f16's range: p is
+//     held as 2^15 p).  The running sum is in f32.
+//   * O' += V' P' with the value words as rows: the result above is, lane by lane, the operand that this
+//     product needs when key k of its 32 is (k / 8, k % 8) -> 16 (k % 8 / 4) + 4 (k / 8) + k % 4.  A lane reads four
+//     tokens' words of 8 elements at once; pairs of tokens of one element are made by byte permutes, so nothing
+//     goes through LDS.  Values are (n - zero) exactly, times the scale, rounded to f16: with
+//     P's rounding that is 2 x 2^-11 of a product, below the output type's rounding for bf16.
 // ---------------------------------------------------------------------------------------
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+
 struct attention_args {
   i64 tokens, batch, width, pages, q_token, q_head, out_token, out_head, window;
+  int slots, splits, by_token;  // row tiles, parts of a context, and how tiles are numbered (tile_of)
 };
 
-// The sequence of a row: the b with starts[b] <= row < starts[b + 1], or -1.
-UNP4_DEV i64 sequence_of(const i32* starts, i64 batch, i64 row) {
-  i64 lo = 0, hi = batch;  // the last b with starts[b] <= row lies in lo .. hi - 1
+// The maximum over the four lanes of a row (lane, lane ^ 16, lane ^ 32, lane ^ 48).
+UNP4_DEV float row_max(float x) {
+  auto a = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(u32, x), __builtin_bit_cast(u32, x), false, false);
+  x = fmaxf(__builtin_bit_cast(float, (u32)a[0]), __builtin_bit_cast(float, (u32)a[1]));
+  a = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(u32, x), __builtin_bit_cast(u32, x), false, false);
+  return fmaxf(__builtin_bit_cast(float, (u32)a[0]), __builtin_bit_cast(float, (u32)a[1]));
+}
+UNP4_DEV float row_sum(float x) {
+  auto a = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(u32, x), __builtin_bit_cast(u32, x), false, false);
+  x = __builtin_bit_cast(float, (u32)a[0]) + __builtin_bit_cast(float, (u32)a[1]);
+  a = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(u32, x), __builtin_bit_cast(u32, x), false, false);
+  return __builtin_bit_cast(float, (u32)a[0]) + __builtin_bit_cast(float, (u32)a[1]);
+}
+
+UNP4_DEV int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+
+// The sequence and tile of a tile number, by one wave.  Tiles are numbered so that a sequence's number is known
+// from its start alone: its first is start * GQ / R + b (its rows fill at most one tile more than they span), or its
+// first token (by_token: a token's GQ rows fit one tile).
+struct tile {
+  int seq, start, rows, length, at;  // rows: tokens of the sequence; at: the tile's number in it, or seq < 0
+};
+template <int GQ, int R>
+UNP4_DEV tile tile_of(const i32* starts, const i32* lengths, const attention_args& a, int slot) {
+  const int lane = threadIdx.x & 63, tokens = (int)a.tokens;
+  auto start_of = [&](i64 b) {
+    const int s = starts[b];
+    return s < 0 ? 0 : s > tokens ? tokens : s;
+  };
+  auto first_of = [&](int s, i64 b) { return a.by_token ? (i64)s : (i64)s * GQ / R + b; };
+  i64 lo = 0, hi = a.batch;
+  for (;;) {  // the last b of lo .. hi - 1 whose first tile is at most slot
+    const i64 step = (hi - lo + 63) / 64, b = lo + lane * step;
+    const bool in = b < hi;
+    const int s = start_of(in ? b : lo), e = start_of((in ? b : lo) + 1), n = lengths[in ? b : lo];
+    const int count = __popcll(__ballot(in && first_of(s, b) <= slot));
+    if (count == 0) return {-1, 0, 0, 0, 0};
+    lo += (count - 1) * step;
+    if (step == 1) {
+      const int st = __builtin_amdgcn_readlane(s, count - 1), en = __builtin_amdgcn_readlane(e, count - 1);
+      tile t{(int)lo, st, en - st, __builtin_amdgcn_readlane(n, count - 1), (int)(slot - first_of(st, lo))};
+      if (t.at < 0 || (i64)t.at * R >= (i64)t.rows * GQ) t.seq = -1;
+      return t;
+    }
+    hi = lo + step < hi ? lo + step : hi;
+  }
+}
+
+template <class T, int H, int QH, int D, int GROUP, int P, bool CAUSAL, int QT> struct attention {
+  typedef record<D, GROUP, P> R;
+  static constexpr int GQ = QH / H, W = R::W, G = R::G, KJ = D / 32, JG = GROUP / 32;
+  // Value tiles: 16 rows of N adjacent elements each, from words FIRST on.  Full tiles of 16 words, then one of
+  // the rest, whose words go to several rows where they are few.
+  static constexpr int FULL = W / 16, REST = W % 16, NT = FULL + (REST ? 1 : 0);
+  static constexpr int NREST = REST == 0 ? 0 : REST <= 4 ? 2 : REST <= 8 ? 4 : 8;
+  static constexpr int NE = FULL * 8 + NREST;  // matrix products of 16 elements that cover a head
+  static constexpr int nibbles(int t) { return t < FULL ? 8 : NREST; }
+
+  struct block {  // what 16 keys' products need, as it lies in memory
+    u32 k[KJ];
+    u32x4 kp[G], v[NT], vp[NT];
+  };
+  int lane, c, g;  // c: the row a lane gives and the column it holds, g: its part of the depth
+  f16x8 q[QT][KJ];
+  float qsum[QT][G], factor[QT];  // of this lane's column; factor: raw scores to log2
+  float m[QT], l[QT];
+  f32x4 o[QT][NE];
+  int end[QT], begin[QT];  // keys that the column sees
+
+  // Rows first .. first + 16 QT - 1 (token * GQ + head of the group) of a sequence.
+  UNP4_DEV void rows(const T* qp, const attention_args& a, const tile& t, int kv, int first, float scale, int cap) {
+    lane = threadIdx.x & 63;
+    c = lane & 15;
+    g = lane >> 4;
+#pragma unroll
+    for (int x = 0; x < QT; ++x) {
+      const int r = first + x * 16 + c;
+      const bool in = r < t.rows * GQ;
+      const int token = in ? r / GQ : 0, head = kv * GQ + (in ? r % GQ : 0);
+      const T* p = qp + (i64)(t.start + token) * a.q_token + (i64)head * a.q_head;
+      T raw[KJ][8];
+      float top = 0.0f;
+#pragma unroll
+      for (int j = 0; j < KJ; ++j)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          raw[j][i] = in ? p[j * 32 + g * 8 + i] : (T)0.0f;
+          top = fmaxf(top, fabsf((float)raw[j][i]));
+        }
+      top = row_max(top);
+      // The power of two that puts the largest element into 2^13 .. 2^14: odd nibbles weigh 16 times as much, so
+      // their elements are scaled down by 16.
+      int up = top > 0.0f && top < __builtin_inff() ? 13 - (int)((__builtin_bit_cast(u32, top) >> 23) & 255) + 127 : 0;
+      up = up > 100 ? 100 : up < -100 ? -100 : up;
+      const float mul = __builtin_bit_cast(float, (u32)(up + 127) << 23);
+#pragma unroll
+      for (int gi = 0; gi < G; ++gi) qsum[x][gi] = 0.0f;
+#pragma unroll
+      for (int j = 0; j < KJ; ++j) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int d = (i >> 1) + 4 * (i & 1);  // the element at place i of a word's operand
+          const _Float16 y = (_Float16)((float)raw[j][d] * ((d & 1) ? mul * 0.0625f : mul));
+          q[x][j][i] = y;
+          qsum[x][j / JG] += (float)y * ((d & 1) ? 0x1p-20f : 0x1p-24f);
+        }
+      }
+#pragma unroll
+      for (int gi = 0; gi < G; ++gi) qsum[x][gi] = row_sum(qsum[x][gi]);
+      factor[x] = fminf(scale * 1.4426950408889634f * 0x1p24f * __builtin_bit_cast(float, (u32)(127 - up) << 23), 0x1p127f);
+      m[x] = -__builtin_inff();
+      l[x] = 0.0f;
+#pragma unroll
+      for (int e = 0; e < NE; ++e) o[x][e] = f32x4{0, 0, 0, 0};
+      const int last = CAUSAL ? t.length - t.rows + token + 1 : t.length;
+      end[x] = in ? (last < cap ? last : cap) : 0;
+      begin[x] = CAUSAL && a.window > 0 && a.window < last ? last - (int)a.window : 0;
+    }
+  }
+
+  UNP4_DEV int word_of(int t) const {  // the value word of this lane's row in tile t
+    const int w = t < FULL ? t * 16 + c : FULL * 16 + c * nibbles(t) / 8;
+    return w < W ? w : W - 1;
+  }
+
+  // 16 keys from token t0 (a multiple of 16) of a record on.
+  UNP4_DEV void load(const u32* rec, int t0, block& b) const {
+    const u32* kp = rec + R::KEYS + t0 * W + (c * W + g * KJ);
+#pragma unroll
+    for (int j = 0; j < KJ; ++j) b.k[j] = kp[j];
+#pragma unroll
+    for (int gi = 0; gi < G; ++gi) b.kp[gi] = *reinterpret_cast<const u32x4*>(rec + R::kpar(t0, gi) + g * 4);
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      const int w = word_of(t);
+      b.v[t] = *reinterpret_cast<const u32x4*>(rec + R::VALUES + t0 * W + (g * W + w) * 4);
+      b.vp[t] = *reinterpret_cast<const u32x4*>(rec + R::VPAR + t0 + (8 * w / GROUP) * P + g * 4);
+    }
+  }
+
+  static UNP4_DEV f16x8 key_operand(u32 x) {
+    const u32 y = x >> 8;
+    const u32x4 b = {x & 0x000F000Fu, x & 0x00F000F0u, y & 0x000F000Fu, y & 0x00F000F0u};
+    return __builtin_bit_cast(f16x8, b);
+  }
+
+  // Value tile t of both blocks: out[e] is the operand of element e of each row's nibbles(t).
+  template <int N> UNP4_DEV void value_operands(const block (&b)[2], int t, f16x8 (&out)[N]) const {
+    u32 part[N][4];
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        u32 wa = b[k].v[t][2 * h], wb = b[k].v[t][2 * h + 1];
+        const u32 pa = b[k].vp[t][2 * h], pb = b[k].vp[t][2 * h + 1];
+        if (N < 8) {  // this row's nibbles of the word
+          const int down = (c * N) % 8 * 4;
+          wa >>= down;
+          wb >>= down;
+        }
+        const f16x2 s = __builtin_bit_cast(f16x2, __builtin_amdgcn_perm(pb, pa, 0x05040100u));
+        const u32 z = __builtin_amdgcn_perm(pb, pa, 0x07060302u);
+        const f16x2 z0 = __builtin_bit_cast(f16x2, z | 0x64006400u), z1 = __builtin_bit_cast(f16x2, (z << 4) | 0x54005400u);
+#pragma unroll
+        for (int e = 0; e < N; e += 4) {
+          const u32 x = __builtin_amdgcn_perm(wb, wa, e ? 0x07060302u : 0x05040100u), y = x >> 8;
+          // 1024 + n in steps of 1, 64 + n in steps of 1/16: both exact, and so is n - zero.
+          part[e][2 * k + h] = pair((x & 0x000F000Fu) | 0x64006400u, z0, s);
+          part[e + 1][2 * k + h] = pair((x & 0x00F000F0u) | 0x54005400u, z1, s);
+          if (N > 2) {
+            part[e + 2 < N ? e + 2 : 0][2 * k + h] = pair((y & 0x000F000Fu) | 0x64006400u, z0, s);
+            part[e + 3 < N ? e + 3 : 0][2 * k + h] = pair((y & 0x00F000F0u) | 0x54005400u, z1, s);
+          }
+        }
+      }
+#pragma unroll
+    for (int e = 0; e < N; ++e)
+      out[e] = __builtin_bit_cast(f16x8, u32x4{part[e][0], part[e][1], part[e][2], part[e][3]});
+  }
+  static UNP4_DEV u32 pair(u32 bits, f16x2 z, f16x2 s) {
+    return __builtin_bit_cast(u32, (__builtin_bit_cast(f16x2, bits) - z) * s);
+  }
+
+  // A value scale that is no number would reach, as 0 x NaN, the columns that do not see its key.  Such words are
+  // taken out of the product, and the elements of the columns that see them become NaN.
+  UNP4_DEV void guard(block (&b)[2], const u32 (&seen)[QT]) {
+    u32 bad[NT], any = 0;
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      bad[t] = 0;
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if ((b[i / 4].vp[t][i % 4] & 0x7C00u) == 0x7C00u) bad[t] |= 1u << i;
+      any |= bad[t];
+    }
+    if (!__any(any != 0)) return;
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (bad[t] >> i & 1) b[i / 4].vp[t][i % 4] = 0;
+      for (int part = 0; part < 4; ++part)  // the keys of each part of the depth
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const u32 row = __shfl(bad[t], part * 16 + g * 4 + r);
+#pragma unroll
+          for (int x = 0; x < QT; ++x)
+            if (row & __shfl(seen[x], part * 16 + c)) {
+#pragma unroll
+              for (int e = 0; e < nibbles(t); ++e) o[x][8 * t + e][r] = __builtin_nanf("");
+            }
+        }
+    }
+  }
+
+  // 32 keys from k0 on; MASKED: some column may not see some of them.  good: whether each block's page is one.
+  template <bool MASKED> UNP4_DEV void step(block (&b)[2], int k0, int cap, bool good0, bool good1) {
+    if (MASKED) {  // what no row may see does not count, whatever it holds
+#pragma unroll
+      for (int k = 0; k < 2; ++k)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (!(k ? good1 : good0) || k0 + 16 * k + 4 * g + i >= cap)
+#pragma unroll
+            for (int t = 0; t < NT; ++t) b[k].vp[t][i] = 0;
+    }
+    f16x8 ka[2][KJ];
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+#pragma unroll
+      for (int j = 0; j < KJ; ++j) ka[k][j] = key_operand(b[k].k[j]);
+    f16x8 p[QT];
+    u32 seen[QT];  // MASKED: which of its 8 keys each of this lane's columns sees
+#pragma unroll
+    for (int x = 0; x < QT; ++x) {
+      float s[8];
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+#pragma unroll
+        for (int gi = 0; gi < G; ++gi) {
+          f32x4 acc = {0, 0, 0, 0};
+#pragma unroll
+          for (int j = gi * JG; j < (gi + 1) * JG; ++j)
+            acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka[k][j], q[x][j], acc, 0, 0, 0);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const u32 w = b[k].kp[gi][i];
+            const float d = fmaf(-zero_of(w), qsum[x][gi], acc[i]);
+            s[4 * k + i] = gi == 0 ? d * scale_of(w) : fmaf(d, scale_of(w), s[4 * k + i]);
+          }
+        }
+      }
+      if (MASKED) {
+        seen[x] = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int key = k0 + 16 * (i / 4) + 4 * g + i % 4;
+          const bool sees = key < end[x] && key >= begin[x] && (i < 4 ? good0 : good1);
+          s[i] = sees ? s[i] : -__builtin_inff();
+          if (sees) seen[x] |= 1u << i;
+        }
+      }
+      float top = s[0];
+#pragma unroll
+      for (int i = 1; i < 8; ++i) top = fmaxf(top, s[i]);
+      if (__any((top - m[x]) * factor[x] > 0.9f)) {
+        const float next = fmaxf(m[x], row_max(top));
+        const float keep = m[x] == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f((m[x] - next) * factor[x]);
+        m[x] = next;
+        l[x] *= keep;
+#pragma unroll
+        for (int e = 0; e < NE; ++e) o[x][e] *= keep;
+      }
+      const float off = m[x] == -__builtin_inff() ? 0.0f : fmaf(-m[x], factor[x], 15.0f);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float e = __builtin_amdgcn_exp2f(fmaf(s[i], factor[x], off));
+        l[x] += e;
+        p[x][i] = (_Float16)e;
+      }
+    }
+    if (MASKED) guard(b, seen);
+    int at = 0;
+#pragma unroll
+    for (int t = 0; t < FULL; ++t) {
+      f16x8 va[8];
+      value_operands<8>(b, t, va);
+#pragma unroll
+      for (int e = 0; e < 8; ++e, ++at)
+#pragma unroll
+        for (int x = 0; x < QT; ++x) o[x][at] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va[e], p[x], o[x][at], 0, 0, 0);
+    }
+    if constexpr (REST > 0) {
+      f16x8 va[NREST];
+      value_operands<NREST>(b, FULL, va);
+#pragma unroll
+      for (int e = 0; e < NREST; ++e, ++at)
+#pragma unroll
+        for (int x = 0; x < QT; ++x) o[x][at] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va[e], p[x], o[x][at], 0, 0, 0);
+    }
+  }
+
+  // The keys of steps first, first + by, .. below last (a step is 32 keys), each step loaded a step ahead.  lo, hi:
+  // the keys from lo on and below hi that every column sees.
+  UNP4_DEV void walk(const u32* cache, const i32* pages, const attention_args& a, int kv, int first, int by, int last,
+                     int cap, int lo, int hi) {
+    if (first >= last) return;
+    auto page = [&](int step, int k) {
+      const int key = step * 32 + 16 * k;
+      return key < cap ? pages[key / P] : -1;  // uniform: cap keys lie in the table's row
+    };
+    auto good = [&](int id) { return (u32)id < (u32)a.pages; };
+    auto fetch = [&](int step, int id0, int id1, block (&b)[2]) {
+      load(cache + ((i64)(good(id0) ? id0 : 0) * H + kv) * (i64)R::WORDS, step * 32 % P, b[0]);
+      load(cache + ((i64)(good(id1) ? id1 : 0) * H + kv) * (i64)R::WORDS, (step * 32 + 16) % P, b[1]);
+    };
+    int id0 = page(first, 0), id1 = page(first, 1);
+    block now[2];
+    fetch(first, id0, id1, now);
+    int next = first + by;
+    int n0 = next < last ? page(next, 0) : -1, n1 = next < last ? page(next, 1) : -1;
+    for (int at = first;;) {
+      block ahead[2];
+      if (next < last) fetch(next, n0, n1, ahead);
+      const int after = next + by;
+      const int f0 = after < last ? page(after, 0) : -1, f1 = after < last ? page(after, 1) : -1;
+      const int k0 = at * 32;
+      if (k0 >= lo && k0 + 32 <= hi && good(id0) && good(id1))
+        step<false>(now, k0, cap, true, true);
+      else
+        step<true>(now, k0, cap, good(id0), good(id1));
+      if (next >= last) return;
+#pragma unroll
+      for (int k = 0; k < 2; ++k) now[k] = ahead[k];
+      id0 = n0;
+      id1 = n1;
+      n0 = f0;
+      n1 = f1;
+      at = next;
+      next = after;
+    }
+  }
+
+  // f(x, element, four-vector part i, value): every element of the lane's columns, N adjacent ones at a time.
+  template <class F> UNP4_DEV void each(F f) const {
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int n = nibbles(t), d = t * 128 + (g * 4 + r) * n;
+        if (t * 128 + 16 * n <= D || d < D) f(t, r, d);
+      }
+  }
+};
+
+// A context's parts in the workspace: [part][token][head] of (maximum in log2, sum), then of D sums.
+template <int QH, int D> struct parts {
+  static UNP4_DEV float* stat(float* ws, const attention_args& a, i64 part, i64 row, int head) {
+    return ws + ((part * a.tokens + row) * QH + head) * 2;
+  }
+  static UNP4_DEV float* sums(float* ws, const attention_args& a, i64 part, i64 row, int head) {
+    return ws + a.splits * a.tokens * QH * 2 + ((part * a.tokens + row) * QH + head) * D;
+  }
+};
+
+// Four elements (two of a narrow tile) of f32 sums.
+UNP4_DEV void put(float* p, const f32x4& o, int n) {
+  if (n >= 4) {
+    *reinterpret_cast<f32x4*>(p) = o;
+  } else {
+    *reinterpret_cast<f32x2*>(p) = f32x2{o[0], o[1]};
+  }
+}
+
+// A row's elements d .. from their sums; top: the maximum in log2, to which p is held as 2^15 p.
+template <class T, int QH, bool LSE>
+UNP4_DEV void finish(T* out, float* lse, const attention_args& a, i64 row, int head, int d, float top, float l, const f32x4& o,
+                     int n = 4) {
+  const float by = l == 0.0f ? 0.0f : 1.0f / l;  // a row that sees nothing gives 0
+  T* p = out + row * a.out_token + head * a.out_head + d;
+  vec<T, 4> y;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) y.v[i] = (T)(l == 0.0f ? 0.0f : o[i] * by);
+  if (n >= 4 && (reinterpret_cast<u64>(p) & 7) == 0) {
+    store<T, 4>(p, y);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (i < n) p[i] = y.v[i];
+  }
+  if (LSE && d == 0) lse[row * QH + head] = l == 0.0f ? -__builtin_inff() : (top - 15.0f + __log2f(l)) * 0.693147180559945309f;
+}
+
+// A block: WR waves of QT x 16 rows each and, for few rows, WK waves of the same rows that take the steps in turn
+// and are joined through LDS.  Blocks are numbered with the heads innermost (consecutive blocks go to different
+// XCDs: with 8 heads each XCD's L2 holds one head's keys), then the parts of a context, then the tiles, last ones
+// first: under a causal mask those have the most keys.
+template <class T, int H, int QH, int D, int GROUP, int P, bool CAUSAL, bool LSE, int QT, int WR, int WK>
+UNP4_DEV void attend(const T* q, const u32* cache, const i32* table, const i32* starts, const i32* lengths, T* out,
+                     float* lse, float* ws, float scale, const attention_args& a) {
+  typedef attention<T, H, QH, D, GROUP, P, CAUSAL, QT> A;
+  constexpr int GQ = QH / H, ROWS = 16 * QT * WR;
+  const int wave = uniform(threadIdx.x >> 6);
+  const int kv = blockIdx.x % H, part = (int)(blockIdx.x / H) % a.splits;
+  const tile t = tile_of<GQ, ROWS>(starts, lengths, a, a.slots - 1 - (int)(blockIdx.x / H) / a.splits);
+  if (t.seq < 0) return;
+  const i64 room = a.width * P;
+  const int cap = t.length < 0 ? 0 : t.length < room ? t.length : (int)room;
+  const int first_row = t.at * ROWS + (WR > 1 ? wave / WK * 16 * QT : 0), all_rows = t.rows * GQ;
+  // Keys that the wave's first and last rows see: some column sees keys from .. to, all see lo .. hi.
+  const int last_row = (first_row + 16 * QT < all_rows ? first_row + 16 * QT : all_rows) - 1;
+  int from = 0, to = cap, lo = 0, hi = cap;
+  if (CAUSAL) {
+    const i64 near = (i64)t.length - t.rows + first_row / GQ + 1, far = (i64)t.length - t.rows + last_row / GQ + 1;
+    to = far < 0 ? 0 : far < cap ? (int)far : cap;
+    hi = near < 0 ? 0 : near < cap ? (int)near : cap;
+    if (a.window > 0) {
+      from = near > a.window ? (int)(near - a.window) : 0;
+      lo = far > a.window ? (int)(far - a.window) : 0;
+    }
+  }
+  if (last_row < first_row) to = 0;
+  // This part's steps.
+  const int step0 = from / 32, steps = to > from ? (to + 31) / 32 - step0 : 0;
+  const int each = (steps + a.splits - 1) / a.splits;
+  const int begin = step0 + (int)min((i64)steps, (i64)part * each);
+  const int end = step0 + (int)min((i64)steps, (i64)(part + 1) * each);
+  A w;
+  w.rows(q, a, t, kv, first_row, scale, cap);
+  w.walk(cache, table + (i64)t.seq * a.width, a, kv, begin + (WK > 1 ? wave % WK : 0), WK, end, cap, lo, hi);
+#pragma unroll
+  for (int x = 0; x < QT; ++x) w.l[x] = row_sum(w.l[x]);
+  if constexpr (WK > 1) {
+    // Join the waves: the rows' maxima and sums, then their elements, each scaled to the common maximum.
+    __shared__ float stat[WK][QT][16][2];
+    __shared__ float sums[WK][QT * 16][D + 4];
+    if (w.g == 0)
+#pragma unroll
+      for (int x = 0; x < QT; ++x) {
+        stat[wave][x][w.c][0] = w.m[x] * w.factor[x];
+        stat[wave][x][w.c][1] = w.l[x];
+      }
+    w.each([&](int tl, int r, int d) {
+#pragma unroll
+      for (int x = 0; x < QT; ++x)
+#pragma unroll
+        for (int e = 0; e < A::nibbles(tl); ++e) sums[wave][x * 16 + w.c][d + e] = w.o[x][8 * tl + e][r];
+    });
+    __syncthreads();
+    const int n = all_rows - first_row < 16 * QT ? all_rows - first_row : 16 * QT;
+    for (int i = threadIdx.x; i < n * (D / 4); i += 64 * WK) {
+      const int row = i / (D / 4), d = i % (D / 4) * 4;
+      float top = -__builtin_inff(), l = 0.0f;
+#pragma unroll
+      for (int v = 0; v < WK; ++v) top = fmaxf(top, stat[v][row / 16][row % 16][0]);
+      const float base = top == -__builtin_inff() ? 0.0f : top;
+      f32x4 o = {0, 0, 0, 0};
+#pragma unroll
+      for (int v = 0; v < WK; ++v) {
+        const float keep = __builtin_amdgcn_exp2f(stat[v][row / 16][row % 16][0] - base);
+        l = fmaf(stat[v][row / 16][row % 16][1], keep, l);
+        o += *reinterpret_cast<const f32x4*>(&sums[v][row][d]) * keep;
+      }
+      const int token = t.start + (first_row + row) / GQ, head = kv * GQ + (first_row + row) % GQ;
+      if (a.splits > 1) {
+        if (d == 0) store<float, 2>(parts<QH, D>::stat(ws, a, part, token, head), {top, l});
+        if (l != 0.0f) *reinterpret_cast<f32x4*>(parts<QH, D>::sums(ws, a, part, token, head) + d) = o;
+      } else {
+        finish<T, QH, LSE>(out, lse, a, token, head, d, top, l, o);
+      }
+    }
+  } else {
+#pragma unroll
+    for (int x = 0; x < QT; ++x) {
+      const int row = first_row + x * 16 + w.c;
+      if (row >= all_rows) continue;
+      const int token = t.start + row / GQ, head = kv * GQ + row % GQ;
+      const float top = w.m[x] * w.factor[x], l = w.l[x];
+      if (a.splits > 1 && w.g == 0) store<float, 2>(parts<QH, D>::stat(ws, a, part, token, head), {top, l});
+      w.each([&](int tl, int r, int d) {
+#pragma unroll
+        for (int e = 0; e < A::nibbles(tl); e += 4) {
+          f32x4 o;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) o[i] = w.o[x][8 * tl + (e + i < A::nibbles(tl) ? e + i : 0)][r];
+          if (a.splits > 1) {
+            if (l != 0.0f) put(parts<QH, D>::sums(ws, a, part, token, head) + d + e, o, A::nibbles(tl));
+          } else {
+            finish<T, QH, LSE>(out, lse, a, token, head, d + e, top, l, o, A::nibbles(tl));
+          }
+        }
+      });
+    }
+  }
+}
+
+// The parts of split contexts: four elements of a row per lane.
+template <class T, int H, int QH, int D, bool LSE>
+UNP4_DEV void join(const i32* starts, T* out, float* lse, float* ws, const attention_args& a) {
+  constexpr int L = D / 4;
+  const i64 n = a.tokens * QH * L, i = (i64)blockIdx.x * 256 + threadIdx.x;
+  if (i >= n) return;
+  const i64 row = i / (QH * L);
+  const int head = (int)(i / L % QH), d = (int)(i % L) * 4;
+  // Rows that no sequence names have no parts.
+  i64 lo = 0, hi = a.batch;
   while (hi - lo > 1) {
     const i64 mid = (lo + hi) >> 1;
     if (starts[mid] <= row) lo = mid; else hi = mid;
   }
-  return starts[lo] <= row && row < starts[lo + 1] ? lo : -1;
-}
-
-// One wave per row and head: 64 keys a step, one per lane, with a running maximum and sum; then each lane
-// adds up its own elements of the output.
-template <class T, int H, int QH, int D, int GROUP, int P, bool CAUSAL, bool LSE>
-UNP4_DEV void attend(const T* q, const u32* cache, const i32* table, const i32* starts, const i32* lengths, T* out,
-                     float* lse, float scale, const attention_args& a) {
-  typedef record<D, GROUP, P> R;
-  constexpr int E = (D + 63) / 64;
-  __shared__ float qs[D], ps[64];
-  __shared__ const u32* recs[64];
-  const int lane = threadIdx.x;
-  for (i64 at = blockIdx.x; at < a.tokens * QH; at += gridDim.x) {
-    const i64 row = at / QH;
-    const int head = (int)(at - row * QH), kv = head / (QH / H);
-    const i64 b = sequence_of(starts, a.batch, row);
-    if (b < 0) continue;
-    const i64 length = lengths[b];
-    i64 end = length, begin = 0;
-    if (CAUSAL) {
-      end = length - starts[b + 1] + row + 1;
-      if (a.window > 0 && end > a.window) begin = end - a.window;
-    }
-    if (end > a.width * P) end = a.width * P;
-    __syncthreads();
-    for (int d = lane; d < D; d += 64) qs[d] = (float)q[row * a.q_token + head * a.q_head + d] * scale;
-    __syncthreads();
-    float m = -__builtin_inff(), sum = 0.0f, o[E];
-    for (int e = 0; e < E; ++e) o[e] = 0.0f;
-    for (i64 j0 = begin; j0 < end; j0 += 64) {
-      const i64 j = j0 + lane;
-      const i32 page = j < end ? table[b * a.width + j / P] : -1;
-      const bool seen = page >= 0 && page < a.pages;
-      const u32* rec = seen ? cache + ((i64)page * H + kv) * (i64)R::WORDS : nullptr;
-      const int t = (int)(j % P);
-      float s = -__builtin_inff();
-      if (seen) {
-        s = 0.0f;
-        for (int w = 0; w < R::W; ++w) {
-          const u32 word = rec[R::key(t, w)], par = rec[R::kpar(t, 8 * w / GROUP)];
-          const float z = zero_of(par);
-          float part = 0.0f;
-          for (int i = 0; i < 8; ++i) part = fmaf(qs[8 * w + i], (float)(word >> (4 * i) & 15u) - z, part);
-          s = fmaf(part, scale_of(par), s);
-        }
-      }
-      float top = s;
-      for (int x = 1; x < 64; x *= 2) top = fmaxf(top, __shfl_xor(top, x));
-      const float next = fmaxf(m, top);
-      const float base = next > -__builtin_inff() ? next : 0.0f;
-      const float p = expf(s - base), keep = expf(m - base);
-      float total = p;
-      for (int x = 1; x < 64; x *= 2) total += __shfl_xor(total, x);
-      sum = fmaf(sum, keep, total);
-      m = next;
-      for (int e = 0; e < E; ++e) o[e] *= keep;
-      __syncthreads();
-      ps[lane] = p;
-      recs[lane] = rec;
-      __syncthreads();
-      for (int i = 0; i < 64; ++i) {
-        const u32* r = recs[i];
-        if (!r) continue;
-        const int ti = (int)((j0 + i) % P);
-        for (int e = 0; e < E; ++e) {
-          const int d = lane + 64 * e;
-          if (D % 64 != 0 && d >= D) continue;
-          const u32 word = r[R::value(ti, d / 8)], par = r[R::vpar(ti, d / GROUP)];
-          o[e] = fmaf(ps[i], ((float)(word >> (4 * (d & 7)) & 15u) - zero_of(par)) * scale_of(par), o[e]);
-        }
-      }
-    }
-    for (int e = 0; e < E; ++e) {
-      const int d = lane + 64 * e;
-      if (D % 64 == 0 || d < D)
-        out[row * a.out_token + head * a.out_head + d] = (T)(sum == 0.0f ? 0.0f : o[e] / sum);
-    }
-    if (LSE && lane == 0) lse[row * QH + head] = sum == 0.0f ? -__builtin_inff() : m + logf(sum);
+  if (starts[lo] > row || row >= starts[lo + 1]) return;
+  float top = -__builtin_inff(), l = 0.0f;
+  for (int s = 0; s < a.splits; ++s) top = fmaxf(top, parts<QH, D>::stat(ws, a, s, row, head)[0]);
+  const float base = top == -__builtin_inff() ? 0.0f : top;
+  f32x4 o = {0, 0, 0, 0};
+  for (int s = 0; s < a.splits; ++s) {
+    const f32x2 st = *reinterpret_cast<const f32x2*>(parts<QH, D>::stat(ws, a, s, row, head));
+    if (st[1] == 0.0f) continue;
+    const float keep = __builtin_amdgcn_exp2f(st[0] - base);
+    l = fmaf(st[1], keep, l);
+    o += *reinterpret_cast<const f32x4*>(parts<QH, D>::sums(ws, a, s, row, head) + d) * keep;
   }
+  finish<T, QH, LSE>(out, lse, a, row, head, d, top, l, o);
 }
 
 }  // namespace unp4

@@ -1874,6 +1874,7 @@ struct cache_args_host {
 };
 struct attention_args_host {
   int64_t tokens, batch, width, pages, q_token, q_head, out_token, out_head, window;
+  int32_t slots, splits, by_token, pad;
 };
 
 constexpr int64_t kMostOffset = (int64_t)1 << 60;
@@ -2038,11 +2039,45 @@ int32_t check_attention(int64_t tokens, int64_t batch, int64_t width, int64_t pa
   return UNP_OK;
 }
 
+// A launch's shape: the entry, its row tiles, how they are numbered (tile_of) and the parts of a context.
+struct AttentionPlan {
+  size_t entry = 0;
+  int64_t slots = 0, splits = 1;
+  bool by_token = false;
+};
+// The workspace of one part of every row: its maximum and sum, and head_dim sums.
+int64_t part_bytes(const unp_exec* x, int64_t tokens) {
+  return tokens * x->l.attention.heads * (x->l.cache4.head_dim + 2) * 4;
+}
+AttentionPlan attention_plan(const unp_exec* x, int64_t tokens, int64_t batch, int64_t width) {
+  const unp_cache4& c = x->l.cache4;
+  const int64_t group = x->l.attention.heads / c.kv_heads;
+  AttentionPlan p;
+  // Waves that share 16 rows where sequences have that many or fewer, waves of rows of their own beyond.
+  p.entry = tokens * group <= 16 * batch ? 0 : 1;
+  const unp::Entry& e = x->l.entries[p.entry];
+  p.slots = tokens * group / e.vec + batch;
+  if (group <= e.vec && tokens <= p.slots) {
+    p.slots = tokens;
+    p.by_token = true;
+  }
+  // As many parts as give every CU two blocks, none shorter than two steps of 32 keys of each wave that shares a
+  // block's rows; with the whole context's pages as its length, which the host does not know.
+  const int64_t blocks = p.slots * c.kv_heads, want = (2LL * x->cu_count + blocks - 1) / blocks;
+  const int64_t most = (width * c.page + 64 * e.k - 1) / (64 * e.k);
+  p.splits = std::max<int64_t>(1, std::min({want, most, (int64_t)128}));
+  return p;
+}
+
 int32_t attention_workspace(const unp_exec* x, const int64_t* sc, size_t n, uint64_t& bytes, unp_error* err) {
   if (x->l.form.kind != UNP_FORM_CACHE4_ATTENTION) return invalid(err, "only a cache attention takes a workspace");
   if (n != 4) return invalid(err, "expected tokens, batch, width and pages");
+  const int32_t rc = check_attention(sc[0], sc[1], sc[2], sc[3], err);
   bytes = 0;
-  return check_attention(sc[0], sc[1], sc[2], sc[3], err);
+  if (rc != UNP_OK || sc[0] == 0 || sc[1] == 0) return rc;
+  const AttentionPlan p = attention_plan(x, sc[0], sc[1], sc[3] > 0 ? sc[2] : 0);
+  if (p.splits > 1) bytes = (uint64_t)(p.splits * part_bytes(x, sc[0]));
+  return UNP_OK;
 }
 
 int32_t run_cache4_attention(unp_exec* x, const unp_arg* a, size_t n, hipStream_t s, unp_error* err) {
@@ -2068,12 +2103,24 @@ int32_t run_cache4_attention(unp_exec* x, const unp_arg* a, size_t n, hipStream_
   if (A.buf[0] % 2 || A.buf[5] % 2 || A.buf[2] % 4 || A.buf[3] % 4 || A.buf[4] % 4 || !aligned16(A.buf[1]) ||
       (at.lse && A.buf[6] % 4) || !aligned16(A.buf[nb - 1]))
     return invalid(err, "buffers are aligned to their elements, the cache and the workspace to 16 bytes");
-  attention_args_host args{tokens, batch, keys ? A.ext[2] : 0, A.ext[3], A.ext[4], A.ext[5], A.ext[6], A.ext[7], A.ext[8]};
+  AttentionPlan p = attention_plan(x, tokens, batch, keys ? A.ext[2] : 0);
+  p.splits = std::max<int64_t>(1, std::min(p.splits, A.ext[9] / part_bytes(x, tokens)));
+  if (p.splits == 1 && A.buf[nb - 1] == 0) A.buf[nb - 1] = A.buf[5];  // not used
+  const int64_t blocks = p.slots * p.splits * c.kv_heads;
+  const int64_t joins = (tokens * at.heads * (c.head_dim / 4) + 255) / 256;
+  if (blocks > 0x7FFFFFFFLL || joins > 0x7FFFFFFFLL) return invalid(err, "tokens: too many rows for one launch");
+  attention_args_host args{tokens, batch, keys ? A.ext[2] : 0, A.ext[3], A.ext[4], A.ext[5], A.ext[6], A.ext[7], A.ext[8],
+                           (int32_t)p.slots, (int32_t)p.splits, p.by_token ? 1 : 0, 0};
   uint64_t q = A.buf[0], cache = A.buf[1], table = A.buf[2], starts = A.buf[3], lengths = A.buf[4], out = A.buf[5];
-  uint64_t lse = at.lse ? A.buf[6] : 0;
+  uint64_t lse = at.lse ? A.buf[6] : 0, ws = A.buf[nb - 1];
   float scale = (float)at.scale;
-  void* params[] = {&q, &cache, &table, &starts, &lengths, &out, &lse, &scale, &args};
-  return launch(x, 0, grid_for(x, tokens * at.heads), params, s, err);
+  void* params[] = {&q, &cache, &table, &starts, &lengths, &out, &lse, &ws, &scale, &args};
+  // A block per tile, part and head: their lengths differ, and the hardware hands blocks out as CUs fall free.
+  x->chunks = p.splits;
+  x->shared = p.splits > 1;
+  if ((rc = launch(x, p.entry, (uint32_t)blocks, params, s, err)) != UNP_OK || p.splits == 1) return rc;
+  void* jparams[] = {&starts, &out, &lse, &ws, &args};
+  return launch(x, 2, (uint32_t)joins, jparams, s, err);
 }
 
 }  // namespace
