@@ -376,7 +376,7 @@ UNP4_DEV tile tile_of(const i32* starts, const i32* lengths, const attention_arg
   }
 }
 
-template <class T, int H, int QH, int D, int GROUP, int P, bool CAUSAL, int QT> struct attention {
+template <class T, int H, int QH, int D, int GROUP, int P, bool CAUSAL, bool LSE, int QT> struct attention {
   typedef record<D, GROUP, P> R;
   static constexpr int GQ = QH / H, W = R::W, G = R::G, KJ = D / 32, JG = GROUP / 32;
   // Value tiles: 16 rows of N adjacent elements each, from words FIRST on.  Full tiles of 16 words, then one of
@@ -391,17 +391,25 @@ template <class T, int H, int QH, int D, int GROUP, int P, bool CAUSAL, int QT> 
     u32x4 kp[G], v[NT], vp[NT];
   };
   int lane, c, g;  // c: the row a lane gives and the column it holds, g: its part of the depth
+  // The nibbles' masks and the exponents they are put under, in registers: as literals each takes an operation more.
+  u32 mask0, mask1, exp0, exp1;
   f16x8 q[QT][KJ];
   float qsum[QT][G], factor[QT];  // of this lane's column; factor: raw scores to log2
-  float m[QT], l[QT];
-  f32x4 o[QT][NE];
+  float m[QT];
+  // The column's sums of p, in l[0] (with LSE this lane's part of it until the end), and of p v.
+  f32x4 l[QT], o[QT][NE];
   int end[QT], begin[QT];  // keys that the column sees
+  u32 poison[QT];          // bit 4t + r: rows r of tile t hold no number (guard)
 
   // Rows first .. first + 16 QT - 1 (token * GQ + head of the group) of a sequence.
   UNP4_DEV void rows(const T* qp, const attention_args& a, const tile& t, int kv, int first, float scale, int cap) {
     lane = threadIdx.x & 63;
     c = lane & 15;
     g = lane >> 4;
+    asm("s_mov_b32 %0, 0x000f000f" : "=s"(mask0));
+    asm("s_mov_b32 %0, 0x00f000f0" : "=s"(mask1));
+    asm("v_mov_b32 %0, 0x64006400" : "=v"(exp0));
+    asm("v_mov_b32 %0, 0x54005400" : "=v"(exp1));
 #pragma unroll
     for (int x = 0; x < QT; ++x) {
       const int r = first + x * 16 + c;
@@ -439,7 +447,8 @@ template <class T, int H, int QH, int D, int GROUP, int P, bool CAUSAL, int QT> 
       for (int gi = 0; gi < G; ++gi) qsum[x][gi] = row_sum(qsum[x][gi]);
       factor[x] = fminf(scale * 1.4426950408889634f * 0x1p24f * __builtin_bit_cast(float, (u32)(127 - up) << 23), 0x1p127f);
       m[x] = -__builtin_inff();
-      l[x] = 0.0f;
+      l[x] = f32x4{0, 0, 0, 0};
+      poison[x] = 0;
 #pragma unroll
       for (int e = 0; e < NE; ++e) o[x][e] = f32x4{0, 0, 0, 0};
       const int last = CAUSAL ? t.length - t.rows + token + 1 : t.length;
@@ -453,13 +462,15 @@ template <class T, int H, int QH, int D, int GROUP, int P, bool CAUSAL, int QT> 
     return w < W ? w : W - 1;
   }
 
-  // 16 keys from token t0 (a multiple of 16) of a record on.
-  UNP4_DEV void load(const u32* rec, int t0, block& b) const {
+  // 16 keys from token t0 (a multiple of 16) of a record on: their key parts, and their value parts.
+  UNP4_DEV void load_keys(const u32* rec, int t0, block& b) const {
     const u32* kp = rec + R::KEYS + t0 * W + (c * W + g * KJ);
 #pragma unroll
     for (int j = 0; j < KJ; ++j) b.k[j] = kp[j];
 #pragma unroll
     for (int gi = 0; gi < G; ++gi) b.kp[gi] = *reinterpret_cast<const u32x4*>(rec + R::kpar(t0, gi) + g * 4);
+  }
+  UNP4_DEV void load_values(const u32* rec, int t0, block& b) const {
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
       const int w = word_of(t);
@@ -468,9 +479,9 @@ template <class T, int H, int QH, int D, int GROUP, int P, bool CAUSAL, int QT> 
     }
   }
 
-  static UNP4_DEV f16x8 key_operand(u32 x) {
+  UNP4_DEV f16x8 key_operand(u32 x) const {
     const u32 y = x >> 8;
-    const u32x4 b = {x & 0x000F000Fu, x & 0x00F000F0u, y & 0x000F000Fu, y & 0x00F000F0u};
+    const u32x4 b = {x & mask0, x & mask1, y & mask0, y & mask1};
     return __builtin_bit_cast(f16x8, b);
   }
 
@@ -490,16 +501,16 @@ template <class T, int H, int QH, int D, int GROUP, int P, bool CAUSAL, int QT> 
         }
         const f16x2 s = __builtin_bit_cast(f16x2, __builtin_amdgcn_perm(pb, pa, 0x05040100u));
         const u32 z = __builtin_amdgcn_perm(pb, pa, 0x07060302u);
-        const f16x2 z0 = __builtin_bit_cast(f16x2, z | 0x64006400u), z1 = __builtin_bit_cast(f16x2, (z << 4) | 0x54005400u);
+        const f16x2 z0 = __builtin_bit_cast(f16x2, z | exp0), z1 = __builtin_bit_cast(f16x2, (z << 4) | exp1);
 #pragma unroll
         for (int e = 0; e < N; e += 4) {
           const u32 x = __builtin_amdgcn_perm(wb, wa, e ? 0x07060302u : 0x05040100u), y = x >> 8;
           // 1024 + n in steps of 1, 64 + n in steps of 1/16: both exact, and so is n - zero.
-          part[e][2 * k + h] = pair((x & 0x000F000Fu) | 0x64006400u, z0, s);
-          part[e + 1][2 * k + h] = pair((x & 0x00F000F0u) | 0x54005400u, z1, s);
+          part[e][2 * k + h] = pair((x & mask0) | exp0, z0, s);
+          part[e + 1][2 * k + h] = pair((x & mask1) | exp1, z1, s);
           if (N > 2) {
-            part[e + 2 < N ? e + 2 : 0][2 * k + h] = pair((y & 0x000F000Fu) | 0x64006400u, z0, s);
-            part[e + 3 < N ? e + 3 : 0][2 * k + h] = pair((y & 0x00F000F0u) | 0x54005400u, z1, s);
+            part[e + 2 < N ? e + 2 : 0][2 * k + h] = pair((y & mask0) | exp0, z0, s);
+            part[e + 3 < N ? e + 3 : 0][2 * k + h] = pair((y & mask1) | exp1, z1, s);
           }
         }
       }
@@ -512,40 +523,80 @@ template <class T, int H, int QH, int D, int GROUP, int P, bool CAUSAL, int QT> 
   }
 
   // A value scale that is no number would reach, as 0 x NaN, the columns that do not see its key.  Such words are
-  // taken out of the product, and the elements of the columns that see them become NaN.
+  // taken out of the product, and the rows of the columns that see them are marked.
   UNP4_DEV void guard(block (&b)[2], const u32 (&seen)[QT]) {
-    u32 bad[NT], any = 0;
+    u32 bad = 0;  // bit 8t + 4k + i
 #pragma unroll
-    for (int t = 0; t < NT; ++t) {
-      bad[t] = 0;
-#pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if ((b[i / 4].vp[t][i % 4] & 0x7C00u) == 0x7C00u) bad[t] |= 1u << i;
-      any |= bad[t];
-    }
-    if (!__any(any != 0)) return;
-#pragma unroll
-    for (int t = 0; t < NT; ++t) {
+    for (int t = 0; t < NT; ++t)
 #pragma unroll
       for (int i = 0; i < 8; ++i)
-        if (bad[t] >> i & 1) b[i / 4].vp[t][i % 4] = 0;
-      for (int part = 0; part < 4; ++part)  // the keys of each part of the depth
+        if ((b[i / 4].vp[t][i % 4] & 0x7C00u) == 0x7C00u) {
+          bad |= 1u << (8 * t + i);
+          b[i / 4].vp[t][i % 4] = 0;
+        }
+    if (!__any(bad != 0)) return;
+    for (int part = 0; part < 4; ++part) {  // the keys of each part of the depth
+      u32 see[QT];
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const u32 row = __shfl(bad[t], part * 16 + g * 4 + r);
+      for (int x = 0; x < QT; ++x) see[x] = __shfl(seen[x], part * 16 + c);
+      for (int r = 0; r < 4; ++r) {
+        const u32 row = __shfl(bad, part * 16 + g * 4 + r);
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
 #pragma unroll
           for (int x = 0; x < QT; ++x)
-            if (row & __shfl(seen[x], part * 16 + c)) {
-#pragma unroll
-              for (int e = 0; e < nibbles(t); ++e) o[x][8 * t + e][r] = __builtin_nanf("");
-            }
-        }
+            if (row >> (8 * t) & see[x] & 255u) poison[x] |= 1u << (4 * t + r);
+      }
     }
   }
 
-  // 32 keys from k0 on; MASKED: some column may not see some of them.  good: whether each block's page is one.
-  template <bool MASKED> UNP4_DEV void step(block (&b)[2], int k0, int cap, bool good0, bool good1) {
-    if (MASKED) {  // what no row may see does not count, whatever it holds
+  // 32 keys from k0 on; masked: some column may not see some of them.  good: whether each block's page is one.
+  // next_keys and next_values load the next step's parts as soon as this one's registers are free.
+  template <class FK, class FV>
+  UNP4_DEV void step(block (&b)[2], bool masked, int k0, int cap, bool good0, bool good1, FK next_keys, FV next_values) {
+    float s[QT][8];
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+#pragma unroll
+      for (int gi = 0; gi < G; ++gi) {
+        f16x8 ka[JG];
+#pragma unroll
+        for (int j = 0; j < JG; ++j) ka[j] = key_operand(b[k].k[gi * JG + j]);
+        f32x4 acc[QT];
+#pragma unroll
+        for (int x = 0; x < QT; ++x) acc[x] = f32x4{0, 0, 0, 0};
+#pragma unroll
+        for (int j = 0; j < JG; ++j)
+#pragma unroll
+          for (int x = 0; x < QT; ++x)
+            acc[x] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka[j], q[x][gi * JG + j], acc[x], 0, 0, 0);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float scale = scale_of(b[k].kp[gi][i]), zero = -zero_of(b[k].kp[gi][i]);
+#pragma unroll
+          for (int x = 0; x < QT; ++x) {
+            const float d = fmaf(zero, qsum[x][gi], acc[x][i]);
+            s[x][4 * k + i] = gi == 0 ? d * scale : fmaf(d, scale, s[x][4 * k + i]);
+          }
+        }
+      }
+    }
+    next_keys();
+    if (masked) {
+      asm volatile("; a branch: not worth computing for every step");
+      u32 seen[QT];  // which of its 8 keys each of this lane's columns sees
+#pragma unroll
+      for (int x = 0; x < QT; ++x) {
+        seen[x] = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int key = k0 + 16 * (i / 4) + 4 * g + i % 4;
+          const bool sees = key < end[x] && key >= begin[x] && (i < 4 ? good0 : good1);
+          s[x][i] = sees ? s[x][i] : -__builtin_inff();
+          if (sees) seen[x] |= 1u << i;
+        }
+      }
+      // What no row may see does not count, whatever it holds.
 #pragma unroll
       for (int k = 0; k < 2; ++k)
 #pragma unroll
@@ -553,46 +604,14 @@ template <class T, int H, int QH, int D, int GROUP, int P, bool CAUSAL, int QT> 
           if (!(k ? good1 : good0) || k0 + 16 * k + 4 * g + i >= cap)
 #pragma unroll
             for (int t = 0; t < NT; ++t) b[k].vp[t][i] = 0;
+      guard(b, seen);
     }
-    f16x8 ka[2][KJ];
-#pragma unroll
-    for (int k = 0; k < 2; ++k)
-#pragma unroll
-      for (int j = 0; j < KJ; ++j) ka[k][j] = key_operand(b[k].k[j]);
     f16x8 p[QT];
-    u32 seen[QT];  // MASKED: which of its 8 keys each of this lane's columns sees
 #pragma unroll
     for (int x = 0; x < QT; ++x) {
-      float s[8];
+      float top = s[x][0];
 #pragma unroll
-      for (int k = 0; k < 2; ++k) {
-#pragma unroll
-        for (int gi = 0; gi < G; ++gi) {
-          f32x4 acc = {0, 0, 0, 0};
-#pragma unroll
-          for (int j = gi * JG; j < (gi + 1) * JG; ++j)
-            acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka[k][j], q[x][j], acc, 0, 0, 0);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const u32 w = b[k].kp[gi][i];
-            const float d = fmaf(-zero_of(w), qsum[x][gi], acc[i]);
-            s[4 * k + i] = gi == 0 ? d * scale_of(w) : fmaf(d, scale_of(w), s[4 * k + i]);
-          }
-        }
-      }
-      if (MASKED) {
-        seen[x] = 0;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const int key = k0 + 16 * (i / 4) + 4 * g + i % 4;
-          const bool sees = key < end[x] && key >= begin[x] && (i < 4 ? good0 : good1);
-          s[i] = sees ? s[i] : -__builtin_inff();
-          if (sees) seen[x] |= 1u << i;
-        }
-      }
-      float top = s[0];
-#pragma unroll
-      for (int i = 1; i < 8; ++i) top = fmaxf(top, s[i]);
+      for (int i = 1; i < 8; ++i) top = fmaxf(top, s[x][i]);
       if (__any((top - m[x]) * factor[x] > 0.9f)) {
         const float next = fmaxf(m[x], row_max(top));
         const float keep = m[x] == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f((m[x] - next) * factor[x]);
@@ -604,12 +623,17 @@ template <class T, int H, int QH, int D, int GROUP, int P, bool CAUSAL, int QT> 
       const float off = m[x] == -__builtin_inff() ? 0.0f : fmaf(-m[x], factor[x], 15.0f);
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const float e = __builtin_amdgcn_exp2f(fmaf(s[i], factor[x], off));
-        l[x] += e;
+        const float e = __builtin_amdgcn_exp2f(fmaf(s[x][i], factor[x], off));
+        if (LSE) l[x][0] += e;
         p[x][i] = (_Float16)e;
       }
     }
-    if (MASKED) guard(b, seen);
+    // Where nobody asks for it, the sum of p is a product too, with ones: of p as rounded, so that the weights' sum
+    // stays 1.  The log-sum-exp takes the sum of what was not rounded.
+    const f16x8 ones = {1, 1, 1, 1, 1, 1, 1, 1};
+    if (!LSE)
+#pragma unroll
+      for (int x = 0; x < QT; ++x) l[x] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, p[x], l[x], 0, 0, 0);
     int at = 0;
 #pragma unroll
     for (int t = 0; t < FULL; ++t) {
@@ -628,47 +652,62 @@ template <class T, int H, int QH, int D, int GROUP, int P, bool CAUSAL, int QT> 
 #pragma unroll
         for (int x = 0; x < QT; ++x) o[x][at] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va[e], p[x], o[x][at], 0, 0, 0);
     }
+    next_values();
   }
 
-  // The keys of steps first, first + by, .. below last (a step is 32 keys), each step loaded a step ahead.  lo, hi:
-  // the keys from lo on and below hi that every column sees.
+  // The keys of steps first, first + by, .. below last (a step is 32 keys), each loaded while the one before is
+  // multiplied.  lo, hi: the keys from lo on and below hi that every column sees.
   UNP4_DEV void walk(const u32* cache, const i32* pages, const attention_args& a, int kv, int first, int by, int last,
                      int cap, int lo, int hi) {
-    if (first >= last) return;
+    if (first >= last) return;  // so cap > 0: there is a page to name
     auto page = [&](int step, int k) {
-      const int key = step * 32 + 16 * k;
-      return key < cap ? pages[key / P] : -1;  // uniform: cap keys lie in the table's row
+      const int key = step * 32 + 16 * k, at = (key < cap ? key : cap - 1) / P;
+      const int id = pages[at];
+      return key < cap && (u32)id < (u32)a.pages ? id : -1;
     };
-    auto good = [&](int id) { return (u32)id < (u32)a.pages; };
-    auto fetch = [&](int step, int id0, int id1, block (&b)[2]) {
-      load(cache + ((i64)(good(id0) ? id0 : 0) * H + kv) * (i64)R::WORDS, step * 32 % P, b[0]);
-      load(cache + ((i64)(good(id1) ? id1 : 0) * H + kv) * (i64)R::WORDS, (step * 32 + 16) % P, b[1]);
-    };
-    int id0 = page(first, 0), id1 = page(first, 1);
-    block now[2];
-    fetch(first, id0, id1, now);
-    int next = first + by;
-    int n0 = next < last ? page(next, 0) : -1, n1 = next < last ? page(next, 1) : -1;
-    for (int at = first;;) {
-      block ahead[2];
-      if (next < last) fetch(next, n0, n1, ahead);
-      const int after = next + by;
-      const int f0 = after < last ? page(after, 0) : -1, f1 = after < last ? page(after, 1) : -1;
-      const int k0 = at * 32;
-      if (k0 >= lo && k0 + 32 <= hi && good(id0) && good(id1))
-        step<false>(now, k0, cap, true, true);
-      else
-        step<true>(now, k0, cap, good(id0), good(id1));
-      if (next >= last) return;
+    auto record_of = [&](int id) { return cache + ((i64)(id < 0 ? 0 : id) * H + kv) * (i64)R::WORDS; };
+    block b[2];
+    int id[2] = {page(first, 0), page(first, 1)};
+    int at = first, next = first + by < last ? first + by : first;
+    int ahead[2] = {page(next, 0), page(next, 1)};
 #pragma unroll
-      for (int k = 0; k < 2; ++k) now[k] = ahead[k];
-      id0 = n0;
-      id1 = n1;
-      n0 = f0;
-      n1 = f1;
-      at = next;
+    for (int k = 0; k < 2; ++k) load_keys(record_of(id[k]), (at * 32 + 16 * k) % P, b[k]);
+#pragma unroll
+    for (int k = 0; k < 2; ++k) load_values(record_of(id[k]), (at * 32 + 16 * k) % P, b[k]);
+    while (at < last) {
+      const int after = next + by < last ? next + by : next;
+      const int far[2] = {page(after, 0), page(after, 1)};
+      const bool masked = at * 32 < lo || at * 32 + 32 > hi || (id[0] | id[1]) < 0;
+      step(
+          b, masked, at * 32, cap, id[0] >= 0, id[1] >= 0,
+          [&] {
+#pragma unroll
+            for (int k = 0; k < 2; ++k) load_keys(record_of(ahead[k]), (next * 32 + 16 * k) % P, b[k]);
+          },
+          [&] {
+#pragma unroll
+            for (int k = 0; k < 2; ++k) load_values(record_of(ahead[k]), (next * 32 + 16 * k) % P, b[k]);
+          });
+      at += by;
       next = after;
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        id[k] = ahead[k];
+        ahead[k] = far[k];
+      }
     }
+    if (LSE)
+#pragma unroll
+      for (int x = 0; x < QT; ++x) l[x][0] = row_sum(l[x][0]);
+#pragma unroll
+    for (int x = 0; x < QT; ++x)
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          if (poison[x] >> (4 * t + r) & 1)
+#pragma unroll
+            for (int e = 0; e < nibbles(t); ++e) o[x][8 * t + e][r] = __builtin_nanf("");
   }
 
   // f(x, element, four-vector part i, value): every element of the lane's columns, N adjacent ones at a time.
@@ -728,7 +767,7 @@ UNP4_DEV void finish(T* out, float* lse, const attention_args& a, i64 row, int h
 template <class T, int H, int QH, int D, int GROUP, int P, bool CAUSAL, bool LSE, int QT, int WR, int WK>
 UNP4_DEV void attend(const T* q, const u32* cache, const i32* table, const i32* starts, const i32* lengths, T* out,
                      float* lse, float* ws, float scale, const attention_args& a) {
-  typedef attention<T, H, QH, D, GROUP, P, CAUSAL, QT> A;
+  typedef attention<T, H, QH, D, GROUP, P, CAUSAL, LSE, QT> A;
   constexpr int GQ = QH / H, ROWS = 16 * QT * WR;
   const int wave = uniform(threadIdx.x >> 6);
   const int kv = blockIdx.x % H, part = (int)(blockIdx.x / H) % a.splits;
@@ -758,8 +797,6 @@ UNP4_DEV void attend(const T* q, const u32* cache, const i32* table, const i32* 
   A w;
   w.rows(q, a, t, kv, first_row, scale, cap);
   w.walk(cache, table + (i64)t.seq * a.width, a, kv, begin + (WK > 1 ? wave % WK : 0), WK, end, cap, lo, hi);
-#pragma unroll
-  for (int x = 0; x < QT; ++x) w.l[x] = row_sum(w.l[x]);
   if constexpr (WK > 1) {
     // Join the waves: the rows' maxima and sums, then their elements, each scaled to the common maximum.
     __shared__ float stat[WK][QT][16][2];
@@ -768,7 +805,7 @@ UNP4_DEV void attend(const T* q, const u32* cache, const i32* table, const i32* 
 #pragma unroll
       for (int x = 0; x < QT; ++x) {
         stat[wave][x][w.c][0] = w.m[x] * w.factor[x];
-        stat[wave][x][w.c][1] = w.l[x];
+        stat[wave][x][w.c][1] = w.l[x][0];
       }
     w.each([&](int tl, int r, int d) {
 #pragma unroll
@@ -805,7 +842,7 @@ UNP4_DEV void attend(const T* q, const u32* cache, const i32* table, const i32* 
       const int row = first_row + x * 16 + w.c;
       if (row >= all_rows) continue;
       const int token = t.start + row / GQ, head = kv * GQ + row % GQ;
-      const float top = w.m[x] * w.factor[x], l = w.l[x];
+      const float top = w.m[x] * w.factor[x], l = w.l[x][0];
       if (a.splits > 1 && w.g == 0) store<float, 2>(parts<QH, D>::stat(ws, a, part, token, head), {top, l});
       w.each([&](int tl, int r, int d) {
 #pragma unroll
