@@ -343,6 +343,9 @@ UNP4_DEV float row_sum(float x) {
 }
 
 UNP4_DEV int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+// Memory that this launch does not write, read at a place all lanes share: a scalar load, which does not queue
+// behind the vector loads in flight.
+typedef const __attribute__((address_space(4))) i32* uniform_ints;
 
 // The sequence and tile of a tile number, by one wave.  Tiles are numbered so that a sequence's number is known
 // from its start alone: its first is start * GQ / R + b (its rows fill at most one tile more than they span), or its
@@ -657,7 +660,7 @@ template <class T, int H, int QH, int D, int GROUP, int P, bool CAUSAL, bool LSE
 
   // The keys of steps first, first + by, .. below last (a step is 32 keys), each loaded while the one before is
   // multiplied.  lo, hi: the keys from lo on and below hi that every column sees.
-  UNP4_DEV void walk(const u32* cache, const i32* pages, const attention_args& a, int kv, int first, int by, int last,
+  UNP4_DEV void walk(const u32* cache, uniform_ints pages, const attention_args& a, int kv, int first, int by, int last,
                      int cap, int lo, int hi) {
     if (first >= last) return;  // so cap > 0: there is a page to name
     auto page = [&](int step, int k) {
@@ -796,7 +799,7 @@ UNP4_DEV void attend(const T* q, const u32* cache, const i32* table, const i32* 
   const int end = step0 + (int)min((i64)steps, (i64)(part + 1) * each);
   A w;
   w.rows(q, a, t, kv, first_row, scale, cap);
-  w.walk(cache, table + (i64)t.seq * a.width, a, kv, begin + (WK > 1 ? wave % WK : 0), WK, end, cap, lo, hi);
+  w.walk(cache, (uniform_ints)(u64)(table + (i64)t.seq * a.width), a, kv, begin + (WK > 1 ? wave % WK : 0), WK, end, cap, lo, hi);
   if constexpr (WK > 1) {
     // Join the waves: the rows' maxima and sums, then their elements, each scaled to the common maximum.
     __shared__ float stat[WK][QT][16][2];
