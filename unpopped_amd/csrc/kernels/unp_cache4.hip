@@ -406,9 +406,6 @@ template <class T, int H, int QH, int D, int GROUP, int P, bool CAUSAL, bool LSE
 
   // Rows first .. first + 16 QT - 1 (token * GQ + head of the group) of a sequence.
   UNP4_DEV void rows(const T* qp, const attention_args& a, const tile& t, int kv, int first, float scale, int cap) {
-    lane = threadIdx.x & 63;
-    c = lane & 15;
-    g = lane >> 4;
     asm("s_mov_b32 %0, 0x000f000f" : "=s"(mask0));
     asm("s_mov_b32 %0, 0x00f000f0" : "=s"(mask1));
     asm("v_mov_b32 %0, 0x64006400" : "=v"(exp0));
@@ -658,45 +655,56 @@ template <class T, int H, int QH, int D, int GROUP, int P, bool CAUSAL, bool LSE
     next_values();
   }
 
-  // The keys of steps first, first + by, .. below last (a step is 32 keys), each loaded while the one before is
+  // The keys of steps at, at + by, .. below last (a step is 32 keys), each loaded while the one before is
   // multiplied.  lo, hi: the keys from lo on and below hi that every column sees.
-  UNP4_DEV void walk(const u32* cache, uniform_ints pages, const attention_args& a, int kv, int first, int by, int last,
-                     int cap, int lo, int hi) {
-    if (first >= last) return;  // so cap > 0: there is a page to name
-    auto page = [&](int step, int k) {
-      const int key = step * 32 + 16 * k, at = (key < cap ? key : cap - 1) / P;
-      const int id = pages[at];
-      return key < cap && (u32)id < (u32)a.pages ? id : -1;
-    };
-    auto record_of = [&](int id) { return cache + ((i64)(id < 0 ? 0 : id) * H + kv) * (i64)R::WORDS; };
+  struct stream {
+    const u32* cache;
+    uniform_ints table;  // the sequence's pages
+    int kv, at, by, last, cap, lo, hi, pages;
+    int next, id[2], ahead[2];  // the step being loaded, and both steps' pages (-1: none)
     block b[2];
-    int id[2] = {page(first, 0), page(first, 1)};
-    int at = first, next = first + by < last ? first + by : first;
-    int ahead[2] = {page(next, 0), page(next, 1)};
+    UNP4_DEV int page(int step, int k) const {  // cap > 0
+      const int key = step * 32 + 16 * k, id = table[(key < cap ? key : cap - 1) / P];
+      return key < cap && (u32)id < (u32)pages ? id : -1;
+    }
+    UNP4_DEV const u32* record_of(int id) const { return cache + ((i64)(id < 0 ? 0 : id) * H + kv) * (i64)R::WORDS; }
+  };
+  UNP4_DEV void open(stream& s) {
+    lane = threadIdx.x & 63;
+    c = lane & 15;
+    g = lane >> 4;
+    if (s.at >= s.last) return;
+    s.next = s.at + s.by < s.last ? s.at + s.by : s.at;
 #pragma unroll
-    for (int k = 0; k < 2; ++k) load_keys(record_of(id[k]), (at * 32 + 16 * k) % P, b[k]);
+    for (int k = 0; k < 2; ++k) s.id[k] = s.page(s.at, k);
 #pragma unroll
-    for (int k = 0; k < 2; ++k) load_values(record_of(id[k]), (at * 32 + 16 * k) % P, b[k]);
-    while (at < last) {
-      const int after = next + by < last ? next + by : next;
-      const int far[2] = {page(after, 0), page(after, 1)};
-      const bool masked = at * 32 < lo || at * 32 + 32 > hi || (id[0] | id[1]) < 0;
+    for (int k = 0; k < 2; ++k) s.ahead[k] = s.page(s.next, k);
+#pragma unroll
+    for (int k = 0; k < 2; ++k) load_keys(s.record_of(s.id[k]), (s.at * 32 + 16 * k) % P, s.b[k]);
+#pragma unroll
+    for (int k = 0; k < 2; ++k) load_values(s.record_of(s.id[k]), (s.at * 32 + 16 * k) % P, s.b[k]);
+  }
+  UNP4_DEV void walk(stream& s) {
+    while (s.at < s.last) {
+      const int after = s.next + s.by < s.last ? s.next + s.by : s.next;
+      const int far[2] = {s.page(after, 0), s.page(after, 1)};
+      const bool masked = s.at * 32 < s.lo || s.at * 32 + 32 > s.hi || (s.id[0] | s.id[1]) < 0;
       step(
-          b, masked, at * 32, cap, id[0] >= 0, id[1] >= 0,
+          s.b, masked, s.at * 32, s.cap, s.id[0] >= 0, s.id[1] >= 0,
           [&] {
 #pragma unroll
-            for (int k = 0; k < 2; ++k) load_keys(record_of(ahead[k]), (next * 32 + 16 * k) % P, b[k]);
+            for (int k = 0; k < 2; ++k) load_keys(s.record_of(s.ahead[k]), (s.next * 32 + 16 * k) % P, s.b[k]);
           },
           [&] {
 #pragma unroll
-            for (int k = 0; k < 2; ++k) load_values(record_of(ahead[k]), (next * 32 + 16 * k) % P, b[k]);
+            for (int k = 0; k < 2; ++k) load_values(s.record_of(s.ahead[k]), (s.next * 32 + 16 * k) % P, s.b[k]);
           });
-      at += by;
-      next = after;
+      s.at += s.by;
+      s.next = after;
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
-        id[k] = ahead[k];
-        ahead[k] = far[k];
+        s.id[k] = s.ahead[k];
+        s.ahead[k] = far[k];
       }
     }
     if (LSE)
@@ -798,8 +806,20 @@ UNP4_DEV void attend(const T* q, const u32* cache, const i32* table, const i32* 
   const int begin = step0 + (int)min((i64)steps, (i64)part * each);
   const int end = step0 + (int)min((i64)steps, (i64)(part + 1) * each);
   A w;
+  typename A::stream s;
+  s.cache = cache;
+  s.table = (uniform_ints)(u64)(table + (i64)t.seq * a.width);
+  s.kv = kv;
+  s.at = begin + (WK > 1 ? wave % WK : 0);
+  s.by = WK;
+  s.last = end;
+  s.cap = cap;
+  s.lo = lo;
+  s.hi = hi;
+  s.pages = (int)a.pages;
+  w.open(s);  // the first keys are on their way while the rows are read
   w.rows(q, a, t, kv, first_row, scale, cap);
-  w.walk(cache, (uniform_ints)(u64)(table + (i64)t.seq * a.width), a, kv, begin + (WK > 1 ? wave % WK : 0), WK, end, cap, lo, hi);
+  w.walk(s);
   if constexpr (WK > 1) {
     // Join the waves: the rows' maxima and sums, then their elements, each scaled to the common maximum.
     __shared__ float stat[WK][QT][16][2];
@@ -864,15 +884,24 @@ UNP4_DEV void attend(const T* q, const u32* cache, const i32* table, const i32* 
   }
 }
 
-// The parts of split contexts: four elements of a row per lane.
+// The parts of split contexts: a block per row and head, whose lanes hold four elements each and take the parts in
+// groups, all of a group's loads in flight at once: with a lane for all parts of its elements, 64 parts took 52 us.
+constexpr int kMostParts = 128;
 template <class T, int H, int QH, int D, bool LSE>
 UNP4_DEV void join(const i32* starts, T* out, float* lse, float* ws, const attention_args& a) {
-  constexpr int L = D / 4;
-  const i64 n = a.tokens * QH * L, i = (i64)blockIdx.x * 256 + threadIdx.x;
-  if (i >= n) return;
-  const i64 row = i / (QH * L);
-  const int head = (int)(i / L % QH), d = (int)(i % L) * 4;
-  // Rows that no sequence names have no parts.
+  constexpr int L = D / 4, GROUPS = 256 / L;
+  __shared__ float weight[kMostParts];
+  __shared__ f32x4 part[GROUPS][L];
+  const i64 row = blockIdx.x / QH;
+  const int head = (int)(blockIdx.x % QH), lane = threadIdx.x & 63, group = threadIdx.x / L, d = threadIdx.x % L * 4;
+  // The parts' maxima and sums, in every wave; rows that no sequence names have none.
+  f32x2 st[kMostParts / 64];
+#pragma unroll
+  for (int i = 0; i < kMostParts / 64; ++i) {
+    const int s = i * 64 + lane;
+    st[i] = s < a.splits ? *reinterpret_cast<const f32x2*>(parts<QH, D>::stat(ws, a, s, row, head))
+                         : f32x2{-__builtin_inff(), 0.0f};
+  }
   i64 lo = 0, hi = a.batch;
   while (hi - lo > 1) {
     const i64 mid = (lo + hi) >> 1;
@@ -880,16 +909,34 @@ UNP4_DEV void join(const i32* starts, T* out, float* lse, float* ws, const atten
   }
   if (starts[lo] > row || row >= starts[lo + 1]) return;
   float top = -__builtin_inff(), l = 0.0f;
-  for (int s = 0; s < a.splits; ++s) top = fmaxf(top, parts<QH, D>::stat(ws, a, s, row, head)[0]);
+#pragma unroll
+  for (int i = 0; i < kMostParts / 64; ++i) top = fmaxf(top, st[i][0]);
+  for (int x = 1; x < 64; x *= 2) top = fmaxf(top, __shfl_xor(top, x));
   const float base = top == -__builtin_inff() ? 0.0f : top;
-  f32x4 o = {0, 0, 0, 0};
-  for (int s = 0; s < a.splits; ++s) {
-    const f32x2 st = *reinterpret_cast<const f32x2*>(parts<QH, D>::stat(ws, a, s, row, head));
-    if (st[1] == 0.0f) continue;
-    const float keep = __builtin_amdgcn_exp2f(st[0] - base);
-    l = fmaf(st[1], keep, l);
-    o += *reinterpret_cast<const f32x4*>(parts<QH, D>::sums(ws, a, s, row, head) + d) * keep;
+#pragma unroll
+  for (int i = 0; i < kMostParts / 64; ++i) {
+    const float keep = __builtin_amdgcn_exp2f(st[i][0] - base);
+    // A part without keys wrote no sums.
+    if (threadIdx.x < 64) weight[i * 64 + lane] = st[i][1] == 0.0f ? -1.0f : keep;
+    l = fmaf(st[i][1], keep, l);
   }
+  for (int x = 1; x < 64; x *= 2) l += __shfl_xor(l, x);
+  __syncthreads();
+  f32x4 o = {0, 0, 0, 0};
+  if (group < GROUPS) {
+#pragma unroll 8
+    for (int s = group; s < a.splits; s += GROUPS) {
+      const f32x4 v = *reinterpret_cast<const f32x4*>(parts<QH, D>::sums(ws, a, s, row, head) + d);
+      const float w = weight[s];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) o[i] = w >= 0.0f ? fmaf(v[i], w, o[i]) : o[i];
+    }
+    part[group][d / 4] = o;
+  }
+  __syncthreads();
+  if (group != 0) return;
+  const int used = a.splits < GROUPS ? a.splits : GROUPS;
+  for (int i = 1; i < used; ++i) o += part[i][d / 4];
   finish<T, QH, LSE>(out, lse, a, row, head, d, top, l, o);
 }
 

@@ -2040,6 +2040,7 @@ int32_t check_attention(int64_t tokens, int64_t batch, int64_t width, int64_t pa
 }
 
 // A launch's shape: the entry, its row tiles, how they are numbered (tile_of) and the parts of a context.
+constexpr int64_t kMostParts = 128;  // the device's kMostParts
 struct AttentionPlan {
   size_t entry = 0;
   int64_t slots = 0, splits = 1;
@@ -2065,7 +2066,7 @@ AttentionPlan attention_plan(const unp_exec* x, int64_t tokens, int64_t batch, i
   // block's rows; with the whole context's pages as its length, which the host does not know.
   const int64_t blocks = p.slots * c.kv_heads, want = (2LL * x->cu_count + blocks - 1) / blocks;
   const int64_t most = (width * c.page + 64 * e.k - 1) / (64 * e.k);
-  p.splits = std::max<int64_t>(1, std::min({want, most, (int64_t)128}));
+  p.splits = std::max<int64_t>(1, std::min({want, most, kMostParts}));
   return p;
 }
 
@@ -2107,7 +2108,7 @@ int32_t run_cache4_attention(unp_exec* x, const unp_arg* a, size_t n, hipStream_
   p.splits = std::max<int64_t>(1, std::min(p.splits, A.ext[9] / part_bytes(x, tokens)));
   if (p.splits == 1 && A.buf[nb - 1] == 0) A.buf[nb - 1] = A.buf[5];  // not used
   const int64_t blocks = p.slots * p.splits * c.kv_heads;
-  const int64_t joins = (tokens * at.heads * (c.head_dim / 4) + 255) / 256;
+  const int64_t joins = tokens * at.heads;
   if (blocks > 0x7FFFFFFFLL || joins > 0x7FFFFFFFLL) return invalid(err, "tokens: too many rows for one launch");
   attention_args_host args{tokens, batch, keys ? A.ext[2] : 0, A.ext[3], A.ext[4], A.ext[5], A.ext[6], A.ext[7], A.ext[8],
                            (int32_t)p.slots, (int32_t)p.splits, p.by_token ? 1 : 0, 0};
