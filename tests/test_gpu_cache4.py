@@ -343,7 +343,8 @@ def attention_case(dtype, heads, kv, dim, group, page, rows, lengths, causal=Tru
     tolerance = ref.attention_tolerance(want, mass, top, reach, max(lengths + [1]), dim, dtype)
     expect[at_o[there]], tol[at_o[there]] = want[there], tolerance[there]
     off = np.abs(got - expect)
-    assert (off <= tol).all(), (np.argwhere(~(off <= tol))[:4].ravel(), float(np.nanmax(off)))
+    wrong = np.argwhere(~(off <= tol)).ravel()
+    assert not len(wrong), [(int(i), got[i], expect[i], tol[i]) for i in wrong[:6]]
     if lse:
         got_lse = lb.download(np.float32, tokens * heads).reshape(tokens, heads).astype(np.float64)
         assert (got_lse[~there] == 77).all()

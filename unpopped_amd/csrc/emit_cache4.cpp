@@ -279,21 +279,24 @@ int32_t lower_cache4_attention(const unp_cache4& c, const unp_attention& a, Lowe
   const std::string same = std::string(T) + ", " + std::to_string(c.kv_heads) + ", " + std::to_string(a.heads) + ", " +
                            std::to_string(c.head_dim);
   const char* lse = a.lse ? "true" : "false";
-  auto add = [&](const char* tail, int qt, int wr, int wk, int per_simd) {
+  // cg groups of columns hold the same 16 / cg rows (few rows); wk waves share a block's rows, or wr have their own.
+  auto add = [&](const char* tail, int qt, int cg, int wr, int wk, int per_simd) {
     Entry e;
     e.symbol = L.name + tail;
     e.threads = 64 * wr * wk;
-    e.vec = 16 * qt * wr;  // rows of a block
-    e.k = wk;              // waves that share them
+    e.vec = 16 / cg * qt * wr;  // rows of a block
+    e.k = wk * 32 * cg;         // keys of a block's step
     L.entries.push_back(e);
-    src << "extern \"C\" __global__ void __launch_bounds__(" << e.threads << ", " << per_simd << ") " << e.symbol << "(const " << T
+    src << "extern \"C\" __global__ void __launch_bounds__(" << e.threads << ", " << per_simd << ") " << e.symbol
+        << "(const " << T
         << "* q, const unsigned* cache, const int* table, const int* starts, const int* lengths, " << T
         << "* out, float* lse, float* ws, float scale, unp4::attention_args a) {\n  unp4::attend<" << same << ", " << c.group
-        << ", " << c.page << ", " << (a.causal ? "true" : "false") << ", " << lse << ", " << qt << ", " << wr << ", " << wk
-        << ">(q, cache, table, starts, lengths, out, lse, ws, scale, a);\n}\n";
+        << ", " << c.page << ", " << (a.causal ? "true" : "false") << ", " << lse << ", " << qt << ", " << cg << ", " << wr
+        << ", " << wk << ">(q, cache, table, starts, lengths, out, lse, ws, scale, a);\n}\n";
   };
-  add("_few", 1, 1, 8, 2);
-  add("_many", 2, 4, 1, c.head_dim <= 128 ? 2 : 1);
+  const int gq = a.heads / c.kv_heads;
+  add("_few", 1, gq <= 4 ? 4 : gq <= 8 ? 2 : 1, 1, 8, 2);
+  add("_many", 2, 1, 4, 1, c.head_dim <= 128 ? 2 : 1);
   Entry e;
   e.symbol = L.name + "_join";
   L.entries.push_back(e);

@@ -304,21 +304,24 @@ UNP4_DEV void read(const I* slots, const u32* cache, T* k, T* v, const cache_arg
 // ---------------------------------------------------------------------------------------
 // Attention over the cache.
 //
-// A wave holds QT x 16 rows of a sequence (its tokens times the query heads of one key/value head) and
-// walks the keys 32 at a time, all in registers:
+// A wave holds QT x 16 / CG rows of a sequence (its tokens times the query heads of one key/value head) and walks
+// the keys in steps of 32 CG, all in registers:
 //   * S' = K Q' by mfma 16x16x32 f16, keys as rows and query rows as columns.  A key word's nibbles are used
 //     as they lie: masked to bits 0..3 or 4..7 of a 16-bit half they are the subnormal f16 numbers n 2^-24
 //     and n 2^-20, so 8 codes cost 5 operations, and the queries carry the powers of two (exactly: each row is
 //     scaled to f16's range, bf16's 8 bits fit in f16's 11).  The group's scale and zero point are applied to the
 //     f32 result: s (sum q n - zero sum q).
-//   * softmax over the columns: a lane holds 8 keys of one row, so the row's maximum needs two exchanges, and
-//     only when some score passes the running one by 2^0.9 (below that p stays in f16's range: p is
-//     held as 2^15 p).  The running sum is in f32.
-//   * O' += V' P' with the value words as rows: the result above is, lane by lane, the operand that this
-//     product needs when key k of its 32 is (k / 8, k % 8) -> 16 (k % 8 / 4) + 4 (k / 8) + k % 4.  A lane reads four
-//     tokens' words of 8 elements at once; pairs of tokens of one element are made by byte permutes, so nothing
-//     goes through LDS.  Values are (n - zero) exactly, times the scale, rounded to f16: with
-//     P's rounding that is 2 x 2^-11 of a product, below the output type's rounding for bf16.
+//   * Few rows (a decode step) would leave most columns empty, and the softmax's cost is the lanes'.  So CG groups
+//     of columns hold the same rows and each keeps the scores of its own 16 of 16 CG keys: columns of one row are
+//     parts of its context, joined at the end as the waves are.
+//   * softmax over the columns: a lane holds 8 keys of one column, so its maximum needs two exchanges, and
+//     only when some score passes the running one by 2^0.9 (below that 2^15 p stays in f16's range).
+//   * O' += V' P' with the value words as rows, again nibbles as they lie: sum p s (n - zero) is the product of n with
+//     p s less the sum of p s zero.  p s is rounded once to f16 (both sums take it as rounded), s relative to a
+//     running power of two that no scale of the column exceeded, so that it stays in f16's range whatever s is.  The
+//     scores are, lane by lane, the operand that this product needs when its key (g, i) of 4 x 8 is key
+//     16 CG (i / 4) + 4 g + i % 4; a lane reads four tokens' words of 8 elements at once and pairs of tokens of one
+//     element are made by byte permutes, so nothing goes through LDS.
 // ---------------------------------------------------------------------------------------
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
@@ -328,14 +331,14 @@ struct attention_args {
   int slots, splits, by_token;  // row tiles, parts of a context, and how tiles are numbered (tile_of)
 };
 
-// The maximum over the four lanes of a row (lane, lane ^ 16, lane ^ 32, lane ^ 48).
-UNP4_DEV float row_max(float x) {
+// The maximum and the sum over the four lanes of a column (lane, lane ^ 16, lane ^ 32, lane ^ 48).
+UNP4_DEV float column_max(float x) {
   auto a = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(u32, x), __builtin_bit_cast(u32, x), false, false);
   x = fmaxf(__builtin_bit_cast(float, (u32)a[0]), __builtin_bit_cast(float, (u32)a[1]));
   a = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(u32, x), __builtin_bit_cast(u32, x), false, false);
   return fmaxf(__builtin_bit_cast(float, (u32)a[0]), __builtin_bit_cast(float, (u32)a[1]));
 }
-UNP4_DEV float row_sum(float x) {
+UNP4_DEV float column_sum(float x) {
   auto a = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(u32, x), __builtin_bit_cast(u32, x), false, false);
   x = __builtin_bit_cast(float, (u32)a[0]) + __builtin_bit_cast(float, (u32)a[1]);
   a = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(u32, x), __builtin_bit_cast(u32, x), false, false);
@@ -379,40 +382,49 @@ UNP4_DEV tile tile_of(const i32* starts, const i32* lengths, const attention_arg
   }
 }
 
-template <class T, int H, int QH, int D, int GROUP, int P, bool CAUSAL, bool LSE, int QT> struct attention {
+template <class T, int H, int QH, int D, int GROUP, int P, bool CAUSAL, int QT, int CG> struct attention {
+  static_assert(QT == 1 || CG == 1, "columns are shared by one row tile");
   typedef record<D, GROUP, P> R;
   static constexpr int GQ = QH / H, W = R::W, G = R::G, KJ = D / 32, JG = GROUP / 32;
-  // Value tiles: 16 rows of N adjacent elements each, from words FIRST on.  Full tiles of 16 words, then one of
-  // the rest, whose words go to several rows where they are few.
-  static constexpr int FULL = W / 16, REST = W % 16, NT = FULL + (REST ? 1 : 0);
+  static constexpr int NB = 2 * CG, KEYS = 16 * NB, ROWS = 16 / CG;  // blocks of 16 keys, keys of a step; rows of a tile
+  // Value tiles: 16 rows of N adjacent elements each.  A group's words in tiles of 16 words, then one of the rest,
+  // whose words go to several rows where they are few.
+  static constexpr int GW = GROUP / 8, FULL = GW / 16, REST = GW % 16, TG = FULL + (REST ? 1 : 0), NT = G * TG;
   static constexpr int NREST = REST == 0 ? 0 : REST <= 4 ? 2 : REST <= 8 ? 4 : 8;
-  static constexpr int NE = FULL * 8 + NREST;  // matrix products of 16 elements that cover a head
-  static constexpr int nibbles(int t) { return t < FULL ? 8 : NREST; }
+  static constexpr int NEG = FULL * 8 + NREST, NE = G * NEG;  // matrix products of 16 elements for a group, a head
+  static constexpr int nibbles(int t) { return t % TG < FULL ? 8 : NREST; }
+  static constexpr int product(int t, int e) { return t / TG * NEG + t % TG * 8 + e; }
 
-  struct block {  // what 16 keys' products need, as it lies in memory
+  struct keys {
     u32 k[KJ];
-    u32x4 kp[G], v[NT], vp[NT];
+  };
+  struct values {
+    u32x4 v[NT];
   };
   int lane, c, g;  // c: the row a lane gives and the column it holds, g: its part of the depth
-  // The nibbles' masks and the exponents they are put under, in registers: as literals each takes an operation more.
-  u32 mask0, mask1, exp0, exp1;
+  int own;         // the column's group: which 16 of 16 CG keys it keeps
+  // The nibbles' masks in registers: as literals each takes an operation more.
+  u32 mask0, mask1;
   f16x8 q[QT][KJ];
   float qsum[QT][G], factor[QT];  // of this lane's column; factor: raw scores to log2
-  float m[QT];
-  // The column's sums of p, in l[0] (with LSE this lane's part of it until the end), and of p v.
-  f32x4 l[QT], o[QT][NE];
+  float m[QT], l[QT];             // running maximum; this lane's part of the sum of p
+  float unit;                     // a power of two: value scales times it are at most 1
+  f32x4 o[QT][NE];
+  // The sums of p s zero by group: this lane's parts, or (one group of columns, few of elements) a product whose rows
+  // are all the same.
+  static constexpr bool ZERO_PRODUCT = CG == 1 && G <= 2;
+  float zs[QT][G];
+  f32x4 zp[QT][ZERO_PRODUCT ? G : 1];
   int end[QT], begin[QT];  // keys that the column sees
-  u32 poison[QT];          // bit 4t + r: rows r of tile t hold no number (guard)
 
-  // Rows first .. first + 16 QT - 1 (token * GQ + head of the group) of a sequence.
+  // Rows first .. first + QT ROWS - 1 (token * GQ + head of the group) of a sequence.
   UNP4_DEV void rows(const T* qp, const attention_args& a, const tile& t, int kv, int first, float scale, int cap) {
     asm("s_mov_b32 %0, 0x000f000f" : "=s"(mask0));
     asm("s_mov_b32 %0, 0x00f000f0" : "=s"(mask1));
-    asm("v_mov_b32 %0, 0x64006400" : "=v"(exp0));
-    asm("v_mov_b32 %0, 0x54005400" : "=v"(exp1));
+    unit = 0x1p60f;
 #pragma unroll
     for (int x = 0; x < QT; ++x) {
-      const int r = first + x * 16 + c;
+      const int r = first + x * 16 + c % ROWS;
       const bool in = r < t.rows * GQ;
       const int token = in ? r / GQ : 0, head = kv * GQ + (in ? r % GQ : 0);
       const T* p = qp + (i64)(t.start + token) * a.q_token + (i64)head * a.q_head;
@@ -425,7 +437,7 @@ template <class T, int H, int QH, int D, int GROUP, int P, bool CAUSAL, bool LSE
           raw[j][i] = in ? p[j * 32 + g * 8 + i] : (T)0.0f;
           top = fmaxf(top, fabsf((float)raw[j][i]));
         }
-      top = row_max(top);
+      top = column_max(top);
       // The power of two that puts the largest element into 2^13 .. 2^14: odd nibbles weigh 16 times as much, so
       // their elements are scaled down by 16.
       int up = top > 0.0f && top < __builtin_inff() ? 13 - (int)((__builtin_bit_cast(u32, top) >> 23) & 255) + 127 : 0;
@@ -444,11 +456,15 @@ template <class T, int H, int QH, int D, int GROUP, int P, bool CAUSAL, bool LSE
         }
       }
 #pragma unroll
-      for (int gi = 0; gi < G; ++gi) qsum[x][gi] = row_sum(qsum[x][gi]);
+      for (int gi = 0; gi < G; ++gi) qsum[x][gi] = column_sum(qsum[x][gi]);
       factor[x] = fminf(scale * 1.4426950408889634f * 0x1p24f * __builtin_bit_cast(float, (u32)(127 - up) << 23), 0x1p127f);
       m[x] = -__builtin_inff();
-      l[x] = f32x4{0, 0, 0, 0};
-      poison[x] = 0;
+      l[x] = 0.0f;
+#pragma unroll
+      for (int gi = 0; gi < G; ++gi) {
+        zs[x][gi] = 0.0f;
+        if (ZERO_PRODUCT) zp[x][ZERO_PRODUCT ? gi : 0] = f32x4{0, 0, 0, 0};
+      }
 #pragma unroll
       for (int e = 0; e < NE; ++e) o[x][e] = f32x4{0, 0, 0, 0};
       const int last = CAUSAL ? t.length - t.rows + token + 1 : t.length;
@@ -457,26 +473,81 @@ template <class T, int H, int QH, int D, int GROUP, int P, bool CAUSAL, bool LSE
     }
   }
 
-  UNP4_DEV int word_of(int t) const {  // the value word of this lane's row in tile t
-    const int w = t < FULL ? t * 16 + c : FULL * 16 + c * nibbles(t) / 8;
-    return w < W ? w : W - 1;
-  }
-
-  // 16 keys from token t0 (a multiple of 16) of a record on: their key parts, and their value parts.
-  UNP4_DEV void load_keys(const u32* rec, int t0, block& b) const {
-    const u32* kp = rec + R::KEYS + t0 * W + (c * W + g * KJ);
-#pragma unroll
-    for (int j = 0; j < KJ; ++j) b.k[j] = kp[j];
-#pragma unroll
-    for (int gi = 0; gi < G; ++gi) b.kp[gi] = *reinterpret_cast<const u32x4*>(rec + R::kpar(t0, gi) + g * 4);
-  }
-  UNP4_DEV void load_values(const u32* rec, int t0, block& b) const {
-#pragma unroll
-    for (int t = 0; t < NT; ++t) {
-      const int w = word_of(t);
-      b.v[t] = *reinterpret_cast<const u32x4*>(rec + R::VALUES + t0 * W + (g * W + w) * 4);
-      b.vp[t] = *reinterpret_cast<const u32x4*>(rec + R::VPAR + t0 + (8 * w / GROUP) * P + g * 4);
+  // The keys of steps at, at + by, .. below last, each loaded while the one before is multiplied.  lo, hi: the keys
+  // from lo on and below hi that every column sees.
+  struct stream {
+    const u32* cache;
+    uniform_ints table;  // the sequence's pages
+    int kv, at, by, last, cap, lo, hi, pages;
+    int next, id[NB], ahead[NB];  // the step being loaded, and both steps' pages by block (-1: none)
+    keys k[NB];
+    values v[NB];
+    u32x4 kp[2][G], vp[2][G];  // the words of the keys that this lane's column keeps
+    UNP4_DEV int page(int step, int k) const {  // cap > 0
+      const int key = step * KEYS + 16 * k, id = table[(key < cap ? key : cap - 1) / P];
+      return key < cap && (u32)id < (u32)pages ? id : -1;
     }
+    UNP4_DEV const u32* record_of(int id) const { return cache + ((i64)(id < 0 ? 0 : id) * H + kv) * (i64)R::WORDS; }
+  };
+  UNP4_DEV void load_keys(stream& s, int step, const int (&id)[NB]) const {
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+      const u32* p = s.record_of(id[b]) + R::KEYS + (step * KEYS + 16 * b) % P * W + (c * W + g * KJ);
+#pragma unroll
+      for (int j = 0; j < KJ; ++j) s.k[b].k[j] = p[j];
+    }
+  }
+  // The first of the column's keys of half h in their record's words: the record, plus their place.
+  UNP4_DEV const u32* own_words(const stream& s, int h, int step, const int (&id)[NB]) const {
+    auto place = [&](int b) { return s.record_of(id[b]) + (step * KEYS + 16 * b) % P; };
+    const u32* p = place(h * CG);
+    if (P >= 16 * CG) return p + 16 * own;  // one page holds them all
+#pragma unroll
+    for (int b = 1; b < CG; ++b) p = own == b ? place(h * CG + b) : p;
+    return p;
+  }
+  UNP4_DEV void load_key_words(stream& s, int step, const int (&id)[NB]) const {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const u32* p = own_words(s, h, step, id) + g * 4;
+#pragma unroll
+      for (int gi = 0; gi < G; ++gi) s.kp[h][gi] = *reinterpret_cast<const u32x4*>(p + R::kpar(0, gi));
+    }
+  }
+  UNP4_DEV void load_value_words(stream& s, int step, const int (&id)[NB]) const {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const u32* p = own_words(s, h, step, id) + g * 4;
+#pragma unroll
+      for (int gi = 0; gi < G; ++gi) s.vp[h][gi] = *reinterpret_cast<const u32x4*>(p + R::vpar(0, gi));
+    }
+  }
+  UNP4_DEV void load_values(stream& s, int step, const int (&id)[NB]) const {
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+      const u32* p = s.record_of(id[b]) + R::VALUES + (step * KEYS + 16 * b) % P * W;
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        const int w = t % TG * 16 + c * nibbles(t) / 8;
+        s.v[b].v[t] = *reinterpret_cast<const u32x4*>(p + (g * W + t / TG * GW + (w < GW ? w : GW - 1)) * 4);
+      }
+    }
+  }
+  UNP4_DEV void open(stream& s) {
+    lane = threadIdx.x & 63;
+    c = lane & 15;
+    g = lane >> 4;
+    own = c / ROWS;
+    if (s.at >= s.last) return;
+    s.next = s.at + s.by < s.last ? s.at + s.by : s.at;
+#pragma unroll
+    for (int b = 0; b < NB; ++b) s.id[b] = s.page(s.at, b);
+#pragma unroll
+    for (int b = 0; b < NB; ++b) s.ahead[b] = s.page(s.next, b);
+    load_keys(s, s.at, s.id);
+    load_key_words(s, s.at, s.id);
+    load_value_words(s, s.at, s.id);
+    load_values(s, s.at, s.id);
   }
 
   UNP4_DEV f16x8 key_operand(u32 x) const {
@@ -484,251 +555,267 @@ template <class T, int H, int QH, int D, int GROUP, int P, bool CAUSAL, bool LSE
     const u32x4 b = {x & mask0, x & mask1, y & mask0, y & mask1};
     return __builtin_bit_cast(f16x8, b);
   }
-
-  // Value tile t of both blocks: out[e] is the operand of element e of each row's nibbles(t).
-  template <int N> UNP4_DEV void value_operands(const block (&b)[2], int t, f16x8 (&out)[N]) const {
+  // Value tile t of two blocks: out[e] is the operand of element e of each row's N.
+  template <int N> UNP4_DEV void value_operands(const values& v0, const values& v1, int t, f16x8 (&out)[N]) const {
     u32 part[N][4];
 #pragma unroll
-    for (int k = 0; k < 2; ++k)
+    for (int k = 0; k < 4; ++k) {
+      u32 wa = k < 2 ? v0.v[t][2 * k] : v1.v[t][2 * k - 4], wb = k < 2 ? v0.v[t][2 * k + 1] : v1.v[t][2 * k - 3];
+      if (N < 8) {  // this row's nibbles of the word
+        wa >>= (c * N) % 8 * 4;
+        wb >>= (c * N) % 8 * 4;
+      }
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        u32 wa = b[k].v[t][2 * h], wb = b[k].v[t][2 * h + 1];
-        const u32 pa = b[k].vp[t][2 * h], pb = b[k].vp[t][2 * h + 1];
-        if (N < 8) {  // this row's nibbles of the word
-          const int down = (c * N) % 8 * 4;
-          wa >>= down;
-          wb >>= down;
-        }
-        const f16x2 s = __builtin_bit_cast(f16x2, __builtin_amdgcn_perm(pb, pa, 0x05040100u));
-        const u32 z = __builtin_amdgcn_perm(pb, pa, 0x07060302u);
-        const f16x2 z0 = __builtin_bit_cast(f16x2, z | exp0), z1 = __builtin_bit_cast(f16x2, (z << 4) | exp1);
-#pragma unroll
-        for (int e = 0; e < N; e += 4) {
-          const u32 x = __builtin_amdgcn_perm(wb, wa, e ? 0x07060302u : 0x05040100u), y = x >> 8;
-          // 1024 + n in steps of 1, 64 + n in steps of 1/16: both exact, and so is n - zero.
-          part[e][2 * k + h] = pair((x & mask0) | exp0, z0, s);
-          part[e + 1][2 * k + h] = pair((x & mask1) | exp1, z1, s);
-          if (N > 2) {
-            part[e + 2 < N ? e + 2 : 0][2 * k + h] = pair((y & mask0) | exp0, z0, s);
-            part[e + 3 < N ? e + 3 : 0][2 * k + h] = pair((y & mask1) | exp1, z1, s);
-          }
+      for (int e = 0; e < N; e += 4) {
+        const u32 x = __builtin_amdgcn_perm(wb, wa, e ? 0x07060302u : 0x05040100u), y = x >> 8;
+        part[e][k] = x & mask0;
+        part[e + 1][k] = x & mask1;
+        if (N > 2) {
+          part[e + 2 < N ? e + 2 : 0][k] = y & mask0;
+          part[e + 3 < N ? e + 3 : 0][k] = y & mask1;
         }
       }
+    }
 #pragma unroll
     for (int e = 0; e < N; ++e)
       out[e] = __builtin_bit_cast(f16x8, u32x4{part[e][0], part[e][1], part[e][2], part[e][3]});
   }
-  static UNP4_DEV u32 pair(u32 bits, f16x2 z, f16x2 s) {
-    return __builtin_bit_cast(u32, (__builtin_bit_cast(f16x2, bits) - z) * s);
+  template <int N> UNP4_DEV void multiply_values(const stream& s, int t, int b, const f16x8 (&p)[QT][G]) {
+    f16x8 va[N];
+    value_operands<N>(s.v[b], s.v[CG + b], t, va);
+#pragma unroll
+    for (int e = 0; e < N; ++e)
+#pragma unroll
+      for (int x = 0; x < QT; ++x)
+        o[x][product(t, e)] =
+            __builtin_amdgcn_mfma_f32_16x16x32_f16(va[e], p[x][t / TG], o[x][product(t, e)], 0, 0, 0);
   }
 
-  // A value scale that is no number would reach, as 0 x NaN, the columns that do not see its key.  Such words are
-  // taken out of the product, and the rows of the columns that see them are marked.
-  UNP4_DEV void guard(block (&b)[2], const u32 (&seen)[QT]) {
-    u32 bad = 0;  // bit 8t + 4k + i
+  UNP4_DEV void step(stream& s) {
+    const int k0 = s.at * KEYS, after = s.next + s.by < s.last ? s.next + s.by : s.next;
+    int far[NB], bad = 0;
 #pragma unroll
-    for (int t = 0; t < NT; ++t)
-#pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if ((b[i / 4].vp[t][i % 4] & 0x7C00u) == 0x7C00u) {
-          bad |= 1u << (8 * t + i);
-          b[i / 4].vp[t][i % 4] = 0;
-        }
-    if (!__any(bad != 0)) return;
-    for (int part = 0; part < 4; ++part) {  // the keys of each part of the depth
-      u32 see[QT];
-#pragma unroll
-      for (int x = 0; x < QT; ++x) see[x] = __shfl(seen[x], part * 16 + c);
-      for (int r = 0; r < 4; ++r) {
-        const u32 row = __shfl(bad, part * 16 + g * 4 + r);
-#pragma unroll
-        for (int t = 0; t < NT; ++t)
-#pragma unroll
-          for (int x = 0; x < QT; ++x)
-            if (row >> (8 * t) & see[x] & 255u) poison[x] |= 1u << (4 * t + r);
-      }
+    for (int b = 0; b < NB; ++b) {
+      far[b] = s.page(after, b);
+      bad |= s.id[b];
     }
-  }
-
-  // 32 keys from k0 on; masked: some column may not see some of them.  good: whether each block's page is one.
-  // next_keys and next_values load the next step's parts as soon as this one's registers are free.
-  template <class FK, class FV>
-  UNP4_DEV void step(block (&b)[2], bool masked, int k0, int cap, bool good0, bool good1, FK next_keys, FV next_values) {
-    float s[QT][8];
+    const bool masked = k0 < s.lo || k0 + KEYS > s.hi || bad < 0;
+    float sc[QT][8];
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {
+    for (int h = 0; h < 2; ++h)
 #pragma unroll
       for (int gi = 0; gi < G; ++gi) {
-        f16x8 ka[JG];
+        f32x4 mine[QT];
 #pragma unroll
-        for (int j = 0; j < JG; ++j) ka[j] = key_operand(b[k].k[gi * JG + j]);
-        f32x4 acc[QT];
+        for (int b = 0; b < CG; ++b) {
+          f16x8 ka[JG];
+          f32x4 acc[QT];
 #pragma unroll
-        for (int x = 0; x < QT; ++x) acc[x] = f32x4{0, 0, 0, 0};
+          for (int j = 0; j < JG; ++j) ka[j] = key_operand(s.k[h * CG + b].k[gi * JG + j]);
 #pragma unroll
-        for (int j = 0; j < JG; ++j)
+          for (int x = 0; x < QT; ++x) acc[x] = f32x4{0, 0, 0, 0};
+#pragma unroll
+          for (int j = 0; j < JG; ++j)
+#pragma unroll
+            for (int x = 0; x < QT; ++x)
+              acc[x] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka[j], q[x][gi * JG + j], acc[x], 0, 0, 0);
 #pragma unroll
           for (int x = 0; x < QT; ++x)
-            acc[x] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka[j], q[x][gi * JG + j], acc[x], 0, 0, 0);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) mine[x][i] = b == 0 || own == b ? acc[x][i] : mine[x][i];
+        }
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const float scale = scale_of(b[k].kp[gi][i]), zero = -zero_of(b[k].kp[gi][i]);
+          const float scale = scale_of(s.kp[h][gi][i]), zero = -zero_of(s.kp[h][gi][i]);
 #pragma unroll
           for (int x = 0; x < QT; ++x) {
-            const float d = fmaf(zero, qsum[x][gi], acc[x][i]);
-            s[x][4 * k + i] = gi == 0 ? d * scale : fmaf(d, scale, s[x][4 * k + i]);
+            const float d = fmaf(zero, qsum[x][gi], mine[x][i]);
+            sc[x][4 * h + i] = gi == 0 ? d * scale : fmaf(d, scale, sc[x][4 * h + i]);
+          }
+        }
+      }
+    load_keys(s, s.next, s.ahead);
+    load_key_words(s, s.next, s.ahead);
+    u32 seen[QT];  // which of its 8 keys each of this lane's columns sees
+    if (masked) {
+      asm volatile("; a branch: not worth computing for every step");
+#pragma unroll
+      for (int x = 0; x < QT; ++x) seen[x] = 0;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        bool there = s.id[h * CG] >= 0;
+#pragma unroll
+        for (int b = 1; b < CG; ++b) there = own == b ? s.id[h * CG + b] >= 0 : there;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int key = k0 + 16 * (h * CG + own) + 4 * g + i;
+          // What no column sees does not count, whatever it holds.
+          if (!there || key >= s.cap)
+#pragma unroll
+            for (int gi = 0; gi < G; ++gi) s.vp[h][gi][i] = 0;
+#pragma unroll
+          for (int x = 0; x < QT; ++x) {
+            const bool sees = there && key < end[x] && key >= begin[x];
+            sc[x][4 * h + i] = sees ? sc[x][4 * h + i] : -__builtin_inff();
+            if (sees) seen[x] |= 1u << (4 * h + i);
           }
         }
       }
     }
-    next_keys();
-    if (masked) {
-      asm volatile("; a branch: not worth computing for every step");
-      u32 seen[QT];  // which of its 8 keys each of this lane's columns sees
-#pragma unroll
-      for (int x = 0; x < QT; ++x) {
-        seen[x] = 0;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const int key = k0 + 16 * (i / 4) + 4 * g + i % 4;
-          const bool sees = key < end[x] && key >= begin[x] && (i < 4 ? good0 : good1);
-          s[x][i] = sees ? s[x][i] : -__builtin_inff();
-          if (sees) seen[x] |= 1u << i;
-        }
-      }
-      // What no row may see does not count, whatever it holds.
-#pragma unroll
-      for (int k = 0; k < 2; ++k)
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (!(k ? good1 : good0) || k0 + 16 * k + 4 * g + i >= cap)
-#pragma unroll
-            for (int t = 0; t < NT; ++t) b[k].vp[t][i] = 0;
-      guard(b, seen);
-    }
-    f16x8 p[QT];
+    // The running maxima and the scales' unit; p of a row against an old maximum may reach 2^0.9.
+    float top[QT], big = 0.0f;
+    bool move = false;
 #pragma unroll
     for (int x = 0; x < QT; ++x) {
-      float top = s[x][0];
+      top[x] = sc[x][0];
 #pragma unroll
-      for (int i = 1; i < 8; ++i) top = fmaxf(top, s[x][i]);
-      if (__any((top - m[x]) * factor[x] > 0.9f)) {
-        const float next = fmaxf(m[x], row_max(top));
+      for (int i = 1; i < 8; ++i) top[x] = fmaxf(top[x], sc[x][i]);
+      move |= (top[x] - m[x]) * factor[x] > 0.9f;
+    }
+    float vs[2][G][4];
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int gi = 0; gi < G; ++gi)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          vs[h][gi][i] = scale_of(s.vp[h][gi][i]);
+          big = fmaxf(big, vs[h][gi][i]);
+        }
+    big = fminf(big, 65504.0f);
+    move |= big * unit > 1.0f;
+    if (__any(move)) {
+      const float all = column_max(big);
+      const float to = all * unit > 1.0f ? __builtin_bit_cast(float, (253u << 23) - (__builtin_bit_cast(u32, all) & 0x7F800000u)) : unit;
+      const float by = to / unit;
+      unit = to;
+#pragma unroll
+      for (int x = 0; x < QT; ++x) {
+        const float next = fmaxf(m[x], column_max(top[x]));
         const float keep = m[x] == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f((m[x] - next) * factor[x]);
         m[x] = next;
         l[x] *= keep;
 #pragma unroll
-        for (int e = 0; e < NE; ++e) o[x][e] *= keep;
+        for (int gi = 0; gi < G; ++gi) {
+          if (ZERO_PRODUCT)
+            zp[x][ZERO_PRODUCT ? gi : 0] *= keep * by;
+          else
+            zs[x][gi] *= keep * by;
+        }
+#pragma unroll
+        for (int e = 0; e < NE; ++e) o[x][e] *= keep * by;
       }
+    }
+    f16x8 zero[G];
+    if (ZERO_PRODUCT) {
+#pragma unroll
+      for (int gi = 0; gi < G; ++gi) {
+        u32 z[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const u32 w = __builtin_amdgcn_perm(s.vp[k / 2][gi][2 * (k % 2) + 1], s.vp[k / 2][gi][2 * (k % 2)], 0x07060302u);
+          const f16x2 y = __builtin_bit_cast(f16x2, (w & mask0) | 0x64006400u) - f16x2{1024, 1024};
+          z[k] = __builtin_bit_cast(u32, y);
+        }
+        zero[gi] = __builtin_bit_cast(f16x8, u32x4{z[0], z[1], z[2], z[3]});
+      }
+    }
+    f16x8 p[QT][G];
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int gi = 0; gi < G; ++gi)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) vs[h][gi][i] *= unit;
+#pragma unroll
+    for (int x = 0; x < QT; ++x) {
       const float off = m[x] == -__builtin_inff() ? 0.0f : fmaf(-m[x], factor[x], 15.0f);
+      float ps[G][8];
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const float e = __builtin_amdgcn_exp2f(fmaf(s[x][i], factor[x], off));
-        if (LSE) l[x][0] += e;
-        p[x][i] = (_Float16)e;
+        const float e = __builtin_amdgcn_exp2f(fmaf(sc[x][i], factor[x], off));
+        l[x] += e;
+#pragma unroll
+        for (int gi = 0; gi < G; ++gi) ps[gi][i] = e * vs[i / 4][gi][i % 4];
+      }
+      if (masked) {  // a scale that is no number does not reach the columns that do not see its key
+        asm volatile("; a branch: not worth computing for every step");
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+#pragma unroll
+          for (int gi = 0; gi < G; ++gi) ps[gi][i] = seen[x] >> i & 1 ? ps[gi][i] : 0.0f;
+      }
+#pragma unroll
+      for (int gi = 0; gi < G; ++gi)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) p[x][gi][i] = (_Float16)ps[gi][i];
+      if (ZERO_PRODUCT) {
+#pragma unroll
+        for (int gi = 0; gi < G; ++gi)
+          zp[x][ZERO_PRODUCT ? gi : 0] =
+              __builtin_amdgcn_mfma_f32_16x16x32_f16(zero[gi], p[x][gi], zp[x][ZERO_PRODUCT ? gi : 0], 0, 0, 0);
+      } else {
+#pragma unroll
+        for (int gi = 0; gi < G; ++gi)
+#pragma unroll
+          for (int i = 0; i < 8; ++i) zs[x][gi] = fmaf((float)p[x][gi][i], zero_of(s.vp[i / 4][gi][i % 4]), zs[x][gi]);
       }
     }
-    // Where nobody asks for it, the sum of p is a product too, with ones: of p as rounded, so that the weights' sum
-    // stays 1.  The log-sum-exp takes the sum of what was not rounded.
-    const f16x8 ones = {1, 1, 1, 1, 1, 1, 1, 1};
-    if (!LSE)
+    load_value_words(s, s.next, s.ahead);
 #pragma unroll
-      for (int x = 0; x < QT; ++x) l[x] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, p[x], l[x], 0, 0, 0);
-    int at = 0;
+    for (int b = 0; b < CG; ++b) {
+      // A column keeps its own keys: the others' products with it are with zeros.
+      f16x8 mine[QT][G];
 #pragma unroll
-    for (int t = 0; t < FULL; ++t) {
-      f16x8 va[8];
-      value_operands<8>(b, t, va);
+      for (int x = 0; x < QT; ++x)
 #pragma unroll
-      for (int e = 0; e < 8; ++e, ++at)
+        for (int gi = 0; gi < G; ++gi) {
+          u32x4 w = __builtin_bit_cast(u32x4, p[x][gi]);
+          if (CG > 1)
 #pragma unroll
-        for (int x = 0; x < QT; ++x) o[x][at] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va[e], p[x], o[x][at], 0, 0, 0);
+            for (int i = 0; i < 4; ++i) w[i] = own == b ? w[i] : 0u;
+          mine[x][gi] = __builtin_bit_cast(f16x8, w);
+        }
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        if constexpr (FULL > 0)
+          if (t % TG < FULL) multiply_values<8>(s, t, b, mine);
+        if constexpr (REST > 0)
+          if (t % TG >= FULL) multiply_values<NREST>(s, t, b, mine);
+      }
     }
-    if constexpr (REST > 0) {
-      f16x8 va[NREST];
-      value_operands<NREST>(b, FULL, va);
+    load_values(s, s.next, s.ahead);
+    s.at += s.by;
+    s.next = after;
 #pragma unroll
-      for (int e = 0; e < NREST; ++e, ++at)
-#pragma unroll
-        for (int x = 0; x < QT; ++x) o[x][at] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va[e], p[x], o[x][at], 0, 0, 0);
+    for (int b = 0; b < NB; ++b) {
+      s.id[b] = s.ahead[b];
+      s.ahead[b] = far[b];
     }
-    next_values();
   }
 
-  // The keys of steps at, at + by, .. below last (a step is 32 keys), each loaded while the one before is
-  // multiplied.  lo, hi: the keys from lo on and below hi that every column sees.
-  struct stream {
-    const u32* cache;
-    uniform_ints table;  // the sequence's pages
-    int kv, at, by, last, cap, lo, hi, pages;
-    int next, id[2], ahead[2];  // the step being loaded, and both steps' pages (-1: none)
-    block b[2];
-    UNP4_DEV int page(int step, int k) const {  // cap > 0
-      const int key = step * 32 + 16 * k, id = table[(key < cap ? key : cap - 1) / P];
-      return key < cap && (u32)id < (u32)pages ? id : -1;
-    }
-    UNP4_DEV const u32* record_of(int id) const { return cache + ((i64)(id < 0 ? 0 : id) * H + kv) * (i64)R::WORDS; }
-  };
-  UNP4_DEV void open(stream& s) {
-    lane = threadIdx.x & 63;
-    c = lane & 15;
-    g = lane >> 4;
-    if (s.at >= s.last) return;
-    s.next = s.at + s.by < s.last ? s.at + s.by : s.at;
-#pragma unroll
-    for (int k = 0; k < 2; ++k) s.id[k] = s.page(s.at, k);
-#pragma unroll
-    for (int k = 0; k < 2; ++k) s.ahead[k] = s.page(s.next, k);
-#pragma unroll
-    for (int k = 0; k < 2; ++k) load_keys(s.record_of(s.id[k]), (s.at * 32 + 16 * k) % P, s.b[k]);
-#pragma unroll
-    for (int k = 0; k < 2; ++k) load_values(s.record_of(s.id[k]), (s.at * 32 + 16 * k) % P, s.b[k]);
-  }
   UNP4_DEV void walk(stream& s) {
-    while (s.at < s.last) {
-      const int after = s.next + s.by < s.last ? s.next + s.by : s.next;
-      const int far[2] = {s.page(after, 0), s.page(after, 1)};
-      const bool masked = s.at * 32 < s.lo || s.at * 32 + 32 > s.hi || (s.id[0] | s.id[1]) < 0;
-      step(
-          s.b, masked, s.at * 32, s.cap, s.id[0] >= 0, s.id[1] >= 0,
-          [&] {
+    while (s.at < s.last) step(s);
 #pragma unroll
-            for (int k = 0; k < 2; ++k) load_keys(s.record_of(s.ahead[k]), (s.next * 32 + 16 * k) % P, s.b[k]);
-          },
-          [&] {
+    for (int x = 0; x < QT; ++x) {
+      l[x] = column_sum(l[x]);
 #pragma unroll
-            for (int k = 0; k < 2; ++k) load_values(s.record_of(s.ahead[k]), (s.next * 32 + 16 * k) % P, s.b[k]);
-          });
-      s.at += s.by;
-      s.next = after;
-#pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        s.id[k] = s.ahead[k];
-        s.ahead[k] = far[k];
-      }
+      for (int gi = 0; gi < G; ++gi) zs[x][gi] = ZERO_PRODUCT ? zp[x][ZERO_PRODUCT ? gi : 0][0] : column_sum(zs[x][gi]);
     }
-    if (LSE)
-#pragma unroll
-      for (int x = 0; x < QT; ++x) l[x][0] = row_sum(l[x][0]);
-#pragma unroll
-    for (int x = 0; x < QT; ++x)
-#pragma unroll
-      for (int t = 0; t < NT; ++t)
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-          if (poison[x] >> (4 * t + r) & 1)
-#pragma unroll
-            for (int e = 0; e < nibbles(t); ++e) o[x][8 * t + e][r] = __builtin_nanf("");
+  }
+  // The sum of p v for element e of row g * 4 + r of tile t.
+  UNP4_DEV float sum_of(int x, int t, int e, int r) const {
+    return (o[x][product(t, e)][r] * ((e & 1) ? 0x1p20f : 0x1p24f) - zs[x][t / TG]) * (1.0f / unit);
   }
 
-  // f(x, element, four-vector part i, value): every element of the lane's columns, N adjacent ones at a time.
+  // f(t, r, d): every run of nibbles(t) adjacent elements d .. of the lane's columns.
   template <class F> UNP4_DEV void each(F f) const {
 #pragma unroll
     for (int t = 0; t < NT; ++t)
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        const int n = nibbles(t), d = t * 128 + (g * 4 + r) * n;
-        if (t * 128 + 16 * n <= D || d < D) f(t, r, d);
+        const int n = nibbles(t), d = t % TG * 128 + (g * 4 + r) * n;
+        if (t % TG * 128 + 16 * n <= GROUP || d < GROUP) f(t, r, t / TG * GROUP + d);
       }
   }
 };
@@ -771,24 +858,24 @@ UNP4_DEV void finish(T* out, float* lse, const attention_args& a, i64 row, int h
   if (LSE && d == 0) lse[row * QH + head] = l == 0.0f ? -__builtin_inff() : (top - 15.0f + __log2f(l)) * 0.693147180559945309f;
 }
 
-// A block: WR waves of QT x 16 rows each and, for few rows, WK waves of the same rows that take the steps in turn
-// and are joined through LDS.  Blocks are numbered with the heads innermost (consecutive blocks go to different
+// A block: WR waves of QT x 16 rows each or, for few rows, WK waves of the same 16 / CG rows that take the steps in
+// turn and are joined through LDS.  Blocks are numbered with the heads innermost (consecutive blocks go to different
 // XCDs: with 8 heads each XCD's L2 holds one head's keys), then the parts of a context, then the tiles, last ones
 // first: under a causal mask those have the most keys.
-template <class T, int H, int QH, int D, int GROUP, int P, bool CAUSAL, bool LSE, int QT, int WR, int WK>
+template <class T, int H, int QH, int D, int GROUP, int P, bool CAUSAL, bool LSE, int QT, int CG, int WR, int WK>
 UNP4_DEV void attend(const T* q, const u32* cache, const i32* table, const i32* starts, const i32* lengths, T* out,
                      float* lse, float* ws, float scale, const attention_args& a) {
-  typedef attention<T, H, QH, D, GROUP, P, CAUSAL, LSE, QT> A;
-  constexpr int GQ = QH / H, ROWS = 16 * QT * WR;
+  typedef attention<T, H, QH, D, GROUP, P, CAUSAL, QT, CG> A;
+  constexpr int GQ = QH / H, WAVE_ROWS = QT * A::ROWS, ROWS = WAVE_ROWS * WR;
   const int wave = uniform(threadIdx.x >> 6);
   const int kv = blockIdx.x % H, part = (int)(blockIdx.x / H) % a.splits;
   const tile t = tile_of<GQ, ROWS>(starts, lengths, a, a.slots - 1 - (int)(blockIdx.x / H) / a.splits);
   if (t.seq < 0) return;
   const i64 room = a.width * P;
   const int cap = t.length < 0 ? 0 : t.length < room ? t.length : (int)room;
-  const int first_row = t.at * ROWS + (WR > 1 ? wave / WK * 16 * QT : 0), all_rows = t.rows * GQ;
+  const int first_row = t.at * ROWS + (WR > 1 ? wave * WAVE_ROWS : 0), all_rows = t.rows * GQ;
   // Keys that the wave's first and last rows see: some column sees keys from .. to, all see lo .. hi.
-  const int last_row = (first_row + 16 * QT < all_rows ? first_row + 16 * QT : all_rows) - 1;
+  const int last_row = (first_row + WAVE_ROWS < all_rows ? first_row + WAVE_ROWS : all_rows) - 1;
   int from = 0, to = cap, lo = 0, hi = cap;
   if (CAUSAL) {
     const i64 near = (i64)t.length - t.rows + first_row / GQ + 1, far = (i64)t.length - t.rows + last_row / GQ + 1;
@@ -801,18 +888,16 @@ UNP4_DEV void attend(const T* q, const u32* cache, const i32* table, const i32* 
   }
   if (last_row < first_row) to = 0;
   // This part's steps.
-  const int step0 = from / 32, steps = to > from ? (to + 31) / 32 - step0 : 0;
+  const int step0 = from / A::KEYS, steps = to > from ? (to + A::KEYS - 1) / A::KEYS - step0 : 0;
   const int each = (steps + a.splits - 1) / a.splits;
-  const int begin = step0 + (int)min((i64)steps, (i64)part * each);
-  const int end = step0 + (int)min((i64)steps, (i64)(part + 1) * each);
   A w;
   typename A::stream s;
   s.cache = cache;
   s.table = (uniform_ints)(u64)(table + (i64)t.seq * a.width);
   s.kv = kv;
-  s.at = begin + (WK > 1 ? wave % WK : 0);
+  s.at = step0 + (int)min((i64)steps, (i64)part * each) + (WK > 1 ? wave : 0);
   s.by = WK;
-  s.last = end;
+  s.last = step0 + (int)min((i64)steps, (i64)(part + 1) * each);
   s.cap = cap;
   s.lo = lo;
   s.hi = hi;
@@ -820,35 +905,34 @@ UNP4_DEV void attend(const T* q, const u32* cache, const i32* table, const i32* 
   w.open(s);  // the first keys are on their way while the rows are read
   w.rows(q, a, t, kv, first_row, scale, cap);
   w.walk(s);
-  if constexpr (WK > 1) {
-    // Join the waves: the rows' maxima and sums, then their elements, each scaled to the common maximum.
-    __shared__ float stat[WK][QT][16][2];
-    __shared__ float sums[WK][QT * 16][D + 4];
-    if (w.g == 0)
-#pragma unroll
-      for (int x = 0; x < QT; ++x) {
-        stat[wave][x][w.c][0] = w.m[x] * w.factor[x];
-        stat[wave][x][w.c][1] = w.l[x][0];
-      }
+  if constexpr (WK > 1 || CG > 1) {
+    // Join the waves and groups of columns: the rows' maxima and sums, then their elements, each scaled to the
+    // common maximum.
+    static_assert(QT == 1 && WR == 1, "a block joins the parts of one tile");
+    __shared__ float stat[WK * CG][A::ROWS][2];
+    __shared__ float sums[WK * CG][A::ROWS][D + 4];
+    const int mine = wave * CG + w.own, r0 = w.c % A::ROWS;
+    if (w.g == 0) {
+      stat[mine][r0][0] = w.m[0] * w.factor[0];
+      stat[mine][r0][1] = w.l[0];
+    }
     w.each([&](int tl, int r, int d) {
 #pragma unroll
-      for (int x = 0; x < QT; ++x)
-#pragma unroll
-        for (int e = 0; e < A::nibbles(tl); ++e) sums[wave][x * 16 + w.c][d + e] = w.o[x][8 * tl + e][r];
+      for (int e = 0; e < A::nibbles(tl); ++e) sums[mine][r0][d + e] = w.sum_of(0, tl, e, r);
     });
     __syncthreads();
-    const int n = all_rows - first_row < 16 * QT ? all_rows - first_row : 16 * QT;
+    const int n = all_rows - first_row < A::ROWS ? all_rows - first_row : A::ROWS;
     for (int i = threadIdx.x; i < n * (D / 4); i += 64 * WK) {
       const int row = i / (D / 4), d = i % (D / 4) * 4;
       float top = -__builtin_inff(), l = 0.0f;
 #pragma unroll
-      for (int v = 0; v < WK; ++v) top = fmaxf(top, stat[v][row / 16][row % 16][0]);
+      for (int v = 0; v < WK * CG; ++v) top = fmaxf(top, stat[v][row][0]);
       const float base = top == -__builtin_inff() ? 0.0f : top;
       f32x4 o = {0, 0, 0, 0};
 #pragma unroll
-      for (int v = 0; v < WK; ++v) {
-        const float keep = __builtin_amdgcn_exp2f(stat[v][row / 16][row % 16][0] - base);
-        l = fmaf(stat[v][row / 16][row % 16][1], keep, l);
+      for (int v = 0; v < WK * CG; ++v) {
+        const float keep = __builtin_amdgcn_exp2f(stat[v][row][0] - base);
+        l = fmaf(stat[v][row][1], keep, l);
         o += *reinterpret_cast<const f32x4*>(&sums[v][row][d]) * keep;
       }
       const int token = t.start + (first_row + row) / GQ, head = kv * GQ + (first_row + row) % GQ;
@@ -865,14 +949,14 @@ UNP4_DEV void attend(const T* q, const u32* cache, const i32* table, const i32* 
       const int row = first_row + x * 16 + w.c;
       if (row >= all_rows) continue;
       const int token = t.start + row / GQ, head = kv * GQ + row % GQ;
-      const float top = w.m[x] * w.factor[x], l = w.l[x][0];
+      const float top = w.m[x] * w.factor[x], l = w.l[x];
       if (a.splits > 1 && w.g == 0) store<float, 2>(parts<QH, D>::stat(ws, a, part, token, head), {top, l});
       w.each([&](int tl, int r, int d) {
 #pragma unroll
         for (int e = 0; e < A::nibbles(tl); e += 4) {
           f32x4 o;
 #pragma unroll
-          for (int i = 0; i < 4; ++i) o[i] = w.o[x][8 * tl + (e + i < A::nibbles(tl) ? e + i : 0)][r];
+          for (int i = 0; i < 4; ++i) o[i] = w.sum_of(x, tl, e + i < A::nibbles(tl) ? e + i : 0, r);
           if (a.splits > 1) {
             if (l != 0.0f) put(parts<QH, D>::sums(ws, a, part, token, head) + d + e, o, A::nibbles(tl));
           } else {

@@ -2054,7 +2054,7 @@ AttentionPlan attention_plan(const unp_exec* x, int64_t tokens, int64_t batch, i
   const unp_cache4& c = x->l.cache4;
   const int64_t group = x->l.attention.heads / c.kv_heads;
   AttentionPlan p;
-  // Waves that share 16 rows where sequences have that many or fewer, waves of rows of their own beyond.
+  // Waves that share their rows where sequences have 16 or fewer, waves of rows of their own beyond.
   p.entry = tokens * group <= 16 * batch ? 0 : 1;
   const unp::Entry& e = x->l.entries[p.entry];
   p.slots = tokens * group / e.vec + batch;
@@ -2062,10 +2062,9 @@ AttentionPlan attention_plan(const unp_exec* x, int64_t tokens, int64_t batch, i
     p.slots = tokens;
     p.by_token = true;
   }
-  // As many parts as give every CU two blocks, none shorter than two steps of 32 keys of each wave that shares a
-  // block's rows; with the whole context's pages as its length, which the host does not know.
+  // As many parts as give every CU two blocks, none shorter than two of a block's steps; with the whole context's pages as its length, which the host does not know.
   const int64_t blocks = p.slots * c.kv_heads, want = (2LL * x->cu_count + blocks - 1) / blocks;
-  const int64_t most = (width * c.page + 64 * e.k - 1) / (64 * e.k);
+  const int64_t most = (width * c.page + 2 * e.k - 1) / (2 * e.k);
   p.splits = std::max<int64_t>(1, std::min({want, most, kMostParts}));
   return p;
 }
