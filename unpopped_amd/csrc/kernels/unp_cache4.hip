@@ -345,6 +345,13 @@ UNP4_DEV float column_sum(float x) {
   return __builtin_bit_cast(float, (u32)a[0]) + __builtin_bit_cast(float, (u32)a[1]);
 }
 
+// The halves of a word as f16, for products that take them as they are: a zero point 0..15 is the subnormal n 2^-24.
+UNP4_DEV float low_half(u32 w) { return (float)__builtin_bit_cast(_Float16, (u16)w); }
+UNP4_DEV float high_half(u32 w) { return (float)__builtin_bit_cast(_Float16, (u16)(w >> 16)); }
+// The low, or high, halves of two words.
+UNP4_DEV u32 low_halves(u32 a, u32 b) { return __builtin_amdgcn_perm(b, a, 0x05040100u); }
+UNP4_DEV u32 high_halves(u32 a, u32 b) { return __builtin_amdgcn_perm(b, a, 0x07060302u); }
+
 UNP4_DEV int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
 // Memory that this launch does not write, read at a place all lanes share: a scalar load, which does not queue
 // behind the vector loads in flight.
@@ -382,7 +389,7 @@ UNP4_DEV tile tile_of(const i32* starts, const i32* lengths, const attention_arg
   }
 }
 
-template <class T, int H, int QH, int D, int GROUP, int P, bool CAUSAL, int QT, int CG> struct attention {
+template <class T, int H, int QH, int D, int GROUP, int P, bool CAUSAL, bool LSE, int QT, int CG> struct attention {
   static_assert(QT == 1 || CG == 1, "columns are shared by one row tile");
   typedef record<D, GROUP, P> R;
   static constexpr int GQ = QH / H, W = R::W, G = R::G, KJ = D / 32, JG = GROUP / 32;
@@ -406,9 +413,10 @@ template <class T, int H, int QH, int D, int GROUP, int P, bool CAUSAL, int QT, 
   // The nibbles' masks in registers: as literals each takes an operation more.
   u32 mask0, mask1;
   f16x8 q[QT][KJ];
-  float qsum[QT][G], factor[QT];  // of this lane's column; factor: raw scores to log2
-  float m[QT], l[QT];             // running maximum; this lane's part of the sum of p
-  float unit;                     // a power of two: value scales times it are at most 1
+  float qsum[QT][G], factor[QT];  // of this lane's column; qsum 2^24 times, as zeros are held; factor: raw scores to log2
+  float m[QT];                    // running maximum
+  f32x4 l[QT];                    // the sum of p, in l[0] (with LSE this lane's part of it until the end)
+  _Float16 unit;                  // a power of two: value scales times it are at most 1
   f32x4 o[QT][NE];
   // The sums of p s zero by group: this lane's parts, or (one group of columns, few of elements) a product whose rows
   // are all the same.
@@ -421,7 +429,7 @@ template <class T, int H, int QH, int D, int GROUP, int P, bool CAUSAL, int QT, 
   UNP4_DEV void rows(const T* qp, const attention_args& a, const tile& t, int kv, int first, float scale, int cap) {
     asm("s_mov_b32 %0, 0x000f000f" : "=s"(mask0));
     asm("s_mov_b32 %0, 0x00f000f0" : "=s"(mask1));
-    unit = 0x1p60f;
+    unit = (_Float16)0x1p15f;
 #pragma unroll
     for (int x = 0; x < QT; ++x) {
       const int r = first + x * 16 + c % ROWS;
@@ -452,14 +460,14 @@ template <class T, int H, int QH, int D, int GROUP, int P, bool CAUSAL, int QT, 
           const int d = (i >> 1) + 4 * (i & 1);  // the element at place i of a word's operand
           const _Float16 y = (_Float16)((float)raw[j][d] * ((d & 1) ? mul * 0.0625f : mul));
           q[x][j][i] = y;
-          qsum[x][j / JG] += (float)y * ((d & 1) ? 0x1p-20f : 0x1p-24f);
+          qsum[x][j / JG] += (float)y * ((d & 1) ? 16.0f : 1.0f);
         }
       }
 #pragma unroll
       for (int gi = 0; gi < G; ++gi) qsum[x][gi] = column_sum(qsum[x][gi]);
       factor[x] = fminf(scale * 1.4426950408889634f * 0x1p24f * __builtin_bit_cast(float, (u32)(127 - up) << 23), 0x1p127f);
       m[x] = -__builtin_inff();
-      l[x] = 0.0f;
+      l[x] = f32x4{0, 0, 0, 0};
 #pragma unroll
       for (int gi = 0; gi < G; ++gi) {
         zs[x][gi] = 0.0f;
@@ -626,11 +634,11 @@ template <class T, int H, int QH, int D, int GROUP, int P, bool CAUSAL, int QT, 
         }
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const float scale = scale_of(s.kp[h][gi][i]), zero = -zero_of(s.kp[h][gi][i]);
+          const u32 w = s.kp[h][gi][i];
 #pragma unroll
           for (int x = 0; x < QT; ++x) {
-            const float d = fmaf(zero, qsum[x][gi], mine[x][i]);
-            sc[x][4 * h + i] = gi == 0 ? d * scale : fmaf(d, scale, sc[x][4 * h + i]);
+            const float d = fmaf(-high_half(w), qsum[x][gi], mine[x][i]);
+            sc[x][4 * h + i] = fmaf(d, low_half(w), gi == 0 ? 0.0f : sc[x][4 * h + i]);
           }
         }
       }
@@ -663,7 +671,7 @@ template <class T, int H, int QH, int D, int GROUP, int P, bool CAUSAL, int QT, 
       }
     }
     // The running maxima and the scales' unit; p of a row against an old maximum may reach 2^0.9.
-    float top[QT], big = 0.0f;
+    float top[QT];
     bool move = false;
 #pragma unroll
     for (int x = 0; x < QT; ++x) {
@@ -672,23 +680,24 @@ template <class T, int H, int QH, int D, int GROUP, int P, bool CAUSAL, int QT, 
       for (int i = 1; i < 8; ++i) top[x] = fmaxf(top[x], sc[x][i]);
       move |= (top[x] - m[x]) * factor[x] > 0.9f;
     }
-    float vs[2][G][4];
+    f16x2 vs[G][4];  // the scales of keys 2k, 2k + 1
+    f16x2 most = {0, 0};
 #pragma unroll
-    for (int h = 0; h < 2; ++h)
+    for (int gi = 0; gi < G; ++gi)
 #pragma unroll
-      for (int gi = 0; gi < G; ++gi)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          vs[h][gi][i] = scale_of(s.vp[h][gi][i]);
-          big = fmaxf(big, vs[h][gi][i]);
-        }
-    big = fminf(big, 65504.0f);
-    move |= big * unit > 1.0f;
+      for (int k = 0; k < 4; ++k) {
+        vs[gi][k] = __builtin_bit_cast(f16x2, low_halves(s.vp[k / 2][gi][2 * (k % 2)], s.vp[k / 2][gi][2 * (k % 2) + 1]));
+        most = __builtin_elementwise_max(most, vs[gi][k]);
+      }
+    const float big = fminf(fmaxf((float)most[0], (float)most[1]), 65504.0f);
+    move |= big * (float)unit > 1.0f;
     if (__any(move)) {
       const float all = column_max(big);
-      const float to = all * unit > 1.0f ? __builtin_bit_cast(float, (253u << 23) - (__builtin_bit_cast(u32, all) & 0x7F800000u)) : unit;
-      const float by = to / unit;
-      unit = to;
+      const float old = (float)unit;
+      // 2^-(exponent + 1), so that the largest scale lies in 1/2 .. 1.
+      const float to = all * old > 1.0f ? __builtin_bit_cast(float, (253u << 23) - (__builtin_bit_cast(u32, all) & 0x7F800000u)) : old;
+      const float by = to / old;
+      unit = (_Float16)to;
 #pragma unroll
       for (int x = 0; x < QT; ++x) {
         const float next = fmaxf(m[x], column_max(top[x]));
@@ -706,59 +715,51 @@ template <class T, int H, int QH, int D, int GROUP, int P, bool CAUSAL, int QT, 
         for (int e = 0; e < NE; ++e) o[x][e] *= keep * by;
       }
     }
-    f16x8 zero[G];
-    if (ZERO_PRODUCT) {
+    u32x4 zero[G];
 #pragma unroll
-      for (int gi = 0; gi < G; ++gi) {
-        u32 z[4];
+    for (int gi = 0; gi < G; ++gi)
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const u32 w = __builtin_amdgcn_perm(s.vp[k / 2][gi][2 * (k % 2) + 1], s.vp[k / 2][gi][2 * (k % 2)], 0x07060302u);
-          const f16x2 y = __builtin_bit_cast(f16x2, (w & mask0) | 0x64006400u) - f16x2{1024, 1024};
-          z[k] = __builtin_bit_cast(u32, y);
-        }
-        zero[gi] = __builtin_bit_cast(f16x8, u32x4{z[0], z[1], z[2], z[3]});
+      for (int k = 0; k < 4; ++k) {
+        vs[gi][k] *= unit;
+        zero[gi][k] = high_halves(s.vp[k / 2][gi][2 * (k % 2)], s.vp[k / 2][gi][2 * (k % 2) + 1]) & mask0;
       }
-    }
-    f16x8 p[QT][G];
-#pragma unroll
-    for (int h = 0; h < 2; ++h)
-#pragma unroll
-      for (int gi = 0; gi < G; ++gi)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) vs[h][gi][i] *= unit;
+    const f16x8 ones = {1, 1, 1, 1, 1, 1, 1, 1};
+    u32x4 p[QT][G];
 #pragma unroll
     for (int x = 0; x < QT; ++x) {
       const float off = m[x] == -__builtin_inff() ? 0.0f : fmaf(-m[x], factor[x], 15.0f);
-      float ps[G][8];
+      f16x8 e;
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const float e = __builtin_amdgcn_exp2f(fmaf(sc[x][i], factor[x], off));
-        l[x] += e;
-#pragma unroll
-        for (int gi = 0; gi < G; ++gi) ps[gi][i] = e * vs[i / 4][gi][i % 4];
+        const float y = __builtin_amdgcn_exp2f(fmaf(sc[x][i], factor[x], off));
+        if (LSE) l[x][0] += y;
+        e[i] = (_Float16)y;
       }
-      if (masked) {  // a scale that is no number does not reach the columns that do not see its key
-        asm volatile("; a branch: not worth computing for every step");
+      // Where nobody asks for it, the sum of p is a product with ones, of p as rounded; the log-sum-exp takes the
+      // sum of what was not rounded.
+      if (!LSE) l[x] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, e, l[x], 0, 0, 0);
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
+      for (int gi = 0; gi < G; ++gi) {
 #pragma unroll
-          for (int gi = 0; gi < G; ++gi) ps[gi][i] = seen[x] >> i & 1 ? ps[gi][i] : 0.0f;
-      }
+        for (int k = 0; k < 4; ++k)
+          p[x][gi][k] = __builtin_bit_cast(u32, f16x2{e[2 * k], e[2 * k + 1]} * vs[gi][k]);
+        if (masked) {  // a scale that is no number does not reach the columns that do not see its key
+          asm volatile("; a branch: not worth computing for every step");
 #pragma unroll
-      for (int gi = 0; gi < G; ++gi)
+          for (int k = 0; k < 4; ++k)
+            p[x][gi][k] &= (seen[x] >> (2 * k) & 1 ? 0xFFFFu : 0u) | (seen[x] >> (2 * k + 1) & 1 ? 0xFFFF0000u : 0u);
+        }
+        if (ZERO_PRODUCT) {
+          f32x4& z = zp[x][ZERO_PRODUCT ? gi : 0];
+          z = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, zero[gi]), __builtin_bit_cast(f16x8, p[x][gi]),
+                                                     z, 0, 0, 0);
+        } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) p[x][gi][i] = (_Float16)ps[gi][i];
-      if (ZERO_PRODUCT) {
-#pragma unroll
-        for (int gi = 0; gi < G; ++gi)
-          zp[x][ZERO_PRODUCT ? gi : 0] =
-              __builtin_amdgcn_mfma_f32_16x16x32_f16(zero[gi], p[x][gi], zp[x][ZERO_PRODUCT ? gi : 0], 0, 0, 0);
-      } else {
-#pragma unroll
-        for (int gi = 0; gi < G; ++gi)
-#pragma unroll
-          for (int i = 0; i < 8; ++i) zs[x][gi] = fmaf((float)p[x][gi][i], zero_of(s.vp[i / 4][gi][i % 4]), zs[x][gi]);
+          for (int k = 0; k < 4; ++k) {
+            zs[x][gi] = fmaf(low_half(p[x][gi][k]), low_half(zero[gi][k]), zs[x][gi]);
+            zs[x][gi] = fmaf(high_half(p[x][gi][k]), high_half(zero[gi][k]), zs[x][gi]);
+          }
+        }
       }
     }
     load_value_words(s, s.next, s.ahead);
@@ -770,7 +771,7 @@ template <class T, int H, int QH, int D, int GROUP, int P, bool CAUSAL, int QT, 
       for (int x = 0; x < QT; ++x)
 #pragma unroll
         for (int gi = 0; gi < G; ++gi) {
-          u32x4 w = __builtin_bit_cast(u32x4, p[x][gi]);
+          u32x4 w = p[x][gi];
           if (CG > 1)
 #pragma unroll
             for (int i = 0; i < 4; ++i) w[i] = own == b ? w[i] : 0u;
@@ -798,14 +799,14 @@ template <class T, int H, int QH, int D, int GROUP, int P, bool CAUSAL, int QT, 
     while (s.at < s.last) step(s);
 #pragma unroll
     for (int x = 0; x < QT; ++x) {
-      l[x] = column_sum(l[x]);
+      if (LSE) l[x][0] = column_sum(l[x][0]);
 #pragma unroll
       for (int gi = 0; gi < G; ++gi) zs[x][gi] = ZERO_PRODUCT ? zp[x][ZERO_PRODUCT ? gi : 0][0] : column_sum(zs[x][gi]);
     }
   }
   // The sum of p v for element e of row g * 4 + r of tile t.
   UNP4_DEV float sum_of(int x, int t, int e, int r) const {
-    return (o[x][product(t, e)][r] * ((e & 1) ? 0x1p20f : 0x1p24f) - zs[x][t / TG]) * (1.0f / unit);
+  return (o[x][product(t, e)][r] * ((e & 1) ? 0x1p20f : 0x1p24f) - zs[x][t / TG] * 0x1p24f) * (1.0f / (float)unit);
   }
 
   // f(t, r, d): every run of nibbles(t) adjacent elements d .. of the lane's columns.
@@ -865,7 +866,7 @@ UNP4_DEV void finish(T* out, float* lse, const attention_args& a, i64 row, int h
 template <class T, int H, int QH, int D, int GROUP, int P, bool CAUSAL, bool LSE, int QT, int CG, int WR, int WK>
 UNP4_DEV void attend(const T* q, const u32* cache, const i32* table, const i32* starts, const i32* lengths, T* out,
                      float* lse, float* ws, float scale, const attention_args& a) {
-  typedef attention<T, H, QH, D, GROUP, P, CAUSAL, QT, CG> A;
+  typedef attention<T, H, QH, D, GROUP, P, CAUSAL, LSE, QT, CG> A;
   constexpr int GQ = QH / H, WAVE_ROWS = QT * A::ROWS, ROWS = WAVE_ROWS * WR;
   const int wave = uniform(threadIdx.x >> 6);
   const int kv = blockIdx.x % H, part = (int)(blockIdx.x / H) % a.splits;
@@ -914,7 +915,7 @@ UNP4_DEV void attend(const T* q, const u32* cache, const i32* table, const i32* 
     const int mine = wave * CG + w.own, r0 = w.c % A::ROWS;
     if (w.g == 0) {
       stat[mine][r0][0] = w.m[0] * w.factor[0];
-      stat[mine][r0][1] = w.l[0];
+      stat[mine][r0][1] = w.l[0][0];
     }
     w.each([&](int tl, int r, int d) {
 #pragma unroll
@@ -949,7 +950,7 @@ UNP4_DEV void attend(const T* q, const u32* cache, const i32* table, const i32* 
       const int row = first_row + x * 16 + w.c;
       if (row >= all_rows) continue;
       const int token = t.start + row / GQ, head = kv * GQ + row % GQ;
-      const float top = w.m[x] * w.factor[x], l = w.l[x];
+      const float top = w.m[x] * w.factor[x], l = w.l[x][0];
       if (a.splits > 1 && w.g == 0) store<float, 2>(parts<QH, D>::stat(ws, a, part, token, head), {top, l});
       w.each([&](int tl, int r, int d) {
 #pragma unroll
