@@ -329,6 +329,7 @@ typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 struct attention_args {
   i64 tokens, batch, width, pages, q_token, q_head, out_token, out_head, window;
   int slots, splits, by_token;  // row tiles, parts of a context, and how tiles are numbered (tile_of)
+  int q_wide, out_wide;         // rows of whole 16-byte vectors
 };
 
 // The maximum and the sum over the four lanes of a column (lane, lane ^ 16, lane ^ 32, lane ^ 48).
@@ -389,11 +390,49 @@ UNP4_DEV tile tile_of(const i32* starts, const i32* lengths, const attention_arg
   }
 }
 
+// N adjacent elements of a row from their sums.
+template <class T, int N> UNP4_DEV void put(T* p, const float (&o)[N], float by, bool wide) {
+  vec<T, N> y;
+#pragma unroll
+  for (int i = 0; i < N; ++i) y.v[i] = (T)(by == 0.0f ? 0.0f : o[i] * by);
+  if (wide) {
+    store<T, N>(p, y);
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) p[i] = y.v[i];
+  }
+}
+// w[r] of part g of a column and w[g] of part r change places, for all four r and g (lanes 16 apart).
+template <int M> UNP4_DEV void transpose(u32 (&w)[4][M]) {
+#pragma unroll
+  for (int i = 0; i < M; ++i) {
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      const auto y = __builtin_amdgcn_permlane32_swap(w[r][i], w[r + 2][i], false, false);
+      w[r][i] = y[0];
+      w[r + 2][i] = y[1];
+    }
+#pragma unroll
+    for (int r = 0; r < 4; r += 2) {
+      const auto y = __builtin_amdgcn_permlane16_swap(w[r][i], w[r + 1][i], false, false);
+      w[r][i] = y[0];
+      w[r + 1][i] = y[1];
+    }
+  }
+}
+// What a row's sums are multiplied with: a row that sees nothing gives 0.
+UNP4_DEV float share_of(float l) { return l == 0.0f ? 0.0f : 1.0f / l; }
+// top: the maximum in log2, to which p is held as 2^15 p.
+UNP4_DEV float log_sum(float top, float l) {
+  return l == 0.0f ? -__builtin_inff() : (top - 15.0f + __log2f(l)) * 0.693147180559945309f;
+}
+
 template <class T, int H, int QH, int D, int GROUP, int P, bool CAUSAL, bool LSE, int QT, int CG> struct attention {
   static_assert(QT == 1 || CG == 1, "columns are shared by one row tile");
   typedef record<D, GROUP, P> R;
   static constexpr int GQ = QH / H, W = R::W, G = R::G, KJ = D / 32, JG = GROUP / 32;
   static constexpr int NB = 2 * CG, KEYS = 16 * NB, ROWS = 16 / CG;  // blocks of 16 keys, keys of a step; rows of a tile
+  static constexpr int NP = KEYS > P ? KEYS / P : 1;                 // pages of a step
   // Value tiles: 16 rows of N adjacent elements each.  A group's words in tiles of 16 words, then one of the rest,
   // whose words go to several rows where they are few.
   static constexpr int GW = GROUP / 8, FULL = GW / 16, REST = GW % 16, TG = FULL + (REST ? 1 : 0), NT = G * TG;
@@ -437,12 +476,19 @@ template <class T, int H, int QH, int D, int GROUP, int P, bool CAUSAL, bool LSE
       const int token = in ? r / GQ : 0, head = kv * GQ + (in ? r % GQ : 0);
       const T* p = qp + (i64)(t.start + token) * a.q_token + (i64)head * a.q_head;
       T raw[KJ][8];
+      if (a.q_wide) {
+#pragma unroll
+        for (int j = 0; j < KJ; ++j) load8<T, true>(p + j * 32 + g * 8, raw[j]);
+      } else {
+#pragma unroll
+        for (int j = 0; j < KJ; ++j) load8<T, false>(p + j * 32 + g * 8, raw[j]);
+      }
       float top = 0.0f;
 #pragma unroll
       for (int j = 0; j < KJ; ++j)
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          raw[j][i] = in ? p[j * 32 + g * 8 + i] : (T)0.0f;
+          raw[j][i] = in ? raw[j][i] : (T)0.0f;
           top = fmaxf(top, fabsf((float)raw[j][i]));
         }
       top = column_max(top);
@@ -487,34 +533,45 @@ template <class T, int H, int QH, int D, int GROUP, int P, bool CAUSAL, bool LSE
     const u32* cache;
     uniform_ints table;  // the sequence's pages
     int kv, at, by, last, cap, lo, hi, pages;
-    int next, id[NB], ahead[NB];  // the step being loaded, and both steps' pages by block (-1: none)
+    // The step being loaded, and the page numbers of both and of the one after as they lie in the table: what is made
+    // of a number a step after its load does not wait for it.
+    int next, id[NP], ahead[NP], far[NP];
     keys k[NB];
     values v[NB];
     u32x4 kp[2][G], vp[2][G];  // the words of the keys that this lane's column keeps
-    UNP4_DEV int page(int step, int k) const {  // cap > 0
-      const int key = step * KEYS + 16 * k, id = table[(key < cap ? key : cap - 1) / P];
-      return key < cap && (u32)id < (u32)pages ? id : -1;
+    UNP4_DEV void number(int step, int (&to)[NP]) const {  // cap > 0
+#pragma unroll
+      for (int k = 0; k < NP; ++k) {
+        const int key = step * KEYS + k * P;
+        to[k] = table[(u32)(key < cap ? key : cap - 1) / P];
+      }
     }
-    UNP4_DEV const u32* record_of(int id) const { return cache + ((i64)(id < 0 ? 0 : id) * H + kv) * (i64)R::WORDS; }
+    UNP4_DEV bool good(int step, int b, const int (&id)[NP]) const {
+      return step * KEYS + 16 * b < cap && (u32)id[b * 16 / P] < (u32)pages;
+    }
+    UNP4_DEV const u32* record_of(int b, const int (&id)[NP]) const {
+      const int page = id[b * 16 / P];
+      return cache + ((i64)((u32)page < (u32)pages ? page : 0) * H + kv) * (i64)R::WORDS;
+    }
   };
-  UNP4_DEV void load_keys(stream& s, int step, const int (&id)[NB]) const {
+  UNP4_DEV void load_keys(stream& s, int step, const int (&id)[NP]) const {
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
-      const u32* p = s.record_of(id[b]) + R::KEYS + (step * KEYS + 16 * b) % P * W + (c * W + g * KJ);
+      const u32* p = s.record_of(b, id) + R::KEYS + (step * KEYS + 16 * b) % P * W + (c * W + g * KJ);
 #pragma unroll
       for (int j = 0; j < KJ; ++j) s.k[b].k[j] = p[j];
     }
   }
   // The first of the column's keys of half h in their record's words: the record, plus their place.
-  UNP4_DEV const u32* own_words(const stream& s, int h, int step, const int (&id)[NB]) const {
-    auto place = [&](int b) { return s.record_of(id[b]) + (step * KEYS + 16 * b) % P; };
+  UNP4_DEV const u32* own_words(const stream& s, int h, int step, const int (&id)[NP]) const {
+    auto place = [&](int b) { return s.record_of(b, id) + (step * KEYS + 16 * b) % P; };
     const u32* p = place(h * CG);
     if (P >= 16 * CG) return p + 16 * own;  // one page holds them all
 #pragma unroll
     for (int b = 1; b < CG; ++b) p = own == b ? place(h * CG + b) : p;
     return p;
   }
-  UNP4_DEV void load_key_words(stream& s, int step, const int (&id)[NB]) const {
+  UNP4_DEV void load_key_words(stream& s, int step, const int (&id)[NP]) const {
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const u32* p = own_words(s, h, step, id) + g * 4;
@@ -522,7 +579,7 @@ template <class T, int H, int QH, int D, int GROUP, int P, bool CAUSAL, bool LSE
       for (int gi = 0; gi < G; ++gi) s.kp[h][gi] = *reinterpret_cast<const u32x4*>(p + R::kpar(0, gi));
     }
   }
-  UNP4_DEV void load_value_words(stream& s, int step, const int (&id)[NB]) const {
+  UNP4_DEV void load_value_words(stream& s, int step, const int (&id)[NP]) const {
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const u32* p = own_words(s, h, step, id) + g * 4;
@@ -530,10 +587,10 @@ template <class T, int H, int QH, int D, int GROUP, int P, bool CAUSAL, bool LSE
       for (int gi = 0; gi < G; ++gi) s.vp[h][gi] = *reinterpret_cast<const u32x4*>(p + R::vpar(0, gi));
     }
   }
-  UNP4_DEV void load_values(stream& s, int step, const int (&id)[NB]) const {
+  UNP4_DEV void load_values(stream& s, int step, const int (&id)[NP]) const {
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
-      const u32* p = s.record_of(id[b]) + R::VALUES + (step * KEYS + 16 * b) % P * W;
+      const u32* p = s.record_of(b, id) + R::VALUES + (step * KEYS + 16 * b) % P * W;
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
         const int w = t % TG * 16 + c * nibbles(t) / 8;
@@ -548,10 +605,8 @@ template <class T, int H, int QH, int D, int GROUP, int P, bool CAUSAL, bool LSE
     own = c / ROWS;
     if (s.at >= s.last) return;
     s.next = s.at + s.by < s.last ? s.at + s.by : s.at;
-#pragma unroll
-    for (int b = 0; b < NB; ++b) s.id[b] = s.page(s.at, b);
-#pragma unroll
-    for (int b = 0; b < NB; ++b) s.ahead[b] = s.page(s.next, b);
+    s.number(s.at, s.id);
+    s.number(s.next, s.ahead);
     load_keys(s, s.at, s.id);
     load_key_words(s, s.at, s.id);
     load_value_words(s, s.at, s.id);
@@ -601,13 +656,11 @@ template <class T, int H, int QH, int D, int GROUP, int P, bool CAUSAL, bool LSE
 
   UNP4_DEV void step(stream& s) {
     const int k0 = s.at * KEYS, after = s.next + s.by < s.last ? s.next + s.by : s.next;
-    int far[NB], bad = 0;
+    s.number(after, s.far);
+    bool whole = k0 >= s.lo && k0 + KEYS <= s.hi;
 #pragma unroll
-    for (int b = 0; b < NB; ++b) {
-      far[b] = s.page(after, b);
-      bad |= s.id[b];
-    }
-    const bool masked = k0 < s.lo || k0 + KEYS > s.hi || bad < 0;
+    for (int k = 0; k < NP; ++k) whole &= (u32)s.id[k] < (u32)s.pages;
+    const bool masked = !whole;
     float sc[QT][8];
 #pragma unroll
     for (int h = 0; h < 2; ++h)
@@ -651,9 +704,9 @@ template <class T, int H, int QH, int D, int GROUP, int P, bool CAUSAL, bool LSE
       for (int x = 0; x < QT; ++x) seen[x] = 0;
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        bool there = s.id[h * CG] >= 0;
+        bool there = s.good(s.at, h * CG, s.id);
 #pragma unroll
-        for (int b = 1; b < CG; ++b) there = own == b ? s.id[h * CG + b] >= 0 : there;
+        for (int b = 1; b < CG; ++b) there = own == b ? s.good(s.at, h * CG + b, s.id) : there;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const int key = k0 + 16 * (h * CG + own) + 4 * g + i;
@@ -789,9 +842,9 @@ template <class T, int H, int QH, int D, int GROUP, int P, bool CAUSAL, bool LSE
     s.at += s.by;
     s.next = after;
 #pragma unroll
-    for (int b = 0; b < NB; ++b) {
-      s.id[b] = s.ahead[b];
-      s.ahead[b] = far[b];
+    for (int k = 0; k < NP; ++k) {
+      s.id[k] = s.ahead[k];
+      s.ahead[k] = s.far[k];
     }
   }
 
@@ -807,6 +860,48 @@ template <class T, int H, int QH, int D, int GROUP, int P, bool CAUSAL, bool LSE
   // The sum of p v for element e of row g * 4 + r of tile t.
   UNP4_DEV float sum_of(int x, int t, int e, int r) const {
   return (o[x][product(t, e)][r] * ((e & 1) ? 0x1p20f : 0x1p24f) - zs[x][t / TG] * 0x1p24f) * (1.0f / (float)unit);
+  }
+
+  // Row x's elements times `by` to p, as U.  A lane's four runs of N elements of a tile lie together, so stores of one
+  // run each would touch 64 places N elements wide; after a transposition four lanes' runs do (a prompt's output
+  // took 170 us without it, of which 16 are its bytes).
+  template <class U, int N> UNP4_DEV void write_tile(int x, int t, U* p, float by, bool there, bool wide) const {
+    constexpr int M = sizeof(U) * N / 4;
+    u32 w[4][M];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      vec<U, N> y;
+#pragma unroll
+      for (int e = 0; e < N; ++e) {
+        const float v = sum_of(x, t, e, r) * by;
+        y.v[e] = (U)(by == 0.0f ? 0.0f : v);
+      }
+      __builtin_memcpy(w[r], &y, sizeof(y));
+    }
+    transpose<M>(w);
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int d = t % TG * 128 + (r * 4 + g) * N;
+      if (!there || d >= GROUP) continue;
+      vec<U, N> y;
+      __builtin_memcpy(&y, w[r], sizeof(y));
+      U* to = p + t / TG * GROUP + d;
+      if (wide) {
+        store<U, N>(to, y);
+      } else {
+#pragma unroll
+        for (int e = 0; e < N; ++e) to[e] = y.v[e];
+      }
+    }
+  }
+  template <class U> UNP4_DEV void write(int x, U* p, float by, bool there, bool wide) const {
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      if constexpr (FULL > 0)
+        if (t % TG < FULL) write_tile<U, 8>(x, t, p, by, there, wide);
+      if constexpr (REST > 0)
+        if (t % TG >= FULL) write_tile<U, NREST>(x, t, p, by, there, wide);
+    }
   }
 
   // f(t, r, d): every run of nibbles(t) adjacent elements d .. of the lane's columns.
@@ -827,37 +922,10 @@ template <int QH, int D> struct parts {
     return ws + ((part * a.tokens + row) * QH + head) * 2;
   }
   static UNP4_DEV float* sums(float* ws, const attention_args& a, i64 part, i64 row, int head) {
-    return ws + a.splits * a.tokens * QH * 2 + ((part * a.tokens + row) * QH + head) * D;
+    const i64 stats = (a.splits * a.tokens * QH * 2 + 3) / 4 * 4;  // the sums stay aligned to 16 bytes
+    return ws + stats + ((part * a.tokens + row) * QH + head) * D;
   }
 };
-
-// Four elements (two of a narrow tile) of f32 sums.
-UNP4_DEV void put(float* p, const f32x4& o, int n) {
-  if (n >= 4) {
-    *reinterpret_cast<f32x4*>(p) = o;
-  } else {
-    *reinterpret_cast<f32x2*>(p) = f32x2{o[0], o[1]};
-  }
-}
-
-// A row's elements d .. from their sums; top: the maximum in log2, to which p is held as 2^15 p.
-template <class T, int QH, bool LSE>
-UNP4_DEV void finish(T* out, float* lse, const attention_args& a, i64 row, int head, int d, float top, float l, const f32x4& o,
-                     int n = 4) {
-  const float by = l == 0.0f ? 0.0f : 1.0f / l;  // a row that sees nothing gives 0
-  T* p = out + row * a.out_token + head * a.out_head + d;
-  vec<T, 4> y;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) y.v[i] = (T)(l == 0.0f ? 0.0f : o[i] * by);
-  if (n >= 4 && (reinterpret_cast<u64>(p) & 7) == 0) {
-    store<T, 4>(p, y);
-  } else {
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (i < n) p[i] = y.v[i];
-  }
-  if (LSE && d == 0) lse[row * QH + head] = l == 0.0f ? -__builtin_inff() : (top - 15.0f + __log2f(l)) * 0.693147180559945309f;
-}
 
 // A block: WR waves of QT x 16 rows each or, for few rows, WK waves of the same 16 / CG rows that take the steps in
 // turn and are joined through LDS.  Blocks are numbered with the heads innermost (consecutive blocks go to different
@@ -941,30 +1009,26 @@ UNP4_DEV void attend(const T* q, const u32* cache, const i32* table, const i32* 
         if (d == 0) store<float, 2>(parts<QH, D>::stat(ws, a, part, token, head), {top, l});
         if (l != 0.0f) *reinterpret_cast<f32x4*>(parts<QH, D>::sums(ws, a, part, token, head) + d) = o;
       } else {
-        finish<T, QH, LSE>(out, lse, a, token, head, d, top, l, o);
+        const float y[4] = {o[0], o[1], o[2], o[3]};
+        put<T, 4>(out + token * a.out_token + head * a.out_head + d, y, share_of(l), a.out_wide);
+        if (LSE && d == 0) lse[(i64)token * QH + head] = log_sum(top, l);
       }
     }
   } else {
 #pragma unroll
     for (int x = 0; x < QT; ++x) {
       const int row = first_row + x * 16 + w.c;
-      if (row >= all_rows) continue;
-      const int token = t.start + row / GQ, head = kv * GQ + row % GQ;
+      const bool there = row < all_rows, split = a.splits > 1;
+      const int token = t.start + (there ? row / GQ : 0), head = kv * GQ + (there ? row % GQ : 0);
       const float top = w.m[x] * w.factor[x], l = w.l[x][0];
-      if (a.splits > 1 && w.g == 0) store<float, 2>(parts<QH, D>::stat(ws, a, part, token, head), {top, l});
-      w.each([&](int tl, int r, int d) {
-#pragma unroll
-        for (int e = 0; e < A::nibbles(tl); e += 4) {
-          f32x4 o;
-#pragma unroll
-          for (int i = 0; i < 4; ++i) o[i] = w.sum_of(x, tl, e + i < A::nibbles(tl) ? e + i : 0, r);
-          if (a.splits > 1) {
-            if (l != 0.0f) put(parts<QH, D>::sums(ws, a, part, token, head) + d + e, o, A::nibbles(tl));
-          } else {
-            finish<T, QH, LSE>(out, lse, a, token, head, d + e, top, l, o, A::nibbles(tl));
-          }
-        }
-      });
+      if (there && w.g == 0) {
+        if (split) store<float, 2>(parts<QH, D>::stat(ws, a, part, token, head), {top, l});
+        if (LSE && !split) lse[(i64)token * QH + head] = log_sum(top, l);
+      }
+      if (split)
+        w.template write<float>(x, parts<QH, D>::sums(ws, a, part, token, head), 1.0f, there && l != 0.0f, true);
+      else
+        w.template write<T>(x, out + token * a.out_token + head * a.out_head, share_of(l), there, a.out_wide);
     }
   }
 }
@@ -1022,7 +1086,9 @@ UNP4_DEV void join(const i32* starts, T* out, float* lse, float* ws, const atten
   if (group != 0) return;
   const int used = a.splits < GROUPS ? a.splits : GROUPS;
   for (int i = 1; i < used; ++i) o += part[i][d / 4];
-  finish<T, QH, LSE>(out, lse, a, row, head, d, top, l, o);
+  const float y[4] = {o[0], o[1], o[2], o[3]};
+  put<T, 4>(out + row * a.out_token + head * a.out_head + d, y, share_of(l), a.out_wide);
+  if (LSE && d == 0) lse[row * QH + head] = log_sum(top, l);
 }
 
 }  // namespace unp4

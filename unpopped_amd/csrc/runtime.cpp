@@ -1874,7 +1874,7 @@ struct cache_args_host {
 };
 struct attention_args_host {
   int64_t tokens, batch, width, pages, q_token, q_head, out_token, out_head, window;
-  int32_t slots, splits, by_token, pad;
+  int32_t slots, splits, by_token, q_wide, out_wide, pad;
 };
 
 constexpr int64_t kMostOffset = (int64_t)1 << 60;
@@ -2046,9 +2046,10 @@ struct AttentionPlan {
   int64_t slots = 0, splits = 1;
   bool by_token = false;
 };
-// The workspace of one part of every row: its maximum and sum, and head_dim sums.
-int64_t part_bytes(const unp_exec* x, int64_t tokens) {
-  return tokens * x->l.attention.heads * (x->l.cache4.head_dim + 2) * 4;
+// The workspace of `parts` parts of every row: maxima and sums, then head_dim sums each.
+int64_t parts_bytes(const unp_exec* x, int64_t tokens, int64_t parts) {
+  const int64_t rows = parts * tokens * x->l.attention.heads;
+  return (rows * 8 + 15) / 16 * 16 + rows * x->l.cache4.head_dim * 4;
 }
 AttentionPlan attention_plan(const unp_exec* x, int64_t tokens, int64_t batch, int64_t width) {
   const unp_cache4& c = x->l.cache4;
@@ -2076,7 +2077,7 @@ int32_t attention_workspace(const unp_exec* x, const int64_t* sc, size_t n, uint
   bytes = 0;
   if (rc != UNP_OK || sc[0] == 0 || sc[1] == 0) return rc;
   const AttentionPlan p = attention_plan(x, sc[0], sc[1], sc[3] > 0 ? sc[2] : 0);
-  if (p.splits > 1) bytes = (uint64_t)(p.splits * part_bytes(x, sc[0]));
+  if (p.splits > 1) bytes = (uint64_t)parts_bytes(x, sc[0], p.splits);
   return UNP_OK;
 }
 
@@ -2104,13 +2105,14 @@ int32_t run_cache4_attention(unp_exec* x, const unp_arg* a, size_t n, hipStream_
       (at.lse && A.buf[6] % 4) || !aligned16(A.buf[nb - 1]))
     return invalid(err, "buffers are aligned to their elements, the cache and the workspace to 16 bytes");
   AttentionPlan p = attention_plan(x, tokens, batch, keys ? A.ext[2] : 0);
-  p.splits = std::max<int64_t>(1, std::min(p.splits, A.ext[9] / part_bytes(x, tokens)));
+  while (p.splits > 1 && parts_bytes(x, tokens, p.splits) > A.ext[9]) --p.splits;
   if (p.splits == 1 && A.buf[nb - 1] == 0) A.buf[nb - 1] = A.buf[5];  // not used
   const int64_t blocks = p.slots * p.splits * c.kv_heads;
   const int64_t joins = tokens * at.heads;
   if (blocks > 0x7FFFFFFFLL || joins > 0x7FFFFFFFLL) return invalid(err, "tokens: too many rows for one launch");
   attention_args_host args{tokens, batch, keys ? A.ext[2] : 0, A.ext[3], A.ext[4], A.ext[5], A.ext[6], A.ext[7], A.ext[8],
-                           (int32_t)p.slots, (int32_t)p.splits, p.by_token ? 1 : 0, 0};
+                           (int32_t)p.slots, (int32_t)p.splits, p.by_token ? 1 : 0,
+                           whole_vectors(A.buf[0], A.ext[4], A.ext[5], 8), whole_vectors(A.buf[5], A.ext[6], A.ext[7], 8), 0};
   uint64_t q = A.buf[0], cache = A.buf[1], table = A.buf[2], starts = A.buf[3], lengths = A.buf[4], out = A.buf[5];
   uint64_t lse = at.lse ? A.buf[6] : 0, ws = A.buf[nb - 1];
   float scale = (float)at.scale;
