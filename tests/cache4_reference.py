@@ -182,10 +182,12 @@ def attention_tolerance(out, mass, top, reach, keys, dim, dtype):
     * Values are added as sum p s n - sum p s zero in f32, codes and zeros of at most 15 steps of at most a seventh of the
       largest |v| (as above), and sum p is 1: (keys + 8) roundings of 2^-23 of 15 / 7 of it in each of the two sums.  So
       an output whose values are all 0 may come out as that much.
-    * Probabilities below 2^-29 of a row's largest are held to 2^-40 of it: keys * 2^-40 of the largest |v|.
+    * A probability p is held as the f16 number 2^11 p: below 2^-25 of the row's largest these are subnormal, a step
+      2^-24 apart, so off by at most 2^-36 of the largest.  With the products that they go into, keys * 2^-35 of the
+      largest |v|.
     * The output is rounded once to its type.
     """
     score = reach[..., None] * (30.0 / 7.0) * (dim + 4) * 2.0 ** -23
     off = mass * (2 * 2.0 ** -11 + 2 * score + (keys + 8) * 2.0 ** -23) + top[..., None] * (
-        keys * 2.0 ** -40 + 2 * 15.0 / 7.0 * (keys + 8) * 2.0 ** -23)
+        keys * 2.0 ** -35 + 2 * 15.0 / 7.0 * (keys + 8) * 2.0 ** -23)
     return off + (np.abs(out) + off) * HALF_STEP[dtype]

@@ -32,6 +32,24 @@ template <class T, int N> struct alignas(sizeof(T) * N) vec {
 };
 template <class T, int N> UNP4_DEV vec<T, N> load(const T* p) { return *reinterpret_cast<const vec<T, N>*>(p); }
 template <class T, int N> UNP4_DEV void store(T* p, const vec<T, N>& x) { *reinterpret_cast<vec<T, N>*>(p) = x; }
+// A store past the caches, for what this launch does not read again.
+template <class T, int N> UNP4_DEV void store_stream(T* p, const vec<T, N>& x) {
+  constexpr int W = sizeof(x) / 4;
+  if constexpr (W % 4 == 0) {
+#pragma unroll
+    for (int i = 0; i < W; i += 4) {
+      u32x4 y;
+      __builtin_memcpy(&y, reinterpret_cast<const char*>(&x) + 4 * i, 16);
+      __builtin_nontemporal_store(y, reinterpret_cast<u32x4*>(p) + i / 4);
+    }
+  } else if constexpr (W == 2) {
+    u64 y;
+    __builtin_memcpy(&y, &x, 8);
+    __builtin_nontemporal_store(y, reinterpret_cast<u64*>(p));
+  } else {
+    store<T, N>(p, x);
+  }
+}
 
 // ---------------------------------------------------------------------------------------
 // Position tables: [count][ROT / 2][cos, sin] of position first + row.
@@ -315,7 +333,8 @@ UNP4_DEV void read(const I* slots, const u32* cache, T* k, T* v, const cache_arg
 //     of columns hold the same rows and each keeps the scores of its own 16 of 16 CG keys: columns of one row are
 //     parts of its context, joined at the end as the waves are.
 //   * softmax over the columns: a lane holds 8 keys of one column, so its maximum needs two exchanges, and
-//     only when some score passes the running one by 2^0.9 (below that 2^15 p stays in f16's range).
+//     only when some score passes the running one by 2^4.9: p is held as 2^11 p in f16, which ends at 2^16
+//     (moving at 2^0.9, with 2^15 p, cost a prompt 8%: the sums are multiplied anew each time).
 //   * O' += V' P' with the value words as rows, again nibbles as they lie: sum p s (n - zero) is the product of n with
 //     p s less the sum of p s zero.  p s is rounded once to f16 (both sums take it as rounded), s relative to a
 //     running power of two that no scale of the column exceeded, so that it stays in f16's range whatever s is.  The
@@ -331,6 +350,8 @@ struct attention_args {
   int slots, splits, by_token;  // row tiles, parts of a context, and how tiles are numbered (tile_of)
   int q_wide, out_wide;         // rows of whole 16-byte vectors
 };
+
+constexpr float kHold = 11.0f, kSlack = 4.9f;
 
 // The maximum and the sum over the four lanes of a column (lane, lane ^ 16, lane ^ 32, lane ^ 48).
 UNP4_DEV float column_max(float x) {
@@ -422,9 +443,9 @@ template <int M> UNP4_DEV void transpose(u32 (&w)[4][M]) {
 }
 // What a row's sums are multiplied with: a row that sees nothing gives 0.
 UNP4_DEV float share_of(float l) { return l == 0.0f ? 0.0f : 1.0f / l; }
-// top: the maximum in log2, to which p is held as 2^15 p.
+// top: the maximum in log2, to which p is held as 2^kHold p.
 UNP4_DEV float log_sum(float top, float l) {
-  return l == 0.0f ? -__builtin_inff() : (top - 15.0f + __log2f(l)) * 0.693147180559945309f;
+  return l == 0.0f ? -__builtin_inff() : (top - kHold + __log2f(l)) * 0.693147180559945309f;
 }
 
 template <class T, int H, int QH, int D, int GROUP, int P, bool CAUSAL, bool LSE, int QT, int CG> struct attention {
@@ -723,7 +744,7 @@ template <class T, int H, int QH, int D, int GROUP, int P, bool CAUSAL, bool LSE
         }
       }
     }
-    // The running maxima and the scales' unit; p of a row against an old maximum may reach 2^0.9.
+    // The running maxima and the scales' unit; p of a row against an old maximum may reach 2^kSlack.
     float top[QT];
     bool move = false;
 #pragma unroll
@@ -731,7 +752,7 @@ template <class T, int H, int QH, int D, int GROUP, int P, bool CAUSAL, bool LSE
       top[x] = sc[x][0];
 #pragma unroll
       for (int i = 1; i < 8; ++i) top[x] = fmaxf(top[x], sc[x][i]);
-      move |= (top[x] - m[x]) * factor[x] > 0.9f;
+      move |= (top[x] - m[x]) * factor[x] > kSlack;
     }
     f16x2 vs[G][4];  // the scales of keys 2k, 2k + 1
     f16x2 most = {0, 0};
@@ -780,7 +801,7 @@ template <class T, int H, int QH, int D, int GROUP, int P, bool CAUSAL, bool LSE
     u32x4 p[QT][G];
 #pragma unroll
     for (int x = 0; x < QT; ++x) {
-      const float off = m[x] == -__builtin_inff() ? 0.0f : fmaf(-m[x], factor[x], 15.0f);
+      const float off = m[x] == -__builtin_inff() ? 0.0f : fmaf(-m[x], factor[x], kHold);
       f16x8 e;
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
@@ -887,7 +908,7 @@ template <class T, int H, int QH, int D, int GROUP, int P, bool CAUSAL, bool LSE
       __builtin_memcpy(&y, w[r], sizeof(y));
       U* to = p + t / TG * GROUP + d;
       if (wide) {
-        store<U, N>(to, y);
+        store_stream<U, N>(to, y);
       } else {
 #pragma unroll
         for (int e = 0; e < N; ++e) to[e] = y.v[e];
