@@ -91,18 +91,26 @@ int32_t lower_rope_table(const unp_rope_table& t, Lowered& L, std::string& why) 
   L.form.dtype = UNP_F32;
   L.rope_table = t;
   L.name = "unp_rope_table_r" + std::to_string(t.rot);
-  Entry e;
-  e.symbol = L.name + "_a";
-  L.entries.push_back(e);
   std::ostringstream src;
-  src << source_head(L.name) << kBounds256 << e.symbol
-      << "(float* table, long long first, long long count, unp4::stretch s) {\n  unp4::rope_table<" << t.rot
-      << ">(table, first, count, s);\n}\n";
+  src << source_head(L.name);
+  std::vector<std::string> when;
+  auto add = [&](const char* tail, int v, const char* cond) {
+    Entry e;
+    e.symbol = L.name + tail;
+    e.fast = v > 1;
+    e.vec = v;
+    L.entries.push_back(e);
+    when.push_back(cond);
+    src << kBounds256 << e.symbol << "(float* table, long long first, long long count, unp4::stretch s) {\n  unp4::rope_table<"
+        << t.rot << ", " << v << ">(table, first, count, s);\n}\n";
+  };
+  if (t.rot % 4 == 0) add("_v", 2, "a 16-byte aligned table");
+  add("_e", 1, "otherwise");
   L.source = src.str();
   L.interface_json = interface(
       L, "rope_table", "\"rot\":" + std::to_string(t.rot),
       {{"table", "Write", "F32"}, {"first", nullptr, "I64"}, {"count", nullptr, "I64"}},
-      "a pair per lane; blocks stride over the pairs", {"always"}, nullptr,
+      "pairs by lanes in order; blocks stride over them", when, nullptr,
       "angles, cosines and sines in f64, rounded once to f32");
   return UNP_OK;
 }

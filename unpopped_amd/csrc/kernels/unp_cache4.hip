@@ -54,7 +54,10 @@ template <class T, int N> UNP4_DEV void store_stream(T* p, const vec<T, N>& x) {
 // ---------------------------------------------------------------------------------------
 // Position tables: [count][ROT / 2][cos, sin] of position first + row.
 //
-// One pair per lane and step; a block computes the ROT / 2 frequencies once, into LDS.
+// A write of what 64-bit arithmetic makes, so the arithmetic is kept below it: the product of position and frequency
+// is taken in turns (frequency / 2 pi), whose whole and quarter part go off exactly, and on the remaining eighth of a turn
+// either side sine and cosine are their series to x^11 and x^10 (off by less than 2^-33, rounded to 2^-24 after).  A
+// lane makes V adjacent pairs; a block computes the ROT / 2 frequencies once, into LDS.
 // ---------------------------------------------------------------------------------------
 struct stretch {
   int kind;
@@ -73,18 +76,53 @@ UNP4_DEV double frequency(int i, const stretch& s) {
   return f;
 }
 
-template <int ROT>
+// The cosine and sine of `turns` turns.
+UNP4_DEV void turn_of(double turns, double& cs, double& sn) {
+  const double part = turns - rint(turns), quarter = rint(part * 4.0);
+  const double x = fma(quarter, -0.25, part) * 6.283185307179586476925, y = x * x;
+  double a = -1.0 / 39916800.0, b = -1.0 / 3628800.0;
+  a = fma(a, y, 1.0 / 362880.0);
+  b = fma(b, y, 1.0 / 40320.0);
+  a = fma(a, y, -1.0 / 5040.0);
+  b = fma(b, y, -1.0 / 720.0);
+  a = fma(a, y, 1.0 / 120.0);
+  b = fma(b, y, 1.0 / 24.0);
+  a = fma(a, y, -1.0 / 6.0);
+  b = fma(b, y, -0.5);
+  a = fma(a * y, x, x);
+  b = fma(b, y, 1.0);
+  const int q = (int)quarter;  // -2 .. 2
+  cs = q & 1 ? a : b;
+  sn = q & 1 ? b : a;
+  cs = q == 1 || q == 2 || q == -2 ? -cs : cs;
+  sn = q == -1 || q == 2 || q == -2 ? -sn : sn;
+}
+
+template <int ROT, int V>
 UNP4_DEV void rope_table(float* out, i64 first, i64 count, const stretch& s) {
-  constexpr int H = ROT / 2;
+  constexpr int H = ROT / 2, U = H / V;
   __shared__ double f[H];
-  for (int i = threadIdx.x; i < H; i += 256) f[i] = frequency<ROT>(i, s);
+  for (int i = threadIdx.x; i < H; i += 256) f[i] = frequency<ROT>(i, s) * 0.15915494309189533576888;
   __syncthreads();
-  const i64 n = count * H;
-  for (i64 at = (i64)blockIdx.x * 256 + threadIdx.x; at < n; at += (i64)gridDim.x * 256) {
-    const i64 row = at / H;
-    double sn, cs;
-    sincos((double)(first + row) * f[at - row * H], &sn, &cs);
-    store<float, 2>(out + 2 * at, {(float)(cs * s.amplitude), (float)(sn * s.amplitude)});
+  // Rows and units of V pairs in order; a step adds whole rows and a rest, so only the first divides.
+  const i64 at = (i64)blockIdx.x * 256 + threadIdx.x, step = (i64)gridDim.x * 256, dr = step / U;
+  const int du = (int)(step - dr * U);
+  i64 row = at / U;
+  for (int unit = (int)(at - row * U);; row += dr, unit += du) {
+    if (unit >= U) {
+      unit -= U;
+      ++row;
+    }
+    if (row >= count) return;
+    vec<float, 2 * V> y;
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      double cs, sn;
+      turn_of((double)(first + row) * f[unit * V + i], cs, sn);
+      y.v[2 * i] = (float)(cs * s.amplitude);
+      y.v[2 * i + 1] = (float)(sn * s.amplitude);
+    }
+    store_stream<float, 2 * V>(out + row * ROT + unit * 2 * V, y);
   }
 }
 
@@ -93,11 +131,14 @@ UNP4_DEV void rope_table(float* out, i64 first, i64 count, const stretch& s) {
 //
 // (x0, x1) -> (x0 c - x1 s, x1 c + x0 s), the sine negated for the inverse.  It reads and writes each
 // element once: a stream.  A unit of the vector entry is V pairs (two 16-byte loads and stores) or 2V
-// elements that are only copied; the plain entry takes a pair or a copied element at a time.
+// elements that are only copied; the plain entry takes a pair or a copied element at a time.  An output larger than half
+// of the last-level cache is stored past the caches: 16384 tokens x 40 heads x 128 bf16 65.2 us against 67.3 (5.3 TB/s),
+// but 4001 x 24 x 128 f32 (49 MB) 19.6 against 17.4.
 // ---------------------------------------------------------------------------------------
 struct rope_args {
   i64 tokens, x_token, x_head, out_token, out_head, first, rows;
   int heads, units;  // units of a head: the rotated ones, and the copied ones unless x and out are one
+  int past, pad;     // store past the caches
 };
 
 template <bool INV> UNP4_DEV void turn(float& a, float& b, float c, float s) {
@@ -105,6 +146,13 @@ template <bool INV> UNP4_DEV void turn(float& a, float& b, float c, float s) {
   const float x0 = a, x1 = b;
   a = fmaf(x0, c, -(x1 * s));
   b = fmaf(x1, c, x0 * s);
+}
+
+template <class T, int V> UNP4_DEV void put_unit(T* p, const vec<T, V>& x, int past) {
+  if (past)
+    store_stream<T, V>(p, x);
+  else
+    store<T, V>(p, x);
 }
 
 template <class T, int D, int ROT, int LAYOUT, bool INV, class I, int V>
@@ -141,13 +189,13 @@ UNP4_DEV void rope(const T* x, const I* positions, const float* table, T* out, c
           e0 = (T)f0;
           e1 = (T)f1;
         }
-        store<T, V>(op + p0, u);
-        store<T, V>(op + p1, w);
+        put_unit(op + p0, u, a.past);
+        put_unit(op + p1, w, a.past);
       } else {
         const int p = ROT + (unit - RU) * 2 * V;
         const vec<T, V> u = load<T, V>(xp + p), w = load<T, V>(xp + p + V);
-        store<T, V>(op + p, u);
-        store<T, V>(op + p + V, w);
+        put_unit(op + p, u, a.past);
+        put_unit(op + p + V, w, a.past);
       }
     } else {
       if (unit < RU) {
@@ -201,46 +249,79 @@ template <class T, bool ALIGNED> UNP4_DEV void load8(const T* p, T (&x)[8]) {
   }
 }
 
+// The maximum over N neighbouring lanes, N a power of two up to 32, by lane permutations within a row of 16 and, for 32,
+// an exchange of two rows.
+template <int CTRL> UNP4_DEV float permuted(float x) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), CTRL, 0xF, 0xF, false));
+}
+template <int N> UNP4_DEV float lane_max(float x) {
+  if (N > 1) x = fmaxf(x, permuted<0xB1>(x));   // pairs
+  if (N > 2) x = fmaxf(x, permuted<0x4E>(x));   // fours
+  if (N > 4) x = fmaxf(x, permuted<0x141>(x));  // eights, mirrored: each four is one value by now
+  if (N > 8) x = fmaxf(x, permuted<0x140>(x));  // the row, mirrored
+  if (N > 16) {
+    const auto y = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(u32, x), __builtin_bit_cast(u32, x), false, false);
+    x = fmaxf(__builtin_bit_cast(float, (u32)y[0]), __builtin_bit_cast(float, (u32)y[1]));
+  }
+  return x;
+}
+
+// Heads of the items that a block takes: a wave's lanes hold the words of one head for several tokens, four in a row
+// first, whose words lie together in the cache.
+template <int H, int W> struct items {
+  static constexpr int L = lanes_of(W), BLOCK = 256 / L;
+  i64 token;
+  int head, w;
+  bool key;
+  static UNP4_DEV i64 count(i64 tokens) { return (tokens + 3) / 4 * (8 * H); }
+  UNP4_DEV explicit items(i64 at) {
+    const i64 four = at / (8 * H);
+    const int in = (int)(at - four * (8 * H)), which = in / 4;
+    token = four * 4 + in % 4;
+    head = which % H;
+    key = which < H;
+    w = threadIdx.x % L;
+  }
+};
+
 // ---------------------------------------------------------------------------------------
 // Append: a lane holds one word's 8 elements of a key or a value head; a group's range is reduced over
-// its lanes.  The rotation's products of a 16-bit element and a 32-bit cosine are exact in f64, so the
-// rotated key is rounded once to 53 bits and once to its type: its code does not depend on how the sum
-// is contracted.  The quotients are correctly rounded f32 divisions; a quotient of an 11-bit by an 11-bit
-// number that is no tie is too far from one (2^-20 of it) for f32 to round onto it, so the codes are those of
-// exact arithmetic.
+// its lanes.  It reads the keys and values once and writes a quarter of that: a stream, if the arithmetic keeps out of
+// its way.
+//
+// The codes are those of exact arithmetic.  The rotation's products of a 16-bit element and a 32-bit cosine are exact in
+// f64, so the rotated key is rounded once to 53 bits and once to its type, however the sum is contracted.  A quotient
+// y / s of two 11-bit numbers that is no tie between two codes is at least 2^-13 from one ((2 y - (2 n + 1) s) / 2 s is
+// a multiple of y's or s's last place), and y times a reciprocal good to 2^-23 is off by less than 2^-17: it rounds
+// as the quotient does, and only where some lane's comes within 2^-16 of a tie the wave divides.
 // ---------------------------------------------------------------------------------------
 template <class T, int H, int D, int GROUP, int P, int ROT, int LAYOUT, class I, bool ALIGNED>
 UNP4_DEV void append(const T* k, const T* v, const I* slots, u32* cache, const I* positions, const float* table,
                      const cache_args& a) {
   typedef record<D, GROUP, P> R;
-  constexpr int L = lanes_of(R::W), IB = 256 / L;
-  const int w = threadIdx.x % L;
-  const i64 n = a.tokens * (2 * H);
-  for (i64 at = (i64)blockIdx.x * IB + threadIdx.x / L; at < n; at += (i64)gridDim.x * IB) {
-    const i64 token = at / (2 * H);
-    const int which = (int)(at - token * (2 * H)), head = which % H;
-    const bool key = which < H;
-    const i64 slot = (i64)slots[token];
-    if (slot < 0 || slot >= a.slots) continue;  // the same in every lane of the item
-    i64 row = 0;
-    if (ROT > 0) {
-      row = (i64)positions[token] - a.first;
-      if (row < 0 || row >= a.rows) continue;
-    }
-    const bool live = w < R::W;
+  typedef items<H, R::W> It;
+  const i64 n = It::count(a.tokens);
+  for (i64 at = (i64)blockIdx.x * It::BLOCK + threadIdx.x / It::L; at < n; at += (i64)gridDim.x * It::BLOCK) {
+    const It it(at);
+    if (it.token >= a.tokens) continue;  // the same in every lane of the item, as below
+    const int w = it.w;
+    const bool live = w < R::W, turns = ROT > 0 && it.key && 8 * w < ROT;
+    const bool second = LAYOUT == HALVES && 8 * w >= ROT / 2;  // of the pairs' elements
+    const int i0 = second ? 8 * w - ROT / 2 : 8 * w;
+    // The elements are on their way before the slot says whether they go anywhere.
+    T x[8], o[8];  // o: the pairs' other elements
+    const T* p = it.key ? k + it.token * a.k_token + it.head * a.k_head : v + it.token * a.v_token + it.head * a.v_head;
+    if (live) load8<T, ALIGNED>(p + 8 * w, x);
+    if (LAYOUT == HALVES && turns) load8<T, ALIGNED>(p + (second ? i0 : i0 + ROT / 2), o);
+    const i64 slot = (i64)slots[it.token];
+    const i64 row = ROT > 0 ? (i64)positions[it.token] - a.first : 0;
+    if (slot < 0 || slot >= a.slots || (ROT > 0 && (row < 0 || row >= a.rows))) continue;
     float y[8];
-    float lo = 0.0f, hi = 0.0f;
+    float lo = 0.0f, hi = 0.0f, not_finite = 0.0f;
     if (live) {
-      const T* p = key ? k + token * a.k_token + head * a.k_head : v + token * a.v_token + head * a.v_head;
-      T x[8];
-      load8<T, ALIGNED>(p + 8 * w, x);
-      if (ROT > 0 && key && 8 * w < ROT) {
+      if (turns) {
         const float* cs = table + row * ROT;
         if (LAYOUT == HALVES) {
-          const bool second = 8 * w >= ROT / 2;
-          const int i0 = second ? 8 * w - ROT / 2 : 8 * w;
-          T o[8];  // the pairs' other elements
-          load8<T, ALIGNED>(p + (second ? i0 : i0 + ROT / 2), o);
           for (int i = 0; i < 8; ++i) {
             const double c = cs[2 * (i0 + i)], s = cs[2 * (i0 + i) + 1];
             const double r = (double)(float)x[i] * c + (second ? 1.0 : -1.0) * ((double)(float)o[i] * s);
@@ -258,31 +339,41 @@ UNP4_DEV void append(const T* k, const T* v, const I* slots, u32* cache, const I
       for (int i = 0; i < 8; ++i) {
         y[i] = (float)x[i];
         lo = fminf(lo, y[i]);
-        // A NaN or an infinity of either sign opens the range to infinity.
-        hi = fmaxf(hi, fabsf(y[i]) < __builtin_inff() ? y[i] : __builtin_inff());
+        hi = fmaxf(hi, y[i]);
+        not_finite = fmaf(y[i], 0.0f, not_finite);  // 0, or no number
       }
+      // A NaN or an infinity of either sign opens the range to infinity.
+      hi = not_finite == 0.0f ? hi : __builtin_inff();
     }
-    constexpr int GL = GROUP == D ? L : GROUP / 8;  // lanes of a group
-    for (int m = 1; m < GL; m *= 2) {
-      lo = fminf(lo, __shfl_xor(lo, m));
-      hi = fmaxf(hi, __shfl_xor(hi, m));
-    }
+    constexpr int GL = GROUP == D ? It::L : GROUP / 8;  // lanes of a group
+    lo = -lane_max<GL>(-lo);
+    hi = lane_max<GL>(hi);
     const _Float16 sh = (_Float16)((hi - lo) / 15.0f);
     const bool finite = (float)sh < __builtin_inff();
     const float s = finite && (float)sh > 0.0f ? (float)sh : 1.0f;
-    const float z = finite ? fminf(15.0f, fmaxf(0.0f, rintf(-lo / s))) : 0.0f;
+    const float inv = __builtin_amdgcn_rcpf(s);
+    const float t0 = -lo * inv;
+    float q[8], z = rintf(t0), near = fabsf(fabsf(t0 - z) - 0.5f);  // near: the least distance to a tie
+    if (__any(near < 0x1p-16f)) z = rintf(-lo / s);
+    z = finite ? __builtin_amdgcn_fmed3f(z, 0.0f, 15.0f) : 0.0f;
     if (!live) continue;
-    u32 word = 0;
+    near = 1.0f;
     for (int i = 0; i < 8; ++i) {
-      const float c = finite ? fminf(15.0f, fmaxf(0.0f, rintf(y[i] / s) + z)) : 0.0f;
-      word |= (u32)c << (4 * i);
+      const float t = y[i] * inv;
+      q[i] = rintf(t);
+      near = fminf(near, fabsf(fabsf(t - q[i]) - 0.5f));
     }
+    if (__any(near < 0x1p-16f))
+      for (int i = 0; i < 8; ++i) q[i] = rintf(y[i] / s);
+    u32 word = 0;
+    for (int i = 0; i < 8; ++i) word |= (u32)__builtin_amdgcn_fmed3f(q[i] + z, 0.0f, 15.0f) << (4 * i);
+    if (!finite) word = 0;
     const int t = (int)(slot % P);
-    u32* rec = cache + ((slot / P) * H + head) * (i64)R::WORDS;
-    rec[key ? R::key(t, w) : R::value(t, w)] = word;
+    u32* rec = cache + ((slot / P) * H + it.head) * (i64)R::WORDS;
+    rec[it.key ? R::key(t, w) : R::value(t, w)] = word;
     if ((8 * w) % GROUP == 0) {
       const u32 bits = finite ? __builtin_bit_cast(u16, sh) : 0x7E00u;
-      rec[key ? R::kpar(t, 8 * w / GROUP) : R::vpar(t, 8 * w / GROUP)] = bits | (u32)z << 16;
+      rec[it.key ? R::kpar(t, 8 * w / GROUP) : R::vpar(t, 8 * w / GROUP)] = bits | (u32)z << 16;
     }
   }
 }
@@ -293,26 +384,27 @@ UNP4_DEV void append(const T* k, const T* v, const I* slots, u32* cache, const I
 template <class T, int H, int D, int GROUP, int P, class I, bool ALIGNED>
 UNP4_DEV void read(const I* slots, const u32* cache, T* k, T* v, const cache_args& a) {
   typedef record<D, GROUP, P> R;
-  const i64 n = a.tokens * (2 * H) * R::W;
-  for (i64 at = (i64)blockIdx.x * 256 + threadIdx.x; at < n; at += (i64)gridDim.x * 256) {
-    const i64 item = at / R::W, token = item / (2 * H);
-    const int w = (int)(at - item * R::W), which = (int)(item - token * (2 * H)), head = which % H;
-    const bool key = which < H;
-    const i64 slot = (i64)slots[token];
+  typedef items<H, R::W> It;
+  const i64 n = It::count(a.tokens);
+  for (i64 at = (i64)blockIdx.x * It::BLOCK + threadIdx.x / It::L; at < n; at += (i64)gridDim.x * It::BLOCK) {
+    const It it(at);
+    const int w = it.w;
+    if (it.token >= a.tokens || w >= R::W) continue;
+    const i64 slot = (i64)slots[it.token];
     vec<T, 8> o;
     if (slot >= 0 && slot < a.slots) {
       const int t = (int)(slot % P), g = 8 * w / GROUP;
-      const u32* rec = cache + ((slot / P) * H + head) * (i64)R::WORDS;
-      const u32 word = rec[key ? R::key(t, w) : R::value(t, w)];
-      const u32 par = rec[key ? R::kpar(t, g) : R::vpar(t, g)];
+      const u32* rec = cache + ((slot / P) * H + it.head) * (i64)R::WORDS;
+      const u32 word = rec[it.key ? R::key(t, w) : R::value(t, w)];
+      const u32 par = rec[it.key ? R::kpar(t, g) : R::vpar(t, g)];
       for (int i = 0; i < 8; ++i)
         o.v[i] = (T)(((float)(word >> (4 * i) & 15u) - zero_of(par)) * scale_of(par));
     } else {
       for (int i = 0; i < 8; ++i) o.v[i] = (T)0.0f;
     }
-    T* p = (key ? k + token * a.k_token + head * a.k_head : v + token * a.v_token + head * a.v_head) + 8 * w;
+    T* p = (it.key ? k + it.token * a.k_token + it.head * a.k_head : v + it.token * a.v_token + it.head * a.v_head) + 8 * w;
     if (ALIGNED) {
-      store<T, 8>(p, o);
+      store_stream<T, 8>(p, o);
     } else {
       for (int i = 0; i < 8; ++i) p[i] = o.v[i];
     }

@@ -1867,7 +1867,7 @@ struct stretch_host {
 };
 struct rope_args_host {
   int64_t tokens, x_token, x_head, out_token, out_head, first, rows;
-  int32_t heads, units;
+  int32_t heads, units, past, pad;
 };
 struct cache_args_host {
   int64_t tokens, slots, k_token, k_head, v_token, v_head, first, rows;
@@ -1927,7 +1927,9 @@ int32_t run_rope_table(unp_exec* x, const unp_arg* a, size_t n, hipStream_t s, u
   stretch_host st{t.scaling, 0, std::log(t.base), t.factor, t.low, t.high, t.original, t.amplitude};
   uint64_t out = A.buf[0];
   void* params[] = {&out, &first, &count, &st};
-  return launch(x, 0, grid_for(x, (count * (t.rot / 2) + 255) / 256), params, s, err);
+  const size_t entry = x->l.entries[0].fast && aligned16(out) ? 0 : x->l.entries.size() - 1;
+  const int64_t units = count * (t.rot / 2 / x->l.entries[entry].vec);
+  return launch(x, entry, grid_for(x, (units + 255) / 256), params, s, err);
 }
 
 int32_t check_rows(int64_t first, int64_t rows, unp_error* err) {
@@ -1962,7 +1964,9 @@ int32_t run_rope(unp_exec* x, const unp_arg* a, size_t n, hipStream_t s, unp_err
   // In place the elements behind rot stay where they are.
   const int unit = fast ? 2 * v : 1;
   rope_args_host args{tokens, A.ext[2], A.ext[3], A.ext[4], A.ext[5], A.ext[6], A.ext[7], (int32_t)heads,
-                      r.rot / 2 / (fast ? v : 1) + (same ? 0 : (r.head_dim - r.rot) / unit)};
+                      r.rot / 2 / (fast ? v : 1) + (same ? 0 : (r.head_dim - r.rot) / unit), 0, 0};
+  // Outputs past half of the 256 MiB last-level cache are not kept in it.
+  args.past = (__int128)tokens * heads * r.head_dim * (int)size > (128 << 20);
   const __int128 items = (__int128)tokens * heads * args.units;
   if (items > kMostOffset) return invalid(err, "x: more than 2^60 elements");
   uint64_t xp = A.buf[0], pos = A.buf[1], tab = A.buf[2], out = A.buf[3];
@@ -1982,6 +1986,15 @@ int32_t cache_scalars(const unp_exec* x, const Args& A, bool written, cache_args
   if ((__int128)tokens * c.kv_heads * c.head_dim > kMostOffset) return invalid(err, "k: more than 2^60 elements");
   out = cache_args_host{tokens, pages * c.page, A.ext[2], A.ext[3], A.ext[4], A.ext[5], 0, 0};
   return UNP_OK;
+}
+
+// Append and read take a head of a token on the next power of two of its words' lanes, four tokens at a time.
+uint32_t cache_grid(const unp_exec* x, int64_t tokens) {
+  const unp_cache4& c = x->l.cache4;
+  int lanes = 1;
+  while (lanes < c.head_dim / 8) lanes *= 2;
+  const int64_t per = 256 / lanes, items = (tokens + 3) / 4 * 8 * c.kv_heads;
+  return grid_for(x, (items + per - 1) / per);
 }
 
 int32_t run_cache4_append(unp_exec* x, const unp_arg* a, size_t n, hipStream_t s, unp_error* err) {
@@ -2004,12 +2017,9 @@ int32_t run_cache4_append(unp_exec* x, const unp_arg* a, size_t n, hipStream_t s
       (rot && (A.buf[4] % ib || !aligned16(A.buf[5]))))
     return invalid(err, "k, v, slots and positions are aligned to their elements, the cache and the table to 16 bytes");
   const bool fast = whole_vectors(A.buf[0], A.ext[2], A.ext[3], 8) && whole_vectors(A.buf[1], A.ext[4], A.ext[5], 8);
-  int lanes = 1;
-  while (lanes < c.head_dim / 8) lanes *= 2;
-  const int64_t items = args.tokens * 2 * c.kv_heads, per = 256 / lanes;
   uint64_t k = A.buf[0], v = A.buf[1], slots = A.buf[2], cache = A.buf[3], pos = rot ? A.buf[4] : 0, tab = rot ? A.buf[5] : 0;
   void* params[] = {&k, &v, &slots, &cache, &pos, &tab, &args};
-  return launch(x, fast ? 0 : 1, grid_for(x, (items + per - 1) / per), params, s, err);
+  return launch(x, fast ? 0 : 1, cache_grid(x, args.tokens), params, s, err);
 }
 
 int32_t run_cache4_read(unp_exec* x, const unp_arg* a, size_t n, hipStream_t s, unp_error* err) {
@@ -2026,10 +2036,9 @@ int32_t run_cache4_read(unp_exec* x, const unp_arg* a, size_t n, hipStream_t s, 
   if (A.buf[2] % 2 || A.buf[3] % 2 || A.buf[0] % unp::kind_bytes(c.index_dtype) || !aligned16(A.buf[1]))
     return invalid(err, "slots, k and v are aligned to their elements, the cache to 16 bytes");
   const bool fast = whole_vectors(A.buf[2], A.ext[2], A.ext[3], 8) && whole_vectors(A.buf[3], A.ext[4], A.ext[5], 8);
-  const int64_t lanes = args.tokens * 2 * c.kv_heads * (c.head_dim / 8);
   uint64_t slots = A.buf[0], cache = A.buf[1], k = A.buf[2], v = A.buf[3];
   void* params[] = {&slots, &cache, &k, &v, &args};
-  return launch(x, fast ? 0 : 1, grid_for(x, (lanes + 255) / 256), params, s, err);
+  return launch(x, fast ? 0 : 1, cache_grid(x, args.tokens), params, s, err);
 }
 
 int32_t check_attention(int64_t tokens, int64_t batch, int64_t width, int64_t pages, unp_error* err) {
