@@ -392,6 +392,7 @@ typedef struct unp_attention {
  * rows are starts[b] .. starts[b + 1] - 1), lengths (I32 [batch]: its keys, its own rows' last), out, with lse
  * lse (F32 [tokens][heads], natural log; -inf for an empty row), workspace; tokens, batch, width, pages, q_token, q_head,
  * out_token, out_head (strides), window, workspace_bytes.
+ *   A context is at most 2^30 keys (width * page), and so are the rows of a key/value head (tokens * heads / kv_heads).
  *   window > 0 (causal only): a row sees its last `window` keys.  A row that sees no key gives 0.
  *   Keys that no row may see do not count, whatever they hold: keys past a sequence's length, keys of a page number
  *   outside the cache, keys past width pages.  Rows that no sequence names are left as they were.  starts do not

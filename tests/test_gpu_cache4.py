@@ -1,9 +1,12 @@
 """The rotary and 4-bit cache forms on the GPU against their numpy reference: values, masks, borders, refusals."""
+import ctypes as C
+
 import numpy as np
 import pytest
 
 import unpopped_amd as u
 from tests import cache4_reference as ref
+from unpopped_amd import _lib
 
 pytestmark = pytest.mark.gpu
 B = u.HipBackend()
@@ -551,3 +554,204 @@ def test_prompt_then_tokens(hip_device):
         out, _, mass, top, reach = ref.attend(q, want, tables, starts, lengths)
         got = ref.loaded(ob.download(np.uint16, q.size), dtype).reshape(q.shape)
         assert (np.abs(got - out) <= ref.attention_tolerance(out, mass, top, reach, int(lengths.max()), dim, dtype)).all()
+
+
+# ---------------------------------------------------------------------------------------
+# Splits, streams, graphs and far places
+# ---------------------------------------------------------------------------------------
+@pytest.mark.parametrize("heads, rows", [(1, [1]), (6, [1]), (12, [1]), (4, [21]), (5, [2, 1])])
+@pytest.mark.parametrize("window", [0, 1500])
+def test_attention_splits_of_every_kind_of_block(hip_device, heads, rows, window):
+    """Contexts that are split over blocks, for each number of rows a block takes; a window leaves parts without keys."""
+    attention_case("F16", heads, 1, 64, 32, 32, rows, [2300, 90][:len(rows)], window=window, seed=heads, lse=heads != 6)
+
+
+def test_attention_of_many_sequences(hip_device):
+    """More sequences than one look of a wave finds, some without rows and some without keys."""
+    rng = np.random.default_rng(3)
+    rows = rng.integers(0, 3, 150).tolist()
+    lengths = [int(n) if i % 9 else 0 for i, n in enumerate(rng.integers(1, 40, 150))]
+    attention_case("Bf16", 2, 1, 32, 32, 16, rows, [max(n, r) for n, r in zip(lengths, rows)], seed=1)
+
+
+def small_step(dtype="Bf16", heads=4, kv=2, dim=64, page=16, rows=(1, 1, 1), lengths=(700, 33, 1200), seed=0):
+    """A decode step's buffers, its reference and a launch: (launch(stream, workspace), out, want, tolerance)."""
+    rng = np.random.default_rng(seed)
+    need = [-(-n // page) for n in lengths]
+    width, pages, tokens = max(need), sum(need), sum(rows)
+    order = rng.permutation(pages)
+    table = np.full((len(rows), width), -1, np.int32)
+    for b in range(len(rows)):
+        table[b, :need[b]] = order[sum(need[:b]):sum(need[:b + 1])]
+    cache = ref.Cache(pages, kv, dim, dim, page)
+    # Random codes and finite scales of every size.
+    cache.bytes[:] = rng.integers(0, 256, cache.bytes.shape, np.uint8)
+    words = cache.bytes[..., page * dim:].copy().view(np.uint16).reshape(pages, kv, -1, 2)
+    words[..., 0] = (rng.random(words.shape[:-1]) * 0.3 + 0.02).astype(np.float16).view(np.uint16)
+    words[..., 1] = rng.integers(0, 16, words.shape[:-1])
+    cache.bytes[..., page * dim:] = words.reshape(pages, kv, -1).view(np.uint8)
+    q = ref.rounded(rng.normal(size=(tokens, heads, dim)), dtype)
+    starts = np.concatenate([[0], np.cumsum(rows)]).astype(np.int32)
+    want, _, mass, top, reach = ref.attend(q, cache, table, starts, np.array(lengths))
+    # With any codes a step may be as large as the largest |v| and |k| themselves, not a seventh of them.
+    tol = ref.attention_tolerance(want, mass, 7 * top, 7 * reach, max(lengths), dim, dtype)
+    ex = executor("lower_cache4_attention", dtype=dtype, heads=heads, kv_heads=kv, head_dim=dim, group=dim, page=page)
+    out = dev(np.zeros(q.size, np.uint16))
+    held = [dev(ref.stored(q, dtype)), dev(cache.bytes), dev(table), dev(starts), dev(np.array(lengths, np.int32))]
+    size = ex.workspace_bytes(tokens, len(rows), width, pages)
+    strides = (heads * dim, dim, heads * dim, dim)
+
+    def launch(stream, ws, how="launch"):
+        getattr(ex, how)(*held, out, ws, tokens, len(rows), width, pages, *strides, 0, size, stream=stream)
+
+    return launch, out, want, tol, size, q.shape, ex
+
+
+def close(out, want, tol, dtype="Bf16"):
+    got = ref.loaded(out.download(np.uint16, want.size), dtype).reshape(want.shape)
+    return bool((np.abs(got - want) <= tol).all())
+
+
+def test_streams_graphs_and_workspaces(hip_device):
+    """A step captured into a graph and replayed between eager work, two graphs with workspaces of their own replayed
+    at once on two streams, and the launches that take no allocation or are timed: each gives the eager bits."""
+    L = _lib.lib()
+    steps = [small_step(seed=s, lengths=n) for s, n in ((0, (700, 33, 1200)), (1, (2048, 1, 3000)))]
+    raw = []
+    for launch, out, want, tol, size, shape, ex in steps:
+        assert size > 0
+        launch(0, u.DeviceBuffer(size))
+        u.synchronize()
+        assert ex.last_launch()["shared"] and ex.last_launch()["entry"].endswith("_join")
+        assert close(out, want, tol)
+        raw.append(out.download(np.uint16, want.size))
+        launch(0, u.DeviceBuffer(size), "launch_static")
+        a, b = u.Event(), u.Event()
+        ex.set_timing(a, b)
+        launch(0, u.DeviceBuffer(size))
+        u.synchronize()
+        assert 0 < a.elapsed_ms(b) < 1000
+        ex.set_timing(None, None)
+        assert np.array_equal(out.download(np.uint16, want.size), raw[-1])
+    workspaces, streams, graphs = [u.DeviceBuffer(s[4]) for s in steps], [], []
+    for (launch, *_), ws in zip(steps, workspaces):
+        st, graph, exe = C.c_void_p(), C.c_void_p(), C.c_void_p()
+        assert L.hipStreamCreate(C.byref(st)) == 0
+        assert L.hipStreamBeginCapture(st, 0) == 0
+        launch(st.value, ws)
+        assert L.hipStreamEndCapture(st, C.byref(graph)) == 0
+        assert L.hipGraphInstantiate(C.byref(exe), graph, None, None, C.c_size_t(0)) == 0
+        streams.append(st)
+        graphs.append((graph, exe))
+    spare = u.DeviceBuffer(steps[0][4])
+    for turn in range(4):
+        for (_, out, *_), ws in zip(steps, workspaces):
+            out.fill(0)
+            ws.fill(0xFF)
+        u.synchronize()
+        for _ in range(3):
+            for (_, exe), st in zip(graphs, streams):
+                assert L.hipGraphLaunch(exe, st) == 0
+        u.synchronize()
+        for (_, out, want, *_), r in zip(steps, raw):
+            assert np.array_equal(out.download(np.uint16, want.size), r), turn
+        steps[0][0](0, spare)  # eager work between the replays
+        u.synchronize()
+    # The same two eagerly, on their streams at once.
+    for (launch, out, *_), ws, st in zip(steps, workspaces, streams):
+        out.fill(0)
+        u.synchronize()
+        launch(st.value, ws)
+    u.synchronize()
+    for (_, out, want, *_), r in zip(steps, raw):
+        assert np.array_equal(out.download(np.uint16, want.size), r)
+    for graph, exe in graphs:
+        assert L.hipGraphExecDestroy(exe) == 0 and L.hipGraphDestroy(graph) == 0
+    for st in streams:
+        assert L.hipStreamDestroy(st) == 0
+
+
+def test_pages_past_four_gigabytes(hip_device):
+    """Slots and pages whose byte offsets need more than 32 bits: appended, read back and attended."""
+    form = dict(dtype="Bf16", kv_heads=2, head_dim=64, group=64, page=16)
+    each = u.cache4_page_bytes(**form)
+    pages = (5 << 30) // each
+    cache = u.DeviceBuffer(pages * each)
+    rng = np.random.default_rng(0)
+    y = ref.rounded(rng.normal(size=(20, 2, 64)), "Bf16")
+    far = [pages - 1, pages // 2]
+    slots = np.array([far[t // 16] * 16 + t % 16 for t in range(20)], np.int64)
+    sb, yb, ko, vo = dev(slots), dev(ref.stored(y, "Bf16")), dev(np.zeros(y.size, np.uint16)), dev(np.zeros(y.size, np.uint16))
+    run(executor("lower_cache4_append", **form, rot=0, index_dtype="I64"), yb, yb, sb, cache, 20, pages, 128, 64, 128, 64)
+    run(executor("lower_cache4_read", **form, index_dtype="I64"), sb, cache, ko, vo, 20, pages, 128, 64, 128, 64)
+    want = ref.Cache(2, 2, 64, 64, 16)
+    for t in range(20):
+        for h in range(2):
+            want.put(t, h, y[t, h], False)
+            want.put(t, h, y[t, h], True)
+    expect = np.array([want.get(t, True) for t in range(20)])
+    for out in (ko, vo):
+        assert np.array_equal(out.download(np.uint16, y.size), ref.stored(expect, "Bf16").ravel())
+    q = ref.rounded(rng.normal(size=(1, 4, 64)), "Bf16")
+    out = dev(np.zeros(256, np.uint16))
+    ex = executor("lower_cache4_attention", **form, heads=4)
+    run(ex, dev(ref.stored(q, "Bf16")), cache, dev(np.array([far], np.int32)), dev(np.array([0, 1], np.int32)),
+        dev(np.array([20], np.int32)), out, dev(np.zeros(16, np.uint8)), 1, 1, 2, pages, 256, 64, 256, 64, 0, 0)
+    o, _, mass, top, reach = ref.attend(q, want, np.array([[0, 1]]), [0, 1], [20])
+    assert close(out, o, ref.attention_tolerance(o, mass, top, reach, 20, 64, "Bf16"))
+
+
+def test_indexes_of_any_value(hip_device):
+    """Positions, slots, lengths and starts at the ends of their types leave what they do not name as it was."""
+    ends = np.array([np.iinfo(np.int64).min, np.iinfo(np.int64).max, -1, 0, 1 << 40, -(1 << 40)], np.int64)
+    x = ref.rounded(np.random.default_rng(0).normal(size=(6, 1, 64)), "Bf16")
+    xb, out, tab = dev(ref.stored(x, "Bf16")), dev(np.full(6 * 64, 0x3333, np.uint16)), dev(ref.table(64, 0, 8).astype(np.float32))
+    for first, row in ((0, 3), (np.iinfo(np.int64).max >> 11, -1)):  # position 0 only, or none
+        out.upload(np.full(6 * 64, 0x3333, np.uint16))
+        run(executor("lower_rope", dtype="Bf16", head_dim=64, index_dtype="I64"), xb, dev(ends), tab, out, 6, 1, 64, 64, 64, 64,
+            int(first), 8)
+        got = out.download(np.uint16, 6 * 64).reshape(6, 64)
+        for t in range(6):
+            assert np.array_equal(got[t], ref.stored(x[t, 0], "Bf16") if t == row else np.full(64, 0x3333, np.uint16))
+    form = dict(dtype="Bf16", kv_heads=1, head_dim=64, group=64, page=16)
+    size = u.cache4_page_bytes(**form)
+    cache = dev(np.full(2 * size, 0x77, np.uint8))
+    slots = np.array([ends[0], ends[1], -1, 3, 32, 31], np.int64)
+    run(executor("lower_cache4_append", **form, rot=64, index_dtype="I64"), xb, xb, dev(slots), cache, dev(ends), tab, 6, 2, 64,
+        64, 64, 64, 0, 8)
+    got = cache.download(np.uint8, 2 * size)
+    want = ref.Cache(2, 1, 64, 64, 16, fill=0x77)
+    for value in (False, True):
+        want.put(3, 0, x[3, 0], value)
+    assert np.array_equal(got, want.bytes.ravel())
+    # Lengths below zero and past the table, starts past the rows: the first sequence's row is the reference's, the
+    # others see all of the table's keys or none, and rows behind the last are left.
+    q = ref.rounded(np.random.default_rng(1).normal(size=(5, 2, 64)), "Bf16")
+    rng = np.random.default_rng(2)
+    full = filled(rng, 2, 1, 64, 64, 16, "Bf16", range(32))
+    table = np.array([[0, 1]] * 4, np.int32)
+    starts, lengths = np.array([0, 1, 2, 3, 4], np.int32), np.array([20, -7, np.iinfo(np.int32).max, np.iinfo(np.int32).min], np.int32)
+    ob = dev(np.full(5 * 128, 0x3333, np.uint16))
+    ex = executor("lower_cache4_attention", **form, heads=2)
+    args = [dev(ref.stored(q, "Bf16")), dev(full.bytes), dev(table), None, None, ob, dev(np.zeros(16, np.uint8)), 5, 4, 2, 2, 128, 64,
+            128, 64, 0, 0]
+    args[3], args[4] = dev(starts), dev(lengths)
+    run(ex, *args)
+    got = ob.download(np.uint16, 5 * 128).reshape(5, 2, 64)
+    o, _, mass, top, reach = ref.attend(q, full, table, starts, [20, 0, 33, 0])
+    tol = ref.attention_tolerance(o, mass, top, reach, 32, 64, "Bf16")
+    for t in (0, 2):
+        assert (np.abs(ref.loaded(got[t], "Bf16") - o[t]) <= tol[t]).all()
+    assert (got[[1, 3]] == 0).all() and (got[4] == 0x3333).all()
+    for wrong in ([0, 9, 9, 9, 9], [5, 3, 1, 0, 0], [-4, -2, 7, 2, 1 << 30], [np.iinfo(np.int32).min] * 2 + [np.iinfo(np.int32).max] * 3):
+        args[3] = dev(np.array(wrong, np.int32))
+        run(ex, *args)  # every access stays inside: the rows are those of 0 .. 4 only
+
+
+def test_attention_limits_refuse(hip_device):
+    ex = executor("lower_cache4_attention", dtype="Bf16", heads=4, kv_heads=2, head_dim=64, group=64, page=16)
+    for shape in ((1, 1, (1 << 26) + 1, 1), ((1 << 29) + 1, 1, 1, 1), (1, 1 << 31, 1, 1)):
+        with pytest.raises(u.UnpError) as e:
+            ex.workspace_bytes(*shape)
+        assert e.value.kind == "InvalidArgument"
+    assert ex.workspace_bytes(0, 5, 5, 5) == 0 and ex.workspace_bytes(5, 0, 5, 5) == 0

@@ -449,10 +449,10 @@ class DeviceBuffer:
 
 
 class _ArgWords(dict):
-    """The packer of n unp_args (native little-endian words), made on first use."""
+    """The packer of n unp_args (native little-endian words, the values signed), made on first use."""
 
     def __missing__(self, n: int):
-        self[n] = struct.Struct(f"{2 * n}Q").pack
+        self[n] = struct.Struct(n * "qq").pack
         return self[n]
 
 
@@ -497,9 +497,18 @@ class Executor:
         # A unp_arg as two words: is_buffer (its low half; the pad is 0), then the value.
         words = []
         for a in args:
-            words += (1, a.ptr) if isinstance(a, DeviceBuffer) else (0, int(a) & 0xFFFFFFFFFFFFFFFF)
+            if a.__class__ is int:
+                words += (0, a)
+            elif isinstance(a, DeviceBuffer):
+                words += (1, a.ptr)
+            else:
+                words += (0, int(a))
         err = _CALL_ERRORS[get_ident()]
-        rc = self._launch(self._h, _ARG_WORDS[len(args)](*words), len(args), stream, err)
+        try:
+            packed = _ARG_WORDS[len(args)](*words)
+        except struct.error:  # a value past 63 bits: its low 64 as they are
+            packed = _ARG_WORDS[len(args)](*[(w + (1 << 63)) % (1 << 64) - (1 << 63) for w in words])
+        rc = self._launch(self._h, packed, len(args), stream, err)
         if rc:
             check(rc, err._obj)
 

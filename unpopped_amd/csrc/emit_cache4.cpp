@@ -303,8 +303,21 @@ int32_t lower_cache4_attention(const unp_cache4& c, const unp_attention& a, Lowe
         << ", " << wk << ">(q, cache, table, starts, lengths, out, lse, ws, scale, a);\n}\n";
   };
   const int gq = a.heads / c.kv_heads;
-  add("_few", 1, gq <= 4 ? 4 : gq <= 8 ? 2 : 1, 1, 8, 2);
-  add("_many", 2, 1, 4, 1, c.head_dim <= 128 ? 2 : 1);
+  // What a wave holds, in registers: the words of a step, the rows, their sums and the words of groups.  The kernels
+  // take about 60 more, and two waves of a SIMD have 256 each (a SIMD's one wave of twice the rows took 646 us for
+  // prompts that two take 380 for).
+  const int deep = c.head_dim / 32, groups = c.head_dim / c.group, words = c.group / 8, rest = words % 16;
+  const int tiles = groups * (words / 16 + (rest > 0));
+  const int products = groups * (words / 16 * 8 + (rest == 0 ? 0 : rest <= 4 ? 2 : rest <= 8 ? 4 : 8));
+  auto held = [&](int cg, int qt) {
+    return 2 * cg * (deep + 4 * tiles) + qt * (4 * deep + 4 * products + (cg == 1 ? 8 * groups : 0)) + 16 * groups;
+  };
+  // As many groups of columns as leave room for a row each, as far as they fit; two row tiles a wave if they fit.
+  int cg = gq <= 4 ? 4 : gq <= 8 ? 2 : 1;
+  while (cg > 1 && held(cg, 1) > 176) cg /= 2;
+  add("_few", 1, cg, 1, 4, held(cg, 1) <= 204 ? 2 : 1);
+  const int qt = held(1, 2) <= 204 ? 2 : 1;
+  add("_many", qt, 1, 4, 1, held(1, qt) <= 204 ? 2 : 1);
   Entry e;
   e.symbol = L.name + "_join";
   L.entries.push_back(e);

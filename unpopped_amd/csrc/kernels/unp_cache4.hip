@@ -168,8 +168,8 @@ UNP4_DEV void rope(const T* x, const I* positions, const float* table, T* out, c
       rest -= per;
       if (++token >= a.tokens) break;
     }
-    const i64 row = (i64)positions[token] - a.first;
-    if (row < 0 || row >= a.rows) continue;
+    const i64 row = (i64)((u64)(i64)positions[token] - (u64)a.first);  // any position, without overflow
+    if ((u64)row >= (u64)a.rows) continue;
     const int head = (int)((u32)rest / (u32)a.units), unit = (int)rest - head * a.units;
     const T* xp = x + token * a.x_token + head * a.x_head;
     T* op = out + token * a.out_token + head * a.out_head;
@@ -314,8 +314,8 @@ UNP4_DEV void append(const T* k, const T* v, const I* slots, u32* cache, const I
     if (live) load8<T, ALIGNED>(p + 8 * w, x);
     if (LAYOUT == HALVES && turns) load8<T, ALIGNED>(p + (second ? i0 : i0 + ROT / 2), o);
     const i64 slot = (i64)slots[it.token];
-    const i64 row = ROT > 0 ? (i64)positions[it.token] - a.first : 0;
-    if (slot < 0 || slot >= a.slots || (ROT > 0 && (row < 0 || row >= a.rows))) continue;
+    const i64 row = ROT > 0 ? (i64)((u64)(i64)positions[it.token] - (u64)a.first) : 0;  // any position, without overflow
+    if ((u64)slot >= (u64)a.slots || (ROT > 0 && (u64)row >= (u64)a.rows)) continue;
     float y[8];
     float lo = 0.0f, hi = 0.0f, not_finite = 0.0f;
     if (live) {
@@ -502,6 +502,10 @@ UNP4_DEV tile tile_of(const i32* starts, const i32* lengths, const attention_arg
     hi = lo + step < hi ? lo + step : hi;
   }
 }
+
+template <int N> struct size {
+  static constexpr int value = N;
+};
 
 // N adjacent elements of a row from their sums.
 template <class T, int N> UNP4_DEV void put(T* p, const float (&o)[N], float by, bool wide) {
@@ -1017,15 +1021,22 @@ template <class T, int H, int QH, int D, int GROUP, int P, bool CAUSAL, bool LSE
     }
   }
 
-  // f(t, r, d): every run of nibbles(t) adjacent elements d .. of the lane's columns.
+  // f(size<N>, t, r, d): every run of N adjacent elements d .. of the lane's columns.
+  template <int N, class F> UNP4_DEV void runs(int t, F f) const {
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int d = t % TG * 128 + (g * 4 + r) * N;
+      if (t % TG * 128 + 16 * N <= GROUP || d < GROUP) f(size<N>{}, t, r, t / TG * GROUP + d);
+    }
+  }
   template <class F> UNP4_DEV void each(F f) const {
 #pragma unroll
-    for (int t = 0; t < NT; ++t)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int n = nibbles(t), d = t % TG * 128 + (g * 4 + r) * n;
-        if (t % TG * 128 + 16 * n <= GROUP || d < GROUP) f(t, r, t / TG * GROUP + d);
-      }
+    for (int t = 0; t < NT; ++t) {
+      if constexpr (FULL > 0)
+        if (t % TG < FULL) runs<8>(t, f);
+      if constexpr (REST > 0)
+        if (t % TG >= FULL) runs<NREST>(t, f);
+    }
   }
 };
 
@@ -1098,9 +1109,9 @@ UNP4_DEV void attend(const T* q, const u32* cache, const i32* table, const i32* 
       stat[mine][r0][0] = w.m[0] * w.factor[0];
       stat[mine][r0][1] = w.l[0][0];
     }
-    w.each([&](int tl, int r, int d) {
+    w.each([&](auto n, int tl, int r, int d) {
 #pragma unroll
-      for (int e = 0; e < A::nibbles(tl); ++e) sums[mine][r0][d + e] = w.sum_of(0, tl, e, r);
+      for (int e = 0; e < decltype(n)::value; ++e) sums[mine][r0][d + e] = w.sum_of(0, tl, e, r);
     });
     __syncthreads();
     const int n = all_rows - first_row < A::ROWS ? all_rows - first_row : A::ROWS;

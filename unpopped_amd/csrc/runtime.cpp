@@ -565,7 +565,7 @@ int32_t unp_hip_exec_create(const unp_generated* g, unp_exec** out, unp_error* e
     }
     x->fns.push_back(f);
     int per_cu = 0;
-    if (x->l.form.kind == UNP_FORM_ROW_REDUCE &&
+    if ((x->l.form.kind == UNP_FORM_ROW_REDUCE || x->l.form.kind == UNP_FORM_CACHE4_ATTENTION) &&
         hipModuleOccupancyMaxActiveBlocksPerMultiprocessor(&per_cu, f, en.threads > 0 ? en.threads : x->l.threads, 0) !=
             hipSuccess)
       per_cu = 0;
@@ -677,6 +677,8 @@ int32_t take_args(const unp_arg* a, size_t n, size_t nbuf, size_t nscal, Args& o
                   std::to_string(n) + " arguments");
     return UNP_INVALID_ARGUMENT;
   }
+  out.buf.reserve(nbuf);
+  out.ext.reserve(nscal);
   for (size_t i = 0; i < n; ++i) {
     const bool want_buf = i < nbuf;
     if ((a[i].is_buffer != 0) != want_buf) {
@@ -2041,10 +2043,14 @@ int32_t run_cache4_read(unp_exec* x, const unp_arg* a, size_t n, hipStream_t s, 
   return launch(x, fast ? 0 : 1, cache_grid(x, args.tokens), params, s, err);
 }
 
-int32_t check_attention(int64_t tokens, int64_t batch, int64_t width, int64_t pages, unp_error* err) {
+int32_t check_attention(const unp_exec* x, int64_t tokens, int64_t batch, int64_t width, int64_t pages, unp_error* err) {
   const int64_t most = 0x7FFFFFFFLL;
   if (tokens < 0 || tokens > most || batch < 0 || batch > most || width < 0 || width > most || pages < 0 || pages > most)
     return invalid(err, "tokens, batch, width and pages are 0..2^31 - 1");
+  // The kernels count keys and rows of a sequence in 32 bits.
+  if (width * x->l.cache4.page > (1LL << 30)) return invalid(err, "width: a context of more than 2^30 keys");
+  if (tokens * x->l.attention.heads > (1LL << 30) * x->l.cache4.kv_heads)
+    return invalid(err, "tokens: more than 2^30 rows of a key/value head");
   return UNP_OK;
 }
 
@@ -2072,17 +2078,22 @@ AttentionPlan attention_plan(const unp_exec* x, int64_t tokens, int64_t batch, i
     p.slots = tokens;
     p.by_token = true;
   }
-  // As many parts as give every CU two blocks, none shorter than two of a block's steps; with the whole context's pages as its length, which the host does not know.
-  const int64_t blocks = p.slots * c.kv_heads, want = (2LL * x->cu_count + blocks - 1) / blocks;
-  const int64_t most = (width * c.page + 2 * e.k - 1) / (2 * e.k);
-  p.splits = std::max<int64_t>(1, std::min({want, most, kMostParts}));
+  // As many parts as fill the CUs with the blocks that they hold at once, none shorter than a step of waves that share
+  // their rows (where no block would be without a CU, none at all) or 128 keys of others, and none of a context that two
+  // such parts would hold: the join costs as much.  The context is its pages' length, as the host knows no other.
+  const int64_t hold = (int64_t)x->cu_count * std::max(1, x->resident[p.entry]), keys = width * c.page;
+  // About the tiles that have rows: a sequence fills its last one by half.
+  const int64_t blocks = p.by_token ? p.slots * c.kv_heads : ((tokens * group + e.vec - 1) / e.vec + (batch - 1) / 2) * c.kv_heads;
+  const int64_t least = p.entry == 0 ? e.k : 128;
+  const int64_t want = p.entry != 0 ? (hold + blocks / 2) / blocks : blocks >= x->cu_count ? 1 : hold / blocks;
+  if (keys > 2 * least) p.splits = std::max<int64_t>(1, std::min({want, (keys + least - 1) / least, kMostParts}));
   return p;
 }
 
 int32_t attention_workspace(const unp_exec* x, const int64_t* sc, size_t n, uint64_t& bytes, unp_error* err) {
   if (x->l.form.kind != UNP_FORM_CACHE4_ATTENTION) return invalid(err, "only a cache attention takes a workspace");
   if (n != 4) return invalid(err, "expected tokens, batch, width and pages");
-  const int32_t rc = check_attention(sc[0], sc[1], sc[2], sc[3], err);
+  const int32_t rc = check_attention(x, sc[0], sc[1], sc[2], sc[3], err);
   bytes = 0;
   if (rc != UNP_OK || sc[0] == 0 || sc[1] == 0) return rc;
   const AttentionPlan p = attention_plan(x, sc[0], sc[1], sc[3] > 0 ? sc[2] : 0);
@@ -2098,7 +2109,7 @@ int32_t run_cache4_attention(unp_exec* x, const unp_arg* a, size_t n, hipStream_
   int32_t rc = take_args(a, n, nb, 10, A, err);
   if (rc != UNP_OK) return rc;
   const int64_t tokens = A.ext[0], batch = A.ext[1];
-  if ((rc = check_attention(tokens, batch, A.ext[2], A.ext[3], err)) != UNP_OK) return rc;
+  if ((rc = check_attention(x, tokens, batch, A.ext[2], A.ext[3], err)) != UNP_OK) return rc;
   if ((rc = check_heads("q", tokens, A.ext[4], at.heads, A.ext[5], c.head_dim, false, err)) != UNP_OK) return rc;
   if ((rc = check_heads("out", tokens, A.ext[6], at.heads, A.ext[7], c.head_dim, true, err)) != UNP_OK) return rc;
   if (A.ext[8] < 0) return invalid(err, "the window is negative");
