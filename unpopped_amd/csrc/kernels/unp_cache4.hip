@@ -428,7 +428,7 @@ UNP4_DEV void read(const I* slots, const u32* cache, T* k, T* v, const cache_arg
 //     only when some score passes the running one by 2^4.9: p is held as 2^11 p in f16, which ends at 2^16
 //     (moving at 2^0.9, with 2^15 p, cost a prompt 8%: the sums are multiplied anew each time).
 //   * O' += V' P' with the value words as rows, again nibbles as they lie: sum p s (n - zero) is the product of n with
-//     p s less the sum of p s zero.  p s is rounded once to f16 (both sums take it as rounded), s relative to a
+//     p s less the sum of p s zero.  p s is rounded to f16 (both sums take it as rounded), s relative to a
 //     running power of two that no scale of the column exceeded, so that it stays in f16's range whatever s is.  The
 //     scores are, lane by lane, the operand that this product needs when its key (g, i) of 4 x 8 is key
 //     16 CG (i / 4) + 4 g + i % 4; a lane reads four tokens' words of 8 elements at once and pairs of tokens of one
@@ -544,6 +544,13 @@ UNP4_DEV float log_sum(float top, float l) {
   return l == 0.0f ? -__builtin_inff() : (top - kHold + __log2f(l)) * 0.693147180559945309f;
 }
 
+template <class T> struct is_half {
+  static constexpr bool value = false;
+};
+template <> struct is_half<_Float16> {
+  static constexpr bool value = true;
+};
+
 template <class T, int H, int QH, int D, int GROUP, int P, bool CAUSAL, bool LSE, int QT, int CG> struct attention {
   static_assert(QT == 1 || CG == 1, "columns are shared by one row tile");
   typedef record<D, GROUP, P> R;
@@ -571,12 +578,15 @@ template <class T, int H, int QH, int D, int GROUP, int P, bool CAUSAL, bool LSE
   f16x8 q[QT][KJ];
   float qsum[QT][G], factor[QT];  // of this lane's column; qsum 2^24 times, as zeros are held; factor: raw scores to log2
   float m[QT];                    // running maximum
-  f32x4 l[QT];                    // the sum of p, in l[0] (with LSE this lane's part of it until the end)
+  f32x4 l[QT];                    // the sum of p, in l[0] (EXACT_SUM: this lane's part of it until the end)
   _Float16 unit;                  // a power of two: value scales times it are at most 1
   f32x4 o[QT][NE];
   // The sums of p s zero by group: this lane's parts, or (one group of columns, few of elements) a product whose rows
   // are all the same.
   static constexpr bool ZERO_PRODUCT = CG == 1 && G <= 2;
+  // F16 outputs: p s is rounded once (bf16's rounding hides that p and then p s are), and the sum of p is of what was not
+  // rounded, as the log-sum-exp's is; otherwise it is a product with ones, of p as rounded.
+  static constexpr bool FINE = is_half<T>::value, EXACT_SUM = LSE || FINE;
   float zs[QT][G];
   f32x4 zp[QT][ZERO_PRODUCT ? G : 1];
   int end[QT], begin[QT];  // keys that the column sees
@@ -898,21 +908,23 @@ template <class T, int H, int QH, int D, int GROUP, int P, bool CAUSAL, bool LSE
 #pragma unroll
     for (int x = 0; x < QT; ++x) {
       const float off = m[x] == -__builtin_inff() ? 0.0f : fmaf(-m[x], factor[x], kHold);
-      f16x8 e;
+      f16x8 e, fine[G];
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         const float y = __builtin_amdgcn_exp2f(fmaf(sc[x][i], factor[x], off));
-        if (LSE) l[x][0] += y;
+        if (EXACT_SUM) l[x][0] += y;
         e[i] = (_Float16)y;
+        if (FINE)
+#pragma unroll
+          for (int gi = 0; gi < G; ++gi) fine[gi][i] = (_Float16)fmaf(y, (float)vs[gi][i / 2][i % 2], 0.0f);
       }
-      // Where nobody asks for it, the sum of p is a product with ones, of p as rounded; the log-sum-exp takes the
-      // sum of what was not rounded.
-      if (!LSE) l[x] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, e, l[x], 0, 0, 0);
+      if (!EXACT_SUM) l[x] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, e, l[x], 0, 0, 0);
 #pragma unroll
       for (int gi = 0; gi < G; ++gi) {
 #pragma unroll
         for (int k = 0; k < 4; ++k)
-          p[x][gi][k] = __builtin_bit_cast(u32, f16x2{e[2 * k], e[2 * k + 1]} * vs[gi][k]);
+          p[x][gi][k] = __builtin_bit_cast(u32, FINE ? f16x2{fine[gi][2 * k], fine[gi][2 * k + 1]}
+                                                     : f16x2{e[2 * k], e[2 * k + 1]} * vs[gi][k]);
         if (masked) {  // a scale that is no number does not reach the columns that do not see its key
           asm volatile("; a branch: not worth computing for every step");
 #pragma unroll
@@ -969,7 +981,7 @@ template <class T, int H, int QH, int D, int GROUP, int P, bool CAUSAL, bool LSE
     while (s.at < s.last) step(s);
 #pragma unroll
     for (int x = 0; x < QT; ++x) {
-      if (LSE) l[x][0] = column_sum(l[x][0]);
+      if (EXACT_SUM) l[x][0] = column_sum(l[x][0]);
 #pragma unroll
       for (int gi = 0; gi < G; ++gi) zs[x][gi] = ZERO_PRODUCT ? zp[x][ZERO_PRODUCT ? gi : 0][0] : column_sum(zs[x][gi]);
     }

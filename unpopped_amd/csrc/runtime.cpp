@@ -2079,14 +2079,14 @@ AttentionPlan attention_plan(const unp_exec* x, int64_t tokens, int64_t batch, i
     p.by_token = true;
   }
   // As many parts as fill the CUs with the blocks that they hold at once, none shorter than a step of waves that share
-  // their rows (where no block would be without a CU, none at all) or 128 keys of others, and none of a context that two
+  // their rows (where no block would be without a CU, none at all) or 128 keys of others, and none of a context that four
   // such parts would hold: the join costs as much.  The context is its pages' length, as the host knows no other.
   const int64_t hold = (int64_t)x->cu_count * std::max(1, x->resident[p.entry]), keys = width * c.page;
   // About the tiles that have rows: a sequence fills its last one by half.
   const int64_t blocks = p.by_token ? p.slots * c.kv_heads : ((tokens * group + e.vec - 1) / e.vec + (batch - 1) / 2) * c.kv_heads;
   const int64_t least = p.entry == 0 ? e.k : 128;
   const int64_t want = p.entry != 0 ? (hold + blocks / 2) / blocks : blocks >= x->cu_count ? 1 : hold / blocks;
-  if (keys > 2 * least) p.splits = std::max<int64_t>(1, std::min({want, (keys + least - 1) / least, kMostParts}));
+  if (keys > 4 * least) p.splits = std::max<int64_t>(1, std::min({want, (keys + least - 1) / least, kMostParts}));
   return p;
 }
 
