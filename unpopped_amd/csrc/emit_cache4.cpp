@@ -316,6 +316,7 @@ int32_t lower_cache4_attention(const unp_cache4& c, const unp_attention& a, Lowe
   int cg = gq <= 4 ? 4 : gq <= 8 ? 2 : 1;
   while (cg > 1 && held(cg, 1) > 176) cg /= 2;
   add("_few", 1, cg, 1, 4, held(cg, 1) <= 204 ? 2 : 1);
+  if (cg > 1) add("_some", 1, 1, 1, 4, held(1, 1) <= 204 ? 2 : 1);
   const int qt = held(1, 2) <= 204 ? 2 : 1;
   add("_many", qt, 1, 4, 1, held(1, qt) <= 204 ? 2 : 1);
   Entry e;
@@ -325,6 +326,10 @@ int32_t lower_cache4_attention(const unp_cache4& c, const unp_attention& a, Lowe
       << "* out, float* lse, float* ws, unp4::attention_args a) {\n  unp4::join<" << same << ", " << lse
       << ">(starts, out, lse, ws, a);\n}\n";
   L.source = src.str();
+  std::vector<std::string> when = {"a sequence has no more rows of a key/value head, on average, than one of its tiles"};
+  if (cg > 1) when.push_back("at most 16 rows");
+  when.push_back("otherwise");
+  when.push_back("after any of them, where a context is split");
   const char* dt = kind_name(c.dtype);
   std::vector<Param> ps = {{"q", "Read", dt}, {"cache", "Read", "U8"}, {"page_table", "Read", "I32"},
                            {"starts", "Read", "I32"}, {"lengths", "Read", "I32"}, {"out", "Write", dt}};
@@ -336,7 +341,7 @@ int32_t lower_cache4_attention(const unp_cache4& c, const unp_attention& a, Lowe
   L.interface_json =
       interface(L, "cache4_attention", cache_fields(c) + ",\"heads\":" + std::to_string(a.heads), ps,
                 "a block per row tile, part of a context and key/value head",
-                {"at most 16 rows of a key/value head per sequence on average", "otherwise", "after either, where a context is split"},
+                when,
                 "the caller's, by unp_hip_exec_workspace",
                 "scores, softmax statistics and sums in f32, probabilities and values as f16 in the products; each output rounded once");
   return UNP_OK;

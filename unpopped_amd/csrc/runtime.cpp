@@ -2070,8 +2070,10 @@ AttentionPlan attention_plan(const unp_exec* x, int64_t tokens, int64_t batch, i
   const unp_cache4& c = x->l.cache4;
   const int64_t group = x->l.attention.heads / c.kv_heads;
   AttentionPlan p;
-  // Waves that share their rows where sequences have 16 or fewer, waves of rows of their own beyond.
-  p.entry = tokens * group <= 16 * batch ? 0 : 1;
+  // The first entry whose tile holds a sequence's rows, of those whose waves share them; beyond 16, waves of rows of
+  // their own.  The last entry joins.
+  const size_t own = x->l.entries.size() - 2;
+  while (p.entry < own && tokens * group > x->l.entries[p.entry].vec * batch) ++p.entry;
   const unp::Entry& e = x->l.entries[p.entry];
   p.slots = tokens * group / e.vec + batch;
   if (group <= e.vec && tokens <= p.slots) {
@@ -2084,8 +2086,8 @@ AttentionPlan attention_plan(const unp_exec* x, int64_t tokens, int64_t batch, i
   const int64_t hold = (int64_t)x->cu_count * std::max(1, x->resident[p.entry]), keys = width * c.page;
   // About the tiles that have rows: a sequence fills its last one by half.
   const int64_t blocks = p.by_token ? p.slots * c.kv_heads : ((tokens * group + e.vec - 1) / e.vec + (batch - 1) / 2) * c.kv_heads;
-  const int64_t least = p.entry == 0 ? e.k : 128;
-  const int64_t want = p.entry != 0 ? (hold + blocks / 2) / blocks : blocks >= x->cu_count ? 1 : hold / blocks;
+  const int64_t least = p.entry < own ? e.k : 128;
+  const int64_t want = p.entry == own ? (hold + blocks / 2) / blocks : blocks >= x->cu_count ? 1 : hold / blocks;
   if (keys > 4 * least) p.splits = std::max<int64_t>(1, std::min({want, (keys + least - 1) / least, kMostParts}));
   return p;
 }
@@ -2142,7 +2144,7 @@ int32_t run_cache4_attention(unp_exec* x, const unp_arg* a, size_t n, hipStream_
   x->shared = p.splits > 1;
   if ((rc = launch(x, p.entry, (uint32_t)blocks, params, s, err)) != UNP_OK || p.splits == 1) return rc;
   void* jparams[] = {&starts, &out, &lse, &ws, &args};
-  return launch(x, 2, (uint32_t)joins, jparams, s, err);
+  return launch(x, x->l.entries.size() - 1, (uint32_t)joins, jparams, s, err);
 }
 
 }  // namespace
