@@ -441,6 +441,37 @@ def test_attention_of_small_and_large_queries(hip_device, q_scale):
         attention_case("Bf16", 4, 2, 64, 64, 16, [1, 9], [30, 29], q_scale=q_scale, seed=11)
 
 
+@pytest.mark.parametrize("rows", [1, 40])
+@pytest.mark.parametrize("q_scale", [1e8, 1e20, 1e30, 1e36])
+def test_attention_of_queries_beyond_every_exponent(hip_device, rows, q_scale):
+    """Scores of which one unit of the last place is more than exp reaches: a row is the value of its highest score."""
+    rng = np.random.default_rng(12)
+    dim, page, n = 64, 16, 40
+    cache = filled(rng, 3, 1, dim, dim, page, "Bf16", range(n))
+    q = ref.rounded(rng.normal(size=(rows, 2, dim)) * q_scale, "Bf16")
+    table, starts, lengths = np.arange(3, dtype=np.int32)[None], np.array([0, rows], np.int32), np.array([n], np.int32)
+    k = np.array([cache.get(s, False)[0] for s in range(n)])
+    v = np.array([cache.get(s, True)[0] for s in range(n)])
+    score = q.reshape(-1, dim) @ k.T / 8.0
+    first = score.argmax(-1)
+    gap = np.sort(score, -1)[:, -1] - np.sort(score, -1)[:, -2]
+    # attention_tolerance's error of a score; the others weigh nothing where they are e^-200 below.
+    err = np.abs(q.reshape(-1, dim)).sum(-1) * np.abs(k).max() / 8.0 * (30 / 7) * (dim + 4) * 2.0 ** -23
+    clear = gap > 2 * err + 200
+    assert clear.any()
+    ex = executor("lower_cache4_attention", dtype="Bf16", heads=2, kv_heads=1, head_dim=dim, group=dim, page=page, causal=False)
+    ob = dev(np.zeros(rows * 2 * dim, np.uint16))
+    run(ex, dev(ref.stored(q, "Bf16")), dev(cache.bytes), dev(table), dev(starts), dev(lengths), ob,
+        dev(np.zeros(16, np.uint8)), rows, 1, 3, 3, 2 * dim, dim, 2 * dim, dim, 0, 0)
+    got = ref.loaded(ob.download(np.uint16, rows * 2 * dim), "Bf16").reshape(-1, dim)
+    want, top = v[first], np.abs(v).max()
+    # A value rounded twice to 11 bits and once to its type, and sums of codes and zeros as in attention_tolerance.
+    off = np.abs(want) * 2 * 2.0 ** -11 + top * (n * 2.0 ** -35 + 30 / 7 * (n + 8) * 2.0 ** -23)
+    off += (np.abs(want) + off) * 2.0 ** -8
+    assert (np.abs(got - want) <= off)[clear].all()
+    assert (np.abs(got) <= top * 1.01).all()  # of the others: some mean of the values
+
+
 def test_attention_keeps_what_no_row_sees_out(hip_device):
     """A value that is no number reaches the rows that see its key, and no other row of the same call."""
     rng = np.random.default_rng(6)

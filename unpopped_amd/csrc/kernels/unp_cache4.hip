@@ -444,6 +444,10 @@ struct attention_args {
 };
 
 constexpr float kHold = 11.0f, kSlack = 4.9f;
+// exp2((score - maximum) factor + kHold) is one product and sum with the rounded maximum * factor - kHold, off by up to
+// 2^-25 of it in log2: below 2^12 that is 2^-13, past 2^21 it would pass f16's end.  Beyond kFar the maximum is subtracted first,
+// for an operation more a score.
+constexpr float kFar = 0x1p12f;
 
 // The maximum and the sum over the four lanes of a column (lane, lane ^ 16, lane ^ 32, lane ^ 48).
 UNP4_DEV float column_max(float x) {
@@ -607,6 +611,7 @@ template <class T, int H, int QH, int D, int GROUP, int P, bool CAUSAL, bool LSE
   f16x8 q[QT][KJ];
   float qsum[QT][G], factor[QT];  // of this lane's column; qsum 2^24 times, as zeros are held; factor: raw scores to log2
   float m[QT];                    // running maximum
+  bool far;                       // some maximum is beyond 2^kFar in log2 (all lanes agree)
   f32x4 l[QT];                    // the sum of p, in l[0] (EXACT_SUM: this lane's part of it until the end)
   _Float16 unit;                  // a power of two: value scales times it are at most 1
   f32x4 o[QT][NE];
@@ -625,6 +630,7 @@ template <class T, int H, int QH, int D, int GROUP, int P, bool CAUSAL, bool LSE
     asm("s_mov_b32 %0, 0x000f000f" : "=s"(mask0));
     asm("s_mov_b32 %0, 0x00f000f0" : "=s"(mask1));
     unit = (_Float16)0x1p15f;
+    far = false;
 #pragma unroll
     for (int x = 0; x < QT; ++x) {
       const int r = first + x * 16 + c % ROWS;
@@ -651,7 +657,7 @@ template <class T, int H, int QH, int D, int GROUP, int P, bool CAUSAL, bool LSE
       // The power of two that puts the largest element into 2^13 .. 2^14: odd nibbles weigh 16 times as much, so
       // their elements are scaled down by 16.
       int up = top > 0.0f && top < __builtin_inff() ? 13 - (int)((__builtin_bit_cast(u32, top) >> 23) & 255) + 127 : 0;
-      up = up > 100 ? 100 : up < -100 ? -100 : up;
+      up = up > 100 ? 100 : up;  // at least -114
       const float mul = __builtin_bit_cast(float, (u32)(up + 127) << 23);
 #pragma unroll
       for (int gi = 0; gi < G; ++gi) qsum[x][gi] = 0.0f;
@@ -667,6 +673,7 @@ template <class T, int H, int QH, int D, int GROUP, int P, bool CAUSAL, bool LSE
       }
 #pragma unroll
       for (int gi = 0; gi < G; ++gi) qsum[x][gi] = column_sum(qsum[x][gi]);
+      // Where this ends at 2^127, two scores that differ at all are further apart than exp reaches either way.
       factor[x] = fminf(scale * 1.4426950408889634f * 0x1p24f * __builtin_bit_cast(float, (u32)(127 - up) << 23), 0x1p127f);
       m[x] = -__builtin_inff();
       l[x] = f32x4{0, 0, 0, 0};
@@ -906,11 +913,13 @@ template <class T, int H, int QH, int D, int GROUP, int P, bool CAUSAL, bool LSE
       const float to = all * old > 1.0f ? __builtin_bit_cast(float, (253u << 23) - (__builtin_bit_cast(u32, all) & 0x7F800000u)) : old;
       const float by = to / old;
       unit = (_Float16)to;
+      bool beyond = false;
 #pragma unroll
       for (int x = 0; x < QT; ++x) {
         const float next = fmaxf(m[x], column_max(top[x]));
         const float keep = m[x] == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f((m[x] - next) * factor[x]);
         m[x] = next;
+        beyond |= next != -__builtin_inff() && !(fabsf(next * factor[x]) <= kFar);
         l[x] *= keep;
 #pragma unroll
         for (int gi = 0; gi < G; ++gi) {
@@ -922,6 +931,14 @@ template <class T, int H, int QH, int D, int GROUP, int P, bool CAUSAL, bool LSE
 #pragma unroll
         for (int e = 0; e < NE; ++e) o[x][e] *= keep * by;
       }
+      far = __any(beyond);
+    }
+    if (far) {
+      asm volatile("; a branch: not worth computing for every step");
+#pragma unroll
+      for (int x = 0; x < QT; ++x)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) sc[x][i] -= m[x] == -__builtin_inff() ? 0.0f : m[x];
     }
     u32x4 zero[G];
 #pragma unroll
@@ -935,7 +952,7 @@ template <class T, int H, int QH, int D, int GROUP, int P, bool CAUSAL, bool LSE
     u32x4 p[QT][G];
 #pragma unroll
     for (int x = 0; x < QT; ++x) {
-      const float off = m[x] == -__builtin_inff() ? 0.0f : fmaf(-m[x], factor[x], kHold);
+      const float off = m[x] == -__builtin_inff() ? 0.0f : far ? kHold : fmaf(-m[x], factor[x], kHold);
       f16x8 e, fine[G];
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
@@ -1016,7 +1033,7 @@ template <class T, int H, int QH, int D, int GROUP, int P, bool CAUSAL, bool LSE
   }
   // The sum of p v for element e of row g * 4 + r of tile t.
   UNP4_DEV float sum_of(int x, int t, int e, int r) const {
-  return (o[x][product(t, e)][r] * ((e & 1) ? 0x1p20f : 0x1p24f) - zs[x][t / TG] * 0x1p24f) * (1.0f / (float)unit);
+    return (o[x][product(t, e)][r] * ((e & 1) ? 0x1p20f : 0x1p24f) - zs[x][t / TG] * 0x1p24f) * (1.0f / (float)unit);
   }
 
   // Row x's elements times `by` to p, as U.  A lane's four runs of N elements of a tile lie together, so stores of one
