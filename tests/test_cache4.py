@@ -150,3 +150,21 @@ def test_a_planted_mistake_in_the_reference_shows():
     for wrong in ((args[0], args[1], np.array([41])), (np.array([[2, 1, 0]]), args[1], args[2])):
         other = ref.attend(q, c, *wrong)[0]
         assert (np.abs(other - out) > tol).mean() > 0.5
+
+
+@pytest.mark.parametrize("owner", [None, 0, object()])
+def test_held_memory_is_not_freed(monkeypatch, owner):
+    freed = []
+
+    class Lib:
+        @staticmethod
+        def unp_hip_free(p):
+            freed.append(p)
+
+    monkeypatch.setattr(u._lib, "lib", lambda: Lib)
+    b = u.DeviceBuffer.held(4096, 64, owner)
+    part = b.at(16)
+    assert (b.ptr, b.nbytes, part.ptr, part.nbytes) == (4096, 64, 4112, 48)
+    b.free()
+    del part, b
+    assert freed == []

@@ -404,9 +404,9 @@ class DeviceBuffer:
     @classmethod
     def held(cls, ptr: int, nbytes: int, owner) -> "DeviceBuffer":
         """Device memory that ``owner`` owns (a tensor of another library) as a launch argument; the
-        buffer keeps ``owner`` alive."""
+        buffer keeps ``owner`` alive (None: the caller does) and never frees the memory."""
         b = cls.__new__(cls)
-        b.nbytes, b.ptr, b._owner = int(nbytes), int(ptr), owner
+        b.nbytes, b.ptr, b._owner = int(nbytes), int(ptr), (owner,)  # never None: that is memory to free
         return b
 
     def upload(self, a: np.ndarray) -> None:
