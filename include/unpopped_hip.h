@@ -321,7 +321,8 @@ typedef struct unp_rope_table {
   double amplitude;  /* multiplies the cosines and sines */
 } unp_rope_table;
 /* Launch: table (F32 [count][rot / 2][2]: cosine, sine); first, count.  Row r holds position first + r
- * (|first| + count <= 2^52).  Angles, cosines and sines are computed in 64 bits and rounded once. */
+ * (within -2^52 .. 2^52).  The table is 8-byte aligned here, 16-byte where it is read.  Angles, cosines
+ * and sines are computed in 64 bits and rounded once. */
 int32_t unp_hip_lower_rope_table(const unp_rope_table* t, unp_generated** out, unp_error* err);
 
 enum unp_rope_layout {
@@ -392,7 +393,9 @@ typedef struct unp_attention {
  * rows are starts[b] .. starts[b + 1] - 1), lengths (I32 [batch]: its keys, its own rows' last), out, with lse
  * lse (F32 [tokens][heads], natural log; -inf for an empty row), workspace; tokens, batch, width, pages, q_token, q_head,
  * out_token, out_head (strides), window, workspace_bytes.
- *   A context is at most 2^30 keys (width * page), and so are the rows of a key/value head (tokens * heads / kv_heads).
+ *   A context is at most 2^30 keys (width * page), and so are the rows of a key/value head (tokens * heads / kv_heads);
+ *   a launch is at most 2^24 - 1 blocks (a tile of rows, of 4 to 128, and a key/value head each; up to one tile more per
+ *   sequence).  out, lse and workspace share no byte with each other or an input.
  *   window > 0 (causal only): a row sees its last `window` keys.  A row that sees no key gives 0.
  *   Keys that no row may see do not count, whatever they hold: keys past a sequence's length, keys of a page number
  *   outside the cache, keys past width pages.  Rows that no sequence names are left as they were.  starts do not

@@ -787,3 +787,11 @@ def test_attention_limits_refuse(hip_device):
             ex.workspace_bytes(*shape)
         assert e.value.kind == "InvalidArgument"
     assert ex.workspace_bytes(0, 5, 5, 5) == 0 and ex.workspace_bytes(5, 0, 5, 5) == 0
+
+
+def test_attention_of_more_blocks_than_a_launch_has_refuses(hip_device):
+    """Shapes whose blocks would pass 2^32 lanes: refused from the scalars, before anything is read."""
+    ex = executor("lower_cache4_attention", dtype="Bf16", heads=4, kv_heads=2, head_dim=64, group=64, page=16)
+    some = dev(np.zeros(64, np.uint8))
+    for tokens, batch in ((1 << 23, 1 << 23), (1 << 29, 1)):
+        invalid(ex, some, some, some, some, some, some, some, tokens, batch, 1, 1, 256, 64, 256, 64, 0, 0)

@@ -2056,6 +2056,7 @@ int32_t check_attention(const unp_exec* x, int64_t tokens, int64_t batch, int64_
 
 // A launch's shape: the entry, its row tiles, how they are numbered (tile_of) and the parts of a context.
 constexpr int64_t kMostParts = 128;  // the device's kMostParts
+constexpr int64_t kMostBlocks = 0xFFFFFF;  // of 256 lanes: a launch has less than 2^32
 struct AttentionPlan {
   size_t entry = 0;
   int64_t slots = 0, splits = 1;
@@ -2129,9 +2130,9 @@ int32_t run_cache4_attention(unp_exec* x, const unp_arg* a, size_t n, hipStream_
   AttentionPlan p = attention_plan(x, tokens, batch, keys ? A.ext[2] : 0);
   while (p.splits > 1 && parts_bytes(x, tokens, p.splits) > A.ext[9]) --p.splits;
   if (p.splits == 1 && A.buf[nb - 1] == 0) A.buf[nb - 1] = A.buf[5];  // not used
-  const int64_t blocks = p.slots * p.splits * c.kv_heads;
-  const int64_t joins = tokens * at.heads;
-  if (blocks > 0x7FFFFFFFLL || joins > 0x7FFFFFFFLL) return invalid(err, "tokens: too many rows for one launch");
+  const int64_t blocks = p.slots * p.splits * c.kv_heads;  // contexts are split where tiles are few: a join's are fewer
+  if (blocks > kMostBlocks)
+    return invalid(err, "more than 2^24 - 1 row tiles times key/value heads: " + std::to_string(blocks));
   attention_args_host args{tokens, batch, keys ? A.ext[2] : 0, A.ext[3], A.ext[4], A.ext[5], A.ext[6], A.ext[7], A.ext[8],
                            (int32_t)p.slots, (int32_t)p.splits, p.by_token ? 1 : 0,
                            whole_vectors(A.buf[0], A.ext[4], A.ext[5], 8), whole_vectors(A.buf[5], A.ext[6], A.ext[7], 8), 0};
@@ -2144,7 +2145,7 @@ int32_t run_cache4_attention(unp_exec* x, const unp_arg* a, size_t n, hipStream_
   x->shared = p.splits > 1;
   if ((rc = launch(x, p.entry, (uint32_t)blocks, params, s, err)) != UNP_OK || p.splits == 1) return rc;
   void* jparams[] = {&starts, &out, &lse, &ws, &args};
-  return launch(x, x->l.entries.size() - 1, (uint32_t)joins, jparams, s, err);
+  return launch(x, x->l.entries.size() - 1, (uint32_t)(tokens * at.heads), jparams, s, err);
 }
 
 }  // namespace
