@@ -1215,16 +1215,60 @@ UNP4_DEV void attend(const T* q, const u32* cache, const i32* table, const i32* 
   }
 }
 
-// The parts of split contexts: a block per row and head, whose lanes hold four elements each and take the parts in
-// groups, all of a group's loads in flight at once: with a lane for all parts of its elements, 64 parts took 52 us.
-constexpr int kMostParts = 128;
+// The last sequence whose start is at most `row`, or -1 where no sequence has the row.
+UNP4_DEV i64 sequence_of(const i32* starts, i64 batch, i64 row) {
+  i64 lo = 0, hi = batch;
+  while (hi - lo > 1) {
+    const i64 mid = (lo + hi) >> 1;
+    if (starts[mid] <= row) lo = mid; else hi = mid;
+  }
+  return starts[lo] > row || row >= starts[lo + 1] ? -1 : lo;
+}
+
+// The parts of split contexts: a lane holds four elements.  Few parts: as many rows and heads a block as its lanes hold, each
+// lane takes all parts, their loads in flight at once (22720 rows of 64 elements in 2 parts: JOINA us, with a block each
+// 27).  Many parts: a block per row and head, whose groups of lanes take parts in turn: with a lane for all parts of its
+// elements, 64 parts took 52 us.
+constexpr int kMostParts = 128, kFewParts = 8;
 template <class T, int H, int QH, int D, bool LSE>
 UNP4_DEV void join(const i32* starts, T* out, float* lse, float* ws, const attention_args& a) {
   constexpr int L = D / 4, GROUPS = 256 / L;
   __shared__ float weight[kMostParts];
   __shared__ f32x4 part[GROUPS][L];
+  const int lane = threadIdx.x & 63, group = threadIdx.x / L, d = threadIdx.x % L * 4;
+  if (a.splits <= kFewParts) {
+    const i64 item = (i64)blockIdx.x * GROUPS + group, row = item / QH;
+    const int head = (int)(item % QH);
+    if (group >= GROUPS || row >= a.tokens) return;
+    f32x2 st[kFewParts];
+    f32x4 v[kFewParts];
+#pragma unroll
+    for (int s = 0; s < kFewParts; ++s) {
+      const int part = s < a.splits ? s : 0;
+      st[s] = *reinterpret_cast<const f32x2*>(parts<QH, D>::stat(ws, a, part, row, head));
+      v[s] = *reinterpret_cast<const f32x4*>(parts<QH, D>::sums(ws, a, part, row, head) + d);
+    }
+    if (sequence_of(starts, a.batch, row) < 0) return;
+    float top = -__builtin_inff(), l = 0.0f;
+#pragma unroll
+    for (int s = 0; s < kFewParts; ++s) top = s < a.splits ? fmaxf(top, st[s][0]) : top;
+    const float base = top == -__builtin_inff() ? 0.0f : top;
+    f32x4 o = {0, 0, 0, 0};
+#pragma unroll
+    for (int s = 0; s < kFewParts; ++s) {
+      if (s >= a.splits || st[s][1] == 0.0f) continue;  // a part without keys wrote no sums
+      const float keep = __builtin_amdgcn_exp2f(st[s][0] - base);
+      l = fmaf(st[s][1], keep, l);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) o[i] = fmaf(v[s][i], keep, o[i]);
+    }
+    const float y[4] = {o[0], o[1], o[2], o[3]};
+    put<T, 4>(out + row * a.out_token + head * a.out_head + d, y, share_of(l), a.out_wide);
+    if (LSE && d == 0) lse[row * QH + head] = log_sum(top, l);
+    return;
+  }
   const i64 row = blockIdx.x / QH;
-  const int head = (int)(blockIdx.x % QH), lane = threadIdx.x & 63, group = threadIdx.x / L, d = threadIdx.x % L * 4;
+  const int head = (int)(blockIdx.x % QH);
   // The parts' maxima and sums, in every wave; rows that no sequence names have none.
   f32x2 st[kMostParts / 64];
 #pragma unroll
@@ -1233,12 +1277,7 @@ UNP4_DEV void join(const i32* starts, T* out, float* lse, float* ws, const atten
     st[i] = s < a.splits ? *reinterpret_cast<const f32x2*>(parts<QH, D>::stat(ws, a, s, row, head))
                          : f32x2{-__builtin_inff(), 0.0f};
   }
-  i64 lo = 0, hi = a.batch;
-  while (hi - lo > 1) {
-    const i64 mid = (lo + hi) >> 1;
-    if (starts[mid] <= row) lo = mid; else hi = mid;
-  }
-  if (starts[lo] > row || row >= starts[lo + 1]) return;
+  if (sequence_of(starts, a.batch, row) < 0) return;
   float top = -__builtin_inff(), l = 0.0f;
 #pragma unroll
   for (int i = 0; i < kMostParts / 64; ++i) top = fmaxf(top, st[i][0]);

@@ -2055,7 +2055,7 @@ int32_t check_attention(const unp_exec* x, int64_t tokens, int64_t batch, int64_
 }
 
 // A launch's shape: the entry, its row tiles, how they are numbered (tile_of) and the parts of a context.
-constexpr int64_t kMostParts = 128;  // the device's kMostParts
+constexpr int64_t kMostParts = 128, kFewParts = 8;  // the device's: a join of few parts takes several rows a block
 constexpr int64_t kMostBlocks = 0xFFFFFF;  // of 256 lanes: a launch has less than 2^32
 struct AttentionPlan {
   size_t entry = 0;
@@ -2145,7 +2145,8 @@ int32_t run_cache4_attention(unp_exec* x, const unp_arg* a, size_t n, hipStream_
   x->shared = p.splits > 1;
   if ((rc = launch(x, p.entry, (uint32_t)blocks, params, s, err)) != UNP_OK || p.splits == 1) return rc;
   void* jparams[] = {&starts, &out, &lse, &ws, &args};
-  return launch(x, x->l.entries.size() - 1, (uint32_t)(tokens * at.heads), jparams, s, err);
+  const int64_t rows = p.splits <= kFewParts ? 256 / (c.head_dim / 4) : 1, joined = tokens * at.heads;
+  return launch(x, x->l.entries.size() - 1, (uint32_t)((joined + rows - 1) / rows), jparams, s, err);
 }
 
 }  // namespace
