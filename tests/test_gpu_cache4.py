@@ -597,6 +597,30 @@ def test_attention_splits_of_every_kind_of_block(hip_device, heads, rows, window
     attention_case("F16", heads, 1, 64, 32, 32, rows, [2300, 90][:len(rows)], window=window, seed=heads, lse=heads != 6)
 
 
+@pytest.mark.parametrize("dtype, heads, kv, dim, group, rows, lengths, entry", [
+    ("Bf16", 8, 2, 64, 64, [9, 3, 12], [700, 520, 12], "_some"),     # several tiles of a sequence
+    ("F16", 12, 1, 64, 32, [4, 1], [600, 601], "_few"),              # the same, of more heads than columns are shared by
+    ("Bf16", 8, 2, 96, 32, [30, 41], [530, 900], "_more"),
+    ("F16", 4, 4, 128, 128, [170, 190, 0, 1], [1300, 190, 7, 5], "_more"),
+    ("Bf16", 6, 2, 32, 32, [60, 61, 90], [200, 150, 90], "_many"),   # a context that is no longer than its steps
+])
+@pytest.mark.parametrize("workspace", [True, 0])
+def test_attention_of_some_tiles_a_sequence(hip_device, dtype, heads, kv, dim, group, rows, lengths, entry, workspace):
+    ex = executor("lower_cache4_attention", dtype=dtype, heads=heads, kv_heads=kv, head_dim=dim, group=group, page=32,
+                  causal=True, lse=True, scale=0.0)
+    attention_case(dtype, heads, kv, dim, group, 32, rows, lengths, workspace=workspace, seed=21)
+    last = ex.last_launch()["entry"]
+    assert last.endswith(entry) or last.endswith("_join"), last
+
+
+@pytest.mark.parametrize("parts", range(1, 12))
+def test_attention_of_every_number_of_parts(hip_device, parts):
+    """Joins of few parts (several rows a block) and of many, by the workspace that they get."""
+    tokens, heads, dim = 2, 3, 96
+    size = (parts * tokens * heads * 8 + 15) // 16 * 16 + parts * tokens * heads * dim * 4
+    attention_case("F16", heads, 1, dim, 96, 16, [1], [1700], behind=1, workspace=size, seed=parts)
+
+
 def test_attention_of_many_sequences(hip_device):
     """More sequences than one look of a wave finds, some without rows and some without keys."""
     rng = np.random.default_rng(3)

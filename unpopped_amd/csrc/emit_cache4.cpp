@@ -288,7 +288,7 @@ int32_t lower_cache4_attention(const unp_cache4& c, const unp_attention& a, Lowe
                            std::to_string(c.head_dim);
   const char* lse = a.lse ? "true" : "false";
   // cg groups of columns hold the same 16 / cg rows (few rows); wk waves share a block's rows, or wr have their own.
-  auto add = [&](const char* tail, int qt, int cg, int wr, int wk, int per_simd) {
+  auto add = [&](const char* tail, int qt, int cg, int wr, int wk, bool once, int per_simd) {
     Entry e;
     e.symbol = L.name + tail;
     e.threads = 64 * wr * wk;
@@ -300,7 +300,7 @@ int32_t lower_cache4_attention(const unp_cache4& c, const unp_attention& a, Lowe
         << "* q, const unsigned* cache, const int* table, const int* starts, const int* lengths, " << T
         << "* out, float* lse, float* ws, float scale, unp4::attention_args a) {\n  unp4::attend<" << same << ", " << c.group
         << ", " << c.page << ", " << (a.causal ? "true" : "false") << ", " << lse << ", " << qt << ", " << cg << ", " << wr
-        << ", " << wk << ">(q, cache, table, starts, lengths, out, lse, ws, scale, a);\n}\n";
+        << ", " << wk << ", " << (once ? "true" : "false") << ">(q, cache, table, starts, lengths, out, lse, ws, scale, a);\n}\n";
   };
   const int gq = a.heads / c.kv_heads;
   // What a wave holds, in registers: the words of a step, the rows, their sums and the words of groups.  The kernels
@@ -315,10 +315,11 @@ int32_t lower_cache4_attention(const unp_cache4& c, const unp_attention& a, Lowe
   // As many groups of columns as leave room for a row each, as far as they fit; two row tiles a wave if they fit.
   int cg = gq <= 4 ? 4 : gq <= 8 ? 2 : 1;
   while (cg > 1 && held(cg, 1) > 176) cg /= 2;
-  add("_few", 1, cg, 1, 4, held(cg, 1) <= 204 ? 2 : 1);
-  if (cg > 1) add("_some", 1, 1, 1, 4, held(1, 1) <= 204 ? 2 : 1);
-  const int qt = held(1, 2) <= 204 ? 2 : 1;
-  add("_many", qt, 1, 4, 1, held(1, qt) <= 204 ? 2 : 1);
+  add("_few", 1, cg, 1, 4, true, held(cg, 1) <= 204 ? 2 : 1);
+  if (cg > 1) add("_some", 1, 1, 1, 4, false, held(1, 1) <= 204 ? 2 : 1);
+  const int qt = held(1, 2) <= 204 ? 2 : 1, per_simd = held(1, qt) <= 204 ? 2 : 1;
+  add("_more", qt, 1, 1, 4, false, per_simd);
+  add("_many", qt, 1, 4, 1, false, per_simd);
   Entry e;
   e.symbol = L.name + "_join";
   L.entries.push_back(e);
@@ -327,7 +328,8 @@ int32_t lower_cache4_attention(const unp_cache4& c, const unp_attention& a, Lowe
       << ">(starts, out, lse, ws, a);\n}\n";
   L.source = src.str();
   std::vector<std::string> when = {"a sequence has no more rows of a key/value head, on average, than one of its tiles"};
-  if (cg > 1) when.push_back("at most 16 rows");
+  if (cg > 1) when.push_back("at most one of its tiles, or four over a long context");
+  when.push_back("a long context and at most eight of its tiles, or too few blocks of the next");
   when.push_back("otherwise");
   when.push_back("after any of them, where a context is split");
   const char* dt = kind_name(c.dtype);

@@ -555,7 +555,7 @@ template <> struct is_half<_Float16> {
   static constexpr bool value = true;
 };
 
-// Adjacent words; ONCE: what this launch reads once goes past the caches (64 single tokens over up to 16384 keys took
+// Adjacent words; ONCE: what this launch reads once (a sequence's rows fill one tile) goes past the caches (64 single tokens over up to 16384 keys took
 // 154 us through them, 141 past them).
 typedef u32 u32x2 __attribute__((ext_vector_type(2)));
 template <class V, bool ONCE> UNP4_DEV V words_at(const u32* p) {
@@ -1112,11 +1112,10 @@ template <int QH, int D> struct parts {
 // turn and are joined through LDS.  Blocks are numbered with the heads innermost (consecutive blocks go to different
 // XCDs: with 8 heads each XCD's L2 holds one head's keys), then the parts of a context, then the tiles, last ones
 // first: under a causal mask those have the most keys.
-template <class T, int H, int QH, int D, int GROUP, int P, bool CAUSAL, bool LSE, int QT, int CG, int WR, int WK>
+template <class T, int H, int QH, int D, int GROUP, int P, bool CAUSAL, bool LSE, int QT, int CG, int WR, int WK, bool ONCE>
 UNP4_DEV void attend(const T* q, const u32* cache, const i32* table, const i32* starts, const i32* lengths, T* out,
                      float* lse, float* ws, float scale, const attention_args& a) {
-  // Waves that share a tile's rows read the keys once, as long as a sequence's rows fill no second tile.
-  typedef attention<T, H, QH, D, GROUP, P, CAUSAL, LSE, QT, CG, (WK > 1)> A;
+  typedef attention<T, H, QH, D, GROUP, P, CAUSAL, LSE, QT, CG, ONCE> A;
   constexpr int GQ = QH / H, WAVE_ROWS = QT * A::ROWS, ROWS = WAVE_ROWS * WR;
   const int wave = uniform(threadIdx.x >> 6);
   const int kv = blockIdx.x % H, part = (int)(blockIdx.x / H) % a.splits;
@@ -1158,42 +1157,46 @@ UNP4_DEV void attend(const T* q, const u32* cache, const i32* table, const i32* 
   w.walk(s);
   if constexpr (WK > 1 || CG > 1) {
     // Join the waves and groups of columns: the rows' maxima and sums, then their elements, each scaled to the
-    // common maximum.
-    static_assert(QT == 1 && WR == 1, "a block joins the parts of one tile");
+    // common maximum; a row tile at a time.
+    static_assert(WR == 1, "a block joins the parts of its waves' rows");
     __shared__ float stat[WK * CG][A::ROWS][2];
     __shared__ float sums[WK * CG][A::ROWS][D + 4];
     const int mine = wave * CG + w.own, r0 = w.c % A::ROWS;
-    if (w.g == 0) {
-      stat[mine][r0][0] = w.m[0] * w.factor[0];
-      stat[mine][r0][1] = w.l[0][0];
-    }
-    w.each([&](auto n, int tl, int r, int d) {
 #pragma unroll
-      for (int e = 0; e < decltype(n)::value; ++e) sums[mine][r0][d + e] = w.sum_of(0, tl, e, r);
-    });
-    __syncthreads();
-    const int n = all_rows - first_row < A::ROWS ? all_rows - first_row : A::ROWS;
-    for (int i = threadIdx.x; i < n * (D / 4); i += 64 * WK) {
-      const int row = i / (D / 4), d = i % (D / 4) * 4;
-      float top = -__builtin_inff(), l = 0.0f;
-#pragma unroll
-      for (int v = 0; v < WK * CG; ++v) top = fmaxf(top, stat[v][row][0]);
-      const float base = top == -__builtin_inff() ? 0.0f : top;
-      f32x4 o = {0, 0, 0, 0};
-#pragma unroll
-      for (int v = 0; v < WK * CG; ++v) {
-        const float keep = __builtin_amdgcn_exp2f(stat[v][row][0] - base);
-        l = fmaf(stat[v][row][1], keep, l);
-        o += *reinterpret_cast<const f32x4*>(&sums[v][row][d]) * keep;
+    for (int x = 0; x < QT; ++x) {
+      if (x > 0) __syncthreads();
+      if (w.g == 0) {
+        stat[mine][r0][0] = w.m[x] * w.factor[x];
+        stat[mine][r0][1] = w.l[x][0];
       }
-      const int token = t.start + (first_row + row) / GQ, head = kv * GQ + (first_row + row) % GQ;
-      if (a.splits > 1) {
-        if (d == 0) store<float, 2>(parts<QH, D>::stat(ws, a, part, token, head), {top, l});
-        if (l != 0.0f) *reinterpret_cast<f32x4*>(parts<QH, D>::sums(ws, a, part, token, head) + d) = o;
-      } else {
-        const float y[4] = {o[0], o[1], o[2], o[3]};
-        put<T, 4>(out + token * a.out_token + head * a.out_head + d, y, share_of(l), a.out_wide);
-        if (LSE && d == 0) lse[(i64)token * QH + head] = log_sum(top, l);
+      w.each([&](auto n, int tl, int r, int d) {
+#pragma unroll
+        for (int e = 0; e < decltype(n)::value; ++e) sums[mine][r0][d + e] = w.sum_of(x, tl, e, r);
+      });
+      __syncthreads();
+      const int at = first_row + x * A::ROWS, n = all_rows - at < A::ROWS ? all_rows - at : A::ROWS;
+      for (int i = threadIdx.x; i < n * (D / 4); i += 64 * WK) {
+        const int row = i / (D / 4), d = i % (D / 4) * 4;
+        float top = -__builtin_inff(), l = 0.0f;
+#pragma unroll
+        for (int v = 0; v < WK * CG; ++v) top = fmaxf(top, stat[v][row][0]);
+        const float base = top == -__builtin_inff() ? 0.0f : top;
+        f32x4 o = {0, 0, 0, 0};
+#pragma unroll
+        for (int v = 0; v < WK * CG; ++v) {
+          const float keep = __builtin_amdgcn_exp2f(stat[v][row][0] - base);
+          l = fmaf(stat[v][row][1], keep, l);
+          o += *reinterpret_cast<const f32x4*>(&sums[v][row][d]) * keep;
+        }
+        const int token = t.start + (at + row) / GQ, head = kv * GQ + (at + row) % GQ;
+        if (a.splits > 1) {
+          if (d == 0) store<float, 2>(parts<QH, D>::stat(ws, a, part, token, head), {top, l});
+          if (l != 0.0f) *reinterpret_cast<f32x4*>(parts<QH, D>::sums(ws, a, part, token, head) + d) = o;
+        } else {
+          const float y[4] = {o[0], o[1], o[2], o[3]};
+          put<T, 4>(out + token * a.out_token + head * a.out_head + d, y, share_of(l), a.out_wide);
+          if (LSE && d == 0) lse[(i64)token * QH + head] = log_sum(top, l);
+        }
       }
     }
   } else {
@@ -1226,7 +1229,7 @@ UNP4_DEV i64 sequence_of(const i32* starts, i64 batch, i64 row) {
 }
 
 // The parts of split contexts: a lane holds four elements.  Few parts: as many rows and heads a block as its lanes hold, each
-// lane takes all parts, their loads in flight at once (22720 rows of 64 elements in 2 parts: JOINA us, with a block each
+// lane takes all parts, their loads in flight at once (22720 rows of 64 elements in 2 parts: 8 us, with a block each
 // 27).  Many parts: a block per row and head, whose groups of lanes take parts in turn: with a lane for all parts of its
 // elements, 64 parts took 52 us.
 constexpr int kMostParts = 128, kFewParts = 8;

@@ -2071,24 +2071,36 @@ AttentionPlan attention_plan(const unp_exec* x, int64_t tokens, int64_t batch, i
   const unp_cache4& c = x->l.cache4;
   const int64_t group = x->l.attention.heads / c.kv_heads;
   AttentionPlan p;
-  // The first entry whose tile holds a sequence's rows, of those whose waves share them; beyond 16, waves of rows of
-  // their own.  The last entry joins.
-  const size_t own = x->l.entries.size() - 2;
-  while (p.entry < own && tokens * group > x->l.entries[p.entry].vec * batch) ++p.entry;
+  // The first entry whose tile holds a sequence's rows, of those whose waves share them, or up to four tiles of the last of
+  // these over a context that is worth its waves' join (a block of rows alone leaves waves without rows: 96 sequences of up
+  // to 40 rows over 2100 keys 117 us, four tiles 63).  Then the one whose waves share two row tiles, where a sequence has
+  // few (64 of up to 256 rows over 4000 keys 228 us, rows alone 264) or blocks of rows alone would fill half of the CUs
+  // at most (2048 rows over 16000 keys 184 and 205; a prompt of 2000 tokens, whose blocks fill them, 78 and 69).  Else
+  // waves of rows of their own.  The last entry joins.
+  const int64_t rows = tokens * group, keys = width * c.page;
+  const size_t own = x->l.entries.size() - 2, more = own - 1;
+  auto holds = [&](size_t entry) { return (int64_t)x->cu_count * std::max(1, x->resident[entry]); };
+  auto tiles = [&](size_t entry) { return rows / x->l.entries[entry].vec * c.kv_heads; };
+  auto at_most = [&](size_t entry, int64_t n) { return rows <= n * x->l.entries[entry].vec * batch; };
+  const bool deep = keys > 4 * x->l.entries[more].k;
+  while (p.entry + 1 < more && !at_most(p.entry, 1)) ++p.entry;
+  if (!at_most(p.entry, deep ? 4 : 1)) p.entry = deep && (at_most(more, 8) || 2 * tiles(own) < holds(own)) ? more : own;
+  const bool several = p.entry >= more || !at_most(p.entry, 1);  // tiles of a sequence
   const unp::Entry& e = x->l.entries[p.entry];
-  p.slots = tokens * group / e.vec + batch;
+  p.slots = rows / e.vec + batch;
   if (group <= e.vec && tokens <= p.slots) {
     p.slots = tokens;
     p.by_token = true;
   }
   // As many parts as fill the CUs with the blocks that they hold at once, none shorter than a step of waves that share
-  // their rows (where no block would be without a CU, none at all) or 128 keys of others, and none of a context that four
-  // such parts would hold: the join costs as much.  The context is its pages' length, as the host knows no other.
-  const int64_t hold = (int64_t)x->cu_count * std::max(1, x->resident[p.entry]), keys = width * c.page;
+  // one tile (where no block would be without a CU, none at all), eight steps where they share several, or 128 keys of
+  // others, and none of a context that four such parts would hold: the join costs as much.  The context is its pages'
+  // length, as the host knows no other.
+  const int64_t hold = holds(p.entry);
   // About the tiles that have rows: a sequence fills its last one by half.
-  const int64_t blocks = p.by_token ? p.slots * c.kv_heads : ((tokens * group + e.vec - 1) / e.vec + (batch - 1) / 2) * c.kv_heads;
-  const int64_t least = p.entry < own ? e.k : 128;
-  const int64_t want = p.entry == own ? (hold + blocks / 2) / blocks : blocks >= x->cu_count ? 1 : hold / blocks;
+  const int64_t blocks = p.by_token ? p.slots * c.kv_heads : ((rows + e.vec - 1) / e.vec + (batch - 1) / 2) * c.kv_heads;
+  const int64_t least = p.entry == own ? 128 : several ? 8 * e.k : e.k;
+  const int64_t want = several ? (hold + blocks / 2) / blocks : blocks >= x->cu_count ? 1 : hold / blocks;
   if (keys > 4 * least) p.splits = std::max<int64_t>(1, std::min({want, (keys + least - 1) / least, kMostParts}));
   return p;
 }
