@@ -2093,13 +2093,14 @@ AttentionPlan attention_plan(const unp_exec* x, int64_t tokens, int64_t batch, i
     p.by_token = true;
   }
   // As many parts as fill the CUs with the blocks that they hold at once, none shorter than a step of waves that share
-  // one tile (where no block would be without a CU, none at all), eight steps where they share several, or 128 keys of
-  // others, and none of a context that four such parts would hold: the join costs as much.  The context is its pages'
+  // one tile (where no block would be without a CU, none at all), eight steps where they share several, or 512 keys of
+  // others (one sequence of 1300 tokens x 4 heads over 16000 keys 532 us in two parts, 654 whole; 2048 tokens x 2 heads of
+  // 192 over themselves 90 and 64), and none of a context that four such parts would hold: the join costs as much.  The context is its pages'
   // length, as the host knows no other.
   const int64_t hold = holds(p.entry);
   // About the tiles that have rows: a sequence fills its last one by half.
   const int64_t blocks = p.by_token ? p.slots * c.kv_heads : ((rows + e.vec - 1) / e.vec + (batch - 1) / 2) * c.kv_heads;
-  const int64_t least = p.entry == own ? 128 : several ? 8 * e.k : e.k;
+  const int64_t least = p.entry == own ? 512 : several ? 8 * e.k : e.k;
   const int64_t want = several ? (hold + blocks / 2) / blocks : blocks >= x->cu_count ? 1 : hold / blocks;
   if (keys > 4 * least) p.splits = std::max<int64_t>(1, std::min({want, (keys + least - 1) / least, kMostParts}));
   return p;
