@@ -346,7 +346,7 @@ int32_t lower_cache4_attention(const unp_cache4& c, const unp_attention& a, Lowe
                 "a block per row tile, part of a context and key/value head",
                 when,
                 "the caller's, by unp_hip_exec_workspace",
-                "scores, softmax statistics and sums in f32, probabilities and values as f16 in the products; each output rounded once");
+                "scores, softmax statistics and sums in f32, probabilities times value scales as f16 in the products; each output rounded once");
   return UNP_OK;
 }
 

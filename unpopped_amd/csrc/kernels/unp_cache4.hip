@@ -431,11 +431,14 @@ UNP4_DEV void read(const I* slots, const u32* cache, T* k, T* v, const cache_arg
 //     only when some score passes the running one by 2^4.9: p is held as 2^11 p in f16, which ends at 2^16
 //     (moving at 2^0.9, with 2^15 p, cost a prompt 8%: the sums are multiplied anew each time).
 //   * O' += V' P' with the value words as rows, again nibbles as they lie: sum p s (n - zero) is the product of n with
-//     p s less the sum of p s zero.  p s is rounded to f16 (both sums take it as rounded), s relative to a
-//     running power of two that no scale of the column exceeded, so that it stays in f16's range whatever s is.  The
-//     scores are, lane by lane, the operand that this product needs when its key (g, i) of 4 x 8 is key
-//     16 CG (i / 4) + 4 g + i % 4; a lane reads four tokens' words of 8 elements at once and pairs of tokens of one
-//     element are made by byte permutes, so nothing goes through LDS.
+//     p s less the sum of p s zero.  p s is rounded to f16 (both sums take it as rounded), s in a unit that puts the
+//     scales that the wave's rows see between 2^-14 and 1, exactly: then what p s loses below f16's normal numbers is less
+//     than 2^-20 of the smallest scale.  Where the scales lie further apart than that, the wave begins anew: p s is made in
+//     f32, and each step of a row and group rounds it in a unit of its own (9847 tokens as below 355 us with and without the
+//     check; 32 sequences of up to 400 x 32 rows 430 us with scales too far apart, 265 without).  The scores are, lane by
+//     lane, the operand that this product needs when its key (g, i) of 4 x 8 is key 16 CG (i / 4) + 4 g + i % 4; a lane reads
+//     four tokens' words of 8 elements at once and pairs of tokens of one element are made by byte permutes, so nothing
+//     goes through LDS.
 //
 // What bounds it: a decode step its reads (64 single tokens x 8 heads over up to 16384 keys 138 us, 5.4 TB/s; one over 262144
 // keys 51, 5.9 TB/s), a prompt the VALU's issue (9847 tokens x 32 heads of three sequences, causal, 355 us, 784
@@ -443,6 +446,7 @@ UNP4_DEV void read(const I* slots, const u32* cache, T* k, T* v, const cache_arg
 // ---------------------------------------------------------------------------------------
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef u16 u16x2 __attribute__((ext_vector_type(2)));
 
 struct attention_args {
   i64 tokens, batch, width, pages, q_token, q_head, out_token, out_head, window;
@@ -620,7 +624,11 @@ template <class T, int H, int QH, int D, int GROUP, int P, bool CAUSAL, bool LSE
   float m[QT];                    // running maximum
   bool far;                       // some maximum is beyond 2^kFar in log2 (all lanes agree)
   f32x4 l[QT];                    // the sum of p, in l[0] (EXACT_SUM: this lane's part of it until the end)
-  _Float16 unit;                  // a power of two: value scales times it are at most 1
+  // The value scales that the wave's rows saw so far, the same in all lanes: but for 0 none is below `least`, their f16 bits
+  // are from `low` (in both halves) to `span` above it, and `unit`, a power of two, puts them between 2^-14 and 1.
+  _Float16 unit;
+  float least;
+  u32 low, span;
   f32x4 o[QT][NE];
   // The sums of p s zero by group: this lane's parts, or (one group of columns, few of elements) a product whose rows
   // are all the same.
@@ -632,12 +640,29 @@ template <class T, int H, int QH, int D, int GROUP, int P, bool CAUSAL, bool LSE
   f32x4 zp[QT][ZERO_PRODUCT ? G : 1];
   int end[QT], begin[QT];  // keys that the column sees
 
+  UNP4_DEV void clear() {
+    unit = (_Float16)1.0f;
+    least = __builtin_inff();
+    low = span = 0;
+    far = false;
+#pragma unroll
+    for (int x = 0; x < QT; ++x) {
+      m[x] = -__builtin_inff();
+      l[x] = f32x4{0, 0, 0, 0};
+#pragma unroll
+      for (int gi = 0; gi < G; ++gi) {
+        zs[x][gi] = 0.0f;
+        if (ZERO_PRODUCT) zp[x][ZERO_PRODUCT ? gi : 0] = f32x4{0, 0, 0, 0};
+      }
+#pragma unroll
+      for (int e = 0; e < NE; ++e) o[x][e] = f32x4{0, 0, 0, 0};
+    }
+  }
   // Rows first .. first + QT ROWS - 1 (token * GQ + head of the group) of a sequence.
   UNP4_DEV void rows(const T* qp, const attention_args& a, const tile& t, int kv, int first, float scale, int cap) {
     asm("s_mov_b32 %0, 0x000f000f" : "=s"(mask0));
     asm("s_mov_b32 %0, 0x00f000f0" : "=s"(mask1));
-    unit = (_Float16)0x1p15f;
-    far = false;
+    clear();
 #pragma unroll
     for (int x = 0; x < QT; ++x) {
       const int r = first + x * 16 + c % ROWS;
@@ -682,15 +707,6 @@ template <class T, int H, int QH, int D, int GROUP, int P, bool CAUSAL, bool LSE
       for (int gi = 0; gi < G; ++gi) qsum[x][gi] = column_sum(qsum[x][gi]);
       // Where this ends at 2^127, two scores that differ at all are further apart than exp reaches either way.
       factor[x] = fminf(scale * 1.4426950408889634f * 0x1p24f * __builtin_bit_cast(float, (u32)(127 - up) << 23), 0x1p127f);
-      m[x] = -__builtin_inff();
-      l[x] = f32x4{0, 0, 0, 0};
-#pragma unroll
-      for (int gi = 0; gi < G; ++gi) {
-        zs[x][gi] = 0.0f;
-        if (ZERO_PRODUCT) zp[x][ZERO_PRODUCT ? gi : 0] = f32x4{0, 0, 0, 0};
-      }
-#pragma unroll
-      for (int e = 0; e < NE; ++e) o[x][e] = f32x4{0, 0, 0, 0};
       const int last = CAUSAL ? t.length - t.rows + token + 1 : t.length;
       end[x] = in ? (last < cap ? last : cap) : 0;
       begin[x] = CAUSAL && a.window > 0 && a.window < last ? last - (int)a.window : 0;
@@ -823,7 +839,80 @@ template <class T, int H, int QH, int D, int GROUP, int P, bool CAUSAL, bool LSE
             __builtin_amdgcn_mfma_f32_16x16x32_f16(va[e], p[x][t / TG], o[x][product(t, e)], 0, 0, 0);
   }
 
-  UNP4_DEV void step(stream& s) {
+  // Whether a value scale of a step lies outside the known range, by its bits; with ZEROS one of 0 does not.
+  template <bool ZEROS> UNP4_DEV bool outside(const f16x2 (&vs)[G][4]) const {
+    u16x2 most = {0, 0};
+#pragma unroll
+    for (int gi = 0; gi < G; ++gi)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const u16x2 b = __builtin_bit_cast(u16x2, vs[gi][k]), over = b - __builtin_bit_cast(u16x2, low);
+        most = __builtin_elementwise_max(most, ZEROS ? over * __builtin_elementwise_min(b, u16x2{1, 1}) : over);
+      }
+    return most[0] > span || most[1] > span;
+  }
+  // Takes a step's value scales (of keys that some row sees) into the known range.  Gives what the sums are multiplied with as
+  // their unit changes: 0 where no unit holds the range.
+  UNP4_DEV float widen(const f16x2 (&vs)[G][4], u32 seen) {
+    u32 top = 0, bottom = 0xFFFF;
+#pragma unroll
+    for (int gi = 0; gi < G; ++gi)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const u32 b = __builtin_bit_cast(u32, vs[gi][i / 2]) >> (16 * (i % 2)) & 0x7FFFu;
+        // Zeros weigh nothing, and no unit makes an infinity or a NaN a number.
+        const bool counts = b != 0 && b < 0x7C00u && (seen >> i & 1);
+        top = counts && b > top ? b : top;
+        bottom = counts && b < bottom ? b : bottom;
+      }
+    top = (u32)uniform((int)lane_max<16>(column_max((float)top)));
+    bottom = (u32)uniform((int)-lane_max<16>(column_max(-(float)bottom)));
+    if (top == 0) return 1.0f;
+    // A bit of room above and two below, so that later scales seldom pass the range.
+    const u32 known = low + span & 0xFFFFu, next = ((top >> 10) + 1) << 10 | 0x3FFu;
+    const u32 end = top <= known ? known : next < 0x7BFFu ? next : 0x7BFFu;
+    const float small = (float)__builtin_bit_cast(_Float16, (u16)bottom);
+    // 2^14 over the exponent's bits: `end` times it is below 1.
+    const float to = __builtin_bit_cast(float, (u32)uniform((int)((141u - (end >> 10)) << 23)));
+    least = fminf(least, fmaxf(small * 0.25f, fminf(small, 0x1p-14f / to)));
+    if (least * to < 0x1p-14f) return 0.0f;
+    const u32 from = (u32)__builtin_bit_cast(u16, (_Float16)least);
+    low = (u32)uniform((int)(from | from << 16));
+    span = (u32)uniform((int)(end - from));
+    const float by = to / (float)unit;
+    unit = (_Float16)to;
+    return by;
+  }
+
+  // The sums of a row tile and group into another unit.
+  UNP4_DEV void rescale(int x, int gi, float by) {
+    if (ZERO_PRODUCT)
+      zp[x][ZERO_PRODUCT ? gi : 0] *= by;
+    else
+      zs[x][gi] *= by;
+#pragma unroll
+    for (int e = 0; e < NEG; ++e) o[x][gi * NEG + e] *= by;
+  }
+  // p s of a step whose scales have no common unit: in f32, then in the one that puts the column's largest into 2^10 .. 2^11
+  // (2^15 at most: below that no p s of a maximal p and any scale is lost).  The sums go into it too; gives the way back.
+  UNP4_DEV float alone(int x, int gi, const float (&y)[8], const f16x2 (&scale)[4], u32 seen, u32x4& p) {
+    float w[8], top = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      w[i] = seen >> i & 1 ? y[i] * (float)scale[i / 2][i % 2] : 0.0f;
+      top = fmaxf(top, fabsf(w[i]));
+    }
+    const int up = 137 - (int)(__builtin_bit_cast(u32, column_max(fminf(top, 0x1p40f))) >> 23);  // 10 less the exponent
+    const float to = __builtin_bit_cast(float, (u32)(127 + (up < 15 ? up : 15)) << 23);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) p[k] = __builtin_bit_cast(u32, f16x2{(_Float16)(w[2 * k] * to), (_Float16)(w[2 * k + 1] * to)});
+    rescale(x, gi, to);
+    return 1.0f / to;
+  }
+
+  // Without APART: a step whose scales have no unit in common with those before is the last (the walk's sums do not count).
+  // The loop keeps its one exit so: from a second one the compiler would have all loads land before each step.
+  template <bool APART> UNP4_DEV void step(stream& s) {
     const int k0 = s.at * KEYS, after = s.next + s.by < s.last ? s.next + s.by : s.next;
     s.number(after, s.far);
     bool whole = k0 >= s.lo && k0 + KEYS <= s.hi;
@@ -879,10 +968,6 @@ template <class T, int H, int QH, int D, int GROUP, int P, bool CAUSAL, bool LSE
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const int key = k0 + 16 * (h * CG + own) + 4 * g + i;
-          // What no column sees does not count, whatever it holds.
-          if (!there || key >= s.cap)
-#pragma unroll
-            for (int gi = 0; gi < G; ++gi) s.vp[h][gi][i] = 0;
 #pragma unroll
           for (int x = 0; x < QT; ++x) {
             const bool sees = there && key < end[x] && key >= begin[x];
@@ -892,53 +977,46 @@ template <class T, int H, int QH, int D, int GROUP, int P, bool CAUSAL, bool LSE
         }
       }
     }
-    // The running maxima and the scales' unit; p of a row against an old maximum may reach 2^kSlack.
+    // The running maxima and the scales' range; p of a row against an old maximum may reach 2^kSlack.
     float top[QT];
-    bool move = false;
+    bool up = false;
 #pragma unroll
     for (int x = 0; x < QT; ++x) {
       top[x] = sc[x][0];
 #pragma unroll
       for (int i = 1; i < 8; ++i) top[x] = fmaxf(top[x], sc[x][i]);
-      move |= (top[x] - m[x]) * factor[x] > kSlack;
+      up |= (top[x] - m[x]) * factor[x] > kSlack;
     }
     f16x2 vs[G][4];  // the scales of keys 2k, 2k + 1
-    f16x2 most = {0, 0};
 #pragma unroll
     for (int gi = 0; gi < G; ++gi)
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
+      for (int k = 0; k < 4; ++k)
         vs[gi][k] = __builtin_bit_cast(f16x2, low_halves(s.vp[k / 2][gi][2 * (k % 2)], s.vp[k / 2][gi][2 * (k % 2) + 1]));
-        most = __builtin_elementwise_max(most, vs[gi][k]);
+    float by = 1.0f;
+    bool past = !APART && outside<false>(vs);
+    if (__any(up || past)) {
+      if (!APART) past = outside<true>(vs);
+      if (__any(past)) {
+        u32 any = masked ? seen[0] : 0xFFu;
+        if (masked && QT > 1) any |= seen[QT - 1];
+        by = widen(vs, any);
+        s.last = by == 0.0f ? s.at : s.last;
       }
-    const float big = fminf(fmaxf((float)most[0], (float)most[1]), 65504.0f);
-    move |= big * (float)unit > 1.0f;
-    if (__any(move)) {
-      const float all = column_max(big);
-      const float old = (float)unit;
-      // 2^-(exponent + 1), so that the largest scale lies in 1/2 .. 1.
-      const float to = all * old > 1.0f ? __builtin_bit_cast(float, (253u << 23) - (__builtin_bit_cast(u32, all) & 0x7F800000u)) : old;
-      const float by = to / old;
-      unit = (_Float16)to;
-      bool beyond = false;
+      if (__any(up || past)) {
+        bool beyond = false;
 #pragma unroll
-      for (int x = 0; x < QT; ++x) {
-        const float next = fmaxf(m[x], column_max(top[x]));
-        const float keep = m[x] == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f((m[x] - next) * factor[x]);
-        m[x] = next;
-        beyond |= next != -__builtin_inff() && !(fabsf(next * factor[x]) <= kFar);
-        l[x] *= keep;
+        for (int x = 0; x < QT; ++x) {
+          const float next = fmaxf(m[x], column_max(top[x]));
+          const float keep = m[x] == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f((m[x] - next) * factor[x]);
+          m[x] = next;
+          beyond |= next != -__builtin_inff() && !(fabsf(next * factor[x]) <= kFar);
+          l[x] *= keep;
 #pragma unroll
-        for (int gi = 0; gi < G; ++gi) {
-          if (ZERO_PRODUCT)
-            zp[x][ZERO_PRODUCT ? gi : 0] *= keep * by;
-          else
-            zs[x][gi] *= keep * by;
+          for (int gi = 0; gi < G; ++gi) rescale(x, gi, keep * by);
         }
-#pragma unroll
-        for (int e = 0; e < NE; ++e) o[x][e] *= keep * by;
+        far = __any(beyond);
       }
-      far = __any(beyond);
     }
     if (far) {
       asm volatile("; a branch: not worth computing for every step");
@@ -952,32 +1030,35 @@ template <class T, int H, int QH, int D, int GROUP, int P, bool CAUSAL, bool LSE
     for (int gi = 0; gi < G; ++gi)
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        vs[gi][k] *= unit;
+        if (!APART) vs[gi][k] *= unit;
         zero[gi][k] = high_halves(s.vp[k / 2][gi][2 * (k % 2)], s.vp[k / 2][gi][2 * (k % 2) + 1]) & mask0;
       }
     const f16x8 ones = {1, 1, 1, 1, 1, 1, 1, 1};
     u32x4 p[QT][G];
+    float back[QT][G];  // APART: from a row's own unit
 #pragma unroll
     for (int x = 0; x < QT; ++x) {
       const float off = m[x] == -__builtin_inff() ? 0.0f : far ? kHold : fmaf(-m[x], factor[x], kHold);
       f16x8 e, fine[G];
+      float y[8];
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const float y = __builtin_amdgcn_exp2f(fmaf(sc[x][i], factor[x], off));
-        if (EXACT_SUM) l[x][0] += y;
-        e[i] = (_Float16)y;
-        if (FINE)
+        y[i] = __builtin_amdgcn_exp2f(fmaf(sc[x][i], factor[x], off));
+        if (EXACT_SUM) l[x][0] += y[i];
+        e[i] = (_Float16)y[i];
+        if (FINE && !APART)
 #pragma unroll
-          for (int gi = 0; gi < G; ++gi) fine[gi][i] = (_Float16)fmaf(y, (float)vs[gi][i / 2][i % 2], 0.0f);
+          for (int gi = 0; gi < G; ++gi) fine[gi][i] = (_Float16)fmaf(y[i], (float)vs[gi][i / 2][i % 2], 0.0f);
       }
       if (!EXACT_SUM) l[x] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, e, l[x], 0, 0, 0);
 #pragma unroll
       for (int gi = 0; gi < G; ++gi) {
+        if (APART) back[x][gi] = alone(x, gi, y, vs[gi], masked ? seen[x] : 0xFFu, p[x][gi]);
 #pragma unroll
-        for (int k = 0; k < 4; ++k)
+        for (int k = 0; k < 4 && !APART; ++k)
           p[x][gi][k] = __builtin_bit_cast(u32, FINE ? f16x2{fine[gi][2 * k], fine[gi][2 * k + 1]}
                                                      : f16x2{e[2 * k], e[2 * k + 1]} * vs[gi][k]);
-        if (masked) {  // a scale that is no number does not reach the columns that do not see its key
+        if (!APART && masked) {  // a scale that is no number does not reach the columns that do not see its key
           asm volatile("; a branch: not worth computing for every step");
 #pragma unroll
           for (int k = 0; k < 4; ++k)
@@ -1019,6 +1100,11 @@ template <class T, int H, int QH, int D, int GROUP, int P, bool CAUSAL, bool LSE
           if (t % TG >= FULL) multiply_values<NREST>(s, t, b, mine);
       }
     }
+    if (APART)
+#pragma unroll
+      for (int x = 0; x < QT; ++x)
+#pragma unroll
+        for (int gi = 0; gi < G; ++gi) rescale(x, gi, back[x][gi]);
     load_values(s, s.next, s.ahead);
     s.at += s.by;
     s.next = after;
@@ -1030,7 +1116,16 @@ template <class T, int H, int QH, int D, int GROUP, int P, bool CAUSAL, bool LSE
   }
 
   UNP4_DEV void walk(stream& s) {
-    while (s.at < s.last) step(s);
+    const int first = s.at, last = s.last;
+    while (s.at < s.last) step<false>(s);
+    if (s.last != last) {
+      // Scales too far apart for one unit, which a cache seldom holds: anew, each step of a row and group in its own.
+      s.at = first;
+      s.last = last;
+      clear();
+      open(s);
+      while (s.at < s.last) step<true>(s);
+    }
 #pragma unroll
     for (int x = 0; x < QT; ++x) {
       if (EXACT_SUM) l[x][0] = column_sum(l[x][0]);
