@@ -365,8 +365,8 @@ typedef struct unp_cache4 {
 int32_t unp_cache4_record_bytes(const unp_cache4* c, uint64_t* bytes, unp_error* err);
 
 /* Quantise a step's keys and values into their slots (page number * page + place).  With rot > 0 the first rot
- * elements of each key are rotated on the way (layout as above): in 64 bits from the 32-bit table, then rounded
- * once to the keys' type.  Each group of a head then takes lo = min(0, smallest), hi = max(0, largest),
+ * elements of each key are rotated on the way (layout as above): in 64 bits from the 32-bit table, then rounded to
+ * 32 bits and from there to the keys' type.  Each group of a head then takes lo = min(0, smallest), hi = max(0, largest),
  * scale = f16((hi - lo) / 15), zero = clamp(round(-lo / scale), 0, 15) and n = clamp(round(y / scale) + zero, 0, 15),
  * the quotients in 32 bits and rounded to even (scale 0 divides as 1); a group that holds a NaN or an infinity, or whose
  * scale overflows f16, takes a NaN scale.

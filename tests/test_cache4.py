@@ -1,6 +1,7 @@
 """The rotary and 4-bit cache forms without a GPU: what they refuse to lower, the sources' compilation, the record's
 size, and the reference that the GPU tests compare with."""
 import ctypes as C
+from fractions import Fraction
 
 import numpy as np
 import pytest
@@ -168,3 +169,28 @@ def test_held_memory_is_not_freed(monkeypatch, owner):
     b.free()
     del part, b
     assert freed == []
+
+
+def nearest(x: Fraction, bits: int) -> Fraction:
+    """x rounded to `bits` significant bits, ties to even (no range)."""
+    step = Fraction(1)
+    while abs(x) >= step * 2 ** bits:
+        step *= 2
+    while abs(x) < step * 2 ** (bits - 1):
+        step /= 2
+    return Fraction(round(x / step)) * step  # Python rounds a tie to the even number
+
+
+@pytest.mark.parametrize("dtype, bits", [("Bf16", 8), ("F16", 11)])
+@pytest.mark.parametrize("rest, sign", [(2.0 ** -30, 1), (-2.0 ** -30, 1), (2.0 ** -30, -1), (2.0 ** -20, 1)])
+def test_a_rotated_key_is_rounded_to_32_bits_and_then_to_its_type(dtype, bits, rest, sign):
+    """A sum beside a tie of the type: 2^-30 beside it the 32-bit number is the tie itself, 2^-20 beside it is not."""
+    x = np.zeros((1, 1, 32))
+    x[0, 0, 0], x[0, 0, 16] = sign, 1.0
+    tab = np.zeros((1, 16, 2), np.float32)
+    tab[0, 0] = 1.0 + 2.0 ** -bits, -rest * sign
+    sum_ = Fraction(float(tab[0, 0, 0])) * sign + Fraction(rest) * sign
+    want = nearest(nearest(nearest(sum_, 53), 24), bits)
+    assert (want == nearest(sum_, bits)) == (rest != 2.0 ** -30)
+    got = ref.rounded(ref.rotate(x, tab.astype(np.float64), 32, "halves"), dtype)
+    assert Fraction(float(got[0, 0, 0])) == want

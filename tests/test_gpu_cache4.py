@@ -819,3 +819,25 @@ def test_attention_of_more_blocks_than_a_launch_has_refuses(hip_device):
     some = dev(np.zeros(64, np.uint8))
     for tokens, batch in ((1 << 23, 1 << 23), (1 << 29, 1)):
         invalid(ex, some, some, some, some, some, some, some, tokens, batch, 1, 1, 256, 64, 256, 64, 0, 0)
+
+
+@pytest.mark.parametrize("dtype, bits", [("Bf16", 8), ("F16", 11)])
+@pytest.mark.parametrize("layout", ["halves", "pairs"])
+def test_append_rounds_a_rotated_key_to_32_bits_and_then_to_its_type(hip_device, dtype, bits, layout):
+    """Sums within 2^-30 and 2^-20 of a tie of the type, each the largest of its group: the scale shows how it was rounded."""
+    dim, rests = 32, [2.0 ** -30, -2.0 ** -30, 2.0 ** -20, -2.0 ** -20]
+    x = np.zeros((len(rests), 1, dim))
+    x[..., 0] = x[..., dim // 2 if layout == "halves" else 1] = 1.0
+    tab = np.zeros((len(rests), dim // 2, 2), np.float32)
+    tab[:, 0, 0], tab[:, 0, 1] = 1.0 + 2.0 ** -bits, np.negative(rests)
+    # Beside the tie by less than half of a 32-bit step: the tie, and so the even one of its neighbours, 1.
+    top = np.array([1.0, 1.0, 1.0 + 2.0 ** (1 - bits), 1.0])
+    form = dict(dtype=dtype, kv_heads=1, head_dim=dim, page=16)
+    cache, some = dev(np.zeros(u.cache4_page_bytes(**form), np.uint8)), dev(np.arange(len(rests), dtype=np.int32))
+    run(executor("lower_cache4_append", **form, rot=dim, layout=layout), dev(ref.stored(x, dtype)), dev(ref.stored(x, dtype)), some,
+        cache, some, dev(tab), len(rests), 1, dim, dim, dim, dim, 0, len(rests))
+    words = cache.download(np.uint8, u.cache4_page_bytes(**form))[16 * dim:16 * dim + 4 * len(rests)].view(np.uint16)[::2]
+    # The other element of the pair is c less s, of a smaller rest: the same largest but for the two sums' signs of it.
+    other = ref.rounded(1.0 + 2.0 ** -bits - np.array(rests), dtype)
+    want = (np.maximum(top, other).astype(np.float32) / np.float32(15)).astype(np.float16)
+    assert np.array_equal(words.view(np.float16), want)

@@ -232,7 +232,7 @@ int32_t lower_cache4_append(const unp_cache4& c, int32_t rot, int32_t layout, Lo
     for (const char* s : {"table_first", "table_rows"}) ps.push_back({s, nullptr, "I64"});
   L.interface_json = interface(L, "cache4_append", cache_fields(c) + ",\"rot\":" + std::to_string(rot), ps,
                                "a word of 8 codes per lane; blocks stride over the heads", {kAlignedWhen, "otherwise"},
-                               nullptr, "keys rotated in f64 and rounded once to their type; codes of correctly rounded quotients");
+                               nullptr, "keys rotated in f64, rounded to f32 and then to their type; codes of correctly rounded quotients");
   return UNP_OK;
 }
 

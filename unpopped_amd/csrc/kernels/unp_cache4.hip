@@ -291,8 +291,9 @@ template <int H, int W> struct items {
 // issuing in 70% of the cycles (a plain stream of these bytes 17).  Four tokens are taken together, whose value words lie
 // together.
 //
-// The codes are those of exact arithmetic.  The rotation's products of a 16-bit element and a 32-bit cosine are exact in
-// f64, so the rotated key is rounded once to 53 bits and once to its type, however the sum is contracted.  A quotient
+// The codes are those of exact arithmetic on the rotated keys.  The rotation's products of a 16-bit element and a 32-bit
+// cosine are exact in f64, so the rotated key is rounded to 53 bits, to 24 and to its type, however the sum is contracted: a key
+// in 32 bits, as a program that rotates before it appends has it, then one in the cache's type.  A quotient
 // y / s of two 11-bit numbers that is no tie between two codes is at least 2^-13 from one ((2 y - (2 n + 1) s) / 2 s is
 // a multiple of y's or s's last place), and y times a reciprocal good to 2^-23 is off by less than 2^-17: it rounds
 // as the quotient does, and only where some lane's comes within 2^-16 of a tie the wave divides.
