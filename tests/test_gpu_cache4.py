@@ -841,3 +841,19 @@ def test_append_rounds_a_rotated_key_to_32_bits_and_then_to_its_type(hip_device,
     other = ref.rounded(1.0 + 2.0 ** -bits - np.array(rests), dtype)
     want = (np.maximum(top, other).astype(np.float32) / np.float32(15)).astype(np.float16)
     assert np.array_equal(words.view(np.float16), want)
+
+
+@pytest.mark.parametrize("dtype, heads, kv, dim, group, rows, lengths, entry", [
+    ("Bf16", 16, 1, 128, 128, [1, 1], [600, 33], "_lse_few"),
+    ("Bf16", 16, 1, 128, 128, [3, 2], [600, 530], "_cached_few"),    # more heads than columns are shared by
+    ("F16", 8, 2, 192, 64, [5, 11], [540, 20], "_more"),             # more words than a wave holds twice
+    ("Bf16", 12, 4, 64, 64, [2, 3], [900, 600], "_some"),
+])
+@pytest.mark.parametrize("workspace", [True, 0])
+def test_attention_reads_what_several_blocks_read_through_the_caches(hip_device, dtype, heads, kv, dim, group, rows, lengths, entry,
+                                                                     workspace):
+    ex = executor("lower_cache4_attention", dtype=dtype, heads=heads, kv_heads=kv, head_dim=dim, group=group, page=32,
+                  causal=True, lse=True, scale=0.0)
+    attention_case(dtype, heads, kv, dim, group, 32, rows, lengths, workspace=workspace, seed=22, behind=0)
+    last = ex.last_launch()["entry"]
+    assert last.endswith(entry) or (workspace and last.endswith("_join")), last

@@ -317,8 +317,12 @@ int32_t lower_cache4_attention(const unp_cache4& c, const unp_attention& a, Lowe
   int cg = gq <= 4 ? 4 : gq <= 8 ? 2 : 1;
   while (cg > 1 && held(cg, 1) > 176) cg /= 2;
   add("_few", 1, cg, 1, 4, true, held(cg, 1) <= 204 ? 2 : 1);
-  if (cg > 1) add("_some", 1, 1, 1, 4, false, held(1, 1) <= 204 ? 2 : 1);
+  // For sequences of several tiles, whose blocks read the same keys: through the caches, and of one row a column where the first
+  // shares them (32 heads over 2, 64 sequences of up to 2 and 4 tokens over 3000 keys 22.7 and 29.2 us, past the caches 26.1 and
+  // 33.0; heads of 192, groups of 64, up to 16 tokens 140 and 152).
   const int qt = held(1, 2) <= 204 ? 2 : 1, per_simd = held(1, qt) <= 204 ? 2 : 1;
+  const bool some = cg > 1 || qt > 1;  // else `_more` has the same tiles
+  if (some) add(cg > 1 ? "_some" : "_cached_few", 1, 1, 1, 4, false, held(1, 1) <= 204 ? 2 : 1);
   add("_more", qt, 1, 1, 4, false, per_simd);
   add("_many", qt, 1, 4, 1, false, per_simd);
   Entry e;
@@ -329,7 +333,7 @@ int32_t lower_cache4_attention(const unp_cache4& c, const unp_attention& a, Lowe
       << ">(starts, out, lse, ws, a);\n}\n";
   L.source = src.str();
   std::vector<std::string> when = {"a sequence has no more rows of a key/value head, on average, than one of its tiles"};
-  if (cg > 1) when.push_back("at most one of its tiles, or four over a long context");
+  if (some) when.push_back("at most one of its tiles, or four over a long context");
   when.push_back("a long context and at most eight of its tiles, or too few blocks of the next");
   when.push_back("otherwise");
   when.push_back("after any of them, where a context is split");

@@ -567,8 +567,8 @@ template <> struct is_half<_Float16> {
   static constexpr bool value = true;
 };
 
-// Adjacent words; ONCE: what this launch reads once (a sequence's rows fill one tile) goes past the caches (64 single tokens over up to 16384 keys took
-// 154 us through them, 141 past them).
+// Adjacent words; ONCE: what this launch reads once (a sequence's rows fill one tile) goes past the caches (64 single tokens
+// over up to 16384 keys took 154 us through them, 141 past them).
 typedef u32 u32x2 __attribute__((ext_vector_type(2)));
 template <class V, bool ONCE> UNP4_DEV V words_at(const u32* p) {
   const V* v = reinterpret_cast<const V*>(p);

@@ -2085,6 +2085,8 @@ AttentionPlan attention_plan(const unp_exec* x, int64_t tokens, int64_t batch, i
   const bool deep = keys > 4 * x->l.entries[more].k;
   while (p.entry + 1 < more && !at_most(p.entry, 1)) ++p.entry;
   if (!at_most(p.entry, deep ? 4 : 1)) p.entry = deep && (at_most(more, 8) || 2 * tiles(own) < holds(own)) ? more : own;
+  // Several tiles of a sequence read its keys through the caches, which the first entry does not.
+  if (p.entry == 0 && !at_most(0, 1)) p.entry = more;
   const bool several = p.entry >= more || !at_most(p.entry, 1);  // tiles of a sequence
   const unp::Entry& e = x->l.entries[p.entry];
   p.slots = rows / e.vec + batch;
