@@ -857,3 +857,48 @@ def test_attention_reads_what_several_blocks_read_through_the_caches(hip_device,
     attention_case(dtype, heads, kv, dim, group, 32, rows, lengths, workspace=workspace, seed=22, behind=0)
     last = ex.last_launch()["entry"]
     assert last.endswith(entry) or (workspace and last.endswith("_join")), last
+
+
+def entry_case(entry, dtype, heads, kv, dim, group, rows, lengths, page=16, lse=False, joined=None, **how):
+    """A launch without a workspace, whose entry it is, and then with one (`joined`: whether that splits the contexts)."""
+    for workspace in (0, True):
+        attention_case(dtype, heads, kv, dim, group, page, rows, lengths, lse=lse, workspace=workspace, behind=0, seed=dim + group + heads,
+                       **how)
+        last = executor("lower_cache4_attention", dtype=dtype, heads=heads, kv_heads=kv, head_dim=dim, group=group, page=page,
+                        causal=True, lse=lse, scale=0.0).last_launch()["entry"]
+        assert last.endswith(entry) or (workspace and last.endswith("_join")), last
+        assert joined is None or not workspace or last.endswith("_join") == joined
+
+
+DECODE = [(128, 128, 16), (128, 64, 64), (64, 64, 32)]
+
+
+@pytest.mark.parametrize("group_heads", [1, 2, 4, 5, 7, 8, 9, 16])
+@pytest.mark.parametrize("dim, group, page", DECODE)
+def test_attention_of_a_decode_step(hip_device, group_heads, dim, group, page):
+    """One token a sequence: the columns shared by four, two and one sets of keys, some of them past the last."""
+    entry_case("_few", ["Bf16", "F16"][group_heads % 2], 2 * group_heads, 2, dim, group, [1, 1, 1], [1, 131, 70], page=page, joined=False)
+
+
+@pytest.mark.parametrize("group_heads", [1, 4, 8, 16])
+@pytest.mark.parametrize("dim, group, page", DECODE)
+def test_attention_of_a_decode_step_over_a_split_context(hip_device, group_heads, dim, group, page):
+    entry_case("_few", ["Bf16", "F16"][group_heads % 2], 2 * group_heads, 2, dim, group, [1, 1], [1400, 33], page=page, width=2400 // page,
+               joined=True)
+
+
+SHAPES = [("Bf16", d, g) for d, g in ((64, 32), (96, 96), (96, 32), (128, 128), (128, 64), (128, 32), (160, 160), (192, 192), (192, 64),
+                                      (224, 224), (224, 32), (256, 256), (256, 128), (256, 32))]
+SHAPES += [("F16", d, g) for d, g in ((64, 32), (128, 128), (128, 64), (160, 32), (192, 192), (256, 64))]
+
+
+@pytest.mark.parametrize("dtype, dim, group", SHAPES)
+def test_attention_of_prompts(hip_device, dtype, dim, group):
+    """Waves of rows of their own: several blocks of a sequence, the last of them in part, and a sequence of one."""
+    entry_case("_many", dtype, 6, 2, dim, group, [101, 1, 37], [101, 20, 60], page=32)
+
+
+@pytest.mark.parametrize("dtype, dim, group", SHAPES)
+def test_attention_of_a_few_dozen_rows(hip_device, dtype, dim, group):
+    """Waves that share the keys of a tile or two, of the last row tile in part."""
+    entry_case("_more", dtype, 6, 2, dim, group, [31, 26], [530, 61], page=32)
