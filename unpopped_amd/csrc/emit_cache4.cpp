@@ -305,8 +305,9 @@ int32_t lower_cache4_attention(const unp_cache4& c, const unp_attention& a, Lowe
   const int gq = a.heads / c.kv_heads;
   // What a wave holds, in registers: the words of a step, the rows, their sums and the words of groups.  The kernels
   // take about 60 more, and two waves of a SIMD have 256 each (a SIMD's one wave of twice the rows took 646 us for
-  // prompts that two take 380 for).  A whole head of 192 is at 204: two of its tiles keep up to 60 words in scratch and
-  // are still the faster (4206 tokens x 16 heads f16 182 us, 191 with one).
+  // prompts that two take 380 for).  A whole head of 192 is at 204: two of its tiles keep up to 50 words in scratch and
+  // are mostly the faster (three prompts of up to 4099 tokens x 16 heads over 8 Bf16 280 us, 315 with one, F16 335 and 328;
+  // 16 sequences of up to 100 rows over 6000 keys 112 and 168, 128 and 172).
   const int deep = c.head_dim / 32, groups = c.head_dim / c.group, words = c.group / 8, rest = words % 16;
   const int tiles = groups * (words / 16 + (rest > 0));
   const int products = groups * (words / 16 * 8 + (rest == 0 ? 0 : rest <= 4 ? 2 : rest <= 8 ? 4 : 8));

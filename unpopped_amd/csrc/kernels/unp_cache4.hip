@@ -435,8 +435,8 @@ UNP4_DEV void read(const I* slots, const u32* cache, T* k, T* v, const cache_arg
 //     p s less the sum of p s zero.  p s is rounded to f16 (both sums take it as rounded), s in a unit that puts the
 //     scales that the wave's rows see between 2^-14 and 1, exactly: then what p s loses below f16's normal numbers is less
 //     than 2^-20 of the smallest scale.  Where the scales lie further apart than that, the wave begins anew: p s is made in
-//     f32, and each step of a row and group rounds it in a unit of its own (9847 tokens as below 355 us with and without the
-//     check; 32 sequences of up to 400 x 32 rows 430 us with scales too far apart, 265 without).  The scores are, lane by
+//     f32, and each step of a row and group rounds it in a unit of its own (9847 tokens as below 355 us without the
+//     check and 353 with it; 32 sequences of up to 400 x 32 rows 265 us, 430 with scales too far apart, 294 with scales of 0).  The scores are, lane by
 //     lane, the operand that this product needs when its key (g, i) of 4 x 8 is key 16 CG (i / 4) + 4 g + i % 4; a lane reads
 //     four tokens' words of 8 elements at once and pairs of tokens of one element are made by byte permutes, so nothing
 //     goes through LDS.
@@ -447,7 +447,6 @@ UNP4_DEV void read(const I* slots, const u32* cache, T* k, T* v, const cache_arg
 // ---------------------------------------------------------------------------------------
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
-typedef u16 u16x2 __attribute__((ext_vector_type(2)));
 
 struct attention_args {
   i64 tokens, batch, width, pages, q_token, q_head, out_token, out_head, window;
@@ -481,6 +480,22 @@ UNP4_DEV float high_half(u32 w) { return (float)__builtin_bit_cast(_Float16, (u1
 // The low, or high, halves of two words.
 UNP4_DEV u32 low_halves(u32 a, u32 b) { return __builtin_amdgcn_perm(b, a, 0x05040100u); }
 UNP4_DEV u32 high_halves(u32 a, u32 b) { return __builtin_amdgcn_perm(b, a, 0x07060302u); }
+
+// The maximum of each half over the wave.
+typedef u16 u16x2 __attribute__((ext_vector_type(2)));
+template <int CTRL> UNP4_DEV u16x2 half_max(u16x2 x) {
+  const u32 w = __builtin_bit_cast(u32, x);
+  return __builtin_elementwise_max(x, __builtin_bit_cast(u16x2, __builtin_amdgcn_update_dpp(w, w, CTRL, 0xF, 0xF, false)));
+}
+UNP4_DEV u16x2 wave_max(u16x2 x) {
+  u32 w = __builtin_bit_cast(u32, x);
+  auto y = __builtin_amdgcn_permlane32_swap(w, w, false, false);
+  x = __builtin_elementwise_max(__builtin_bit_cast(u16x2, (u32)y[0]), __builtin_bit_cast(u16x2, (u32)y[1]));
+  w = __builtin_bit_cast(u32, x);
+  y = __builtin_amdgcn_permlane16_swap(w, w, false, false);
+  x = __builtin_elementwise_max(__builtin_bit_cast(u16x2, (u32)y[0]), __builtin_bit_cast(u16x2, (u32)y[1]));
+  return half_max<0x140>(half_max<0x141>(half_max<0x4E>(half_max<0xB1>(x))));  // pairs, fours, eights, the row
+}
 
 UNP4_DEV int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
 // Memory that this launch does not write, read at a place all lanes share: a scalar load, which does not queue
@@ -625,10 +640,9 @@ template <class T, int H, int QH, int D, int GROUP, int P, bool CAUSAL, bool LSE
   float m[QT];                    // running maximum
   bool far;                       // some maximum is beyond 2^kFar in log2 (all lanes agree)
   f32x4 l[QT];                    // the sum of p, in l[0] (EXACT_SUM: this lane's part of it until the end)
-  // The value scales that the wave's rows saw so far, the same in all lanes: but for 0 none is below `least`, their f16 bits
-  // are from `low` (in both halves) to `span` above it, and `unit`, a power of two, puts them between 2^-14 and 1.
+  // The value scales that the wave's rows saw so far, the same in all lanes: their f16 bits, but for zeros, are from `low` (in
+  // both halves) to `span` above it, and `unit`, a power of two, puts them between 2^-14 and 1.
   _Float16 unit;
-  float least;
   u32 low, span;
   f32x4 o[QT][NE];
   // The sums of p s zero by group: this lane's parts, or (one group of columns, few of elements) a product whose rows
@@ -642,9 +656,8 @@ template <class T, int H, int QH, int D, int GROUP, int P, bool CAUSAL, bool LSE
   int end[QT], begin[QT];  // keys that the column sees
 
   UNP4_DEV void clear() {
-    unit = (_Float16)1.0f;
-    least = __builtin_inff();
-    low = span = 0;
+    unit = (_Float16)0x1p14f;
+    low = span = 0;  // no scales yet
     far = false;
 #pragma unroll
     for (int x = 0; x < QT; ++x) {
@@ -852,37 +865,37 @@ template <class T, int H, int QH, int D, int GROUP, int P, bool CAUSAL, bool LSE
       }
     return most[0] > span || most[1] > span;
   }
-  // Takes a step's value scales (of keys that some row sees) into the known range.  Gives what the sums are multiplied with as
-  // their unit changes: 0 where no unit holds the range.
-  UNP4_DEV float widen(const f16x2 (&vs)[G][4], u32 seen) {
-    u32 top = 0, bottom = 0xFFFF;
+  // Takes a step's value scales (under a mask those of keys that some row sees) into the known range, by their bits.  Gives what
+  // the sums are multiplied with as their unit changes: 0 where no unit holds the range.
+  UNP4_DEV float widen(const f16x2 (&vs)[G][4], bool mask, u32 seen) {
+    u16x2 top = {0, 0}, bottom = {0, 0};  // bottom: 2^16 less the smallest, 0 for none
 #pragma unroll
     for (int gi = 0; gi < G; ++gi)
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const u32 b = __builtin_bit_cast(u32, vs[gi][i / 2]) >> (16 * (i % 2)) & 0x7FFFu;
-        // Zeros weigh nothing, and no unit makes an infinity or a NaN a number.
-        const bool counts = b != 0 && b < 0x7C00u && (seen >> i & 1);
-        top = counts && b > top ? b : top;
-        bottom = counts && b < bottom ? b : bottom;
+      for (int k = 0; k < 4; ++k) {
+        u16x2 b = __builtin_bit_cast(u16x2, __builtin_bit_cast(u32, vs[gi][k]) & 0x7FFF7FFFu);
+        // No unit makes an infinity or a NaN a number.
+        b *= __builtin_elementwise_min(__builtin_elementwise_sub_sat(u16x2{0x7C00, 0x7C00}, b), u16x2{1, 1});
+        if (mask) b *= u16x2{(u16)(seen >> (2 * k) & 1), (u16)(seen >> (2 * k + 1) & 1)};
+        top = __builtin_elementwise_max(top, b);
+        bottom = __builtin_elementwise_max(bottom, (u16x2)(u16x2{0, 0} - b));
       }
-    top = (u32)uniform((int)lane_max<16>(column_max((float)top)));
-    bottom = (u32)uniform((int)-lane_max<16>(column_max(-(float)bottom)));
-    if (top == 0) return 1.0f;
+    const u16x2 ends = wave_max(__builtin_elementwise_max(u16x2{top[0], bottom[0]}, u16x2{top[1], bottom[1]}));
+    const u32 both = (u32)uniform(__builtin_bit_cast(int, ends)), most = both & 0xFFFFu, least = 0x10000u - (both >> 16);
+    if (most == 0) return 1.0f;
     // A bit of room above and two below, so that later scales seldom pass the range.
-    const u32 known = low + span & 0xFFFFu, next = ((top >> 10) + 1) << 10 | 0x3FFu;
-    const u32 end = top <= known ? known : next < 0x7BFFu ? next : 0x7BFFu;
-    const float small = (float)__builtin_bit_cast(_Float16, (u16)bottom);
-    // 2^14 over the exponent's bits: `end` times it is below 1.
-    const float to = __builtin_bit_cast(float, (u32)uniform((int)((141u - (end >> 10)) << 23)));
-    least = fminf(least, fmaxf(small * 0.25f, fminf(small, 0x1p-14f / to)));
-    if (least * to < 0x1p-14f) return 0.0f;
-    const u32 from = (u32)__builtin_bit_cast(u16, (_Float16)least);
-    low = (u32)uniform((int)(from | from << 16));
-    span = (u32)uniform((int)(end - from));
-    const float by = to / (float)unit;
-    unit = (_Float16)to;
-    return by;
+    const u32 known = low + span & 0xFFFFu, next = ((most >> 10) + 1) << 10 | 0x3FFu;
+    const u32 end = most <= known ? known : next < 0x7BFFu ? next : 0x7BFFu;
+    const int exponent = (int)(end >> 10);  // of `end`, 15 too large: 2^14 over it times `end` is below 1
+    const u32 limit = exponent >= 14 ? (u32)(exponent - 13) << 10 : exponent >= 4 ? 1u << (exponent - 4) : 0u;  // 2^-14 in it
+    u32 from = least > 0xC00u ? least - 0x800u : 1u;
+    from = from > limit ? from : least < limit ? least : limit;
+    from = span != 0 && (low & 0xFFFFu) < from ? low & 0xFFFFu : from;
+    if (from < limit) return 0.0f;
+    low = from | from << 16;
+    span = end - from;
+    unit = (_Float16)__builtin_bit_cast(float, (u32)(141 - exponent) << 23);
+    return __builtin_bit_cast(float, (u32)(127 + (int)(known >> 10) - exponent) << 23);
   }
 
   // The sums of a row tile and group into another unit.
@@ -999,9 +1012,7 @@ template <class T, int H, int QH, int D, int GROUP, int P, bool CAUSAL, bool LSE
     if (__any(up || past)) {
       if (!APART) past = outside<true>(vs);
       if (__any(past)) {
-        u32 any = masked ? seen[0] : 0xFFu;
-        if (masked && QT > 1) any |= seen[QT - 1];
-        by = widen(vs, any);
+        by = widen(vs, masked, masked ? seen[0] | seen[QT - 1] : 0xFFu);
         s.last = by == 0.0f ? s.at : s.last;
       }
       if (__any(up || past)) {
@@ -1119,11 +1130,12 @@ template <class T, int H, int QH, int D, int GROUP, int P, bool CAUSAL, bool LSE
   UNP4_DEV void walk(stream& s) {
     const int first = s.at, last = s.last;
     while (s.at < s.last) step<false>(s);
-    if (s.last != last) {
+    if (__builtin_expect(s.last != last, 0)) {
       // Scales too far apart for one unit, which a cache seldom holds: anew, each step of a row and group in its own.
       s.at = first;
       s.last = last;
       clear();
+      unit = (_Float16)1.0f;
       open(s);
       while (s.at < s.last) step<true>(s);
     }
