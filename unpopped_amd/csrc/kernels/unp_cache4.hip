@@ -54,10 +54,11 @@ template <class T, int N> UNP4_DEV void store_stream(T* p, const vec<T, N>& x) {
 // ---------------------------------------------------------------------------------------
 // Position tables: [count][ROT / 2][cos, sin] of position first + row.
 //
-// A write of what 64-bit arithmetic makes (262144 x 64 pairs 30 us, 4.5 TB/s), so the arithmetic is kept below it: the product of position and frequency
-// is taken in turns (frequency / 2 pi), whose whole and quarter part go off exactly, and on the remaining eighth of a turn
-// either side sine and cosine are their series to x^11 and x^10 (off by less than 2^-33, rounded to 2^-24 after).  A
-// lane makes V adjacent pairs; a block computes the ROT / 2 frequencies once, into LDS.
+// 64-bit arithmetic beside a write of what it makes: 262144 x 64 pairs take 30 us, a plain write of them 21, and the VALU
+// issues in 60% of the cycles.  The product of position and frequency is taken in turns (frequency / 2 pi), whose whole and
+// quarter part go off exactly, and on the remaining eighth of a turn either side sine and cosine are their series to x^11
+// and x^10 (off by less than 2^-33, rounded to 2^-24 after).  A lane makes V adjacent pairs; a block computes the ROT / 2
+// frequencies once, into LDS.
 // ---------------------------------------------------------------------------------------
 struct stretch {
   int kind;
@@ -131,9 +132,10 @@ UNP4_DEV void rope_table(float* out, i64 first, i64 count, const stretch& s) {
 //
 // (x0, x1) -> (x0 c - x1 s, x1 c + x0 s), the sine negated for the inverse.  It reads and writes each
 // element once: a stream.  A unit of the vector entry is V pairs (two 16-byte loads and stores) or 2V
-// elements that are only copied; the plain entry takes a pair or a copied element at a time.  An output larger than half
-// of the last-level cache is stored past the caches: 16384 tokens x 40 heads x 128 bf16 65.2 us against 67.3 (5.3 TB/s),
-// but 4001 x 24 x 128 f32 (49 MB) 19.6 against 17.4.
+// elements that are only copied; the plain entry takes a pair or a copied element at a time (16384 tokens x 40 heads of 100,
+// all of it rotated, 135 us, 2.0 TB/s; of 80, of which 20, 187 us).  An output larger than half of the last-level cache is
+// stored past the caches: 16384 tokens x 40 heads x 128 bf16 65.2 us against 67.3 (5.3 TB/s, a plain copy 6.35), but
+// 4001 x 24 x 128 f32 (49 MB) 19.6 against 17.4.
 // ---------------------------------------------------------------------------------------
 struct rope_args {
   i64 tokens, x_token, x_head, out_token, out_head, first, rows;
@@ -288,7 +290,7 @@ template <int H, int W> struct items {
 // Append: a lane holds one word's 8 elements of a key or a value head; a group's range is reduced over
 // its lanes.  It reads the keys and values once and writes a quarter of that: a stream, if the arithmetic keeps out of
 // its way.  It does not quite: 16384 tokens x 8 heads x 128 bf16 take 42 us, of which the exact rotation is 7, with the VALU
-// issuing in 70% of the cycles (a plain stream of these bytes 17).  Four tokens are taken together, whose value words lie
+// issuing in 70% of the cycles (a plain copy of these bytes 15).  Four tokens are taken together, whose value words lie
 // together.
 //
 // The codes are those of exact arithmetic on the rotated keys.  The rotation's products of a 16-bit element and a 32-bit
@@ -436,14 +438,15 @@ UNP4_DEV void read(const I* slots, const u32* cache, T* k, T* v, const cache_arg
 //     scales that the wave's rows see between 2^-14 and 1, exactly: then what p s loses below f16's normal numbers is less
 //     than 2^-20 of the smallest scale.  Where the scales lie further apart than that, the wave begins anew: p s is made in
 //     f32, and each step of a row and group rounds it in a unit of its own (9847 tokens as below 355 us without the
-//     check and 353 with it; 32 sequences of up to 400 x 32 rows 265 us, 430 with scales too far apart, 294 with scales of 0).  The scores are, lane by
-//     lane, the operand that this product needs when its key (g, i) of 4 x 8 is key 16 CG (i / 4) + 4 g + i % 4; a lane reads
-//     four tokens' words of 8 elements at once and pairs of tokens of one element are made by byte permutes, so nothing
-//     goes through LDS.
+//     check and 353 with it; 32 sequences of up to 400 x 32 rows 265 us, 430 with scales too far apart, 294 with every
+//     fifth of them 0).  The scores are, lane by lane, the operand that this product needs when its key (g, i) of 4 x 8 is key
+//     16 CG (i / 4) + 4 g + i % 4; a lane reads four tokens' words of 8 elements at once and pairs of tokens of one
+//     element are made by byte permutes, so nothing goes through LDS.
 //
-// What bounds it: a decode step its reads (64 single tokens x 8 heads over up to 16384 keys 138 us, 5.4 TB/s; one over 262144
-// keys 51, 5.9 TB/s), a prompt the VALU's issue (9847 tokens x 32 heads of three sequences, causal, 355 us, 784
-// TFLOP/s: 78% of the cycles issue VALU or matrix instructions, about 300 for 32 rows and 32 keys).
+// What bounds it: a decode step its reads (64 single tokens x 8 heads over up to 16384 keys 139 us, 5.4 TB/s, a plain read
+// 7.07; one over 262144 keys 52, 5.8 TB/s), a prompt the VALU's issue (9847 tokens x 32 heads of three sequences, causal,
+// 350-355 us one after another, 790 TFLOP/s: 77% of the cycles issue VALU or matrix instructions, about 300 for 32 rows
+// and 32 keys; 425 on a card that was idle before).
 // ---------------------------------------------------------------------------------------
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
