@@ -400,9 +400,10 @@ typedef struct unp_attention {
  *   Keys that no row may see do not count, whatever they hold: keys past a sequence's length, keys of a page number
  *   outside the cache, keys past width pages.  Rows that no sequence names are left as they were.  starts do not
  *   decrease; in a list that does, which sequence takes a row, if any, is not said.
- *   The scores, the softmax's statistics and the sums are held in 32 bits.  A query's elements are held to 2^-34 of its
- *   row's largest.  A probability (Bf16) and its product with a value's scale are rounded to f16, of a unit that follows
- *   the scales: relative to what they are, and to less than 2^-20 of the smallest scale that the row sees or 2^-35 of the
+ *   The scores, the softmax's statistics and the sums are held in 32 bits, to which the matrix unit adds the products of
+ *   32 keys or elements at a time: of an element and a key's code to 2^-14 of the row's largest element, of a probability
+ *   and a value's code to 2^-16 of the largest of those keys', together to 2^-11 of the largest scale.  A probability (Bf16) and its product with a value's scale are rounded to f16, of a unit that follows
+ *   the scales: relative to what they are, and to less than 2^-20 of the smallest scale but 0 that the row sees or 2^-35 of the
  *   largest product.  So other groups, keys that a row does not see and keys of little weight cost its values no bits,
  *   whatever their scales.  The workspace (16-byte aligned) holds the parts
  *   of a context that is split over blocks; one smaller than unp_hip_exec_workspace says, 0 among them, lowers the

@@ -176,3 +176,39 @@ def test_a_scale_that_is_no_number_stays_with_its_group(hip_device, bad, spread)
     hit[25:, :, :group] = True
     assert not np.isfinite(got[hit]).any()
     assert (np.abs(got - want) <= tolerance(want, mass, fifteen, reach, n, dim, "Bf16"))[~hit].all()
+
+
+@pytest.mark.parametrize("code, zero", [(0, 15), (15, 0), (15, 7)])
+@pytest.mark.parametrize("dtype, heads, dim, group, rows", [("F16", 16, 64, 64, 1), ("Bf16", 2, 64, 32, 20), ("F16", 2, 128, 32, 70),
+                                                            ("Bf16", 4, 128, 128, 90)])
+def test_faint_keys_beside_one_whose_value_is_zero(hip_device, dtype, heads, dim, group, rows, code, zero):
+    """A key that takes all but 2^-13 of the weight and whose value is 0: the output is the others'.  Products of theirs, of a
+    code or a zero point with 2^-18.2 of the largest weight, are among the smallest that a step's sums hold."""
+    n, page, scale = 32, 16, 0.25
+    cache = ref.Cache(2, 1, dim, group, page)
+    slots = np.arange(n)
+    for s in slots:
+        cache.put(s, 0, np.where((np.arange(dim) == 3) & (s > 0), -1.0, 0.0), False)
+        for d in range(dim):
+            at, shift = cache.code_at(s % page, d, True)
+            cache.bytes[s // page, 0, at] |= np.uint8((8 if s == 0 else code) << shift)
+    zeros = np.full((n, 1, dim // group), zero)
+    zeros[0] = 8
+    with_value_scales(cache, slots, np.full(zeros.shape, scale), zeros)
+    q = np.zeros((rows, heads, dim))
+    q[..., 3] = ref.rounded(np.float32(18.2 * np.log(2) * np.sqrt(dim)), dtype)
+    args = (np.arange(2, dtype=np.int32)[None], np.array([0, rows], np.int32), np.array([n], np.int32))
+    want, _, mass, _, reach = ref.attend(q, cache, *args, causal=False)
+    ex = executor("lower_cache4_attention", dtype=dtype, heads=heads, kv_heads=1, head_dim=dim, group=group, page=page, causal=False)
+    out = dev(np.zeros(q.size, np.uint16))
+    run(ex, dev(ref.stored(q, dtype)), dev(cache.bytes), *(dev(a) for a in args), out, dev(np.zeros(16, np.uint8)), rows, 1, 2, 2,
+        heads * dim, dim, heads * dim, dim, 0, 0)
+    got = ref.loaded(out.download(np.uint16, q.size), dtype).reshape(q.shape)
+    # As tolerance() has them: the roundings of p and p s and the scores', and f32 sums of at most (8 + 31 x 15 x 2^-18) p s.
+    # A product of a code is held to 2^-16 (odd elements 2^-20) of the step's largest p s, one of a zero point to 2^-21.
+    score = reach[..., None] * (30.0 / 7.0) * (dim + 4) * 2.0 ** -23
+    off = mass * (2 * 2.0 ** -11 + 2 * score + (n + 8) * 2.0 ** -23) + 2 * 8.1 * scale * (n + 8) * 2.0 ** -23
+    off += (n - 1) * scale * (np.where(np.arange(dim) % 2 == 0, 2.0 ** -16, 2.0 ** -20) * (code > 0) + 2.0 ** -21 * (zero > 0))
+    off += (np.abs(want) + off) * ref.HALF_STEP[dtype] + (2.0 ** -25 if dtype == "F16" else 0.0)
+    print("largest error / tolerance %.3g" % (np.abs(got - want) / off).max(), np.abs(want).max(), flush=True)
+    assert (np.abs(got - want) <= off).all()

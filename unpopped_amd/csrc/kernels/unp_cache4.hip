@@ -433,10 +433,17 @@ UNP4_DEV void read(const I* slots, const u32* cache, T* k, T* v, const cache_arg
 //   * softmax over the columns: a lane holds 8 keys of one column, so its maximum needs two exchanges, and
 //     only when some score passes the running one by 2^4.9: p is held as 2^11 p in f16, which ends at 2^16
 //     (moving at 2^0.9, with 2^15 p, cost a prompt 8%: the sums are multiplied anew each time).
-//   * O' += V' P' with the value words as rows, again nibbles as they lie: sum p s (n - zero) is the product of n with
-//     p s less the sum of p s zero.  p s is rounded to f16 (both sums take it as rounded), s in a unit that puts the
-//     scales that the wave's rows see between 2^-14 and 1, exactly: then what p s loses below f16's normal numbers is less
-//     than 2^-20 of the smallest scale.  Where the scales lie further apart than that, the wave begins anew: p s is made in
+//     The unit adds 32 products in 24 bits from the largest one's on, a subnormal number counting as one of 2^-14 there: what is
+//     dropped of a code's product with an element is below 2^-14 of the row's largest element.
+//   * O' += V' P' with the value words as rows: sum p s (n - zero) is the product of n with p s less the sum of p s zero.
+//     The nibbles are two bits up, n 2^-22 and n 2^-18, and the zero points normal numbers, so that no more is dropped of a
+//     product than 2^-16 (odd elements 2^-20, zero points 2^-21) of the step's largest p s: less than 2^-11 of the largest
+//     scale over all steps.  As they lie it is four times that, and all of one sign: one token over 200000 keys was off by
+//     1.72e-3 in Bf16 and is by 1.66e-3 (its rounding alone 1.64e-3), over 65536 in F16 3.6e-4 and 2.5e-4, for 3% of a
+//     prompt's time.  Key codes two bits up cost 1% more and gave nothing.
+//     p s is rounded to f16 (both sums take it as rounded), s in a unit that puts the scales that the wave's rows see
+//     between 2^-14 and 1, exactly: then what p s loses below f16's normal numbers is less than 2^-20 of the smallest
+//     scale.  Where the scales lie further apart than that, the wave begins anew: p s is made in
 //     f32, and each step of a row and group rounds it in a unit of its own (9847 tokens as below 355 us without the
 //     check and 353 with it; 32 sequences of up to 400 x 32 rows 265 us, 430 with scales too far apart, 294 with every
 //     fifth of them 0).  The scores are, lane by lane, the operand that this product needs when its key (g, i) of 4 x 8 is key
@@ -477,7 +484,7 @@ UNP4_DEV float column_sum(float x) {
   return __builtin_bit_cast(float, (u32)a[0]) + __builtin_bit_cast(float, (u32)a[1]);
 }
 
-// The halves of a word as f16, for products that take them as they are: a zero point 0..15 is the subnormal n 2^-24.
+// The halves of a word as f16, for products that take them as they are: a zero point n of 0..15 is the subnormal n 2^-24.
 UNP4_DEV float low_half(u32 w) { return (float)__builtin_bit_cast(_Float16, (u16)w); }
 UNP4_DEV float high_half(u32 w) { return (float)__builtin_bit_cast(_Float16, (u16)(w >> 16)); }
 // The low, or high, halves of two words.
@@ -637,7 +644,8 @@ template <class T, int H, int QH, int D, int GROUP, int P, bool CAUSAL, bool LSE
   int lane, c, g;  // c: the row a lane gives and the column it holds, g: its part of the depth
   int own;         // the column's group: which 16 of 16 CG keys it keeps
   // The nibbles' masks in registers: as literals each takes an operation more.
-  u32 mask0, mask1;
+  // mask0, mask1: nibbles at bits 0 and 4 of a half; mask2, mask6: at bits 2 and 6.
+  u32 mask0, mask1, mask2, mask6;
   f16x8 q[QT][KJ];
   float qsum[QT][G], factor[QT];  // of this lane's column; qsum 2^24 times, as zeros are held; factor: raw scores to log2
   float m[QT];                    // running maximum
@@ -679,6 +687,8 @@ template <class T, int H, int QH, int D, int GROUP, int P, bool CAUSAL, bool LSE
   UNP4_DEV void rows(const T* qp, const attention_args& a, const tile& t, int kv, int first, float scale, int cap) {
     asm("s_mov_b32 %0, 0x000f000f" : "=s"(mask0));
     asm("s_mov_b32 %0, 0x00f000f0" : "=s"(mask1));
+    asm("s_mov_b32 %0, 0x003c003c" : "=s"(mask2));
+    asm("s_mov_b32 %0, 0x03c003c0" : "=s"(mask6));
     clear();
 #pragma unroll
     for (int x = 0; x < QT; ++x) {
@@ -832,12 +842,12 @@ template <class T, int H, int QH, int D, int GROUP, int P, bool CAUSAL, bool LSE
       }
 #pragma unroll
       for (int e = 0; e < N; e += 4) {
-        const u32 x = __builtin_amdgcn_perm(wb, wa, e ? 0x07060302u : 0x05040100u), y = x >> 8;
-        part[e][k] = x & mask0;
-        part[e + 1][k] = x & mask1;
+        const u32 x = __builtin_amdgcn_perm(wb, wa, e ? 0x07060302u : 0x05040100u), x2 = x << 2, y = x >> 6;
+        part[e][k] = x2 & mask2;
+        part[e + 1][k] = x2 & mask6;
         if (N > 2) {
-          part[e + 2 < N ? e + 2 : 0][k] = y & mask0;
-          part[e + 3 < N ? e + 3 : 0][k] = y & mask1;
+          part[e + 2 < N ? e + 2 : 0][k] = y & mask2;
+          part[e + 3 < N ? e + 3 : 0][k] = y & mask6;
         }
       }
     }
@@ -1046,7 +1056,9 @@ template <class T, int H, int QH, int D, int GROUP, int P, bool CAUSAL, bool LSE
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         if (!APART) vs[gi][k] *= unit;
-        zero[gi][k] = high_halves(s.vp[k / 2][gi][2 * (k % 2)], s.vp[k / 2][gi][2 * (k % 2) + 1]) & mask0;
+        // A zero point n as the normal number n 2^-9.
+        const u32 z = high_halves(s.vp[k / 2][gi][2 * (k % 2)], s.vp[k / 2][gi][2 * (k % 2) + 1]) & mask0;
+        zero[gi][k] = __builtin_bit_cast(u32, __builtin_bit_cast(f16x2, z) * f16x2{(_Float16)0x1p15f, (_Float16)0x1p15f});
       }
     const f16x8 ones = {1, 1, 1, 1, 1, 1, 1, 1};
     u32x4 p[QT][G];
@@ -1151,7 +1163,7 @@ template <class T, int H, int QH, int D, int GROUP, int P, bool CAUSAL, bool LSE
   }
   // The sum of p v for element e of row g * 4 + r of tile t.
   UNP4_DEV float sum_of(int x, int t, int e, int r) const {
-    return (o[x][product(t, e)][r] * ((e & 1) ? 0x1p20f : 0x1p24f) - zs[x][t / TG] * 0x1p24f) * (1.0f / (float)unit);
+    return (o[x][product(t, e)][r] * ((e & 1) ? 0x1p18f : 0x1p22f) - zs[x][t / TG] * 0x1p9f) * (1.0f / (float)unit);
   }
 
   // Row x's elements times `by` to p, as U.  A lane's four runs of N elements of a tile lie together, so stores of one
