@@ -444,16 +444,15 @@ UNP4_DEV void read(const I* slots, const u32* cache, T* k, T* v, const cache_arg
 //     p s is rounded to f16 (both sums take it as rounded), s in a unit that puts the scales that the wave's rows see
 //     between 2^-14 and 1, exactly: then what p s loses below f16's normal numbers is less than 2^-20 of the smallest
 //     scale.  Where the scales lie further apart than that, the wave begins anew: p s is made in
-//     f32, and each step of a row and group rounds it in a unit of its own (9847 tokens as below 355 us without the
-//     check and 353 with it; 32 sequences of up to 400 x 32 rows 265 us, 430 with scales too far apart, 294 with every
-//     fifth of them 0).  The scores are, lane by lane, the operand that this product needs when its key (g, i) of 4 x 8 is key
+//     f32, and each step of a row and group rounds it in a unit of its own (the check cost a prompt
+//     nothing; 32 sequences of up to 400 x 32 rows take 269 us, 434 with scales too far apart, 296 with every fifth of them 0).  The scores are, lane by lane, the operand that this product needs when its key (g, i) of 4 x 8 is key
 //     16 CG (i / 4) + 4 g + i % 4; a lane reads four tokens' words of 8 elements at once and pairs of tokens of one
 //     element are made by byte permutes, so nothing goes through LDS.
 //
-// What bounds it: a decode step its reads (64 single tokens x 8 heads over up to 16384 keys 139 us, 5.4 TB/s, a plain read
-// 7.07; one over 262144 keys 52, 5.8 TB/s), a prompt the VALU's issue (9847 tokens x 32 heads of three sequences, causal,
-// 350-355 us one after another, 790 TFLOP/s: 77% of the cycles issue VALU or matrix instructions, about 300 for 32 rows
-// and 32 keys; 425 on a card that was idle before).
+// What bounds it: a decode step its reads (64 single tokens x 8 heads over up to 16384 keys 140 us, 5.4 TB/s, a plain read
+// 7.07; one over 262144 keys 53, 5.7 TB/s), a prompt the VALU's issue (9847 tokens x 32 heads of three sequences, causal,
+// 362 us one after another, 769 TFLOP/s: 78% of the cycles issue VALU or matrix instructions, about 310 for 32 rows and 32
+// keys; 412-425 on a card that was idle before).
 // ---------------------------------------------------------------------------------------
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
