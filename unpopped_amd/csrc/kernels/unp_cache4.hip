@@ -426,15 +426,14 @@ UNP4_DEV void read(const I* slots, const u32* cache, T* k, T* v, const cache_arg
 //     as they lie: masked to bits 0..3 or 4..7 of a 16-bit half they are the subnormal f16 numbers n 2^-24
 //     and n 2^-20, so 8 codes cost 5 operations, and the queries carry the powers of two (exactly: each row is
 //     scaled to f16's range, bf16's 8 bits fit in f16's 11).  The group's scale and zero point are applied to the
-//     f32 result: s (sum q n - zero sum q).
+//     f32 result: s (sum q n - zero sum q).  The unit adds 32 products in 24 bits from the largest one's on, a subnormal
+//     number counting as one of 2^-14 there: less than 2^-14 of the row's largest element is dropped of a product.
 //   * Few rows (a decode step) would leave most columns empty, and the softmax's cost is the lanes'.  So CG groups
 //     of columns hold the same rows and each keeps the scores of its own 16 of 16 CG keys: columns of one row are
 //     parts of its context, joined at the end as the waves are.
 //   * softmax over the columns: a lane holds 8 keys of one column, so its maximum needs two exchanges, and
 //     only when some score passes the running one by 2^4.9: p is held as 2^11 p in f16, which ends at 2^16
 //     (moving at 2^0.9, with 2^15 p, cost a prompt 8%: the sums are multiplied anew each time).
-//     The unit adds 32 products in 24 bits from the largest one's on, a subnormal number counting as one of 2^-14 there: what is
-//     dropped of a code's product with an element is below 2^-14 of the row's largest element.
 //   * O' += V' P' with the value words as rows: sum p s (n - zero) is the product of n with p s less the sum of p s zero.
 //     The nibbles are two bits up, n 2^-22 and n 2^-18, and the zero points normal numbers, so that no more is dropped of a
 //     product than 2^-16 (odd elements 2^-20, zero points 2^-21) of the step's largest p s: less than 2^-11 of the largest
@@ -444,8 +443,9 @@ UNP4_DEV void read(const I* slots, const u32* cache, T* k, T* v, const cache_arg
 //     p s is rounded to f16 (both sums take it as rounded), s in a unit that puts the scales that the wave's rows see
 //     between 2^-14 and 1, exactly: then what p s loses below f16's normal numbers is less than 2^-20 of the smallest
 //     scale.  Where the scales lie further apart than that, the wave begins anew: p s is made in
-//     f32, and each step of a row and group rounds it in a unit of its own (the check cost a prompt
-//     nothing; 32 sequences of up to 400 x 32 rows take 269 us, 434 with scales too far apart, 296 with every fifth of them 0).  The scores are, lane by lane, the operand that this product needs when its key (g, i) of 4 x 8 is key
+//     f32, and each step of a row and group rounds it in a unit of its own (the check cost a prompt nothing; 32 sequences of
+//     up to 400 x 32 rows take 269 us, 434 with scales too far apart, 296 with every fifth of them 0).
+//     The scores are, lane by lane, the operand that this product needs when its key (g, i) of 4 x 8 is key
 //     16 CG (i / 4) + 4 g + i % 4; a lane reads four tokens' words of 8 elements at once and pairs of tokens of one
 //     element are made by byte permutes, so nothing goes through LDS.
 //
