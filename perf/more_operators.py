@@ -89,7 +89,7 @@ def draw(rng) -> dict:
         # Codes of 8 bits lie in rows of whole vectors: an odd length is padded (a gradient's sum over tokens).
         return {"kind": kind, "m": m, "n": n if rng.random() < 0.4 else max(64, n // 64 * 64), "k": k if rng.random() < 0.2 else k // 16 * 16,
                 "a": rng.choice(["Fp8E4M3FN", "Fp8E4M3FN", "Fp8E5M2"]), "b": rng.choice(["Fp8E4M3FN", "Fp8E4M3FN", "Fp8E5M2"]),
-                "b_rows": rng.choice([128, 128, 1]), "out": rng.choice(["Bf16", "Bf16", "F16", "F32"]), "groups": groups}
+                "b_rows": rng.choice([128, 128, 1]), "out": rng.choice(["Bf16", "Bf16", "F16"]), "groups": groups}
     if kind == "experts":
         while True:
             rows, groups = rng.choice([rng.randint(1, 128), _log(rng, 1, 16384)]), _log(rng, 1, 128)
