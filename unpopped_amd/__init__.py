@@ -40,6 +40,7 @@ FORMS = {"reduction": 0, "scan": 1, "gather": 2, "dequant4": 3, "row_reduce2": 4
 DTYPE_SUPPORT = {0: "Supported", 1: "Unsupported", 2: "NotExpressible"}
 ROPE_SCALINGS = {"none": 0, "linear": 1, "ramp": 2}
 ROPE_LAYOUTS = {"halves": 0, "pairs": 1}
+GROUPED_DIRECTIONS = {"forward": 0, "input": 1, "weight": 2}
 ARTIFACT_KINDS = {0: "Ptx", 1: "Cubin", 2: "HipCodeObject", 3: "SpirV", 4: "Stub"}
 
 
@@ -187,6 +188,40 @@ class HipBackend:
         c = _cache4(dtype, kv_heads, head_dim, group, page, "I32")
         a = _lib.Attention(heads, int(causal), int(lse), 0, scale)
         return self._wrap(lambda out, err: _lib.lib().unp_hip_lower_cache4_attention(C.byref(c), C.byref(a), out, err))
+
+    def lower_quant8(self, dtype: str, kind: str = "Fp8E4M3FN", block_rows: int = 1,
+                     transpose: bool = False) -> GeneratedKernel:
+        """The 8-bit codes of a matrix, or of its transpose, with an F32 scale for each block of ``block_rows`` (1 or
+        128) rows and 128 columns (``unp_hip_lower_quant8``).  Launch: x, codes, scales; rows, cols, x_row,
+        code_row, scale_row (strides in elements)."""
+        q = _lib.Quant8(ELEMENT_KINDS[dtype], ELEMENT_KINDS[kind], block_rows, int(transpose))
+        return self._wrap(lambda out, err: _lib.lib().unp_hip_lower_quant8(C.byref(q), out, err))
+
+    def lower_matmul8(self, a_kind: str = "Fp8E4M3FN", b_kind: str = "Fp8E4M3FN", out: str = "Bf16", b_rows: int = 128,
+                      grouped: bool = False) -> GeneratedKernel:
+        """Rows of 8-bit codes times a matrix of them, or times their group's, with the scales of blocks of 128 columns
+        (``unp_hip_lower_matmul8``): out[i][j] = sum of a[i][l] b[j][l], Bf16 or F16.  Launch: a, a_scales, b, b_scales, with ``grouped``
+        starts, out, workspace; m, n, k, with ``grouped`` groups, a_row, a_scale_row, b_row, b_scale_row, with ``grouped``
+        b_group, b_scale_group, out_row, workspace_bytes (:meth:`Executor.workspace_bytes` of m, n, k and groups)."""
+        m = _lib.Matmul8(ELEMENT_KINDS[a_kind], ELEMENT_KINDS[b_kind], ELEMENT_KINDS[out], b_rows, int(grouped))
+        return self._wrap(lambda o, err: _lib.lib().unp_hip_lower_matmul8(C.byref(m), o, err))
+
+    def lower_grouped_matmul(self, dtype: str, out: str | None = None, direction: str = "forward") -> GeneratedKernel:
+        """Rows times their group's matrix, or a gradient of that (``unp_hip_lower_grouped_matmul``): ``"forward"``
+        out[r][j] = sum of x[r][l] w[g][j][l], ``"input"`` out[r][l] = sum of x[r][j] w[g][j][l], ``"weight"``
+        out[g][j][l] = sum over g's rows of x[r][j] y[r][l].  Launch: x, w (``"weight"``: y), starts, out, workspace;
+        rows, n, k, groups, x_row, then w_group, w_row, out_row (``"weight"``: y_row, out_group, out_row),
+        workspace_bytes (:meth:`Executor.workspace_bytes` of rows, n, k and groups)."""
+        m = _lib.GroupedMatmul(ELEMENT_KINDS[dtype], ELEMENT_KINDS[dtype if out is None else out],
+                               GROUPED_DIRECTIONS[direction])
+        return self._wrap(lambda o, err: _lib.lib().unp_hip_lower_grouped_matmul(C.byref(m), o, err))
+
+    def lower_group_rows(self, index_dtype: str = "I32") -> GeneratedKernel:
+        """Where each group's rows begin, which token each row takes and where each choice went, from the group that each
+        choice names (``unp_hip_lower_group_rows``).  Launch: ids, starts, rows, place, workspace; count, per, groups,
+        workspace_bytes (:meth:`Executor.workspace_bytes` of count, per and groups)."""
+        r = _lib.GroupRows(ELEMENT_KINDS[index_dtype])
+        return self._wrap(lambda out, err: _lib.lib().unp_hip_lower_group_rows(C.byref(r), out, err))
 
     @staticmethod
     def _wrap(call) -> GeneratedKernel:
@@ -512,12 +547,20 @@ class Executor:
         if rc:
             check(rc, err._obj)
 
-    def workspace_bytes(self, tokens: int, batch: int, width: int, pages: int) -> int:
-        """The workspace with which a cache attention launch of these scalars splits as far as it would."""
-        sc = (C.c_int64 * 4)(tokens, batch, width, pages)
+    def workspace_bytes(self, *scalars: int, **named: int) -> int:
+        """The workspace with which a launch of these scalars splits as far as it would: the form's first scalars, in order or
+        by name (a cache attention's ``tokens``, ``batch``, ``width``, ``pages``; a product's extents and groups; the
+        ``count``, ``per`` and ``groups`` of group rows)."""
+        if named:
+            names = [p["name"] for p in self.kernel.interface["params"] if p["kind"] == "scalar"]
+            rest = names[len(scalars):len(scalars) + len(named)]
+            if set(rest) != set(named):
+                raise TypeError(f"workspace_bytes takes {', '.join(names)}, not {', '.join(named)}")
+            scalars += tuple(named[n] for n in rest)
+        sc = (C.c_int64 * max(1, len(scalars)))(*scalars)
         n = C.c_uint64()
         err = _lib.Error()
-        check(_lib.lib().unp_hip_exec_workspace(self._h, sc, 4, C.byref(n), C.byref(err)), err)
+        check(_lib.lib().unp_hip_exec_workspace(self._h, sc, len(scalars), C.byref(n), C.byref(err)), err)
         return int(n.value)
 
     def launch_static(self, *args, stream: int = 0) -> None:

@@ -86,6 +86,26 @@ class Attention(C.Structure):
     _fields_ = [(n, C.c_int32) for n in ("heads", "causal", "lse", "pad")] + [("scale", C.c_double)]
 
 
+class Quant8(C.Structure):
+    """unp_quant8: a quantisation to 8-bit floating point."""
+    _fields_ = [(n, C.c_int32) for n in ("dtype", "kind", "block_rows", "transpose")]
+
+
+class Matmul8(C.Structure):
+    """unp_matmul8: a product of 8-bit codes with scales."""
+    _fields_ = [(n, C.c_int32) for n in ("a_kind", "b_kind", "out", "b_rows", "grouped")]
+
+
+class GroupedMatmul(C.Structure):
+    """unp_grouped_matmul: products by group, or their gradients."""
+    _fields_ = [(n, C.c_int32) for n in ("dtype", "out", "direction")]
+
+
+class GroupRows(C.Structure):
+    """unp_group_rows: the rows of each group."""
+    _fields_ = [("index_dtype", C.c_int32)]
+
+
 _lib = None
 
 
@@ -136,6 +156,10 @@ def lib() -> C.CDLL:
         "unp_hip_lower_cache4_append": (i32, [C.POINTER(Cache4), i32, i32, C.POINTER(P), E]),
         "unp_hip_lower_cache4_read": (i32, [C.POINTER(Cache4), C.POINTER(P), E]),
         "unp_hip_lower_cache4_attention": (i32, [C.POINTER(Cache4), C.POINTER(Attention), C.POINTER(P), E]),
+        "unp_hip_lower_quant8": (i32, [C.POINTER(Quant8), C.POINTER(P), E]),
+        "unp_hip_lower_matmul8": (i32, [C.POINTER(Matmul8), C.POINTER(P), E]),
+        "unp_hip_lower_grouped_matmul": (i32, [C.POINTER(GroupedMatmul), C.POINTER(P), E]),
+        "unp_hip_lower_group_rows": (i32, [C.POINTER(GroupRows), C.POINTER(P), E]),
         "unp_hip_exec_workspace": (i32, [P, C.POINTER(C.c_int64), sz, C.POINTER(u64), E]),
         "unp_hip_compile": (i32, [C.c_char_p, C.c_char_p, u32, C.POINTER(C.POINTER(C.c_uint8)),
                                   C.POINTER(sz), C.POINTER(C.c_void_p)]),

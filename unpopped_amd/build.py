@@ -22,7 +22,7 @@ LIB = HERE / "libunpopped_hip.so"
 SYNTH_LIB = HERE / "libunpopped_synth.so"
 ROCM = Path(os.environ.get("ROCM_PATH", "/opt/rocm"))
 
-HOST_SOURCES = ["emit_hip.cpp", "emit_cache4.cpp", "compile_rtc.cpp", "runtime.cpp", "kernel_ir.cpp", "lifts.cpp"]
+HOST_SOURCES = ["emit_hip.cpp", "emit_cache4.cpp", "emit_matmul.cpp", "compile_rtc.cpp", "runtime.cpp", "kernel_ir.cpp", "lifts.cpp"]
 
 HIPCC_DEVICE_FLAGS = [
     "--offload-arch=gfx950", "-O3", "-std=c++17", "-ffp-contract=off",
@@ -55,7 +55,8 @@ def embed_device_library(source: str, name: str) -> Path:
 
 def build_host() -> Path:
     embedded = [embed_device_library("unp_device.hip", "kDeviceLibrary"),
-                embed_device_library("unp_cache4.hip", "kCache4Library")]
+                embed_device_library("unp_cache4.hip", "kCache4Library"),
+                embed_device_library("unp_matmul.hip", "kMatmulLibrary")]
     objs = []
     for src in HOST_SOURCES + [str(e) for e in embedded]:
         path = Path(src) if os.path.isabs(src) else CSRC / src

@@ -41,15 +41,17 @@ bool layout_ok(int32_t l, std::string& why) {
   return false;
 }
 
-// One parameter of the interface JSON.
-struct Param {
-  const char* name;
-  const char* role;  // "Read", "Write", "ReadWrite"; null: a scalar
-  const char* dtype;
-};
-std::string interface(const Lowered& L, const char* form, const std::string& fields, const std::vector<Param>& ps,
-                      const char* policy, const std::vector<std::string>& when, const char* workspace,
-                      const char* note) {
+std::string source_head(const std::string& name) {
+  return "// unpopped-hip kernel `" + name + "` for rocm:gfx950.\n" + kCache4Library + "\n";
+}
+
+const char* kBounds256 = "extern \"C\" __global__ void __launch_bounds__(256) ";
+
+}  // namespace
+
+std::string form_interface(const Lowered& L, const char* form, const std::string& fields, const std::vector<FormParam>& ps,
+                           const char* policy, const std::vector<std::string>& when, const char* workspace,
+                           const char* note) {
   std::ostringstream j;
   j << "{\"backend\":\"hip\",\"target\":\"rocm:gfx950\",\"form\":\"" << form << "\"," << fields << ",\"params\":[";
   for (size_t i = 0; i < ps.size(); ++i) {
@@ -65,14 +67,6 @@ std::string interface(const Lowered& L, const char* form, const std::string& fie
     << ",\"fidelity_notes\":[\"" << note << "\"]}";
   return j.str();
 }
-
-std::string source_head(const std::string& name) {
-  return "// unpopped-hip kernel `" + name + "` for rocm:gfx950.\n" + kCache4Library + "\n";
-}
-
-const char* kBounds256 = "extern \"C\" __global__ void __launch_bounds__(256) ";
-
-}  // namespace
 
 int32_t lower_rope_table(const unp_rope_table& t, Lowered& L, std::string& why) {
   L = Lowered{};
@@ -107,7 +101,7 @@ int32_t lower_rope_table(const unp_rope_table& t, Lowered& L, std::string& why) 
   if (t.rot % 4 == 0) add("_v", 2, "a 16-byte aligned table");
   add("_e", 1, "otherwise");
   L.source = src.str();
-  L.interface_json = interface(
+  L.interface_json = form_interface(
       L, "rope_table", "\"rot\":" + std::to_string(t.rot),
       {{"table", "Write", "F32"}, {"first", nullptr, "I64"}, {"count", nullptr, "I64"}},
       "pairs by lanes in order; blocks stride over them", when, nullptr,
@@ -151,7 +145,7 @@ int32_t lower_rope(const unp_rope& r, Lowered& L, std::string& why) {
   add("_e", 0, "otherwise");
   L.source = src.str();
   const char *dt = kind_name(r.dtype), *ix = kind_name(r.index_dtype);
-  L.interface_json = interface(
+  L.interface_json = form_interface(
       L, "rope", "\"head_dim\":" + std::to_string(r.head_dim) + ",\"rot\":" + std::to_string(r.rot),
       {{"x", "Read", dt}, {"positions", "Read", ix}, {"table", "Read", "F32"}, {"out", "Write", dt},
        {"tokens", nullptr, "I64"}, {"heads", nullptr, "I64"}, {"x_token", nullptr, "I64"}, {"x_head", nullptr, "I64"},
@@ -222,7 +216,7 @@ int32_t lower_cache4_append(const unp_cache4& c, int32_t rot, int32_t layout, Lo
   }
   L.source = src.str();
   const char *dt = kind_name(c.dtype), *ix = kind_name(c.index_dtype);
-  std::vector<Param> ps = {{"k", "Read", dt}, {"v", "Read", dt}, {"slots", "Read", ix}, {"cache", "ReadWrite", "U8"}};
+  std::vector<FormParam> ps = {{"k", "Read", dt}, {"v", "Read", dt}, {"slots", "Read", ix}, {"cache", "ReadWrite", "U8"}};
   if (rot > 0) {
     ps.push_back({"positions", "Read", ix});
     ps.push_back({"table", "Read", "F32"});
@@ -230,7 +224,7 @@ int32_t lower_cache4_append(const unp_cache4& c, int32_t rot, int32_t layout, Lo
   for (const char* s : {"tokens", "pages", "k_token", "k_head", "v_token", "v_head"}) ps.push_back({s, nullptr, "I64"});
   if (rot > 0)
     for (const char* s : {"table_first", "table_rows"}) ps.push_back({s, nullptr, "I64"});
-  L.interface_json = interface(L, "cache4_append", cache_fields(c) + ",\"rot\":" + std::to_string(rot), ps,
+  L.interface_json = form_interface(L, "cache4_append", cache_fields(c) + ",\"rot\":" + std::to_string(rot), ps,
                                "a word of 8 codes per lane; blocks stride over the heads", {kAlignedWhen, "otherwise"},
                                nullptr, "keys rotated in f64, rounded to f32 and then to their type; codes of correctly rounded quotients");
   return UNP_OK;
@@ -257,9 +251,9 @@ int32_t lower_cache4_read(const unp_cache4& c, Lowered& L, std::string& why) {
   }
   L.source = src.str();
   const char *dt = kind_name(c.dtype), *ix = kind_name(c.index_dtype);
-  std::vector<Param> ps = {{"slots", "Read", ix}, {"cache", "Read", "U8"}, {"k", "Write", dt}, {"v", "Write", dt}};
+  std::vector<FormParam> ps = {{"slots", "Read", ix}, {"cache", "Read", "U8"}, {"k", "Write", dt}, {"v", "Write", dt}};
   for (const char* s : {"tokens", "pages", "k_token", "k_head", "v_token", "v_head"}) ps.push_back({s, nullptr, "I64"});
-  L.interface_json = interface(L, "cache4_read", cache_fields(c), ps, "a word of 8 codes per lane, striding over the grid",
+  L.interface_json = form_interface(L, "cache4_read", cache_fields(c), ps, "a word of 8 codes per lane, striding over the grid",
                                {kAlignedWhen, "otherwise"}, nullptr,
                                "exact integer difference and f32 product; one round-to-nearest-even to the type: bit-exact");
   return UNP_OK;
@@ -339,7 +333,7 @@ int32_t lower_cache4_attention(const unp_cache4& c, const unp_attention& a, Lowe
   when.push_back("otherwise");
   when.push_back("after any of them, where a context is split");
   const char* dt = kind_name(c.dtype);
-  std::vector<Param> ps = {{"q", "Read", dt}, {"cache", "Read", "U8"}, {"page_table", "Read", "I32"},
+  std::vector<FormParam> ps = {{"q", "Read", dt}, {"cache", "Read", "U8"}, {"page_table", "Read", "I32"},
                            {"starts", "Read", "I32"}, {"lengths", "Read", "I32"}, {"out", "Write", dt}};
   if (a.lse) ps.push_back({"lse", "Write", "F32"});
   ps.push_back({"workspace", "ReadWrite", "U8"});
@@ -347,7 +341,7 @@ int32_t lower_cache4_attention(const unp_cache4& c, const unp_attention& a, Lowe
                         "workspace_bytes"})
     ps.push_back({s, nullptr, "I64"});
   L.interface_json =
-      interface(L, "cache4_attention", cache_fields(c) + ",\"heads\":" + std::to_string(a.heads), ps,
+      form_interface(L, "cache4_attention", cache_fields(c) + ",\"heads\":" + std::to_string(a.heads), ps,
                 "a block per row tile, part of a context and key/value head",
                 when,
                 "the caller's, by unp_hip_exec_workspace",

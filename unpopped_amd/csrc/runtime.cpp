@@ -157,7 +157,7 @@ size_t split_bytes(const unp_exec* x) {
   return split_counter_bytes(x) + split_items(x) * values * 16;
 }
 
-int32_t attention_workspace(const unp_exec* x, const int64_t* sc, size_t n, uint64_t& bytes, unp_error* err);
+int32_t form_workspace(const unp_exec* x, const int64_t* sc, size_t n, uint64_t& bytes, unp_error* err);
 
 bool splits(const unp_exec* x) {
   if (x->l.form.kind == UNP_FORM_ROW_REDUCE) return true;
@@ -280,6 +280,19 @@ int32_t unp_hip_lower_cache4_attention(const unp_cache4* c, const unp_attention*
   return lower_into(c && a, out, err, [&](unp::Lowered& l, std::string& why) {
     return unp::lower_cache4_attention(*c, *a, l, why);
   });
+}
+
+int32_t unp_hip_lower_quant8(const unp_quant8* q, unp_generated** out, unp_error* err) {
+  return lower_into(q, out, err, [&](unp::Lowered& l, std::string& why) { return unp::lower_quant8(*q, l, why); });
+}
+int32_t unp_hip_lower_matmul8(const unp_matmul8* m, unp_generated** out, unp_error* err) {
+  return lower_into(m, out, err, [&](unp::Lowered& l, std::string& why) { return unp::lower_matmul8(*m, l, why); });
+}
+int32_t unp_hip_lower_grouped_matmul(const unp_grouped_matmul* m, unp_generated** out, unp_error* err) {
+  return lower_into(m, out, err, [&](unp::Lowered& l, std::string& why) { return unp::lower_grouped_matmul(*m, l, why); });
+}
+int32_t unp_hip_lower_group_rows(const unp_group_rows* r, unp_generated** out, unp_error* err) {
+  return lower_into(r, out, err, [&](unp::Lowered& l, std::string& why) { return unp::lower_group_rows(*r, l, why); });
 }
 
 int32_t unp_hip_form_variants(const unp_form* form, unp_variant* out, size_t cap, size_t* count, unp_error* err) {
@@ -644,7 +657,7 @@ int32_t unp_hip_exec_workspace(const unp_exec* x, const int64_t* scalars, size_t
   }
   *bytes = 0;
   set_error(err, UNP_OK, "");
-  return attention_workspace(x, scalars, nscalars, *bytes, err);
+  return form_workspace(x, scalars, nscalars, *bytes, err);
 }
 
 int32_t unp_hip_exec_last_launch(const unp_exec* x, uint32_t grid[3], uint32_t block[3], char* entry,
@@ -2109,7 +2122,6 @@ AttentionPlan attention_plan(const unp_exec* x, int64_t tokens, int64_t batch, i
 }
 
 int32_t attention_workspace(const unp_exec* x, const int64_t* sc, size_t n, uint64_t& bytes, unp_error* err) {
-  if (x->l.form.kind != UNP_FORM_CACHE4_ATTENTION) return invalid(err, "only a cache attention takes a workspace");
   if (n != 4) return invalid(err, "expected tokens, batch, width and pages");
   const int32_t rc = check_attention(x, sc[0], sc[1], sc[2], sc[3], err);
   bytes = 0;
@@ -2162,6 +2174,303 @@ int32_t run_cache4_attention(unp_exec* x, const unp_arg* a, size_t n, hipStream_
   void* jparams[] = {&starts, &out, &lse, &ws, &args};
   const int64_t rows = p.splits <= kFewParts ? 256 / (c.head_dim / 4) : 1, joined = tokens * at.heads;
   return launch(x, x->l.entries.size() - 1, (uint32_t)((joined + rows - 1) / rows), jparams, s, err);
+}
+
+// ---------------------------------------------------------------------------------------
+// The floating point products.  Rows, columns and depths are at most 2^28, so that the kernels' counts of tiles and their
+// offsets inside a tile stay in 32 bits.
+// ---------------------------------------------------------------------------------------
+
+// Host images of the kernels' argument structs (passed by value).
+struct product_args_host {
+  int64_t m, n, depth, x_row, w_row, w_group, xs_row, ws_row, ws_group, out_row, out_group;
+  int32_t groups, tiles_m, tiles_n, parts, x_vectors, w_vectors, wide, pad;
+};
+struct quant_args_host {
+  int64_t rows, cols, x_row, code_row, scale_row;
+  int32_t x_vectors, code_vectors;
+};
+struct rows_args_host {
+  int64_t n, per, chunk;
+  int32_t groups, chunks;
+};
+
+constexpr int64_t kMostExtent = (int64_t)1 << 28, kMostGroups = 1024;
+
+// A product's extents: rows and columns of out (by group where the depth is), the depth, and the groups.
+struct Extents {
+  int64_t m, n, depth, groups;
+  bool by_row, by_depth;  // what the groups divide
+  int64_t rows() const { return by_depth ? groups * m : m; }  // of the result
+};
+struct ProductPlan {
+  size_t entry = 0;
+  int64_t tiles_m = 0, tiles_n = 0, parts = 1;
+};
+
+int32_t check_extents(const Extents& e, unp_error* err) {
+  for (int64_t v : {e.m, e.n, e.depth})
+    if (v < 0 || v > kMostExtent) return invalid(err, "rows, columns and depths are 0..2^28");
+  if (e.groups < 0 || e.groups > kMostGroups) return invalid(err, "groups is 0..1024");
+  return UNP_OK;
+}
+
+int64_t parts_bytes(const Extents& e, int64_t parts) { return parts * e.rows() * ((e.n + 3) / 4 * 4) * 4; }
+
+// Tiles of `t` rows that e's rows fill at most: a group's last one is not shared.
+int64_t row_tiles(const Extents& e, int64_t t) {
+  if (e.by_depth) return e.groups * ((e.m + t - 1) / t);
+  if (!e.by_row) return (e.m + t - 1) / t;
+  return e.m / t + std::min(e.groups, e.m);
+}
+
+ProductPlan product_plan(const unp_exec* x, const Extents& e, bool direct) {
+  (void)direct;
+  ProductPlan p;
+  const unp::Entry& k = x->l.entries[p.entry];
+  p.tiles_m = row_tiles(e, k.vec);
+  p.tiles_n = (e.n + k.cols - 1) / k.cols;
+  return p;
+}
+
+// The launch of a product whose strides and buffers are checked: x, w, their scales, starts, out and workspace.
+int32_t launch_product(unp_exec* x, const Extents& e, product_args_host args, const uint64_t (&buf)[7], int64_t workspace_bytes,
+                       bool direct, hipStream_t s, unp_error* err) {
+  ProductPlan p = product_plan(x, e, direct);
+  while (p.parts > 1 && parts_bytes(e, p.parts) > workspace_bytes) --p.parts;
+  const int64_t blocks = p.tiles_m * p.tiles_n * p.parts;
+  if (blocks > kMostBlocks) return invalid(err, "more than 2^24 - 1 tiles of the result: " + std::to_string(blocks));
+  args.m = e.m;
+  args.n = e.n;
+  args.depth = e.depth;
+  args.groups = (int32_t)e.groups;
+  args.tiles_m = (int32_t)p.tiles_m;
+  args.tiles_n = (int32_t)p.tiles_n;
+  args.parts = (int32_t)p.parts;
+  uint64_t xp = buf[0], wp = buf[1], xs = buf[2], ws = buf[3], starts = buf[4], out = buf[5], parts = buf[6];
+  void* params[] = {&xp, &wp, &xs, &ws, &starts, &out, &parts, &args};
+  x->chunks = p.parts;
+  x->shared = p.parts > 1;
+  const int32_t rc = launch(x, p.entry, (uint32_t)blocks, params, s, err);
+  if (rc != UNP_OK || p.parts == 1) return rc;
+  void* jparams[] = {&starts, &out, &parts, &args};
+  return launch(x, x->l.entries.size() - 1, grid_for(x, (e.rows() * ((e.n + 3) / 4) + 255) / 256), jparams, s, err);
+}
+
+// Rows of whole 16-byte vectors at `p`, stride in elements of `size` bytes.
+bool vectors(uint64_t p, int64_t stride, int64_t size) { return aligned16(p) && stride * size % 16 == 0; }
+// A stride (in bytes) with which the offsets inside a tile stay below 2^31.
+bool near(int64_t stride) { return stride <= (1 << 22); }
+
+int32_t run_matmul8(unp_exec* x, const unp_arg* a, size_t n, hipStream_t s, unp_error* err) {
+  Args A;
+  const unp_matmul8& f = x->l.matmul8;
+  const bool grouped = f.grouped != 0;
+  int32_t rc = take_args(a, n, grouped ? 7 : 6, grouped ? 12 : 9, A, err);
+  if (rc != UNP_OK) return rc;
+  size_t i = 0;
+  auto next = [&] { return A.ext[i++]; };
+  Extents e{};
+  e.m = next(), e.n = next(), e.depth = next();
+  e.groups = grouped ? next() : 1;
+  e.by_row = grouped;
+  const int64_t a_row = next(), as_row = next(), b_row = next(), bs_row = next();
+  const int64_t b_group = grouped ? next() : 0, bs_group = grouped ? next() : 0, out_row = next(), bytes = next();
+  if ((rc = check_extents(e, err)) != UNP_OK) return rc;
+  const int64_t blocks = (e.depth + 127) / 128, scale_rows = (e.n + f.b_rows - 1) / f.b_rows;
+  if ((rc = check_heads("a", e.m, a_row, 1, 0, e.depth, false, err)) != UNP_OK ||
+      (rc = check_heads("a_scales", e.m, as_row, 1, 0, blocks, false, err)) != UNP_OK ||
+      (rc = check_heads("b", e.groups, b_group, e.n, b_row, e.depth, false, err)) != UNP_OK ||
+      (rc = check_heads("b_scales", e.groups, bs_group, scale_rows, bs_row, blocks, false, err)) != UNP_OK ||
+      (rc = check_heads("out", e.m, out_row, 1, 0, e.n, e.n > 0, err)) != UNP_OK)
+    return rc;
+  if (bytes < 0) return invalid(err, "workspace_bytes is negative");
+  if (e.m == 0 || e.n == 0 || e.groups == 0) return UNP_OK;
+  const size_t out = grouped ? 5 : 4;
+  for (size_t b = 0; b < A.buf.size(); ++b)
+    if (A.buf[b] == 0 && !(b < 4 && e.depth == 0) && !(b == out + 1 && bytes == 0))
+      return invalid(err, "buffer argument " + std::to_string(b) + " is null");
+  const uint64_t starts = grouped ? A.buf[4] : 0;
+  const int64_t size = (int64_t)unp::kind_bytes(f.out);
+  if (A.buf[1] % 4 || A.buf[3] % 4 || starts % 4 || A.buf[out] % (uint64_t)size || !aligned16(A.buf[out + 1]))
+    return invalid(err, "buffers are aligned to their elements, the workspace to 16 bytes");
+  product_args_host args{};
+  args.x_row = a_row;
+  args.w_row = b_row;
+  args.w_group = b_group;
+  args.xs_row = as_row;
+  args.ws_row = bs_row;
+  args.ws_group = bs_group;
+  args.out_row = out_row;
+  args.x_vectors = vectors(A.buf[0], a_row, 1);
+  args.w_vectors = vectors(A.buf[2], b_row, 1) && b_group % 16 == 0;
+  args.wide = A.buf[out] % (uint64_t)(4 * size) == 0 && out_row % 4 == 0;
+  const bool direct = args.x_vectors && args.w_vectors && e.depth % 16 == 0 && near(a_row) && near(b_row);
+  const uint64_t buf[7] = {A.buf[0], A.buf[2], A.buf[1], A.buf[3], starts, A.buf[out], A.buf[out + 1]};
+  return launch_product(x, e, args, buf, bytes, direct, s, err);
+}
+
+int32_t run_grouped_matmul(unp_exec* x, const unp_arg* a, size_t n, hipStream_t s, unp_error* err) {
+  Args A;
+  const unp_grouped_matmul& f = x->l.grouped_matmul;
+  const bool weight = f.direction == UNP_GROUPED_WEIGHT, input = f.direction == UNP_GROUPED_INPUT;
+  int32_t rc = take_args(a, n, 5, 9, A, err);
+  if (rc != UNP_OK) return rc;
+  const int64_t rows = A.ext[0], nn = A.ext[1], kk = A.ext[2], groups = A.ext[3], x_row = A.ext[4], bytes = A.ext[8];
+  Extents e{};
+  e.m = weight ? nn : rows;
+  e.n = weight || input ? kk : nn;
+  e.depth = weight ? rows : input ? nn : kk;
+  e.groups = groups;
+  e.by_row = !weight;
+  e.by_depth = weight;
+  if ((rc = check_extents(e, err)) != UNP_OK) return rc;
+  const int64_t w_group = weight ? 0 : A.ext[5], w_row = weight ? A.ext[5] : A.ext[6];
+  const int64_t out_group = weight ? A.ext[6] : 0, out_row = A.ext[7];
+  if ((rc = check_heads("x", rows, x_row, 1, 0, weight || input ? nn : kk, false, err)) != UNP_OK) return rc;
+  if (weight)
+    rc = check_heads("y", rows, w_row, 1, 0, kk, false, err);
+  else
+    rc = check_heads("w", groups, w_group, nn, w_row, kk, false, err);
+  if (rc != UNP_OK) return rc;
+  if (weight)
+    rc = check_heads("out", groups, out_group, nn, out_row, kk, kk > 0, err);
+  else
+    rc = check_heads("out", rows, out_row, 1, 0, e.n, e.n > 0, err);
+  if (rc != UNP_OK) return rc;
+  if (bytes < 0) return invalid(err, "workspace_bytes is negative");
+  if (e.m == 0 || e.n == 0 || groups == 0) return UNP_OK;
+  if ((__int128)e.rows() * e.n > kMostOffset) return invalid(err, "out: more than 2^60 elements");
+  for (size_t b = 0; b < 5; ++b)
+    if (A.buf[b] == 0 && !(b < 2 && e.depth == 0) && !(b == 4 && bytes == 0))
+      return invalid(err, "buffer argument " + std::to_string(b) + " is null");
+  const int64_t size = (int64_t)unp::kind_bytes(f.out);
+  if (A.buf[0] % 2 || A.buf[1] % 2 || A.buf[2] % 4 || A.buf[3] % (uint64_t)size || !aligned16(A.buf[4]))
+    return invalid(err, "buffers are aligned to their elements, the workspace to 16 bytes");
+  product_args_host args{};
+  args.x_row = 2 * x_row;
+  args.w_row = 2 * w_row;
+  args.w_group = 2 * w_group;
+  args.out_row = out_row;
+  args.out_group = out_group;
+  args.x_vectors = vectors(A.buf[0], x_row, 2);
+  args.w_vectors = vectors(A.buf[1], w_row, 2) && w_group % 8 == 0;
+  args.wide = A.buf[3] % (uint64_t)(4 * size) == 0 && out_row % 4 == 0 && out_group % 4 == 0;
+  // What lies along the rows in memory is whole vectors: the depth, or columns of out.
+  const bool whole = weight ? nn % 8 == 0 && kk % 8 == 0 : input ? nn % 8 == 0 && kk % 8 == 0 : kk % 8 == 0;
+  const bool direct = args.x_vectors && args.w_vectors && whole && near(2 * x_row) && near(2 * w_row);
+  const uint64_t buf[7] = {A.buf[0], A.buf[1], 0, 0, A.buf[2], A.buf[3], A.buf[4]};
+  return launch_product(x, e, args, buf, bytes, direct, s, err);
+}
+
+int32_t run_quant8(unp_exec* x, const unp_arg* a, size_t n, hipStream_t s, unp_error* err) {
+  Args A;
+  int32_t rc = take_args(a, n, 3, 5, A, err);
+  if (rc != UNP_OK) return rc;
+  const unp_quant8& q = x->l.quant8;
+  const int64_t rows = A.ext[0], cols = A.ext[1];
+  if (rows < 0 || cols < 0 || rows > kMostExtent || cols > kMostExtent) return invalid(err, "rows and cols are 0..2^28");
+  const int64_t yr = q.transpose ? cols : rows, yc = q.transpose ? rows : cols;
+  const int64_t sr = (yr + q.block_rows - 1) / q.block_rows, sc = (yc + 127) / 128;
+  if ((rc = check_heads("x", rows, A.ext[2], 1, 0, cols, false, err)) != UNP_OK ||
+      (rc = check_heads("codes", yr, A.ext[3], 1, 0, yc, true, err)) != UNP_OK ||
+      (rc = check_heads("scales", sr, A.ext[4], 1, 0, sc, true, err)) != UNP_OK)
+    return rc;
+  if (rows == 0 || cols == 0) return UNP_OK;
+  if ((rc = need_buffers(A, true, err)) != UNP_OK) return rc;
+  const int64_t size = (int64_t)unp::kind_bytes(q.dtype);
+  if (A.buf[0] % (uint64_t)size || A.buf[2] % 4) return invalid(err, "x and scales are aligned to their elements");
+  quant_args_host args{rows, cols, A.ext[2], A.ext[3], A.ext[4], vectors(A.buf[0], A.ext[2], size), vectors(A.buf[1], A.ext[3], 1)};
+  uint64_t xp = A.buf[0], codes = A.buf[1], scales = A.buf[2];
+  void* params[] = {&xp, &codes, &scales, &args};
+  const bool by_rows = q.block_rows == 1 && !q.transpose;
+  const int64_t blocks = by_rows ? (rows * ((cols + 127) / 128) + 31) / 32 : ((rows + 127) / 128) * ((cols + 127) / 128);
+  return launch(x, 0, grid_for(x, blocks), params, s, err);
+}
+
+// A chunk is a block's: a few ids a lane.  All in one up to 4096 ids; as many chunks as the workspace holds counts of.
+constexpr int64_t kSortStep = 512, kMostChunks = 128;
+struct RowsPlan {
+  int64_t chunk = 0, chunks = 1;
+};
+RowsPlan rows_plan(int64_t n, int64_t groups, int64_t bytes) {
+  RowsPlan p;
+  int64_t want = n <= 4096 ? 1 : std::min(kMostChunks, (n + 2 * kSortStep - 1) / (2 * kSortStep));
+  want = std::max<int64_t>(1, std::min(want, bytes / (4 * groups)));
+  p.chunk = ((n + want - 1) / want + kSortStep - 1) / kSortStep * kSortStep;
+  p.chunks = (n + p.chunk - 1) / p.chunk;
+  return p;
+}
+
+int32_t check_group_rows(int64_t n, int64_t per, int64_t groups, unp_error* err) {
+  if (n < 0 || n > kMostExtent) return invalid(err, "count is 0..2^28");
+  if (per < 1) return invalid(err, "per is at least 1");
+  if (groups < 1 || groups > kMostGroups) return invalid(err, "groups is 1..1024");
+  return UNP_OK;
+}
+
+int32_t run_group_rows(unp_exec* x, const unp_arg* a, size_t n, hipStream_t s, unp_error* err) {
+  Args A;
+  int32_t rc = take_args(a, n, 5, 4, A, err);
+  if (rc != UNP_OK) return rc;
+  const int64_t count = A.ext[0], per = A.ext[1], groups = A.ext[2], bytes = A.ext[3];
+  if ((rc = check_group_rows(count, per, groups, err)) != UNP_OK) return rc;
+  if (bytes < 0) return invalid(err, "workspace_bytes is negative");
+  for (size_t b = 0; b < 5; ++b)
+    if (A.buf[b] == 0 && !(b != 1 && b != 4 && count == 0) && !(b == 4 && bytes == 0))
+      return invalid(err, "buffer argument " + std::to_string(b) + " is null");
+  if (A.buf[0] % unp::kind_bytes(x->l.group_rows.index_dtype) || A.buf[1] % 4 || A.buf[2] % 4 || A.buf[3] % 4 || !aligned16(A.buf[4]))
+    return invalid(err, "buffers are aligned to their elements, the workspace to 16 bytes");
+  RowsPlan p = rows_plan(std::max<int64_t>(count, 1), groups, bytes);
+  rows_args_host args{count, per, p.chunk, (int32_t)groups, (int32_t)p.chunks};
+  uint64_t ids = A.buf[0], starts = A.buf[1], rows = A.buf[2], place = A.buf[3], counted = A.buf[4];
+  x->chunks = p.chunks;
+  x->shared = p.chunks > 1;
+  if (p.chunks > 1) {
+    void* params[] = {&ids, &counted, &args};
+    if ((rc = launch(x, 1, (uint32_t)p.chunks, params, s, err)) != UNP_OK) return rc;
+  }
+  void* params[] = {&ids, &starts, &rows, &place, &counted, &args};
+  return launch(x, 0, (uint32_t)p.chunks, params, s, err);
+}
+
+int32_t product_workspace(const unp_exec* x, const int64_t* sc, size_t n, uint64_t& bytes, unp_error* err) {
+  Extents e{};
+  if (x->l.form.kind == UNP_FORM_MATMUL8) {
+    const bool grouped = x->l.matmul8.grouped != 0;
+    if (n != (grouped ? 4u : 3u)) return invalid(err, grouped ? "expected m, n, k and groups" : "expected m, n and k");
+    e = Extents{sc[0], sc[1], sc[2], grouped ? sc[3] : 1, grouped, false};
+  } else {
+    if (n != 4) return invalid(err, "expected rows, n, k and groups");
+    const int32_t d = x->l.grouped_matmul.direction;
+    const bool weight = d == UNP_GROUPED_WEIGHT, input = d == UNP_GROUPED_INPUT;
+    e = Extents{weight ? sc[1] : sc[0], weight || input ? sc[2] : sc[1], weight ? sc[0] : input ? sc[1] : sc[2], sc[3], !weight, weight};
+  }
+  const int32_t rc = check_extents(e, err);
+  if (rc != UNP_OK || e.m == 0 || e.n == 0 || e.groups == 0) return rc;
+  const ProductPlan p = product_plan(x, e, true);
+  if (p.parts > 1) bytes = (uint64_t)parts_bytes(e, p.parts);
+  return UNP_OK;
+}
+
+int32_t form_workspace(const unp_exec* x, const int64_t* sc, size_t n, uint64_t& bytes, unp_error* err) {
+  switch (x->l.form.kind) {
+    case UNP_FORM_CACHE4_ATTENTION:
+      return attention_workspace(x, sc, n, bytes, err);
+    case UNP_FORM_MATMUL8:
+    case UNP_FORM_GROUPED_MATMUL:
+      return product_workspace(x, sc, n, bytes, err);
+    case UNP_FORM_GROUP_ROWS: {
+      if (n != 3) return invalid(err, "expected count, per and groups");
+      const int32_t rc = check_group_rows(sc[0], sc[1], sc[2], err);
+      if (rc != UNP_OK || sc[0] == 0) return rc;
+      const RowsPlan p = rows_plan(sc[0], sc[2], (int64_t)1 << 40);
+      if (p.chunks > 1) bytes = (uint64_t)(p.chunks * sc[2] * 4);
+      return UNP_OK;
+    }
+    default:
+      return invalid(err, "only a cache attention, a floating point product and group rows take a workspace");
+  }
 }
 
 }  // namespace
@@ -2640,7 +2949,7 @@ extern "C" int32_t unp_hip_exec_launch_views(unp_exec* x, const unp_view* views,
   if ((nviews && !views) || (nscalars && !scalars)) return invalid(err, "null views or scalars");
   const unp_form& f = x->l.form;
   if (f.kind >= UNP_FORM_ROPE_TABLE)
-    return invalid(err, "a rotary or cache form takes its strides as scalars (unp_hip_exec_launch)");
+    return invalid(err, "a descriptor's form takes its strides as scalars (unp_hip_exec_launch)");
   size_t nbuf = 0, nscal = 0;
   param_counts(x, nbuf, nscal);
   if (nviews != nbuf || nscalars != nscal)
@@ -2742,6 +3051,14 @@ extern "C" int32_t unp_hip_exec_launch(unp_exec* x, const unp_arg* args, size_t 
       return run_cache4_read(x, args, nargs, s, err);
     case UNP_FORM_CACHE4_ATTENTION:
       return run_cache4_attention(x, args, nargs, s, err);
+    case UNP_FORM_QUANT8:
+      return run_quant8(x, args, nargs, s, err);
+    case UNP_FORM_MATMUL8:
+      return run_matmul8(x, args, nargs, s, err);
+    case UNP_FORM_GROUPED_MATMUL:
+      return run_grouped_matmul(x, args, nargs, s, err);
+    case UNP_FORM_GROUP_ROWS:
+      return run_group_rows(x, args, nargs, s, err);
     default:
       set_error(err, UNP_UNSUPPORTED_KERNEL, "unknown form");
       return UNP_UNSUPPORTED_KERNEL;

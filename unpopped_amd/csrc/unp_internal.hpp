@@ -183,7 +183,21 @@ struct Lowered {
   unp_rope rope{};              // UNP_FORM_ROPE; UNP_FORM_CACHE4_APPEND: its rot
   unp_cache4 cache4{};          // the UNP_FORM_CACHE4_* forms
   unp_attention attention{};    // UNP_FORM_CACHE4_ATTENTION, its scale resolved
+  unp_quant8 quant8{};                  // UNP_FORM_QUANT8
+  unp_matmul8 matmul8{};                // UNP_FORM_MATMUL8
+  unp_grouped_matmul grouped_matmul{};  // UNP_FORM_GROUPED_MATMUL
+  unp_group_rows group_rows{};          // UNP_FORM_GROUP_ROWS
 };
+
+// The interface JSON of a descriptor's form: its own fields, parameters and entries (each with its condition).
+struct FormParam {
+  const char* name;
+  const char* role;  // "Read", "Write", "ReadWrite"; null: a scalar
+  const char* dtype;
+};
+std::string form_interface(const Lowered& l, const char* form, const std::string& fields, const std::vector<FormParam>& params,
+                           const char* grid_policy, const std::vector<std::string>& when, const char* workspace,
+                           const char* note);
 
 // Emit the HIP source and interface for `f`; on refusal returns a nonzero unp_status and
 // fills `detail`.
@@ -206,6 +220,11 @@ int32_t lower_rope(const unp_rope& r, Lowered& out, std::string& why);
 int32_t lower_cache4_append(const unp_cache4& c, int32_t rot, int32_t layout, Lowered& out, std::string& why);
 int32_t lower_cache4_read(const unp_cache4& c, Lowered& out, std::string& why);
 int32_t lower_cache4_attention(const unp_cache4& c, const unp_attention& a, Lowered& out, std::string& why);
+// The floating point products (emit_matmul.cpp).
+int32_t lower_quant8(const unp_quant8& q, Lowered& out, std::string& why);
+int32_t lower_matmul8(const unp_matmul8& m, Lowered& out, std::string& why);
+int32_t lower_grouped_matmul(const unp_grouped_matmul& m, Lowered& out, std::string& why);
+int32_t lower_group_rows(const unp_group_rows& r, Lowered& out, std::string& why);
 int32_t check_cache4(const unp_cache4& c, std::string& why);  // a nonzero unp_status where no cache form takes it
 inline uint64_t cache4_record_bytes(const unp_cache4& c) {
   return (uint64_t)c.page * (uint64_t)(c.head_dim + 8 * (c.head_dim / c.group));
