@@ -431,9 +431,9 @@ typedef struct unp_quant8 {
   int32_t block_rows; /* rows of a block: 1 or 128 */
   int32_t transpose;  /* 1: y is x transposed, else y is x */
 } unp_quant8;
-/* A scale for each block of block_rows rows and 128 columns of y: the largest magnitude of the block over the largest code
- * (448 or 57344).  A code is its element over the scale, rounded to even; both quotients are correctly rounded to f32
- * first.  A block of zeros has the scale 0 and codes 0; one that holds a NaN or an infinity has a NaN scale and codes 0.
+/* A scale for each block of block_rows rows and 128 columns of y: the largest magnitude of the block times the f32 number
+ * nearest to 1 / 448 (or 1 / 57344), the largest code's inverse.  A code is its element over the scale, correctly rounded to f32
+ * and from there to even.  A block of zeros has the scale 0 and codes 0; one that holds a NaN or an infinity has a NaN scale and codes 0.
  * Launch: x ([rows][cols]), codes (y's shape), scales (F32 [y's rows / block_rows][y's columns / 128], both rounded up);
  * rows, cols, x_row, code_row, scale_row (strides).  Bytes of a row of codes behind its columns are not written. */
 int32_t unp_hip_lower_quant8(const unp_quant8* q, unp_generated** out, unp_error* err);

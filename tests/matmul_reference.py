@@ -51,21 +51,23 @@ def quantised(x: np.ndarray, kind: str, block_rows: int, transpose: bool):
                 if not np.isfinite(most):
                     scales[i, j] = np.nan
                     continue
-                scales[i, j] = most / np.float32(LARGEST[kind])
+                scales[i, j] = most * np.float32(1.0 / LARGEST[kind])
                 unit = scales[i, j] if scales[i, j] > 0 else np.float32(1)
                 codes[at] = encoded(y[at] / unit, kind)
     return codes, scales
 
 
-def product8(a, sa, b, sb, b_rows):
+def product8(a, sa, b, sb, b_rows, sizes=True):
     """a [m, k] and b [n, k] as numbers, their scales: the product in 64 bits, the sum of its terms' magnitudes, and that of the
-    largest term of each 16 neighbours."""
+    largest term of each 16 neighbours (both 0 without `sizes`)."""
     k = a.shape[1]
     out, size, tops = (np.zeros((a.shape[0], b.shape[0])) for _ in range(3))
     for c in range(-(-k // 128)):
         at = slice(128 * c, 128 * (c + 1))
         s = sa[:, c, None].astype(np.float64) * np.repeat(sb[:, c].astype(np.float64), b_rows)[None, :b.shape[0]]
         out += s * (a[:, at] @ b[:, at].T)
+        if not sizes:
+            continue
         size += np.abs(s) * (np.abs(a[:, at]) @ np.abs(b[:, at]).T)
         for i in range(128 * c, min(k, 128 * (c + 1)), 16):
             tops += np.abs(s) * (np.abs(a[:, None, i:i + 16]) * np.abs(b[None, :, i:i + 16])).max(-1)

@@ -61,6 +61,25 @@ void add_product(Lowered& L, const Product& p, std::ostringstream& src, std::vec
         << types << ", " << tm << ", " << tn << ", " << wm << ", " << wn << ", " << split << ", " << stages << ", "
         << (direct ? "true" : "false") << ">(x, w, xs, ws, starts, out, parts, a);\n}\n";
   };
+  // The entries in the order of their tiles' rows.  Few rows: the weights' bytes count, and waves share a tile's depth so that
+  // enough loads are on their way (64 x 8192 by 28672 codes: 64 x 128 tiles 38.9 us, 128 x 128 in 16-row tiles 79.6; 16 rows of
+  // it: 32 x 64 tiles 34.9, 16 x 16 51.3, the weights alone at a read's rate 33; one row by 4096 x 4096: 16 x 16 5.2, 32 x 64 9.9).
+  const bool few = std::string(p.by) != "DEPTH";
+  if (few) {
+    add("_one", 16, 16, 1, 1, 8, 4, true, "vectors, and too few tiles of the next");
+    add("_few", 32, 64, 1, 4, 2, 3, true, "vectors, up to 32 rows a group");
+    add("_some", 64, 128, 1, 4, 2, 3, true, "vectors, up to 64 rows a group");
+  }
+  add("_tile", 128, 128, 2, 2, 1, 2, true, "vectors, and few tiles of the next");
+  Entry wide;
+  wide.symbol = L.name + "_wide";
+  wide.threads = 512;
+  wide.vec = wide.cols = 256;
+  wide.fast = true;
+  L.entries.push_back(wide);
+  when.push_back("vectors: 16-byte aligned operands, strides and lengths along them");
+  src << "extern \"C\" __global__ void __launch_bounds__(512) " << wide.symbol << params << " {\n  unpm::matmul_wide<" << types
+      << ">(x, w, xs, ws, starts, out, parts, a);\n}\n";
   add("_any", 128, 128, 2, 2, 1, 2, false, "otherwise");
   Entry e;
   e.symbol = L.name + "_join";
@@ -106,7 +125,7 @@ int32_t lower_quant8(const unp_quant8& q, Lowered& L, std::string& why) {
        {"rows", nullptr, "I64"}, {"cols", nullptr, "I64"}, {"x_row", nullptr, "I64"}, {"code_row", nullptr, "I64"},
        {"scale_row", nullptr, "I64"}},
       rows ? "8 lanes a block; blocks of lanes stride over them" : "a block per 128 x 128 elements, striding over them",
-      {"always"}, nullptr, "scales and quotients correctly rounded to f32, codes rounded to even: bit-exact");
+      {"always"}, nullptr, "scales as the largest magnitude times an f32 constant, quotients correctly rounded to f32, codes rounded to even: bit-exact");
   return UNP_OK;
 }
 
@@ -152,7 +171,7 @@ int32_t lower_grouped_matmul(const unp_grouped_matmul& m, Lowered& L, std::strin
     return why = "an unknown direction of a grouped product", UNP_UNSUPPORTED_OP;
   const bool weight = m.direction == UNP_GROUPED_WEIGHT;
   L.form.kind = UNP_FORM_GROUPED_MATMUL;
-  L.form.dtype = m.dtype;
+  L.form.dtype = m.out;
   L.grouped_matmul = m;
   const char* way = weight ? "weight" : m.direction == UNP_GROUPED_INPUT ? "input" : "forward";
   L.name = std::string("unp_grouped_matmul_") + short_name(m.dtype) + "_" + short_name(m.out) + "_" + way;

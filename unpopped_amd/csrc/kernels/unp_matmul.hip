@@ -45,6 +45,11 @@ template <int N> UNPM_DEV void wait_loads() { asm volatile("s_waitcnt vmcnt(%0)"
 UNPM_DEV void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 UNPM_DEV u32 lds_address(const void* p) { return (u32)(size_t)(lds_void*)p; }
 UNPM_DEV i64 least(i64 a, i64 b) { return a < b ? a : b; }
+// What every lane of a wave has, in scalar registers.
+UNPM_DEV u32 scalar(u32 x) { return __builtin_amdgcn_readfirstlane(x); }
+UNPM_DEV i64 uniform(i64 x) {
+  return (i64)((u64)(u32)__builtin_amdgcn_readfirstlane((i32)(x >> 32)) << 32 | (u32)__builtin_amdgcn_readfirstlane((i32)x));
+}
 
 // ---------------------------------------------------------------------------------------
 // Products: out[i][j] = sum over d of x[i][d] * w[j][d], of 16-bit numbers, or of 8-bit codes with an f32 scale for 128
@@ -67,29 +72,25 @@ struct product_args {
   i64 out_row, out_group;          // in elements
   i32 groups, tiles_m, tiles_n, parts;
   i32 x_vectors, w_vectors;        // rows of whole 16-byte vectors
-  i32 wide;                        // out takes four columns at once
-  i32 pad;
+  i32 wide;                        // out takes vectors of 16 bytes: 1, or 2 past the caches
+  i32 tail;                        // bytes of a row's last 16 along d that exist, where not all do
 };
 
 constexpr u32 OUTSIDE = 0x80000000u;  // an offset past every buffer: loads of it give zeros
 
 UNPM_DEV u32x4 resource(const u8* p) {
   const u64 a = (u64)p;
-  u32x4 r;
-  r[0] = __builtin_amdgcn_readfirstlane((u32)a);
-  r[1] = __builtin_amdgcn_readfirstlane((u32)(a >> 32) & 0xFFFFu);
-  r[2] = OUTSIDE;
-  r[3] = 0x00020000u;
-  return r;
+  return u32x4{scalar((u32)a), scalar((u32)(a >> 32) & 0xFFFFu), OUTSIDE, 0x00020000u};
 }
-// 16 bytes of each lane from p + offset to LDS, lane after lane from `to` on; zeros where the offset is OUTSIDE.
+// 16 bytes of each lane from p + offset to LDS, lane after lane from `to` on; zeros where the offset is OUTSIDE.  (Nothing
+// else here uses M0, which no clobber list may name.)
 UNPM_DEV void load_to_lds(const u8* p, u32 offset, u32 to) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(to), "v"(offset),
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(scalar(to)), "v"(offset),
                "s"(resource(p))
-               : "memory", "m0");
+               : "memory");
 }
 UNPM_DEV void load_word_to_lds(const float* p, u32 to) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" ::"s"(to), "v"(p) : "memory", "m0");
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" ::"s"(scalar(to)), "v"(p) : "memory");
 }
 
 // 16 bytes at p of which `there` exist (elements of E bytes), zeros for the others.
@@ -105,10 +106,11 @@ template <int E> UNPM_DEV u32x4 fetch16(const u8* p, i64 there, bool vector) {
   return x;
 }
 
-// Where the 16 bytes of a tile's row lie: a row of 128 bytes along d has 8 slots, the slot of a chunk goes by the row's
-// low bits and those above them.  A transposed row (2 T bytes) moves pairs of slots: the four rows that 16 lanes read, and
-// the four that lie eight further, are in different banks.
-UNPM_DEV int straight_slot(int row, int chunk) { return chunk ^ ((row ^ (row >> 3)) & 7); }
+// Where the 16 bytes of a tile's row lie: a row of 128 bytes along d has 8 slots, and the slot of a chunk goes by bits 1 to
+// 3 of the row (bit 0 is half of the banks).  Then the 16 lanes that one cycle of a read serves, eight rows' chunk g and eight
+// others' chunk g + 1, are in different banks.  A transposed row (2 T bytes) moves pairs of slots: the four rows that 16
+// lanes read, and the four that lie eight further, are in different banks.
+UNPM_DEV int straight_slot(int row, int chunk) { return chunk ^ ((row >> 1) & 7); }
 template <int T> UNPM_DEV int turned_slot(int row, int chunk) {
   constexpr int PAIRS = T / 16;
   const int f = PAIRS >= 8 ? (row & 3) | ((row >> 3) & 1) << 2 : row & (PAIRS - 1);
@@ -142,6 +144,34 @@ template <int KIND, bool TURNED, int T> struct side {
   // What of the step's length has to be left for the lane's 16 bytes to exist, in bytes or TURNED rows.
   static UNPM_DEV int after(int u, int lane) { return TURNED ? row_of(u, lane) : chunk_of(u, lane) * 16; }
   static UNPM_DEV i64 left(i64 elements) { return TURNED ? elements : elements * E; }
+  static UNPM_DEV bool exists(int after, i64 left) { return TURNED ? after < left : after + 16 <= left; }
+  // Row r of the last step: the first `bytes` of 16 that do not all exist, which no load to LDS took (it wrote zeros).
+  UNPM_DEV void patch(u8* lds, int r, i64 step, i64 elements, int bytes) const {
+    if (TURNED || r >= there) return;
+    const int c = (int)elements * E / 16;
+    const u8* from = at(step) + r * row + c * 16;
+    u8* to = lds + r * 128 + straight_slot(r, c) * 16;
+#pragma clang loop unroll(disable)
+    for (int i = 0; i < bytes; i += E) {
+      if constexpr (E == 1)
+        to[i] = from[i];
+      else
+        *reinterpret_cast<u16*>(to + i) = *reinterpret_cast<const u16*>(from + i);
+    }
+  }
+  // 16 bytes (the q-th) of a step that holds those alone, as its first elements along d.
+  UNPM_DEV void alone(u8* lds, int q, i64 step, i64 elements) const {
+    const i64 first = elements * E / 16 * (16 / E);
+    u32x4 v = {0, 0, 0, 0};
+    const int r = q / CHUNKS, c = q % CHUNKS;
+    if constexpr (TURNED) {
+      if (r < elements - first) v = fetch16<E>(at(step) + (first + r) * row + c * 16, there - c * 16, vectors);
+      *reinterpret_cast<u32x4*>(lds + r * (T * 2) + turned_slot<T>(r, c) * 16) = v;
+    } else {
+      if (c == 0 && r < there) v = fetch16<E>(at(step) + r * row + first * E, (elements - first) * E, false);
+      *reinterpret_cast<u32x4*>(lds + r * 128 + straight_slot(r, c) * 16) = v;
+    }
+  }
   UNPM_DEV const u8* at(i64 step) const { return p + (TURNED ? step * D * row : step * 128); }
   UNPM_DEV u32x4 fetch(int u, int lane, i64 step, i64 elements) const {
     const int r = row_of(u, lane), c = chunk_of(u, lane);
@@ -185,20 +215,30 @@ template <int KA, int KB> UNPM_DEV f32x4 multiply8(const u32x4 (&a)[2], const u3
   return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(x, y, f32x4{0, 0, 0, 0}, KA - E4M3, KB - E4M3, 0, 0, 0, 0);
 }
 
-// Blocks are dealt to the 8 XCDs in turn: each takes a run of the tiles, so that its L2 holds what they share, in bands of
-// 8 tiles along out's rows.
+// Blocks are dealt to the 8 XCDs in turn.  Each takes a run of as many neighbouring tiles as its CUs hold at once, so that
+// its L2 holds what they share; the runs of the XCDs lie side by side, so that groups of any size load them alike.
+// Tiles are counted in bands of 8 along out's rows.
 struct tile_at {
   i64 m, n;
   int part;
 };
-UNPM_DEV tile_at tile_of(const product_args& a) {
-  const u32 b = blockIdx.x, blocks = gridDim.x, each = blocks / 8, rest = blocks % 8, xcd = b % 8;
-  const u32 id = xcd * each + (xcd < rest ? xcd : rest) + b / 8;
-  const u32 tiles = (u32)a.tiles_m * (u32)a.tiles_n, part = id / tiles, t = id % tiles;
+template <u32 RUN> UNPM_DEV bool tile_of(const product_args& a, u32 tiles_m, tile_at& at) {
+  const u32 tiles = tiles_m * (u32)a.tiles_n, all = tiles * (u32)a.parts, b = blockIdx.x;
+  if (b >= all) return false;
+  const u32 turn = b / (8 * RUN) * (8 * RUN), in = b - turn, rest = all - turn;
+  u32 id = turn;
+  if (rest >= 8 * RUN) {
+    id += in % 8 * RUN + in / 8;
+  } else {  // the last turn: runs as equal as they can be
+    const u32 each = rest / 8, more = rest % 8, xcd = in % 8;
+    id += xcd * each + (xcd < more ? xcd : more) + in / 8;
+  }
+  const u32 part = id / tiles, t = id % tiles;
   constexpr u32 BAND = 8;
-  const u32 per = BAND * (u32)a.tiles_n, band = t / per, in = t % per;
-  const u32 first = band * BAND, high = (u32)a.tiles_m - first < BAND ? (u32)a.tiles_m - first : BAND;
-  return {(i64)(first + in % high), (i64)(in / high), (int)part};
+  const u32 per = BAND * (u32)a.tiles_n, band = t / per, of = t % per;
+  const u32 first = band * BAND, high = tiles_m - first < BAND ? tiles_m - first : BAND;
+  at = {(i64)(first + of % high), (i64)(of / high), (int)part};
+  return true;
 }
 
 // The rows of group g, whatever the starts are: within 0 .. rows.
@@ -206,47 +246,70 @@ UNPM_DEV void group_rows(const i32* starts, int g, i64 rows, i64& r0, i64& r1) {
   r0 = least(starts[g] < 0 ? 0 : starts[g], rows);
   r1 = least(starts[g + 1] < 0 ? 0 : starts[g + 1], rows);
 }
-// Tile t of T rows of the groups that have rows: its group and rows, or no such tile.  Every lane of a wave asks alike.
-template <int T> UNPM_DEV bool find_group(const i32* starts, int groups, i64 rows, i64 t, int& group, i64& r0, i64& r1) {
+// How many tiles of T rows this lane's group has, of the 64 groups from `first` on, and how many those up to it have.
+struct tiles_upto {
+  i32 own, upto;
+  i64 r0, r1;
+};
+template <int T> UNPM_DEV tiles_upto group_tiles(const i32* starts, int groups, i64 rows, int first) {
   const int lane = threadIdx.x & 63;
-  i64 past = 0;
-  for (int first = 0; first < groups; first += 64) {
-    i64 s0 = 0, s1 = 0;
-    if (first + lane < groups) group_rows(starts, first + lane, rows, s0, s1);
-    const i32 own = s1 > s0 ? (i32)((s1 - s0 + T - 1) / T) : 0;
-    i32 upto = own;
+  tiles_upto t{0, 0, 0, 0};
+  if (first + lane < groups) group_rows(starts, first + lane, rows, t.r0, t.r1);
+  t.own = t.r1 > t.r0 ? (i32)((t.r1 - t.r0 + T - 1) / T) : 0;
+  t.upto = t.own;
 #pragma unroll
-    for (int d = 1; d < 64; d *= 2) {
-      const i32 v = __shfl_up(upto, d);
-      if (lane >= d) upto += v;
-    }
-    const u64 has = __ballot(past + upto > t);
+  for (int d = 1; d < 64; d *= 2) {
+    const i32 v = __shfl_up(t.upto, d);
+    if (lane >= d) t.upto += v;
+  }
+  return t;
+}
+// This block's tile of T rows of the groups that have rows: its place, group and rows, or none.  Every wave finds it alike.
+template <int T, u32 RUN>
+UNPM_DEV bool find_group(const i32* starts, const product_args& a, tile_at& at, int& group, i64& r0, i64& r1) {
+  tiles_upto t = group_tiles<T>(starts, a.groups, a.m, 0);
+  i64 all = __shfl(t.upto, 63);
+  for (int first = 64; first < a.groups; first += 64) all += __shfl(group_tiles<T>(starts, a.groups, a.m, first).upto, 63);
+  // Starts that decrease may name more tiles than there are blocks.
+  if (!tile_of<RUN>(a, (u32)__builtin_amdgcn_readfirstlane((i32)least(all, a.tiles_m)), at)) return false;
+  i64 past = 0;
+  for (int first = 0;; first += 64) {
+    if (first > 0) t = group_tiles<T>(starts, a.groups, a.m, first);
+    const u64 has = __ballot(past + t.upto > at.m);
     if (has) {
       const int l = __builtin_ctzll(has);
       group = first + l;
-      const i64 tile = t - past - (__shfl(upto, l) - __shfl(own, l));
-      r0 = __shfl((i32)s0, l) + tile * T;
-      r1 = __shfl((i32)s1, l);
+      const i64 tile = at.m - past - (__shfl(t.upto, l) - __shfl(t.own, l));
+      r0 = uniform(__shfl((i32)t.r0, l) + tile * T);
+      r1 = uniform(__shfl((i32)t.r1, l));
       return true;
     }
-    past += __shfl(upto, 63);
+    past += __shfl(t.upto, 63);
+    if (first + 64 >= a.groups) return false;
   }
-  return false;
 }
 
-template <class OUT> UNPM_DEV void store4(OUT* p, const f32x4& v, i64 there, bool wide) {
-  struct alignas(4 * sizeof(OUT)) quad {
-    OUT v[4];
+// N adjacent columns of out, `there` of which exist; `wide`: out takes vectors of 16 bytes, 2: and is larger than what the
+// caches keep (12001 x 8192 results of 16 bits 380 us past them, 394 through; 16 x 8192 x 2048 of 32 bits 482 and 536).
+template <class OUT, int N> UNPM_DEV void store_columns(OUT* p, const float (&v)[N], i64 there, i32 wide) {
+  constexpr int V = 16 / sizeof(OUT);
+  struct alignas(16) vec {
+    OUT v[V];
   };
-  quad q;
 #pragma unroll
-  for (int j = 0; j < 4; ++j) q.v[j] = (OUT)v[j];
-  if (wide && there >= 4) {
-    *reinterpret_cast<quad*>(p) = q;
-  } else {
+  for (int i = 0; i < N; i += V) {
+    vec q;
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-      if (j < there) p[j] = q.v[j];
+    for (int j = 0; j < V; ++j) q.v[j] = (OUT)v[i + j];
+    if (wide == 2 && there >= i + V) {
+      __builtin_nontemporal_store(bits<u32x4>(q), reinterpret_cast<u32x4*>(p + i));
+    } else if (wide && there >= i + V) {
+      *reinterpret_cast<vec*>(p + i) = q;
+    } else {
+#pragma unroll
+      for (int j = 0; j < V; ++j)
+        if (i + j < there) p[i + j] = q.v[j];
+    }
   }
 }
 
@@ -259,42 +322,46 @@ template <int XK, int WK_, bool XT, bool WT, int BY, int TM, int TN> struct plac
   const float *xs, *ws;  // scales of the first rows
   i64 xs_last, ws_last;  // the tile's last rows that have scales
   i64 first, last;       // steps
-  i64 end;               // elements along d of this part
+  i64 end, depth;        // elements along d up to this part's end, and in all
   i64 m0, n0, m_there;   // the tile in out
   i64 row0;              // the tile's first row among all rows (of all groups) of the result
 };
 
-template <int XK, int WKIND, bool XT, bool WT, int BY, int SB, int TM, int TN>
+template <int XK, int WKIND, bool XT, bool WT, int BY, int SB, int TM, int TN, u32 RUN>
 UNPM_DEV bool find_place(const u8* x, const u8* w, const float* xs, const float* ws, const i32* starts,
                          const product_args& a, int& part, place<XK, WKIND, XT, WT, BY, TM, TN>& o) {
   constexpr int E = XK >= E4M3 ? 1 : 2, D = 128 / E;
-  const tile_at t = tile_of(a);
-  part = t.part;
+  tile_at t;
   i64 depth = a.depth;
-  o.n0 = t.n * TN;
-  if constexpr (BY == DEPTH) {
-    const int g = (int)(t.m / ((a.m + TM - 1) / TM));
-    const i64 tm = t.m % ((a.m + TM - 1) / TM);
-    i64 r0, r1;
-    group_rows(starts, g, a.depth, r0, r1);
-    depth = r1 > r0 ? r1 - r0 : 0;
-    o.m0 = tm * TM;
-    o.m_there = a.m - o.m0;
-    o.row0 = g * a.m + o.m0;
-    x += r0 * a.x_row;
-    w += r0 * a.w_row;
-  } else if constexpr (BY == ROWS) {
+  if constexpr (BY == ROWS) {
     int g;
     i64 r0, r1;
-    if (!find_group<TM>(starts, a.groups, a.m, t.m, g, r0, r1)) return false;
+    if (!find_group<TM, RUN>(starts, a, t, g, r0, r1)) return false;
+    g = __builtin_amdgcn_readfirstlane(g);
     o.m0 = o.row0 = r0;
     o.m_there = r1 - r0;
     w += g * a.w_group;
     ws += g * a.ws_group;
   } else {
-    o.m0 = o.row0 = t.m * TM;
+    if (!tile_of<RUN>(a, (u32)a.tiles_m, t)) return false;
+    o.m0 = t.m * TM;
+    o.row0 = o.m0;
+    if constexpr (BY == DEPTH) {
+      const u32 each = (u32)a.tiles_m / (u32)a.groups, g = (u32)t.m / each;
+      i64 r0, r1;
+      group_rows(starts, (int)g, a.depth, r0, r1);
+      r0 = uniform(r0);
+      r1 = uniform(r1);
+      depth = r1 > r0 ? r1 - r0 : 0;
+      o.m0 = (t.m - g * each) * TM;
+      o.row0 = g * a.m + o.m0;
+      x += r0 * a.x_row;
+      w += r0 * a.w_row;
+    }
     o.m_there = a.m - o.m0;
   }
+  part = t.part;
+  o.n0 = t.n * TN;
   const i64 n_there = a.n - o.n0;
   if (o.m_there > TM) o.m_there = TM;
   o.x.p = XT ? x + o.m0 * 2 : x + o.m0 * a.x_row;
@@ -315,21 +382,45 @@ UNPM_DEV bool find_place(const u8* x, const u8* w, const float* xs, const float*
   o.first = steps * part / a.parts;
   o.last = steps * (part + 1) / a.parts;
   o.end = least(depth, o.last * D);
+  o.depth = depth;
   return true;
 }
 
-// The sums of one 16 x 16 tile to out or, where the depth is split, to this part's sums.
-template <class OUT, int BY>
-UNPM_DEV void put(OUT* out, float* parts, const product_args& a, int part, i64 row0, i64 m0, i64 n0, i64 m_there, int m, int n,
-                  const f32x4& v) {
-  const i64 n_there = a.n - n0 - n;
-  if (m >= m_there || n_there <= 0) return;
-  if (a.parts > 1) {
-    const i64 rows = BY == DEPTH ? a.groups * a.m : a.m, wide = (a.n + 3) / 4 * 4;
-    *reinterpret_cast<f32x4*>(parts + (part * rows + row0 + m) * wide + n0 + n) = v;
-  } else {
-    const i64 g = BY == DEPTH ? (row0 - m0) / a.m : 0;
-    store4<OUT>(out + g * a.out_group + (m0 + m) * a.out_row + n0 + n, v, n_there, a.wide);
+// A tile's sums in LDS, [SPLIT][TM][TN] in f32: a row's quads of columns are moved by the row's low bits, so that the 16 rows
+// that a wave's sums of a 16 x 16 product lie in are in different banks.
+template <int TM, int TN> UNPM_DEV int sum_at(int split, int m, int n) {
+  constexpr int Q = TN / 4 < 16 ? TN / 4 : 16;
+  return (split * TM + m) * TN + ((n / 4) ^ (m & (Q - 1))) * 4;
+}
+// From there to out, or where the depth is split to this part's sums: whole rows at a time, as columns written where the
+// matrix instruction leaves them would be 32 bytes of each of 16 rows (a launch of 12001 x 8192 results of 16 bits took 468 us,
+// 343 without its stores).  Row 0 of the sums is row `first` of the block's tile.
+template <class OUT, int BY, int TM, int TN, int SPLIT, int THREADS>
+UNPM_DEV void store_sums(const float* sums, OUT* out, float* parts, const product_args& a, int part, i64 row0, i64 m0, i64 n0,
+                         i64 m_there, int first) {
+  constexpr int V = 16 / sizeof(OUT) < TN ? 16 / sizeof(OUT) : TN;
+  for (int q = threadIdx.x; q < TM * TN / V; q += THREADS) {
+    const int m = q / (TN / V), n = q % (TN / V) * V;
+    const i64 there = a.n - n0 - n;
+    if (first + m >= m_there || there <= 0) continue;
+    float v[V];
+#pragma unroll
+    for (int i = 0; i < V; i += 4) {
+      f32x4 t = *reinterpret_cast<const f32x4*>(sums + sum_at<TM, TN>(0, m, n + i));
+#pragma unroll
+      for (int s = 1; s < SPLIT; ++s) t += *reinterpret_cast<const f32x4*>(sums + sum_at<TM, TN>(s, m, n + i));
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[i + j] = t[j];
+    }
+    if (a.parts > 1) {
+      const i64 rows = BY == DEPTH ? a.groups * a.m : a.m, wide = (a.n + 7) / 8 * 8;
+      float* p = parts + (part * rows + row0 + first + m) * wide + n0 + n;
+#pragma unroll
+      for (int i = 0; i < V; i += 4) *reinterpret_cast<f32x4*>(p + i) = f32x4{v[i], v[i + 1], v[i + 2], v[i + 3]};
+    } else {
+      const i64 g = BY == DEPTH ? (row0 - m0) / a.m : 0;
+      store_columns<OUT>(out + g * a.out_group + (m0 + first + m) * a.out_row + n0 + n, v, there, a.wide);
+    }
   }
 }
 
@@ -353,7 +444,7 @@ UNPM_DEV void matmul(const u8* xp, const u8* wp, const float* xsp, const float* 
 
   place<XK, WKIND, XT, WT, BY, TM, TN> o;
   int part;
-  if (!find_place<XK, WKIND, XT, WT, BY, SB, TM, TN>(xp, wp, xsp, wsp, starts, a, part, o)) return;
+  if (!find_place<XK, WKIND, XT, WT, BY, SB, TM, TN, 64>(xp, wp, xsp, wsp, starts, a, part, o)) return;
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int wm = wave % WM, wn = wave / WM % WN, own = wave / (WM * WN);
   f32x4 acc[NT][MT];
@@ -395,7 +486,7 @@ UNPM_DEV void matmul(const u8* xp, const u8* wp, const float* xsp, const float* 
         const bool isx = u < xside::UNITS;
         const i64 rest = isx ? xside::left(left) : wside::left(left);
         const u8* p = isx ? o.x.at(step) : o.w.at(step);
-        load_to_lds(p, after[i] < rest ? offset[i] : OUTSIDE, lds0 + at);
+        load_to_lds(p, (isx ? xside::exists(after[i], rest) : wside::exists(after[i], rest)) ? offset[i] : OUTSIDE, lds0 + at);
       } else {
         const u32x4 y = u < xside::UNITS ? o.x.fetch(u, lane, step, left) : o.w.fetch(u - xside::UNITS, lane, step, left);
         *reinterpret_cast<u32x4*>(lds + at + lane * 16) = y;
@@ -468,62 +559,295 @@ UNPM_DEV void matmul(const u8* xp, const u8* wp, const float* xsp, const float* 
       if constexpr (DIRECT) wait_loads<(STAGES - 2) * LOADS>();
       lds_barrier();
       issue(s + STAGES - 1, slot == 0 ? STAGES - 1 : slot - 1);
+      if (DIRECT && a.tail && s == stages - 1 && o.end == o.depth) {
+        const i64 last = o.last - 1, left = o.end - last * D;
+        u8* at = lds + slot * STAGE + (int)((last - o.first) % SPLIT) * STEP;
+        for (int r = threadIdx.x; r < TM + TN; r += WAVES * 64) {
+          if (r < TM)
+            o.x.patch(at, r, last, left, a.tail);
+          else
+            o.w.patch(at + xside::BYTES, r - TM, last, left, a.tail);
+        }
+        lds_barrier();
+      }
       compute(slot);
       slot = slot == STAGES - 1 ? 0 : slot + 1;
     }
     if constexpr (DIRECT) wait_loads<0>();  // LDS is not written after the block's end
   }
 
-  if constexpr (SPLIT > 1) {
-    lds_barrier();
-    float* sums = reinterpret_cast<float*>(lds);  // [SPLIT][TM][TN]
+  lds_barrier();
+  float* sums = reinterpret_cast<float*>(lds);
 #pragma unroll
-    for (int n = 0; n < NT; ++n)
+  for (int n = 0; n < NT; ++n)
 #pragma unroll
-      for (int m = 0; m < MT; ++m)
-        *reinterpret_cast<f32x4*>(sums + (own * TM + (wm * MT + m) * 16 + (lane & 15)) * TN + (wn * NT + n) * 16 + (lane >> 4) * 4) =
-            acc[n][m];
-    lds_barrier();
-    for (int q = threadIdx.x; q < TM * TN / 4; q += WAVES * 64) {
-      const int m = q / (TN / 4), n = q % (TN / 4) * 4;
-      f32x4 v = *reinterpret_cast<const f32x4*>(sums + m * TN + n);
+    for (int m = 0; m < MT; ++m)
+      *reinterpret_cast<f32x4*>(sums + sum_at<TM, TN>(own, (wm * MT + m) * 16 + (lane & 15), (wn * NT + n) * 16 + (lane >> 4) * 4)) =
+          acc[n][m];
+  lds_barrier();
+  store_sums<OUT, BY, TM, TN, SPLIT, WAVES * 64>(sums, out, parts, a, part, o.row0, o.m0, o.n0, o.m_there, 0);
+}
+
+// Tiles of 256 x 256 for much work: eight waves, two on each SIMD, of which one multiplies while the other reads LDS and
+// starts loads (the second set runs one barrier behind the first).  A wave has four blocks of 64 x 32, one in each quarter of
+// the tile; the halves of the operands' tiles lie in LDS twice, and as a half has been read by every wave, the loads of
+// the same half two steps on go there: five halves are on their way at any time.
+//   phase  reads     multiplies  loads
+//   0      X0 W0     X0 W0       scales and X1 of the next step
+//   1      W1        X0 W1       X0 of the one after it
+//   2      X1        X1 W1       W0
+//   3                X1 W0       W1
+// A wave waits for its own loads of what the next phase reads before the barrier that ends its reads: all but those that it
+// has started since.
+template <int XK, int WKIND, bool XT, bool WT, class OUT, int BY, int SB>
+UNPM_DEV void matmul_wide(const u8* xp, const u8* wp, const float* xsp, const float* wsp, const i32* starts, OUT* out, float* parts,
+                          const product_args& a) {
+  constexpr int E = XK >= E4M3 ? 1 : 2, D = 128 / E;
+  typedef side<XK, XT, 128> xside;
+  typedef side<WKIND, WT, 128> wside;
+  constexpr int HALF = 16384, SCALES = E == 1 ? 2048 : 0, STAGE = 4 * HALF + SCALES;
+  __shared__ __attribute__((aligned(1024))) u8 lds[2 * STAGE];
+
+  place<XK, WKIND, XT, WT, BY, 256, 256> o;
+  int part;
+  if (!find_place<XK, WKIND, XT, WT, BY, SB, 256, 256, 32>(xp, wp, xsp, wsp, starts, a, part, o)) return;
+  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int wm = wave >> 2, wn = wave & 3;
+  const u32 lds0 = lds_address(lds);
+
+  // The halves of the operands: X0, X1, W0, W1.  Two loads of a wave each.
+  xside xh[2];
+  wside wh[2];
 #pragma unroll
-      for (int s = 1; s < SPLIT; ++s) v += *reinterpret_cast<const f32x4*>(sums + (s * TM + m) * TN + n);
-      put<OUT, BY>(out, parts, a, part, o.row0, o.m0, o.n0, o.m_there, m, n, v);
+  for (int h = 0; h < 2; ++h) {
+    xh[h].row = a.x_row;
+    xh[h].p = XT ? o.x.p + h * 256 : o.x.p + h * 128 * a.x_row;
+    xh[h].there = o.x.there - h * (XT ? 256 : 128);
+    wh[h].row = a.w_row;
+    wh[h].p = WT ? o.w.p + h * 256 : o.w.p + h * 128 * a.w_row;
+    wh[h].there = o.w.there - h * (WT ? 256 : 128);
+    xh[h].vectors = wh[h].vectors = true;
+  }
+  u32 offset[4][2];
+#pragma unroll
+  for (int h = 0; h < 2; ++h)
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      offset[h][i] = xh[h].offset(i * 8 + wave, lane);
+      offset[2 + h][i] = wh[h].offset(i * 8 + wave, lane);
     }
-  } else {
+  const float* scale = nullptr;
+  if constexpr (E == 1) {
+    const int f = wave * 64 + lane;
+    scale = f < 256 ? o.xs + least(f, o.xs_last) * a.xs_row : o.ws + least((f - 256) / SB, o.ws_last) * a.ws_row;
+  }
+  // What of a step has to be left for a lane's 16 bytes to exist is the same for every load of it along d.
+  const i32 x_after = xside::after(wave, lane), w_after = wside::after(wave, lane);
+  auto issue = [&](int half, i64 step) {
+    const bool isx = half < 2;
+    const i32 left = (i32)(o.end - (o.first + step) * D);
+    const u8* p = isx ? xh[half & 1].at(o.first + step) : wh[half & 1].at(o.first + step);
+    const u32 to = lds0 + (u32)(step & 1) * STAGE + half * HALF + wave * 1024;
 #pragma unroll
-    for (int n = 0; n < NT; ++n)
+    for (int i = 0; i < 2; ++i) {
+      const i32 after = (isx ? x_after + (XT ? i * 32 : 0) : w_after + (WT ? i * 32 : 0));
+      const i32 rest = (i32)(isx ? xside::left(left) : wside::left(left));
+      load_to_lds(p, (isx ? xside::exists(after, rest) : wside::exists(after, rest)) ? offset[half][i] : OUTSIDE, to + i * 8192);
+    }
+  };
+  auto issue_scales = [&](i64 step) {
+    if constexpr (E == 1)
+      load_word_to_lds(scale + least(o.first + step, o.last - 1), lds0 + (u32)(step & 1) * STAGE + 4 * HALF + wave * 256);
+  };
+
+  f32x4 acc[2][2][2][4];  // of W half, X half, tile of W, tile of X
 #pragma unroll
-      for (int m = 0; m < MT; ++m)
-        put<OUT, BY>(out, parts, a, part, o.row0, o.m0, o.n0, o.m_there, (wm * MT + m) * 16 + (lane & 15),
-                     (wn * NT + n) * 16 + (lane >> 4) * 4, acc[n][m]);
+  for (int i = 0; i < 32; ++i) (&acc[0][0][0][0])[i] = f32x4{0, 0, 0, 0};
+  const i64 steps = o.last - o.first;
+  if (steps > 0) {
+    issue(0, 0);
+    issue(2, 0);
+    issue(3, 0);
+    issue_scales(0);
+    issue(1, 0);
+    issue(0, 1);
+    issue(2, 1);
+    issue(3, 1);
+    wait_loads<E == 1 ? 8 : 10>();
+    lds_barrier();
+    if (wm == 1) lds_barrier();
+
+    u32x4 xf[4][2], wf[2][2][2];
+    float xsc[4], wsc = 0;  // of the halves at hand
+    f32x4 wrow[2];
+    auto read_x = [&](const u8* at, int h) {
+#pragma unroll
+      for (int m = 0; m < 4; ++m)
+#pragma unroll
+        for (int k = 0; k < 2; ++k) xf[m][k] = xside::read(at + h * HALF, wm * 64 + m * 16, k, lane);
+      if constexpr (E == 1)
+#pragma unroll
+        for (int m = 0; m < 4; ++m)
+          xsc[m] = reinterpret_cast<const float*>(at + 4 * HALF)[h * 128 + wm * 64 + m * 16 + (lane & 15)];
+    };
+    auto read_w_scales = [&](const u8* at, int h) {
+      const float* s = reinterpret_cast<const float*>(at + 4 * HALF) + 256 + h * 128;
+      if constexpr (E == 1 && SB == 1)
+#pragma unroll
+        for (int n = 0; n < 2; ++n) wrow[n] = *reinterpret_cast<const f32x4*>(s + wn * 32 + n * 16 + (lane >> 4) * 4);
+      if constexpr (E == 1 && SB > 1) wsc = *s;
+    };
+    auto read_w = [&](const u8* at, int h) {
+#pragma unroll
+      for (int n = 0; n < 2; ++n)
+#pragma unroll
+        for (int k = 0; k < 2; ++k) wf[h][n][k] = wside::read(at + (2 + h) * HALF, wn * 32 + n * 16, k, lane);
+      read_w_scales(at, h);
+    };
+    auto products = [&](int hw, int hx) {
+      __builtin_amdgcn_s_setprio(1);
+      if constexpr (E == 2) {
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+#pragma unroll
+          for (int n = 0; n < 2; ++n)
+#pragma unroll
+            for (int m = 0; m < 4; ++m) acc[hw][hx][n][m] = multiply<XK>(wf[hw][n][k], xf[m][k], acc[hw][hx][n][m]);
+      } else {
+        // A product's sums are taken up two instructions later, when they are there: three are held, not eight.
+        constexpr int LATE = 2;
+        f32x4 p[LATE + 1];
+        float both[4];
+#pragma unroll
+        for (int m = 0; m < 4; ++m) both[m] = SB == 1 ? xsc[m] : xsc[m] * wsc;
+#pragma unroll
+        for (int i = 0; i < 8 + LATE; ++i) {
+          if (i < 8) p[i % (LATE + 1)] = multiply8<WKIND, XK>(wf[hw][i / 4], xf[i % 4]);
+          __builtin_amdgcn_sched_barrier(0);
+          if (i >= LATE) {
+            const int n = (i - LATE) / 4, m = (i - LATE) % 4;
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              acc[hw][hx][n][m][j] =
+                  __builtin_fmaf(p[(i - LATE) % (LATE + 1)][j], SB == 1 ? both[m] * wrow[n][j] : both[m], acc[hw][hx][n][m][j]);
+          }
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      }
+      __builtin_amdgcn_s_setprio(0);
+    };
+    auto meet = [&] {
+      __builtin_amdgcn_sched_barrier(0);
+      asm volatile("s_barrier" ::: "memory");
+      __builtin_amdgcn_sched_barrier(0);
+    };
+    auto read_done = [&] {
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      meet();
+    };
+    for (i64 s = 0; s < steps; ++s) {
+      const u8* at = lds + (u32)(s & 1) * STAGE;
+      read_x(at, 0);
+      read_w(at, 0);
+      issue_scales(s + 1);
+      issue(1, s + 1);
+      wait_loads<E == 1 ? 12 : 10>();
+      read_done();
+      products(0, 0);
+      meet();
+      read_w(at, 1);
+      issue(0, s + 2);
+      wait_loads<E == 1 ? 11 : 10>();
+      read_done();
+      products(1, 0);
+      meet();
+      read_x(at, 1);
+      issue(2, s + 2);
+      read_done();
+      products(1, 1);
+      meet();
+      read_w_scales(at, 0);
+      issue(3, s + 2);
+      wait_loads<E == 1 ? 8 : 10>();
+      read_done();
+      products(0, 1);
+      meet();
+    }
+    if (wm == 0) lds_barrier();
+    wait_loads<0>();
+    if (a.tail && o.end == o.depth) {
+      // The bytes of the last 16 that exist, which the last step had as zeros: one more step of them alone.
+      const i64 last = o.last - 1, left = o.end - last * D;
+      lds_barrier();
+#pragma clang loop unroll(disable)
+      for (int q = threadIdx.x; q < 1024; q += 512) {
+        xh[0].alone(lds, q, last, left);
+        xh[1].alone(lds + HALF, q, last, left);
+        wh[0].alone(lds + 2 * HALF, q, last, left);
+        wh[1].alone(lds + 3 * HALF, q, last, left);
+      }
+      if constexpr (E == 1) *reinterpret_cast<float*>(lds + 4 * HALF + threadIdx.x * 4) = scale[last];
+      lds_barrier();
+      read_x(lds, 0);
+      read_w(lds, 0);
+      products(0, 0);
+      read_w(lds, 1);
+      products(1, 0);
+      read_x(lds, 1);
+      products(1, 1);
+      read_w_scales(lds, 0);
+      products(0, 1);
+    }
+  }
+  // A half of X at a time: 128 rows of sums fill what held the steps.
+  float* sums = reinterpret_cast<float*>(lds);
+#pragma unroll
+  for (int hx = 0; hx < 2; ++hx) {
+    lds_barrier();
+#pragma unroll
+    for (int hw = 0; hw < 2; ++hw)
+#pragma unroll
+      for (int n = 0; n < 2; ++n)
+#pragma unroll
+        for (int m = 0; m < 4; ++m)
+          *reinterpret_cast<f32x4*>(sums + sum_at<128, 256>(0, wm * 64 + m * 16 + (lane & 15),
+                                                            hw * 128 + wn * 32 + n * 16 + (lane >> 4) * 4)) = acc[hw][hx][n][m];
+    lds_barrier();
+    store_sums<OUT, BY, 128, 256, 1, 512>(sums, out, parts, a, part, o.row0, o.m0, o.n0, o.m_there, hx * 128);
   }
 }
 
 // The sums of a split depth, part after part.
 template <class OUT, int BY>
 UNPM_DEV void join(const i32* starts, OUT* out, const float* parts, const product_args& a) {
-  const i64 rows = BY == DEPTH ? a.groups * a.m : a.m, quads = (a.n + 3) / 4;
+  const i64 rows = BY == DEPTH ? a.groups * a.m : a.m, units = (a.n + 7) / 8;
   i64 r0 = 0, r1 = rows;
   if constexpr (BY == ROWS) {
     i64 skip;
     group_rows(starts, 0, rows, r0, skip);
     group_rows(starts, a.groups - 1, rows, skip, r1);
   }
-  for (i64 i = r0 * quads + (i64)blockIdx.x * 256 + threadIdx.x; i < r1 * quads; i += (i64)gridDim.x * 256) {
-    const i64 r = i / quads, n = i % quads * 4;
-    f32x4 v = *reinterpret_cast<const f32x4*>(parts + r * quads * 4 + n);
-    for (int p = 1; p < a.parts; ++p) v += *reinterpret_cast<const f32x4*>(parts + (p * rows + r) * quads * 4 + n);
+  for (i64 i = r0 * units + (i64)blockIdx.x * 256 + threadIdx.x; i < r1 * units; i += (i64)gridDim.x * 256) {
+    const i64 r = i / units, n = i % units * 8;
+    float v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+    for (int p = 0; p < a.parts; ++p) {
+      const f32x4* q = reinterpret_cast<const f32x4*>(parts + (p * rows + r) * units * 8 + n);
+      const f32x4 x = q[0], y = n + 4 < a.n ? q[1] : f32x4{0, 0, 0, 0};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        v[j] += x[j];
+        v[4 + j] += y[j];
+      }
+    }
     const i64 g = BY == DEPTH ? r / a.m : 0;
-    store4<OUT>(out + g * a.out_group + (r - g * a.m * (BY == DEPTH)) * a.out_row + n, v, a.n - n, a.wide);
+    store_columns<OUT>(out + g * a.out_group + (BY == DEPTH ? r - g * a.m : r) * a.out_row + n, v, a.n - n, a.wide);
   }
 }
 
 // ---------------------------------------------------------------------------------------
 // Quantisation: codes of y = x or its transpose, and the f32 scale of each block of 128 columns and RB rows of y:
-// scale = most / largest code, code = y / scale rounded to even, both quotients correctly rounded.  A block of zeros has the
-// scale 0 and divides as by 1; one that holds a NaN or an infinity has a NaN scale and codes 0.
+// scale = most times the f32 nearest to 1 / largest code, code = y / scale rounded to even from the correctly rounded quotient.
+// A block of zeros has the scale 0 and divides as by 1; one that holds a NaN or an infinity has a NaN scale and codes 0.
 //
 // Magnitudes are compared as integers (NaN above infinity above every number).  The quotient of two f32 numbers is taken
 // from the divisor's reciprocal by one correction (P. Markstein, 1990), exact while the remainder is a normal number;
@@ -535,7 +859,7 @@ struct quant_args {
   i32 x_vectors, code_vectors;
 };
 
-template <int KIND> UNPM_DEV float largest() { return KIND == E4M3 ? 448.0f : 57344.0f; }
+template <int KIND> UNPM_DEV float inverse_largest() { return KIND == E4M3 ? 1.0f / 448.0f : 1.0f / 57344.0f; }
 
 struct step_of {
   float scale, unit, inverse;
@@ -544,7 +868,7 @@ struct step_of {
 template <int KIND> UNPM_DEV step_of block_step(u32 most) {
   step_of s;
   s.none = most >= 0x7F800000u;
-  s.scale = s.none ? __builtin_nanf("") : bits<float>(most) / largest<KIND>();
+  s.scale = s.none ? __builtin_nanf("") : bits<float>(most) * inverse_largest<KIND>();
   s.unit = s.scale > 0.0f ? s.scale : 1.0f;
   s.inverse = 1.0f / s.unit;
   s.divide = s.unit < 0x1p-90f;

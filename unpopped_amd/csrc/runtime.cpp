@@ -578,7 +578,9 @@ int32_t unp_hip_exec_create(const unp_generated* g, unp_exec** out, unp_error* e
     }
     x->fns.push_back(f);
     int per_cu = 0;
-    if ((x->l.form.kind == UNP_FORM_ROW_REDUCE || x->l.form.kind == UNP_FORM_CACHE4_ATTENTION) &&
+    const int32_t kind = x->l.form.kind;
+    if ((kind == UNP_FORM_ROW_REDUCE || kind == UNP_FORM_CACHE4_ATTENTION || kind == UNP_FORM_MATMUL8 ||
+         kind == UNP_FORM_GROUPED_MATMUL) &&
         hipModuleOccupancyMaxActiveBlocksPerMultiprocessor(&per_cu, f, en.threads > 0 ? en.threads : x->l.threads, 0) !=
             hipSuccess)
       per_cu = 0;
@@ -2184,7 +2186,7 @@ int32_t run_cache4_attention(unp_exec* x, const unp_arg* a, size_t n, hipStream_
 // Host images of the kernels' argument structs (passed by value).
 struct product_args_host {
   int64_t m, n, depth, x_row, w_row, w_group, xs_row, ws_row, ws_group, out_row, out_group;
-  int32_t groups, tiles_m, tiles_n, parts, x_vectors, w_vectors, wide, pad;
+  int32_t groups, tiles_m, tiles_n, parts, x_vectors, w_vectors, wide, tail;
 };
 struct quant_args_host {
   int64_t rows, cols, x_row, code_row, scale_row;
@@ -2195,7 +2197,7 @@ struct rows_args_host {
   int32_t groups, chunks;
 };
 
-constexpr int64_t kMostExtent = (int64_t)1 << 28, kMostGroups = 1024;
+constexpr int64_t kMostExtent = (int64_t)1 << 28, kMostGroups = 1024, kMostSplit = 16;
 
 // A product's extents: rows and columns of out (by group where the depth is), the depth, and the groups.
 struct Extents {
@@ -2215,7 +2217,7 @@ int32_t check_extents(const Extents& e, unp_error* err) {
   return UNP_OK;
 }
 
-int64_t parts_bytes(const Extents& e, int64_t parts) { return parts * e.rows() * ((e.n + 3) / 4 * 4) * 4; }
+int64_t parts_bytes(const Extents& e, int64_t parts) { return parts * e.rows() * ((e.n + 7) / 8 * 8) * 4; }
 
 // Tiles of `t` rows that e's rows fill at most: a group's last one is not shared.
 int64_t row_tiles(const Extents& e, int64_t t) {
@@ -2225,11 +2227,25 @@ int64_t row_tiles(const Extents& e, int64_t t) {
 }
 
 ProductPlan product_plan(const unp_exec* x, const Extents& e, bool direct) {
-  (void)direct;
   ProductPlan p;
-  const unp::Entry& k = x->l.entries[p.entry];
-  p.tiles_m = row_tiles(e, k.vec);
-  p.tiles_n = (e.n + k.cols - 1) / k.cols;
+  const std::vector<unp::Entry>& es = x->l.entries;
+  const size_t any = es.size() - 2, wide = any - 1, tile = any - 2;
+  auto tiles = [&](size_t k) { return row_tiles(e, es[k].vec) * ((e.n + es[k].cols - 1) / es[k].cols); };
+  auto holds = [&](size_t k) { return (int64_t)x->cu_count * std::max(1, x->resident[k]); };
+  p.entry = any;
+  if (direct) {
+    // Rows of a group, on average over the groups that can have some.
+    const int64_t used = e.by_row ? std::max<int64_t>(1, std::min(e.groups, e.m)) : 1, rows = (e.m + used - 1) / used;
+    p.entry = tiles(wide) >= x->cu_count / 2 ? wide : tile;
+    if (!e.by_depth && rows <= 64) p.entry = rows <= 32 ? 1 : 2;
+    if (!e.by_depth && rows <= 16 && tiles(1) < x->cu_count) p.entry = 0;
+  }
+  p.tiles_m = row_tiles(e, es[p.entry].vec);
+  p.tiles_n = (e.n + es[p.entry].cols - 1) / es[p.entry].cols;
+  // Few tiles: the depth in as many parts as the CUs hold blocks, each at least eight steps of the waves that share it.
+  const int64_t steps = (e.depth * (x->l.form.kind == UNP_FORM_MATMUL8 ? 1 : 2) + 127) / 128, all = p.tiles_m * p.tiles_n;
+  if (direct && 2 * all <= holds(p.entry))
+    p.parts = std::max<int64_t>(1, std::min({holds(p.entry) / all, steps / (8 * std::max(1, es[p.entry].k)), kMostSplit}));
   return p;
 }
 
@@ -2247,6 +2263,8 @@ int32_t launch_product(unp_exec* x, const Extents& e, product_args_host args, co
   args.tiles_m = (int32_t)p.tiles_m;
   args.tiles_n = (int32_t)p.tiles_n;
   args.parts = (int32_t)p.parts;
+  // Results past half of the 256 MiB last-level cache are not kept in it.
+  if (args.wide && (__int128)e.rows() * e.n * (int64_t)unp::kind_bytes(x->l.form.dtype) > (128 << 20)) args.wide = 2;
   uint64_t xp = buf[0], wp = buf[1], xs = buf[2], ws = buf[3], starts = buf[4], out = buf[5], parts = buf[6];
   void* params[] = {&xp, &wp, &xs, &ws, &starts, &out, &parts, &args};
   x->chunks = p.parts;
@@ -2254,7 +2272,7 @@ int32_t launch_product(unp_exec* x, const Extents& e, product_args_host args, co
   const int32_t rc = launch(x, p.entry, (uint32_t)blocks, params, s, err);
   if (rc != UNP_OK || p.parts == 1) return rc;
   void* jparams[] = {&starts, &out, &parts, &args};
-  return launch(x, x->l.entries.size() - 1, grid_for(x, (e.rows() * ((e.n + 3) / 4) + 255) / 256), jparams, s, err);
+  return launch(x, x->l.entries.size() - 1, grid_for(x, (e.rows() * ((e.n + 7) / 8) + 255) / 256), jparams, s, err);
 }
 
 // Rows of whole 16-byte vectors at `p`, stride in elements of `size` bytes.
@@ -2304,8 +2322,9 @@ int32_t run_matmul8(unp_exec* x, const unp_arg* a, size_t n, hipStream_t s, unp_
   args.out_row = out_row;
   args.x_vectors = vectors(A.buf[0], a_row, 1);
   args.w_vectors = vectors(A.buf[2], b_row, 1) && b_group % 16 == 0;
-  args.wide = A.buf[out] % (uint64_t)(4 * size) == 0 && out_row % 4 == 0;
-  const bool direct = args.x_vectors && args.w_vectors && e.depth % 16 == 0 && near(a_row) && near(b_row);
+  args.wide = vectors(A.buf[out], out_row, size);
+  args.tail = (int32_t)(e.depth % 16);
+  const bool direct = args.x_vectors && args.w_vectors && near(a_row) && near(b_row);
   const uint64_t buf[7] = {A.buf[0], A.buf[2], A.buf[1], A.buf[3], starts, A.buf[out], A.buf[out + 1]};
   return launch_product(x, e, args, buf, bytes, direct, s, err);
 }
@@ -2355,9 +2374,10 @@ int32_t run_grouped_matmul(unp_exec* x, const unp_arg* a, size_t n, hipStream_t 
   args.out_group = out_group;
   args.x_vectors = vectors(A.buf[0], x_row, 2);
   args.w_vectors = vectors(A.buf[1], w_row, 2) && w_group % 8 == 0;
-  args.wide = A.buf[3] % (uint64_t)(4 * size) == 0 && out_row % 4 == 0 && out_group % 4 == 0;
-  // What lies along the rows in memory is whole vectors: the depth, or columns of out.
-  const bool whole = weight ? nn % 8 == 0 && kk % 8 == 0 : input ? nn % 8 == 0 && kk % 8 == 0 : kk % 8 == 0;
+  args.wide = vectors(A.buf[3], out_row, size) && out_group * size % 16 == 0;
+  // Columns of out that lie along an operand's rows are whole vectors; a depth that does may end inside one.
+  const bool whole = weight ? nn % 8 == 0 && kk % 8 == 0 : input ? kk % 8 == 0 : true;
+  args.tail = weight ? 0 : (int32_t)(2 * e.depth % 16);
   const bool direct = args.x_vectors && args.w_vectors && whole && near(2 * x_row) && near(2 * w_row);
   const uint64_t buf[7] = {A.buf[0], A.buf[1], 0, 0, A.buf[2], A.buf[3], A.buf[4]};
   return launch_product(x, e, args, buf, bytes, direct, s, err);
