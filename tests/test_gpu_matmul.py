@@ -155,13 +155,12 @@ def starts_of(rng, rows, groups, way):
 
 
 def matmul8_case(m, n, k, a_kind="Fp8E4M3FN", b_kind="Fp8E4M3FN", out="Bf16", b_rows=128, groups=0, way="all", pad=0, first=0, seed=0,
-                 whole=True, workspace=None, nan_scale=False, starts=None, out_pad=0):
+                 whole=True, workspace=None, nan_scale=False, starts=None, out_pad=0, top=4):
     """whole: numbers and scales whose products and sums are exact in 32 bits, so that the result has to be."""
     rng = np.random.default_rng(seed)
     nb, nr = -(-k // 128), -(-n // b_rows)
     g = max(1, groups)
     if whole:
-        top = 4
         a, b = (rng.integers(-top, top + 1, s).astype(float) for s in ((m, k), (g, n, k)))
         sa, sb = (np.exp2(rng.integers(-2, 3, s)).astype(np.float32) for s in ((m, nb), (g, nr, nb)))
         assert top * top * k * 16 * 16 <= 1 << 24  # in units of 2^-4
@@ -457,41 +456,50 @@ def test_rows_of_groups_refuse(hip_device):
 # Each kernel, at the edges of its tiles
 # ---------------------------------------------------------------------------------------
 @pytest.mark.parametrize("m, n, k, kw, entry", [
-    (1, 100, 2048, {}, "_one"), (16, 33, 1040, {}, "_one"), (17, 64, 1024, {}, "_few"), (32, 2100, 272, {}, "_few"),
-    (33, 128, 1024, {}, "_some"), (64, 130, 2176, dict(b_rows=1), "_some"), (65, 129, 1168, {}, "_tile"), (200, 300, 128, dict(b_rows=1), "_tile"),
-    (2049, 3849, 144, {}, "_wide"), (2817, 2820, 400, dict(b_rows=1), "_wide"), (2817, 2561, 16, dict(a_kind="Fp8E5M2"), "_wide"),
-    (2817, 2700, 272, dict(out="F16", out_pad=1), "_wide"), (130, 140, 200, dict(pad=1), "_any"), (3, 5, 128, dict(pad=1), "_any"),
+    (1, 100, 2048, {}, "_one"), (16, 33, 1040, {}, "_one"), (17, 64, 1024, {}, "_slim"), (32, 2100, 272, {}, "_slim"),
+    (33, 128, 1024, {}, "_slim"), (64, 130, 2176, dict(b_rows=1), "_one"), (65, 129, 1168, {}, "_one"), (200, 300, 128, dict(b_rows=1), "_slim"),
+    (2049, 3849, 144, {}, "_wide"), (2817, 2820, 400, dict(b_rows=1), "_wide"), (2817, 2561, 16, dict(a_kind="Fp8E5M2"), "_tile"),
+    (2817, 2700, 272, dict(out="F16", out_pad=1), "_tile"), (130, 140, 200, dict(pad=1), "_any"), (3, 5, 128, dict(pad=1), "_any"),
     # Lengths that end inside 16 bytes, in rows of whole vectors.
-    (1, 100, 2001, dict(pad=15), "_one"), (20, 100, 1039, dict(pad=1), "_few"), (60, 130, 129, dict(pad=15), "_some"), (70, 129, 1151, dict(pad=1), "_tile"),
-    (2817, 2561, 257, dict(pad=15), "_wide"), (2817, 2561, 7, dict(pad=9, first=16), "_wide"), (2817, 2561, 143, dict(pad=1, b_rows=1), "_wide"),
+    (1, 100, 2001, dict(pad=15), "_one"), (20, 100, 1039, dict(pad=1), "_one"), (60, 130, 129, dict(pad=15), "_slim"), (70, 129, 1151, dict(pad=1), "_one"),
+    (2817, 2561, 257, dict(pad=15), "_tile"), (2817, 2561, 7, dict(pad=9, first=16), "_tile"), (2817, 2561, 143, dict(pad=1, b_rows=1), "_tile"),
+    (100, 2100, 16, {}, "_few"), (33, 8200, 143, dict(pad=1), "_few"), (65, 4100, 272, dict(b_rows=1), "_few"), (31, 8200, 1039, dict(pad=1), "_few"),
+    (100, 8200, 143, dict(pad=1), "_some"), (600, 2100, 272, dict(b_rows=1), "_some"), (4000, 264, 144, dict(a_kind="Fp8E5M2"), "_some"),
+    (1000, 2100, 16, {}, "_tile"), (2049, 2561, 257, dict(pad=15), "_tile"), (4000, 2561, 272, {}, "_wide"), (4000, 2100, 143, dict(pad=1, b_rows=1), "_wide"),
+    (2817, 4100, 257, dict(pad=15, out="F16", out_pad=1), "_wide"), (4000, 8200, 7, dict(pad=9, first=16), "_wide"),
 ])
 def test_product_of_codes_by_kernel(hip_device, m, n, k, kw, entry):
     assert matmul8_case(m, n, k, **kw)["entry"].endswith(entry)
 
 
 @pytest.mark.parametrize("m, n, k, groups, way, entry", [
-    (40, 48, 256, 8, "all", "_one"), (500, 2100, 144, 40, "gaps", "_few"), (500, 260, 640, 10, "all", "_some"), (900, 300, 272, 6, "gaps", "_tile"),
+    (40, 48, 256, 8, "all", "_slim"), (500, 2100, 144, 40, "gaps", "_few"), (500, 260, 640, 10, "all", "_slim"), (900, 300, 272, 6, "gaps", "_few"),
     (4000, 2300, 144, 5, "gaps", "_wide"), (3500, 2561, 272, 2, "one", "_wide"),
+    (40, 48, 1040, 8, "all", "_one"), (500, 1100, 640, 10, "all", "_few"), (900, 1300, 272, 6, "gaps", "_some"), (2000, 2100, 272, 6, "gaps", "_tile"),
 ])
 def test_product_of_codes_by_group_and_kernel(hip_device, m, n, k, groups, way, entry):
     assert matmul8_case(m, n, k, groups=groups, way=way)["entry"].endswith(entry)
 
 
 @pytest.mark.parametrize("direction, rows, n, k, groups, way, entry", [
-    ("forward", 40, 48, 256, 8, "all", "_one"), ("forward", 500, 2104, 136, 40, "gaps", "_few"), ("forward", 500, 264, 640, 10, "all", "_some"),
-    ("forward", 900, 304, 72, 6, "gaps", "_tile"), ("forward", 4000, 2304, 72, 5, "gaps", "_wide"), ("forward", 3500, 2561, 200, 2, "one", "_wide"),
-    ("input", 40, 256, 48, 8, "all", "_one"), ("input", 500, 136, 2104, 40, "gaps", "_few"), ("input", 500, 640, 264, 10, "all", "_some"),
-    ("input", 900, 72, 304, 6, "gaps", "_tile"), ("input", 4000, 72, 2304, 5, "gaps", "_wide"), ("input", 3500, 200, 2568, 2, "one", "_wide"),
+    ("forward", 40, 48, 256, 8, "all", "_slim"), ("forward", 500, 2104, 136, 40, "gaps", "_few"), ("forward", 500, 264, 640, 10, "all", "_slim"),
+    ("forward", 900, 304, 72, 6, "gaps", "_few"), ("forward", 4000, 2304, 72, 5, "gaps", "_wide"), ("forward", 3500, 2561, 200, 2, "one", "_wide"),
+    ("input", 40, 256, 48, 8, "all", "_slim"), ("input", 500, 136, 2104, 40, "gaps", "_few"), ("input", 500, 640, 264, 10, "all", "_slim"),
+    ("input", 900, 72, 304, 6, "gaps", "_few"), ("input", 4000, 72, 2304, 5, "gaps", "_wide"), ("input", 3500, 200, 2568, 2, "one", "_wide"),
     ("weight", 300, 264, 520, 3, "gaps", "_tile"), ("weight", 700, 1104, 1288, 6, "gaps", "_wide"), ("weight", 131, 2312, 2824, 2, "one", "_wide"),
     ("weight", 300, 2056, 2056, 2, "all", "_wide"),
+    ("forward", 40, 48, 1040, 8, "all", "_one"), ("forward", 900, 1304, 136, 6, "gaps", "_some"), ("forward", 2000, 2104, 136, 6, "gaps", "_tile"),
+    ("input", 40, 1040, 48, 8, "all", "_one"), ("input", 900, 136, 1304, 6, "gaps", "_some"), ("input", 2000, 136, 2104, 6, "gaps", "_tile"),
 ])
 def test_grouped_product_by_kernel(hip_device, direction, rows, n, k, groups, way, entry):
     assert grouped_case(direction, rows, n, k, groups, way=way)["entry"].endswith(entry)
 
 
 @pytest.mark.parametrize("direction, rows, n, k, groups, pad, entry", [
-    ("forward", 40, 48, 257, 8, 7, "_one"), ("forward", 900, 304, 71, 6, 1, "_tile"), ("forward", 4000, 2304, 129, 5, 7, "_wide"),
-    ("input", 40, 257, 48, 8, 7, "_one"), ("input", 900, 71, 304, 6, 1, "_tile"), ("input", 4000, 129, 2304, 5, 7, "_wide"),
+    ("forward", 40, 48, 257, 8, 7, "_slim"), ("forward", 900, 304, 71, 6, 1, "_few"), ("forward", 4000, 2304, 129, 5, 7, "_wide"),
+    ("input", 40, 257, 48, 8, 7, "_slim"), ("input", 900, 71, 304, 6, 1, "_few"), ("input", 4000, 129, 2304, 5, 7, "_wide"),
+    ("forward", 40, 48, 1041, 8, 7, "_one"), ("forward", 900, 1304, 135, 6, 1, "_some"), ("forward", 2000, 2104, 71, 6, 1, "_tile"),
+    ("input", 40, 1041, 48, 8, 7, "_one"), ("input", 900, 135, 1304, 6, 1, "_some"), ("input", 2000, 71, 2104, 6, 1, "_tile"),
 ])
 def test_grouped_product_of_lengths_inside_a_vector(hip_device, direction, rows, n, k, groups, pad, entry):
     """The depth alone; the columns of an operand that lie along out are whole vectors."""
@@ -503,8 +511,8 @@ def test_grouped_product_of_lengths_inside_a_vector(hip_device, direction, rows,
 
 @pytest.mark.parametrize("workspace", [None, 0])
 def test_a_split_depth_gives_the_same_whole_numbers(hip_device, workspace):
-    parts = [matmul8_case(60, 200, 4096, workspace=workspace)["chunks"],
-             grouped_case("forward", 60, 136, 4096, 2, way="gaps", workspace=workspace)["chunks"],
-             grouped_case("input", 60, 4096, 136, 1, workspace=workspace)["chunks"],
+    parts = [matmul8_case(60, 200, 28000, top=1, workspace=workspace)["chunks"],
+             grouped_case("forward", 60, 136, 16384, 2, way="gaps", workspace=workspace)["chunks"],
+             grouped_case("input", 60, 16384, 136, 1, workspace=workspace)["chunks"],
              grouped_case("weight", 4096, 136, 200, 2, out="F32", workspace=workspace)["chunks"]]
     assert all(p > 1 for p in parts) if workspace is None else parts == [1] * 4

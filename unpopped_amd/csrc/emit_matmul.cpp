@@ -41,6 +41,8 @@ struct Product {
   int scale_rows;
 };
 
+const char* kFewest = "16-byte aligned operands and strides, columns of out along an operand's rows in whole vectors; the least time";
+
 void add_product(Lowered& L, const Product& p, std::ostringstream& src, std::vector<std::string>& when) {
   const std::string types = std::string(p.x) + ", " + p.w + ", " + (p.x_turned ? "true" : "false") + ", " +
                             (p.w_turned ? "true" : "false") + ", " + p.out + ", unpm::" + p.by + ", " +
@@ -61,23 +63,22 @@ void add_product(Lowered& L, const Product& p, std::ostringstream& src, std::vec
         << types << ", " << tm << ", " << tn << ", " << wm << ", " << wn << ", " << split << ", " << stages << ", "
         << (direct ? "true" : "false") << ">(x, w, xs, ws, starts, out, parts, a);\n}\n";
   };
-  // The entries in the order of their tiles' rows.  Few rows: the weights' bytes count, and waves share a tile's depth so that
-  // enough loads are on their way (64 x 8192 by 28672 codes: 64 x 128 tiles 38.9 us, 128 x 128 in 16-row tiles 79.6; 16 rows of
-  // it: 32 x 64 tiles 34.9, 16 x 16 51.3, the weights alone at a read's rate 33; one row by 4096 x 4096: 16 x 16 5.2, 32 x 64 9.9).
-  const bool few = std::string(p.by) != "DEPTH";
-  if (few) {
-    add("_one", 16, 16, 1, 1, 8, 4, true, "vectors, and too few tiles of the next");
-    add("_few", 32, 64, 1, 4, 2, 3, true, "vectors, up to 32 rows a group");
-    add("_some", 64, 128, 1, 4, 2, 3, true, "vectors, up to 64 rows a group");
+  // In the order of their tiles; product_plan says which of them a launch takes.  Few rows: the weights' bytes count, and waves
+  // share a tile's steps so that enough loads are on their way.
+  if (std::string(p.by) != "DEPTH") {
+    add("_one", 16, 16, 1, 1, 8, 4, true, kFewest);
+    add("_slim", 32, 32, 1, 2, 4, 3, true, kFewest);
+    add("_few", 32, 64, 1, 4, 2, 3, true, kFewest);
+    add("_some", 64, 128, 1, 4, 2, 3, true, kFewest);
   }
-  add("_tile", 128, 128, 2, 2, 1, 2, true, "vectors, and few tiles of the next");
+  add("_tile", 128, 128, 2, 4, 1, 2, true, kFewest);
   Entry wide;
   wide.symbol = L.name + "_wide";
   wide.threads = 512;
   wide.vec = wide.cols = 256;
   wide.fast = true;
   L.entries.push_back(wide);
-  when.push_back("vectors: 16-byte aligned operands, strides and lengths along them");
+  when.push_back(kFewest);
   src << "extern \"C\" __global__ void __launch_bounds__(512) " << wide.symbol << params << " {\n  unpm::matmul_wide<" << types
       << ">(x, w, xs, ws, starts, out, parts, a);\n}\n";
   add("_any", 128, 128, 2, 2, 1, 2, false, "otherwise");

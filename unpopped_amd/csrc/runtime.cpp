@@ -2186,7 +2186,7 @@ int32_t run_cache4_attention(unp_exec* x, const unp_arg* a, size_t n, hipStream_
 // Host images of the kernels' argument structs (passed by value).
 struct product_args_host {
   int64_t m, n, depth, x_row, w_row, w_group, xs_row, ws_row, ws_group, out_row, out_group;
-  int32_t groups, tiles_m, tiles_n, parts, x_vectors, w_vectors, wide, tail;
+  int32_t groups, tiles_m, tiles_n, parts, x_vectors, w_vectors, wide, tail, turn, pad;
 };
 struct quant_args_host {
   int64_t rows, cols, x_row, code_row, scale_row;
@@ -2197,7 +2197,7 @@ struct rows_args_host {
   int32_t groups, chunks;
 };
 
-constexpr int64_t kMostExtent = (int64_t)1 << 28, kMostGroups = 1024, kMostSplit = 16;
+constexpr int64_t kMostExtent = (int64_t)1 << 28, kMostGroups = 1024;
 
 // A product's extents: rows and columns of out (by group where the depth is), the depth, and the groups.
 struct Extents {
@@ -2226,34 +2226,65 @@ int64_t row_tiles(const Extents& e, int64_t t) {
   return e.m / t + std::min(e.groups, e.m);
 }
 
-ProductPlan product_plan(const unp_exec* x, const Extents& e, bool direct) {
-  ProductPlan p;
-  const std::vector<unp::Entry>& es = x->l.entries;
-  const size_t any = es.size() - 2, wide = any - 1, tile = any - 2;
-  auto tiles = [&](size_t k) { return row_tiles(e, es[k].vec) * ((e.n + es[k].cols - 1) / es[k].cols); };
-  auto holds = [&](size_t k) { return (int64_t)x->cu_count * std::max(1, x->resident[k]); };
-  p.entry = any;
-  if (direct) {
-    // Rows of a group, on average over the groups that can have some.
-    const int64_t used = e.by_row ? std::max<int64_t>(1, std::min(e.groups, e.m)) : 1, rows = (e.m + used - 1) / used;
-    p.entry = tiles(wide) >= x->cu_count / 2 ? wide : tile;
-    if (!e.by_depth && rows <= 64) p.entry = rows <= 32 ? 1 : 2;
-    if (!e.by_depth && rows <= 16 && tiles(1) < x->cu_count) p.entry = 0;
+// What a direct entry takes, in microseconds: to begin and end, and a step (128 bytes along the depth) of the blocks of a CU,
+// of one block and of as many as the CU holds; and the TB/s at which it reads weights that no cache holds.  Fitted to times of
+// 78 shapes of 1 to 16000 rows, 72 to 28672 columns, depths of 64 to 28672 and 1 to 64 groups, where it chooses entries and parts
+// that are 4 % slower than the best of each (geometric mean; over 12 % at 7 shapes, 43 % at the worst).
+struct EntryCost {
+  double fixed, alone, full, rate;
+};
+EntryCost entry_cost(int tile, bool codes) {
+  switch (tile) {  // rows x columns
+    case 16 * 16: return {4.4, 0.05, 0.13, 4.0};
+    case 32 * 32: return {3.5, 0.16, 0.21, 4.8};
+    case 32 * 64: return {4.3, 0.21, 0.38, 5.3};
+    case 64 * 128: return {4.3, 0.39, 0.50, 5.2};
+    case 128 * 128: return codes ? EntryCost{4.6, 0.80, 1.55, 3.6} : EntryCost{4.6, 0.80, 1.20, 4.4};
+    default: return codes ? EntryCost{8.0, 1.60, 2.00, 3.5} : EntryCost{5.0, 1.18, 1.46, 3.2};
   }
-  p.tiles_m = row_tiles(e, es[p.entry].vec);
-  p.tiles_n = (e.n + es[p.entry].cols - 1) / es[p.entry].cols;
-  // Few tiles: the depth in as many parts as the CUs hold blocks, each at least eight steps of the waves that share it.
-  const int64_t steps = (e.depth * (x->l.form.kind == UNP_FORM_MATMUL8 ? 1 : 2) + 127) / 128, all = p.tiles_m * p.tiles_n;
-  if (direct && 2 * all <= holds(p.entry))
-    p.parts = std::max<int64_t>(1, std::min({holds(p.entry) / all, steps / (8 * std::max(1, es[p.entry].k)), kMostSplit}));
-  return p;
+}
+
+// The entry and the number of parts of the depth that take the least time.  Operands that no entry loads directly, or rows of
+// other sizes than whole vectors along out, go to the last one but the join, unsplit.
+ProductPlan product_plan(const unp_exec* x, const Extents& e, bool direct, int64_t workspace_bytes) {
+  const std::vector<unp::Entry>& es = x->l.entries;
+  ProductPlan best;
+  best.entry = es.size() - 2;
+  if (direct) {
+    const bool codes = x->l.form.kind == UNP_FORM_MATMUL8;
+    // Groups that have rows, as rows thrown at them leave, and their rows or their depth on average.
+    const double groups = (double)std::max<int64_t>(1, e.groups), n = e.by_row ? (double)e.m : e.by_depth ? (double)e.depth : 1.0;
+    const double used = e.by_row ? std::max(1.0, groups * (1.0 - std::exp(-n / groups))) : 1.0;
+    const double depth = (double)e.depth / (e.by_depth ? groups : 1.0), steps = std::max(1.0, std::ceil(depth * (codes ? 1 : 2) / 128.0));
+    const double weights = used * (double)e.n * depth * (codes ? 1 : 2) / 1e6;  // that no entry can do without
+    double least = 0;
+    for (size_t k = 0; k + 2 < es.size(); ++k) {
+      const double rows = e.by_row ? used * std::max(1.0, (double)e.m / used / es[k].vec + 0.5) : (double)row_tiles(e, es[k].vec);
+      const double tiles = rows * (double)((e.n + es[k].cols - 1) / es[k].cols);
+      const double hold = (double)x->cu_count * std::max(1, x->resident[k]);
+      const EntryCost c = entry_cost(es[k].vec * es[k].cols, codes);
+      const double read = weights / c.rate;
+      for (int64_t parts : {1, 2, 3, 4, 6, 8, 12, 16}) {
+        if (parts > 1 && (steps < 4.0 * es[k].k * (double)parts || parts_bytes(e, parts) > workspace_bytes)) break;
+        const double blocks = tiles * (double)parts, each = std::ceil(steps / (double)parts), rounds = std::ceil(blocks / hold);
+        double t = std::max(read, blocks <= x->cu_count ? each * c.alone : rounds * each * c.full) + c.fixed + 1.5 * (rounds - 1);
+        if (parts > 1) t += 4.0 + 2.0 * (double)parts_bytes(e, parts) / 3.2e6;
+        if (least > 0 && t >= least) continue;
+        least = t;
+        best.entry = k;
+        best.parts = parts;
+      }
+    }
+  }
+  best.tiles_m = row_tiles(e, es[best.entry].vec);
+  best.tiles_n = (e.n + es[best.entry].cols - 1) / es[best.entry].cols;
+  return best;
 }
 
 // The launch of a product whose strides and buffers are checked: x, w, their scales, starts, out and workspace.
 int32_t launch_product(unp_exec* x, const Extents& e, product_args_host args, const uint64_t (&buf)[7], int64_t workspace_bytes,
                        bool direct, hipStream_t s, unp_error* err) {
-  ProductPlan p = product_plan(x, e, direct);
-  while (p.parts > 1 && parts_bytes(e, p.parts) > workspace_bytes) --p.parts;
+  const ProductPlan p = product_plan(x, e, direct, workspace_bytes);
   const int64_t blocks = p.tiles_m * p.tiles_n * p.parts;
   if (blocks > kMostBlocks) return invalid(err, "more than 2^24 - 1 tiles of the result: " + std::to_string(blocks));
   args.m = e.m;
@@ -2263,6 +2294,7 @@ int32_t launch_product(unp_exec* x, const Extents& e, product_args_host args, co
   args.tiles_m = (int32_t)p.tiles_m;
   args.tiles_n = (int32_t)p.tiles_n;
   args.parts = (int32_t)p.parts;
+  args.turn = x->l.entries[p.entry].vec <= 64 && x->l.entries[p.entry].fast;
   // Results past half of the 256 MiB last-level cache are not kept in it.
   if (args.wide && (__int128)e.rows() * e.n * (int64_t)unp::kind_bytes(x->l.form.dtype) > (128 << 20)) args.wide = 2;
   uint64_t xp = buf[0], wp = buf[1], xs = buf[2], ws = buf[3], starts = buf[4], out = buf[5], parts = buf[6];
@@ -2468,7 +2500,7 @@ int32_t product_workspace(const unp_exec* x, const int64_t* sc, size_t n, uint64
   }
   const int32_t rc = check_extents(e, err);
   if (rc != UNP_OK || e.m == 0 || e.n == 0 || e.groups == 0) return rc;
-  const ProductPlan p = product_plan(x, e, true);
+  const ProductPlan p = product_plan(x, e, true, kMostOffset);
   if (p.parts > 1) bytes = (uint64_t)parts_bytes(e, p.parts);
   return UNP_OK;
 }
