@@ -112,9 +112,10 @@ int32_t lower_quant8(const unp_quant8& q, Lowered& L, std::string& why) {
   const bool rows = q.block_rows == 1 && !q.transpose;
   Entry e;
   e.symbol = L.name + "_k";
+  e.threads = rows ? 256 : 512;
   L.entries.push_back(e);
   const std::string T = device_type(q.dtype);
-  src << "extern \"C\" __global__ void __launch_bounds__(256) " << e.symbol << "(const " << T
+  src << "extern \"C\" __global__ void __launch_bounds__(" << e.threads << ") " << e.symbol << "(const " << T
       << "* x, unpm::u8* codes, float* scales, unpm::quant_args a) {\n  unpm::quantise_" << (rows ? "rows<" : "tiles<") << T << ", "
       << operand(q.kind);
   if (!rows) src << ", " << q.block_rows << ", " << (q.transpose ? "true" : "false");
@@ -125,7 +126,7 @@ int32_t lower_quant8(const unp_quant8& q, Lowered& L, std::string& why) {
       {{"x", "Read", kind_name(q.dtype)}, {"codes", "Write", kind_name(q.kind)}, {"scales", "Write", "F32"},
        {"rows", nullptr, "I64"}, {"cols", nullptr, "I64"}, {"x_row", nullptr, "I64"}, {"code_row", nullptr, "I64"},
        {"scale_row", nullptr, "I64"}},
-      rows ? "8 lanes a block; blocks of lanes stride over them" : "a block per 128 x 128 elements, striding over them",
+      rows ? "8 lanes a block of 128 elements" : "a block of lanes per 128 x 128 elements",
       {"always"}, nullptr, "scales as the largest magnitude times an f32 constant, quotients correctly rounded to f32, codes rounded to even: bit-exact");
   return UNP_OK;
 }

@@ -887,11 +887,18 @@ template <int KIND> UNPM_DEV step_of block_step(u32 most) {
   s.divide = s.unit < 0x1p-90f;
   return s;
 }
-UNPM_DEV float quotient(float y, const step_of& s) {
-  if (s.none) return 0.0f;
-  if (s.divide) return y / s.unit;
-  const float q = y * s.inverse;
-  return __builtin_fmaf(-__builtin_fmaf(q, s.unit, -y), s.inverse, q);  // in this order a zero keeps its sign
+// Numbers of one block over its step; where it is none, whatever comes out.  A wave divides or multiplies as one.
+template <int N> UNPM_DEV void quotients(float (&y)[N], const step_of& s) {
+  if (__any(s.divide)) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) y[i] = y[i] / s.unit;
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const float q = y[i] * s.inverse;
+      y[i] = __builtin_fmaf(-__builtin_fmaf(q, s.unit, -y[i]), s.inverse, q);  // in this order a zero keeps its sign
+    }
+  }
 }
 // Four codes as a word.
 template <int KIND> UNPM_DEV u32 codes4(float a, float b, float c, float d) {
@@ -903,26 +910,20 @@ template <int KIND> UNPM_DEV u32 codes4(float a, float b, float c, float d) {
 UNPM_DEV u32 magnitude(float x) { return bits<u32>(x) & 0x7FFFFFFFu; }
 UNPM_DEV u32 more(u32 a, u32 b) { return a > b ? a : b; }
 
-// N elements of a row from column c on, zeros past the last one.
-template <class T, int N> UNPM_DEV void load_row(const T* row, i64 c, i64 cols, bool vectors, float (&y)[N]) {
-  if (vectors && c + N <= cols) {
-    constexpr int V = 16 / sizeof(T);
-    struct alignas(16) vec {
-      T v[V];
-    };
+// 16 bytes of a row from column c on, zeros past the last one (whole: known to be there and aligned).
+template <class T> struct alignas(16) vec_of {
+  T v[16 / sizeof(T)];
+};
+template <class T> UNPM_DEV vec_of<T> load_vec(const T* row, i64 c, i64 cols, bool whole) {
+  constexpr int V = 16 / sizeof(T);
+  if (whole) return *reinterpret_cast<const vec_of<T>*>(row + c);
+  vec_of<T> v;
 #pragma unroll
-    for (int i = 0; i < N; i += V) {
-      const vec v = *reinterpret_cast<const vec*>(row + c + i);
-#pragma unroll
-      for (int j = 0; j < V; ++j) y[i + j] = (float)v.v[j];
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < N; ++i) y[i] = c + i < cols ? (float)row[c + i] : 0.0f;
-  }
+  for (int i = 0; i < V; ++i) v.v[i] = c + i < cols ? row[c + i] : (T)0.0f;
+  return v;
 }
-template <int W> UNPM_DEV void store_codes(u8* row, i64 c, i64 cols, bool vectors, const u32 (&w)[W]) {
-  if (vectors && c + 4 * W <= cols) {
+template <int W> UNPM_DEV void store_codes(u8* row, i64 c, i64 cols, bool whole, const u32 (&w)[W]) {
+  if (whole) {
     struct alignas(4 * W) vec {
       u32 v[W];
     };
@@ -936,59 +937,99 @@ template <int W> UNPM_DEV void store_codes(u8* row, i64 c, i64 cols, bool vector
       if (c + i < cols) row[c + i] = (u8)(w[i / 4] >> (i % 4 * 8));
   }
 }
+// The largest of 8 neighbouring lanes' numbers: within pairs, within fours, and of the two fours.
+UNPM_DEV u32 most_of_8(u32 m) {
+  m = more(m, (u32)__builtin_amdgcn_mov_dpp((i32)m, 0xB1, 0xF, 0xF, true));
+  m = more(m, (u32)__builtin_amdgcn_mov_dpp((i32)m, 0x4E, 0xF, 0xF, true));
+  return more(m, (u32)__builtin_amdgcn_mov_dpp((i32)m, 0x141, 0xF, 0xF, true));
+}
 
-// A scale per row and block: 8 lanes hold its 128 elements, 16 each.
+// A scale per row and block: 8 lanes hold its 128 elements, 16 bytes of each run of 128 (so a load covers whole lines).
+// Memory bounds it: 69 microseconds for 16384 x 8192 16-bit numbers (5.9 TB/s), 68 for a loop that only reads and writes as much.
 template <class T, int KIND> UNPM_DEV void quantise_rows(const T* x, u8* codes, float* scales, const quant_args& a) {
+  constexpr int V = 16 / sizeof(T), PIECES = 16 / V;
   const i64 blocks = (a.cols + 127) / 128, all = a.rows * blocks;
   const int lane = threadIdx.x & 7;
-  for (i64 i = ((i64)blockIdx.x * 256 + threadIdx.x) / 8; i < all; i += (i64)gridDim.x * 32) {
-    const i64 r = i / blocks, b = i % blocks, c = b * 128 + lane * 16;
-    float y[16];
-    load_row<T, 16>(x + r * a.x_row, c, a.cols, a.x_vectors, y);
+  for (i64 first = (i64)blockIdx.x * 32; first < all; first += (i64)gridDim.x * 32) {
+    const i64 r0 = first >> 31 ? first / blocks : (u32)first / (u32)blocks;
+    const u32 b0 = (u32)(first - r0 * blocks) + threadIdx.x / 8, b = b0 % (u32)blocks;
+    const i64 r = r0 + b0 / (u32)blocks;
+    if (r >= a.rows) break;
+    const i64 c = (i64)b * 128 + lane * V;
+    // A wave whose blocks are all there loads and stores without a look at each vector: its loads are then in flight together.
+    const bool there = __all((i64)b * 128 + 128 <= a.cols), loads = there && a.x_vectors, stores = there && a.code_vectors;
+    vec_of<T> v[PIECES];
+    if (loads) {
+#pragma unroll
+      for (int p = 0; p < PIECES; ++p) v[p] = load_vec<T>(x + r * a.x_row, c + p * 8 * V, a.cols, true);
+    } else {
+#pragma unroll
+      for (int p = 0; p < PIECES; ++p) v[p] = load_vec<T>(x + r * a.x_row, c + p * 8 * V, a.cols, false);
+    }
+    float y[PIECES * V];
     u32 most = 0;
 #pragma unroll
-    for (int j = 0; j < 16; ++j) most = more(most, magnitude(y[j]));
+    for (int j = 0; j < 16; ++j) {
+      y[j] = (float)v[j / V].v[j % V];
+      most = more(most, magnitude(y[j]));
+    }
+    const step_of s = block_step<KIND>(most_of_8(most));
+    quotients(y, s);
 #pragma unroll
-    for (int d = 1; d < 8; d *= 2) most = more(most, (u32)__shfl_xor((i32)most, d));
-    const step_of s = block_step<KIND>(most);
-    u32 w[4];
+    for (int p = 0; p < PIECES; ++p) {
+      u32 w[V / 4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-      w[j] = codes4<KIND>(quotient(y[4 * j], s), quotient(y[4 * j + 1], s), quotient(y[4 * j + 2], s), quotient(y[4 * j + 3], s));
-    store_codes<4>(codes + r * a.code_row, c, a.cols, a.code_vectors, w);
+      for (int j = 0; j < V / 4; ++j) {
+        const float* z = y + p * V + 4 * j;
+        w[j] = s.none ? 0 : codes4<KIND>(z[0], z[1], z[2], z[3]);
+      }
+      store_codes<V / 4>(codes + r * a.code_row, c + p * 8 * V, a.cols, stores, w);
+    }
     if (lane == 0) scales[r * a.scale_row + b] = s.scale;
   }
 }
 
-// The other forms: a block takes 128 x 128 elements of x; thread (i, j) rows 8 i .. 8 i + 7 and columns 8 j .. 8 j + 7.
-// One scale for all of them, or (TURNED) one for each column, whose 128 rows lie along y's row.
-template <class T, int KIND, int RB, bool TURNED>
+// The other forms: a block takes 128 x 128 elements of x; thread (i, j) R rows from R i on and 8 columns, 16 bytes of each run
+// of 16 lanes.  One scale for all of them, or (TURNED) one for each column, whose 128 rows lie along y's row.
+// 34.5 microseconds for 8192 x 4096 of 32 bits (4.9 TB/s), 30 for a copy; threads of 8 rows each, half as many, took 35.4.
+template <class T, int KIND, int RB, bool TURNED, int THREADS = 512>
 UNPM_DEV void quantise_tiles(const T* x, u8* codes, float* scales, const quant_args& a) {
   static_assert(RB == 128 || TURNED, "scales of rows are quantise_rows's");
   constexpr int ROW = 128 + 16;  // of a transposed tile in LDS
-  __shared__ u32 tops[16][128];
+  constexpr int V = 16 / sizeof(T), PIECES = 8 / V, R = 2048 / THREADS, TEAMS = 128 / R;
+  __shared__ u32 tops[TEAMS][128];
   __shared__ __attribute__((aligned(16))) u8 turned[TURNED ? 128 * ROW : 16];
   const i64 across = (a.cols + 127) / 128, all = (a.rows + 127) / 128 * across;
   const int i = threadIdx.x / 16, j = threadIdx.x % 16;
   for (i64 t = blockIdx.x; t < all; t += gridDim.x) {
-    const i64 tr = t / across, tc = t % across, r0 = tr * 128 + i * 8, c0 = tc * 128 + j * 8;
-    float y[8][8];
+    const i64 tr = t / across, tc = t % across, r0 = tr * 128 + i * R, c0 = tc * 128 + j * V;
+    const bool there = tr * 128 + 128 <= a.rows && tc * 128 + 128 <= a.cols, loads = there && a.x_vectors, stores = there && a.code_vectors;
+    vec_of<T> v[R][PIECES];
+    if (loads) {
 #pragma unroll
-    for (int r = 0; r < 8; ++r) {
-      if (r0 + r < a.rows) {
-        load_row<T, 8>(x + (r0 + r) * a.x_row, c0, a.cols, a.x_vectors, y[r]);
-      } else {
+      for (int r = 0; r < R; ++r)
 #pragma unroll
-        for (int c = 0; c < 8; ++c) y[r][c] = 0.0f;
-      }
+        for (int p = 0; p < PIECES; ++p) v[r][p] = load_vec<T>(x + (r0 + r) * a.x_row, c0 + p * 16 * V, a.cols, true);
+    } else {
+#pragma unroll
+      for (int r = 0; r < R; ++r)
+#pragma unroll
+        for (int p = 0; p < PIECES; ++p)
+          v[r][p] = load_vec<T>(x + (r0 + r) * a.x_row, r0 + r < a.rows ? c0 + p * 16 * V : a.cols, a.cols, false);
     }
+    float y[8][R];  // of a column, then a row
     u32 top[8];
 #pragma unroll
     for (int c = 0; c < 8; ++c) {
       top[c] = 0;
 #pragma unroll
-      for (int r = 0; r < 8; ++r) top[c] = more(top[c], magnitude(y[r][c]));
+      for (int r = 0; r < R; ++r) {
+        y[c][r] = (float)v[r][c / V].v[c % V];
+        top[c] = more(top[c], magnitude(y[c][r]));
+      }
     }
+    auto column = [&](int c) { return c / V * 16 * V + j * V + c % V; };
+    bool none[8];
     if constexpr (RB == 128) {
       u32 most = 0;
 #pragma unroll
@@ -997,54 +1038,69 @@ UNPM_DEV void quantise_tiles(const T* x, u8* codes, float* scales, const quant_a
       for (int d = 1; d < 64; d *= 2) most = more(most, (u32)__shfl_xor((i32)most, d));
       if ((threadIdx.x & 63) == 0) tops[0][threadIdx.x / 64] = most;
       __syncthreads();
-      most = more(more(tops[0][0], tops[0][1]), more(tops[0][2], tops[0][3]));
+      most = 0;
+#pragma unroll
+      for (int w = 0; w < THREADS / 64; ++w) most = more(most, tops[0][w]);
       const step_of s = block_step<KIND>(most);
       if (threadIdx.x == 0) scales[(TURNED ? tc : tr) * a.scale_row + (TURNED ? tr : tc)] = s.scale;
 #pragma unroll
-      for (int r = 0; r < 8; ++r)
-#pragma unroll
-        for (int c = 0; c < 8; ++c) y[r][c] = quotient(y[r][c], s);
+      for (int c = 0; c < 8; ++c) {
+        quotients(y[c], s);
+        none[c] = s.none;
+      }
     } else {
 #pragma unroll
-      for (int c = 0; c < 8; ++c) tops[i][j * 8 + c] = top[c];
+      for (int c = 0; c < 8; ++c) tops[i][column(c)] = top[c];
       __syncthreads();
       if (threadIdx.x < 128) {
         u32 most = 0;
 #pragma unroll
-        for (int k = 0; k < 16; ++k) most = more(most, tops[k][threadIdx.x]);
+        for (int k = 0; k < TEAMS; ++k) most = more(most, tops[k][threadIdx.x]);
         tops[0][threadIdx.x] = most;
         if (tc * 128 + threadIdx.x < a.cols) scales[(tc * 128 + threadIdx.x) * a.scale_row + tr] = block_step<KIND>(most).scale;
       }
       __syncthreads();
 #pragma unroll
       for (int c = 0; c < 8; ++c) {
-        const step_of s = block_step<KIND>(tops[0][j * 8 + c]);
-#pragma unroll
-        for (int r = 0; r < 8; ++r) y[r][c] = quotient(y[r][c], s);
+        const step_of s = block_step<KIND>(tops[0][column(c)]);
+        quotients(y[c], s);
+        none[c] = s.none;
       }
     }
     if constexpr (TURNED) {
 #pragma unroll
-      for (int c = 0; c < 8; ++c)
-        *reinterpret_cast<u32x2*>(turned + (j * 8 + c) * ROW + i * 8) =
-            u32x2{codes4<KIND>(y[0][c], y[1][c], y[2][c], y[3][c]), codes4<KIND>(y[4][c], y[5][c], y[6][c], y[7][c])};
+      for (int c = 0; c < 8; ++c) {
+        struct alignas(R) codes_of {
+          u32 v[R / 4];
+        } w;
+#pragma unroll
+        for (int k = 0; k < R / 4; ++k) w.v[k] = none[c] ? 0 : codes4<KIND>(y[c][4 * k], y[c][4 * k + 1], y[c][4 * k + 2], y[c][4 * k + 3]);
+        *reinterpret_cast<codes_of*>(turned + column(c) * ROW + i * R) = w;
+      }
       __syncthreads();
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const int c = k * 32 + threadIdx.x / 8, part = threadIdx.x % 8;
+      for (int k = 0; k < 1024 / THREADS; ++k) {
+        const int c = k * (THREADS / 8) + threadIdx.x / 8, part = threadIdx.x % 8;
         if (tc * 128 + c < a.cols) {
-          const u32x4 v = *reinterpret_cast<const u32x4*>(turned + c * ROW + part * 16);
-          const u32 w[4] = {v[0], v[1], v[2], v[3]};
-          store_codes<4>(codes + (tc * 128 + c) * a.code_row, tr * 128 + part * 16, a.rows, a.code_vectors, w);
+          const u32x4 u = *reinterpret_cast<const u32x4*>(turned + c * ROW + part * 16);
+          const u32 w[4] = {u[0], u[1], u[2], u[3]};
+          store_codes<4>(codes + (tc * 128 + c) * a.code_row, tr * 128 + part * 16, a.rows, stores, w);
         }
       }
     } else {
 #pragma unroll
-      for (int r = 0; r < 8; ++r)
-        if (r0 + r < a.rows) {
-          const u32 w[2] = {codes4<KIND>(y[r][0], y[r][1], y[r][2], y[r][3]), codes4<KIND>(y[r][4], y[r][5], y[r][6], y[r][7])};
-          store_codes<2>(codes + (r0 + r) * a.code_row, c0, a.cols, a.code_vectors, w);
-        }
+      for (int r = 0; r < R; ++r)
+        if (r0 + r < a.rows)
+#pragma unroll
+          for (int p = 0; p < PIECES; ++p) {
+            u32 w[V / 4];
+#pragma unroll
+            for (int k = 0; k < V / 4; ++k) {
+              const int c = p * V + 4 * k;
+              w[k] = none[0] ? 0 : codes4<KIND>(y[c][r], y[c + 1][r], y[c + 2][r], y[c + 3][r]);
+            }
+            store_codes<V / 4>(codes + (r0 + r) * a.code_row, c0 + p * 16 * V, a.cols, stores, w);
+          }
     }
     __syncthreads();
   }
@@ -1055,12 +1111,14 @@ UNPM_DEV void quantise_tiles(const T* x, u8* codes, float* scales, const quant_a
 // where i went (-1: an id of no group), rows[p] = i / per of the i that went to p (-1 behind the last).
 //
 // Chunks of ids in order: count() writes each chunk's ids per group, and place() adds up those of the chunks before its own.
-// With one chunk, one block does both.  Inside a chunk a wave takes a run of ids, 64 at a time; the lanes of one
+// With one chunk, one block does both.  131072 ids of 128 groups take 13 microseconds in 128 chunks, mostly two launches; adding
+// the chunks up one after another took 49.  Inside a chunk a wave takes a run of ids, 64 at a time; the lanes of one
 // id find each other by its bits, so their order is that of the lanes.
 // ---------------------------------------------------------------------------------------
 struct rows_args {
-  i64 n, per, chunk;  // ids, ids of a row, ids of a block: a multiple of 64 times the waves
+  i64 n, chunk;  // ids, ids of a block: a multiple of 64 times the waves
   i32 groups, chunks;
+  u32 per, pad;  // ids of a row
 };
 constexpr int MOST_GROUPS = 1024, SORT_WAVES = 8;
 
@@ -1074,7 +1132,9 @@ UNPM_DEV run_of wave_run(const rows_args& a) {
 }
 // counts[wave][group] of the block's chunk.
 template <class I> UNPM_DEV void count_runs(const I* ids, const rows_args& a, i32 (*counts)[MOST_GROUPS]) {
-  for (int g = threadIdx.x; g < SORT_WAVES * MOST_GROUPS; g += SORT_WAVES * 64) (&counts[0][0])[g] = 0;
+#pragma unroll
+  for (int w = 0; w < SORT_WAVES; ++w)
+    for (int g = threadIdx.x; g < a.groups; g += SORT_WAVES * 64) counts[w][g] = 0;
   __syncthreads();
   const run_of r = wave_run(a);
   for (i64 i = r.first + (threadIdx.x & 63); i < r.last; i += 64) {
@@ -1102,24 +1162,45 @@ UNPM_DEV void place_rows(const I* ids, i32* starts, i32* rows, i32* place, const
   constexpr int THREADS = SORT_WAVES * 64, EACH = MOST_GROUPS / THREADS;
   count_runs<I>(ids, a, counts);
   const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
-  // This thread's groups t * EACH ..: how many ids they have in all, and in the chunks before this one.
-  i32 all[EACH], ahead[EACH], own = 0;
+  // How many ids the groups have in all, and in the chunks before this one.  With several chunks each thread adds up one
+  // group's counts of some of them, 16 at a time.
+  __shared__ i32 every[MOST_GROUPS];
+  const int teams = a.groups < THREADS ? THREADS / a.groups : 1;
+  for (int g = t; g < a.groups; g += THREADS) {
+    i32 c = 0;
+    if (a.chunks == 1) {
+#pragma unroll
+      for (int w = 0; w < SORT_WAVES; ++w) c += counts[w][g];
+    }
+    every[g] = c;
+    before[g] = 0;
+  }
+  __syncthreads();
+  if (a.chunks > 1 && t < teams * (a.groups < THREADS ? a.groups : THREADS)) {
+    const int team = teams > 1 ? t / a.groups : 0;
+    for (int g = teams > 1 ? t % a.groups : t; g < a.groups; g += THREADS) {
+      i32 c_all = 0, c_ahead = 0;
+      for (int c = team; c < a.chunks; c += 16 * teams) {
+        i32 v[16];
+#pragma unroll
+        for (int k = 0; k < 16; ++k) v[k] = c + k * teams < a.chunks ? counted[(c + k * teams) * a.groups + g] : 0;
+#pragma unroll
+        for (int k = 0; k < 16; ++k) {
+          c_all += v[k];
+          c_ahead += c + k * teams < (int)blockIdx.x ? v[k] : 0;
+        }
+      }
+      atomicAdd(&every[g], c_all);
+      atomicAdd(&before[g], c_ahead);
+    }
+  }
+  __syncthreads();
+  // Where they begin: this thread's groups t * EACH ...
+  i32 all[EACH], own = 0;
 #pragma unroll
   for (int e = 0; e < EACH; ++e) {
     const int g = t * EACH + e;
-    all[e] = ahead[e] = 0;
-    if (g < a.groups) {
-      if (a.chunks > 1) {
-        for (int c = 0; c < a.chunks; ++c) {
-          const i32 v = counted[(i64)c * a.groups + g];
-          all[e] += v;
-          ahead[e] += c < (int)blockIdx.x ? v : 0;
-        }
-      } else {
-#pragma unroll
-        for (int w = 0; w < SORT_WAVES; ++w) all[e] += counts[w][g];
-      }
-    }
+    all[e] = g < a.groups ? every[g] : 0;
     own += all[e];
   }
   i32 upto = own;
@@ -1141,7 +1222,7 @@ UNPM_DEV void place_rows(const I* ids, i32* starts, i32* rows, i32* place, const
     const int g = t * EACH + e;
     if (g < a.groups) {
       if (blockIdx.x == 0) starts[g] = start;
-      before[g] = start + ahead[e];
+      before[g] += start;
     }
     start += all[e];
   }
@@ -1174,7 +1255,7 @@ UNPM_DEV void place_rows(const I* ids, i32* starts, i32* rows, i32* place, const
       const int rank = __builtin_popcountll(same & ((1ull << lane) - 1));
       const i32 at = counts[wave][g] + rank;
       place[i] = at;
-      rows[at] = (i32)(i / a.per);
+      rows[at] = (i32)((u32)i / a.per);
       // The last of the lanes moves the count on; the wave has read it by then.
       if ((same >> lane) == 1) counts[wave][g] = at + 1;
     } else if (i < r.last) {
