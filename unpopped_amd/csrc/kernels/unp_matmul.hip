@@ -611,15 +611,16 @@ UNPM_DEV void matmul(const u8* xp, const u8* wp, const float* xsp, const float* 
 //   2      X1        X1 W1       W0
 //   3                X1 W0       W1
 // A wave waits for its own loads of what the next phase reads before the barrier that ends its reads: all but those that it
-// has started since.
+// has started since.  A tile of at most 128 rows, the last of a group, has the first two phases alone: they load scales two
+// steps ahead and W1 of the next, then X0 and W0 two ahead.
 template <int XK, int WKIND, bool XT, bool WT, class OUT, int BY, int SB>
 UNPM_DEV void matmul_wide(const u8* xp, const u8* wp, const float* xsp, const float* wsp, const i32* starts, OUT* out, float* parts,
                           const product_args& a) {
   constexpr int E = XK >= E4M3 ? 1 : 2, D = 128 / E;
   typedef side<XK, XT, 128> xside;
   typedef side<WKIND, WT, 128> wside;
-  constexpr int HALF = 16384, SCALES = E == 1 ? 2048 : 0, STAGE = 4 * HALF + SCALES;
-  __shared__ __attribute__((aligned(1024))) u8 lds[2 * STAGE];
+  constexpr int HALF = 16384, STAGE = 4 * HALF, SCALES = E == 1 ? 2048 : 0;
+  __shared__ __attribute__((aligned(1024))) u8 lds[2 * STAGE + 4 * SCALES];  // the scales of four steps
 
   place<XK, WKIND, XT, WT, BY, 256, 256> o;
   int part;
@@ -670,30 +671,38 @@ UNPM_DEV void matmul_wide(const u8* xp, const u8* wp, const float* xsp, const fl
   };
   auto issue_scales = [&](i64 step) {
     if constexpr (E == 1)
-      load_word_to_lds(scale + least(o.first + step, o.last - 1), lds0 + (u32)(step & 1) * STAGE + 4 * HALF + wave * 256);
+      load_word_to_lds(scale + least(o.first + step, o.last - 1), lds0 + 2 * STAGE + (u32)(step & 3) * SCALES + wave * 256);
   };
 
   f32x4 acc[2][2][2][4];  // of W half, X half, tile of W, tile of X
 #pragma unroll
   for (int i = 0; i < 32; ++i) (&acc[0][0][0][0])[i] = f32x4{0, 0, 0, 0};
   const i64 steps = o.last - o.first;
+  const bool low = o.m_there <= 128;
   if (steps > 0) {
     issue(0, 0);
     issue(2, 0);
     issue(3, 0);
     issue_scales(0);
-    issue(1, 0);
-    issue(0, 1);
-    issue(2, 1);
-    issue(3, 1);
-    wait_loads<E == 1 ? 8 : 10>();
+    if (low) {
+      issue_scales(1);
+      issue(0, 1);
+      issue(2, 1);
+      wait_loads<E == 1 ? 5 : 4>();
+    } else {
+      issue(1, 0);
+      issue(0, 1);
+      issue(2, 1);
+      issue(3, 1);
+      wait_loads<E == 1 ? 8 : 10>();
+    }
     lds_barrier();
     if (wm == 1) lds_barrier();
 
     u32x4 xf[4][2], wf[2][2][2];
     float xsc[4], wsc = 0;  // of the halves at hand
     f32x4 wrow[2];
-    auto read_x = [&](const u8* at, int h) {
+    auto read_x = [&](const u8* at, const float* scales, int h) {
 #pragma unroll
       for (int m = 0; m < 4; ++m)
 #pragma unroll
@@ -701,21 +710,21 @@ UNPM_DEV void matmul_wide(const u8* xp, const u8* wp, const float* xsp, const fl
       if constexpr (E == 1)
 #pragma unroll
         for (int m = 0; m < 4; ++m)
-          xsc[m] = reinterpret_cast<const float*>(at + 4 * HALF)[h * 128 + wm * 64 + m * 16 + (lane & 15)];
+          xsc[m] = scales[h * 128 + wm * 64 + m * 16 + (lane & 15)];
     };
-    auto read_w_scales = [&](const u8* at, int h) {
-      const float* s = reinterpret_cast<const float*>(at + 4 * HALF) + 256 + h * 128;
+    auto read_w_scales = [&](const float* scales, int h) {
+      const float* s = scales + 256 + h * 128;
       if constexpr (E == 1 && SB == 1)
 #pragma unroll
         for (int n = 0; n < 2; ++n) wrow[n] = *reinterpret_cast<const f32x4*>(s + wn * 32 + n * 16 + (lane >> 4) * 4);
       if constexpr (E == 1 && SB > 1) wsc = *s;
     };
-    auto read_w = [&](const u8* at, int h) {
+    auto read_w = [&](const u8* at, const float* scales, int h) {
 #pragma unroll
       for (int n = 0; n < 2; ++n)
 #pragma unroll
         for (int k = 0; k < 2; ++k) wf[h][n][k] = wside::read(at + (2 + h) * HALF, wn * 32 + n * 16, k, lane);
-      read_w_scales(at, h);
+      read_w_scales(scales, h);
     };
     auto products = [&](int hw, int hx) {
       __builtin_amdgcn_s_setprio(1);
@@ -758,28 +767,48 @@ UNPM_DEV void matmul_wide(const u8* xp, const u8* wp, const float* xsp, const fl
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
       meet();
     };
-    for (i64 s = 0; s < steps; ++s) {
+    for (i64 s = 0; low && s < steps; ++s) {
       const u8* at = lds + (u32)(s & 1) * STAGE;
-      read_x(at, 0);
-      read_w(at, 0);
+      const float* sc = reinterpret_cast<const float*>(lds + 2 * STAGE + (u32)(s & 3) * SCALES);
+      read_x(at, sc, 0);
+      read_w(at, sc, 0);
+      issue_scales(s + 2);
+      issue(3, s + 1);
+      wait_loads<E == 1 ? 7 : 6>();
+      read_done();
+      products(0, 0);
+      meet();
+      read_w(at, sc, 1);
+      issue(0, s + 2);
+      issue(2, s + 2);
+      wait_loads<E == 1 ? 7 : 6>();
+      read_done();
+      products(1, 0);
+      meet();
+    }
+    for (i64 s = 0; !low && s < steps; ++s) {
+      const u8* at = lds + (u32)(s & 1) * STAGE;
+      const float* sc = reinterpret_cast<const float*>(lds + 2 * STAGE + (u32)(s & 3) * SCALES);
+      read_x(at, sc, 0);
+      read_w(at, sc, 0);
       issue_scales(s + 1);
       issue(1, s + 1);
       wait_loads<E == 1 ? 12 : 10>();
       read_done();
       products(0, 0);
       meet();
-      read_w(at, 1);
+      read_w(at, sc, 1);
       issue(0, s + 2);
       wait_loads<E == 1 ? 11 : 10>();
       read_done();
       products(1, 0);
       meet();
-      read_x(at, 1);
+      read_x(at, sc, 1);
       issue(2, s + 2);
       read_done();
       products(1, 1);
       meet();
-      read_w_scales(at, 0);
+      read_w_scales(sc, 0);
       issue(3, s + 2);
       wait_loads<E == 1 ? 8 : 10>();
       read_done();
@@ -799,16 +828,17 @@ UNPM_DEV void matmul_wide(const u8* xp, const u8* wp, const float* xsp, const fl
         wh[0].alone(lds + 2 * HALF, q, last, left);
         wh[1].alone(lds + 3 * HALF, q, last, left);
       }
-      if constexpr (E == 1) *reinterpret_cast<float*>(lds + 4 * HALF + threadIdx.x * 4) = scale[last];
+      if constexpr (E == 1) *reinterpret_cast<float*>(lds + 2 * STAGE + threadIdx.x * 4) = scale[last];
       lds_barrier();
-      read_x(lds, 0);
-      read_w(lds, 0);
+      const float* sc = reinterpret_cast<const float*>(lds + 2 * STAGE);
+      read_x(lds, sc, 0);
+      read_w(lds, sc, 0);
       products(0, 0);
-      read_w(lds, 1);
+      read_w(lds, sc, 1);
       products(1, 0);
-      read_x(lds, 1);
+      read_x(lds, sc, 1);
       products(1, 1);
-      read_w_scales(lds, 0);
+      read_w_scales(sc, 0);
       products(0, 1);
     }
   }
@@ -816,6 +846,7 @@ UNPM_DEV void matmul_wide(const u8* xp, const u8* wp, const float* xsp, const fl
   float* sums = reinterpret_cast<float*>(lds);
 #pragma unroll
   for (int hx = 0; hx < 2; ++hx) {
+    if (hx && low) break;
     lds_barrier();
 #pragma unroll
     for (int hw = 0; hw < 2; ++hw)
