@@ -84,9 +84,11 @@ UNPM_DEV u32x4 resource(const u8* p) {
   return u32x4{scalar((u32)a), scalar((u32)(a >> 32) & 0xFFFFu), OUTSIDE, 0x00020000u};
 }
 // 16 bytes of each lane from p + offset to LDS, lane after lane from `to` on; zeros where the offset is OUTSIDE.  (Nothing
-// else here uses M0, which no clobber list may name.)
+// else here uses M0, which no clobber list may name.)  A scalar register that a vector instruction wrote, as reading the
+// first lane or a spilled register back does, may be read by a load or store five wait states later; within assembly the
+// compiler adds none.
 UNPM_DEV void load_to_lds(const u8* p, u32 offset, u32 to) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(scalar(to)), "v"(offset),
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(scalar(to)), "v"(offset),
                "s"(resource(p))
                : "memory");
 }
