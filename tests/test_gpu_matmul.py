@@ -1,8 +1,11 @@
 """The floating point products on the GPU against their numpy reference: values, odd and empty sizes, strides, groups, refusals."""
+import ctypes as C
+
 import numpy as np
 import pytest
 
 import unpopped_amd as u
+from unpopped_amd import _lib
 from tests import matmul_reference as ref
 from tests.cache4_reference import loaded, rounded, stored
 
@@ -516,3 +519,224 @@ def test_a_split_depth_gives_the_same_whole_numbers(hip_device, workspace):
              grouped_case("input", 60, 16384, 136, 1, workspace=workspace)["chunks"],
              grouped_case("weight", 4096, 136, 200, 2, out="F32", workspace=workspace)["chunks"]]
     assert all(p > 1 for p in parts) if workspace is None else parts == [1] * 4
+
+
+@pytest.mark.parametrize("case", ["codes", "forward", "input", "weight", "weight16"])
+def test_more_wide_tiles_than_compute_units(hip_device, case):
+    """Tiles of 256 x 256, of whole and half heights, at the edges of each operand."""
+    if case == "codes":
+        starts = [0, 700, 700, 1000, 3111, 3240, 4200]
+        got = matmul8_case(4300, 8200, 272, groups=6, starts=starts, out_pad=8)
+    elif case == "forward":
+        got = grouped_case("forward", 4300, 8200, 136, 6, way="gaps")
+    elif case == "input":
+        got = grouped_case("input", 4300, 136, 8200, 6, way="gaps")
+    else:
+        got = grouped_case("weight", 1000, 2104, 1544, 8, way="gaps", out="F32" if case == "weight" else "Bf16")
+    assert got["entry"].endswith("_wide") and got["grid"][0] > 256, got
+
+
+# ---------------------------------------------------------------------------------------
+# As they are used: together, for gradients, on streams, in graphs and far apart
+# ---------------------------------------------------------------------------------------
+def gather(table, rows, out, n, cols, extent, dtype="Bf16"):
+    key = ("gather", dtype)
+    if key not in _execs:
+        _execs[key] = u.Executor(B.lower_form(kind="gather", dtype=dtype, rank=2, index_dtype="I32", oob="ZeroFill"))
+    _execs[key].launch(table, rows, out, n, cols, extent)
+
+
+def test_experts_of_tokens_together(hip_device):
+    """Choices to rows by expert, the tokens' rows gathered, their products in 16 bits and from codes, and the results gathered
+    back to the choices, on the device from end to end."""
+    rng = np.random.default_rng(5)
+    tokens, per, groups, n, k = 37, 3, 6, 72, 136
+    count = tokens * per
+    ids = rng.integers(0, groups, count)
+    ids[ids == 2] = 4  # an expert of no rows
+    ids[::11] = -1     # choices of none
+    x, w = rng.integers(-1, 2, (tokens, k)).astype(float), rng.integers(-1, 2, (groups, n, k)).astype(float)
+    starts, rows, place = ref.group_rows(ids, per, groups)
+    d_starts, d_rows, d_place = (u.DeviceBuffer(4 * s) for s in (groups + 1, count, count))
+    sort = executor("lower_group_rows", index_dtype="I32")
+    sort.launch(dev(ids.astype(np.int32)), d_starts, d_rows, d_place, u.DeviceBuffer(16), count, per, groups, 0)
+    d_x, d_xs = dev(held(x, "Bf16")), u.DeviceBuffer(2 * count * k)
+    gather(d_x, d_rows, d_xs, count, k, tokens)
+    # In 16 bits: sums of at most k products of -1, 0 and 1 are whole numbers that bf16 holds.
+    ex = executor("lower_grouped_matmul", dtype="Bf16", out="Bf16", direction="forward")
+    d_y, d_out = dev(np.zeros(count * n, np.uint16)), u.DeviceBuffer(2 * count * n)
+    need = ex.workspace_bytes(count, n, k, groups)
+    ex.launch(d_xs, dev(held(w, "Bf16")), d_starts, d_y, u.DeviceBuffer(max(need, 16)), count, n, k, groups, k, n * k, k, n, need)
+    gather(d_y, d_place, d_out, count, n, count)
+    u.synchronize()
+    assert np.array_equal(d_starts.download(np.int32, groups + 1), starts)
+    want = np.zeros((count, n))
+    for i, g in enumerate(ids):
+        if g >= 0:
+            want[i] = w[g] @ x[i // per]
+    assert np.array_equal(read(d_out, count * n, "Bf16").reshape(count, n), want)
+    # From codes: the rows' and the weights' scales are the device's own.
+    blocks = -(-k // 128)
+    quant = executor("lower_quant8", dtype="Bf16", kind="Fp8E4M3FN", block_rows=1, transpose=False)
+    d_a, d_sa = u.DeviceBuffer(count * k), u.DeviceBuffer(4 * count * blocks)
+    quant.launch(d_xs, d_a, d_sa, count, k, k, k, blocks)
+    wide = executor("lower_quant8", dtype="F32", kind="Fp8E4M3FN", block_rows=128, transpose=False)
+    d_b, d_sb = u.DeviceBuffer(groups * n * k), u.DeviceBuffer(4 * groups * blocks)
+    for g in range(groups):
+        wide.launch(dev(w[g].astype(np.float32)), d_b.at(g * n * k), d_sb.at(4 * g * blocks), n, k, k, k, blocks)
+        u.synchronize()
+    ex = executor("lower_matmul8", a_kind="Fp8E4M3FN", b_kind="Fp8E4M3FN", out="Bf16", b_rows=128, grouped=True)
+    need = ex.workspace_bytes(count, n, k, groups)
+    ex.launch(d_a, d_sa, d_b, d_sb, d_starts, d_y, u.DeviceBuffer(max(need, 16)), count, n, k, groups, k, blocks, k, blocks, n * k, blocks,
+              n, need)
+    gather(d_y, d_place, d_out, count, n, count)
+    u.synchronize()
+    got = read(d_out, count * n, "Bf16").reshape(count, n)
+    # 1 is the code 448 times f32(1 / 448), off by 2^-24: a product of two is off by 2^-23 and two blocks' sum of magnitudes is at
+    # most k.  Two of the matrix unit's sums of 16 keep 2^-13 of the largest term, which is 1, in each of k / 16 + 1 runs for 15
+    # products; then sums of 11 steps a block to 2^-23, and bf16's half step.
+    tol = k * (2.0 ** -22 + (8 + 3 * blocks) * 2.0 ** -23) + (k / 16 + 1) * 15 * 2.0 ** -13
+    assert (np.abs(got - want) <= tol + (np.abs(want) + tol) * 2.0 ** -8).all()
+    assert (got[ids < 0] == 0).all()
+
+
+def test_gradients_against_differences(hip_device):
+    """A product is linear in its rows and in its weights: the change of sum(c * y) over any step is the gradient's sum."""
+    rng = np.random.default_rng(8)
+    rows, n, k, groups = 150, 88, 104, 5
+    starts = starts_of(rng, rows, groups, "all")
+    whole = lambda s: rng.integers(-2, 3, s).astype(float)  # noqa: E731
+    x, w, c, dx, dw = whole((rows, k)), whole((groups, n, k)), whole((rows, n)), whole((rows, k)), whole((groups, n, k))
+
+    def product(direction, a, b, shape, strides):
+        out = "F32"
+        ex = executor("lower_grouped_matmul", dtype="F16", out=out, direction=direction)
+        size, buf = ex.workspace_bytes(rows, n, k, groups), dev(np.zeros(shape, np.float32))
+        ex.launch(dev(held(a, "F16")), dev(held(b, "F16")), dev(starts.astype(np.int32)), buf, u.DeviceBuffer(max(size, 16)), rows, n, k,
+                  groups, *strides, size)
+        u.synchronize()
+        return read(buf, int(np.prod(shape)), out).reshape(shape)
+
+    forward = lambda x, w: (c * product("forward", x, w, (rows, n), (k, n * k, k, n))).sum()  # noqa: E731
+    gx = product("input", c, w, (rows, k), (n, n * k, k, k))
+    gw = product("weight", c, x, (groups, n, k), (n, k, n * k, k))
+    at = forward(x, w)
+    assert forward(x + dx, w) - at == (gx * dx).sum() != 0
+    assert forward(x, w + dw) - at == (gw * dw).sum() != 0
+
+
+def steps_for_streams():
+    """Launches of each form with every buffer of their own: (launch(stream, how), output, bytes of it, workspace or None)."""
+    rng = np.random.default_rng(2)
+    found = []
+
+    def codes(shape):
+        return dev(ref.encoded(rng.normal(size=shape), "Fp8E4M3FN"))
+
+    def add(ex, buffers, out, size, need, scalars):
+        ws = u.DeviceBuffer(max(need, 16)) if need is not None else None
+        args = [*buffers, *([ws] if ws else []), *scalars, *([need] if ws else [])]
+        found.append((lambda stream, how="launch", ex=ex, args=args: getattr(ex, how)(*args, stream=stream), out, size, ws, ex))
+
+    m, n, k = 60, 200, 28000
+    blocks, sides = -(-k // 128), -(-n // 128)
+    ex, out = executor("lower_matmul8", a_kind="Fp8E4M3FN", b_kind="Fp8E4M3FN", out="F16", b_rows=128, grouped=False), u.DeviceBuffer(2 * m * n)
+    add(ex, [codes((m, k)), dev(np.exp(rng.normal(size=(m, blocks))).astype(np.float32)), codes((n, k)),
+             dev(np.exp(rng.normal(size=(sides, blocks))).astype(np.float32) / 100), out], out, 2 * m * n,
+        ex.workspace_bytes(m, n, k), [m, n, k, k, blocks, k, blocks, n])
+    rows, n, k, g = 5000, 136, 200, 2
+    starts = dev(np.array([0, 2100, 5000], np.int32))
+    ex, out = executor("lower_grouped_matmul", dtype="Bf16", out="F32", direction="weight"), u.DeviceBuffer(4 * g * n * k)
+    add(ex, [dev(held(rng.normal(size=(rows, n)), "Bf16")), dev(held(rng.normal(size=(rows, k)), "Bf16")), starts, out], out, 4 * g * n * k,
+        ex.workspace_bytes(rows, n, k, g), [rows, n, k, g, n, k, n * k, k])
+    m, n, k, g = 4300, 2304, 264, 3
+    ex, out = executor("lower_grouped_matmul", dtype="Bf16", out="Bf16", direction="forward"), u.DeviceBuffer(2 * m * n)
+    add(ex, [dev(held(rng.normal(size=(m, k)), "Bf16")), dev(held(rng.normal(size=(g, n, k)), "Bf16")),
+             dev(np.array([0, 1000, 4200, 4300], np.int32)), out], out, 2 * m * n, ex.workspace_bytes(m, n, k, g),
+        [m, n, k, g, k, n * k, k, n])
+    r, c = 700, 900
+    ex, out = executor("lower_quant8", dtype="F32", kind="Fp8E5M2", block_rows=128, transpose=True), u.DeviceBuffer(r * c)
+    add(ex, [dev(rng.normal(size=(r, c)).astype(np.float32)), out, u.DeviceBuffer(4 * 64)], out, r * c, None, [r, c, c, r, 6])
+    count, g = 20000, 64
+    ex, out = executor("lower_group_rows", index_dtype="I32"), u.DeviceBuffer(4 * count)
+    add(ex, [dev(rng.integers(-1, g, count).astype(np.int32)), u.DeviceBuffer(4 * (g + 1)), out, u.DeviceBuffer(4 * count)], out, 4 * count,
+        ex.workspace_bytes(count, 4, g), [count, 4, g])
+    return found
+
+
+def test_streams_graphs_and_workspaces(hip_device):
+    """Each form captured into a graph and replayed between eager work, all of them at once on streams of their own, timed and
+    without allocation: the same bits every time."""
+    L = _lib.lib()
+    steps, raw, streams, graphs = steps_for_streams(), [], [], []
+    split = 0
+    for launch, out, size, ws, ex in steps:
+        launch(0)
+        u.synchronize()
+        split += ex.last_launch()["shared"]
+        raw.append(out.download(np.uint8, size))
+        out.fill(0x5A)
+        launch(0, "launch_static")
+        a, b = u.Event(), u.Event()
+        ex.set_timing(a, b)
+        launch(0)
+        u.synchronize()
+        assert 0 < a.elapsed_ms(b) < 1000
+        ex.set_timing(None, None)
+        assert np.array_equal(out.download(np.uint8, size), raw[-1])
+    assert split >= 3  # the split products and the rows of groups have kernels that follow one another
+    for launch, *_ in steps:
+        st, graph, exe = C.c_void_p(), C.c_void_p(), C.c_void_p()
+        assert L.hipStreamCreate(C.byref(st)) == 0
+        assert L.hipStreamBeginCapture(st, 0) == 0
+        launch(st.value)
+        assert L.hipStreamEndCapture(st, C.byref(graph)) == 0
+        assert L.hipGraphInstantiate(C.byref(exe), graph, None, None, C.c_size_t(0)) == 0
+        streams.append(st)
+        graphs.append((graph, exe))
+    others = steps_for_streams()
+    for turn in range(4):
+        for _, out, _, ws, _ in steps:
+            out.fill(0)
+            if ws:
+                ws.fill(0xFF)
+        u.synchronize()
+        for _ in range(3):
+            for (_, exe), st in zip(graphs, streams):
+                assert L.hipGraphLaunch(exe, st) == 0
+        others[turn][0](0)  # eager work on buffers of its own beside them
+        u.synchronize()
+        for (_, out, size, _, _), r in zip(steps, raw):
+            assert np.array_equal(out.download(np.uint8, size), r), turn
+    for (launch, out, *_), st in zip(steps, streams):
+        out.fill(0)
+        u.synchronize()
+        launch(st.value)
+    u.synchronize()
+    for (_, out, size, _, _), r in zip(steps, raw):
+        assert np.array_equal(out.download(np.uint8, size), r)
+    for graph, exe in graphs:
+        assert L.hipGraphExecDestroy(exe) == 0 and L.hipGraphDestroy(graph) == 0
+    for st in streams:
+        assert L.hipStreamDestroy(st) == 0
+
+
+@pytest.mark.parametrize("direct", [True, False])
+def test_products_past_four_gigabytes(hip_device, direct):
+    """Rows, groups and results at byte offsets that need more than 32 bits, in rows that load directly and in others."""
+    rng = np.random.default_rng(4)
+    m, n, k, groups = 1300, 17, 256, 2
+    a_row, b_row, out_row, b_group = (1 << 22) if direct else (1 << 22) + 1, 256, 1 << 21, (5 << 30) + (0 if direct else 2)
+    a, b = rng.integers(-4, 5, (m, k)).astype(float), rng.integers(-4, 5, (groups, n, k)).astype(float)
+    da, db, do = u.DeviceBuffer(m * a_row + 16), u.DeviceBuffer(b_group + n * b_row), u.DeviceBuffer(m * out_row * 2)
+    for i in range(m):
+        da.at(i * a_row).upload(ref.encoded(a[i], "Fp8E4M3FN"))
+    for g in range(groups):
+        db.at(g * b_group).upload(ref.encoded(b[g], "Fp8E4M3FN"))
+    ones = dev(np.ones(2 * m, np.float32))
+    starts = dev(np.array([0, 70, m], np.int32))
+    ex = executor("lower_matmul8", a_kind="Fp8E4M3FN", b_kind="Fp8E4M3FN", out="Bf16", b_rows=128, grouped=True)
+    run(ex, da, ones, db, ones, starts, do, u.DeviceBuffer(16), m, n, k, groups, a_row, 2, b_row, 2, b_group, 2, out_row, 0)
+    assert ex.last_launch()["entry"].endswith("_any") != direct
+    for i in (0, 1, 69, 70, 500, 1024, 1025, m - 1):
+        assert np.array_equal(read(do.at(2 * i * out_row), n, "Bf16"), once(b[int(i >= 70)] @ a[i], "Bf16")), i
