@@ -138,11 +138,15 @@ template <int KIND, bool TURNED, int T> struct side {
     const int r = row_of(u, lane), s = lane % CHUNKS;
     return TURNED ? turned_slot<T>(r, s) : straight_slot(r, s);
   }
-  // The offset of the lane's 16 bytes from the step's first; OUTSIDE where its row or column does not exist.
-  UNPM_DEV u32 offset(int u, int lane) const {
-    const int r = row_of(u, lane), c = chunk_of(u, lane);
+  // The offset of the lane's 16 bytes from the step's first; OUTSIDE where its row or column does not exist.  The tile's row
+  // (TURNED: chunk of columns) i is number map(i) from p on.
+  template <class M> UNPM_DEV u32 offset(int u, int lane, M map) const {
+    const int r = TURNED ? row_of(u, lane) : map(row_of(u, lane)), c = TURNED ? map(chunk_of(u, lane)) : chunk_of(u, lane);
     const bool in = TURNED ? c * 16 < there : r < there;
     return in ? (u32)(r * (i32)row + c * 16) : OUTSIDE;
+  }
+  UNPM_DEV u32 offset(int u, int lane) const {
+    return offset(u, lane, [](int i) { return i; });
   }
   // What of the step's length has to be left for the lane's 16 bytes to exist, in bytes or TURNED rows.
   static UNPM_DEV int after(int u, int lane) { return TURNED ? row_of(u, lane) : chunk_of(u, lane) * 16; }
@@ -163,15 +167,17 @@ template <int KIND, bool TURNED, int T> struct side {
     }
   }
   // 16 bytes (the q-th) of a step that holds those alone, as its first elements along d.
-  UNPM_DEV void alone(u8* lds, int q, i64 step, i64 elements) const {
+  template <class M> UNPM_DEV void alone(u8* lds, int q, i64 step, i64 elements, M map) const {
     const i64 first = elements * E / 16 * (16 / E);
     u32x4 v = {0, 0, 0, 0};
     const int r = q / CHUNKS, c = q % CHUNKS;
     if constexpr (TURNED) {
-      if (r < elements - first) v = fetch16<E>(at(step) + (first + r) * row + c * 16, there - c * 16, vectors);
+      const int from = map(c);
+      if (r < elements - first) v = fetch16<E>(at(step) + (first + r) * row + from * 16, there - from * 16, vectors);
       *reinterpret_cast<u32x4*>(lds + r * (T * 2) + turned_slot<T>(r, c) * 16) = v;
     } else {
-      if (c == 0 && r < there) v = fetch16<E>(at(step) + r * row + first * E, (elements - first) * E, false);
+      const int from = map(r);
+      if (c == 0 && from < there) v = fetch16<E>(at(step) + from * row + first * E, (elements - first) * E, false);
       *reinterpret_cast<u32x4*>(lds + r * 128 + straight_slot(r, c) * 16) = v;
     }
   }
@@ -603,10 +609,57 @@ UNPM_DEV void matmul(const u8* xp, const u8* wp, const float* xsp, const float* 
   store_sums<OUT, BY, TM, TN, SPLIT, WAVES * 64>(sums, out, parts, a, part, o.row0, o.m0, o.n0, o.m_there, 0);
 }
 
+// A wave's 16 x 64 (of 16 bits) or 16 x 32 sums on their way out: 2 KB of LDS that no other wave uses turn the rows that the
+// matrix instruction gives a lane's quad of into 128 bytes of eight rows a store, which are whole lines of the caches.  Without
+// barriers and of half the bytes it takes 1 us a tile of 256 x 256 less than store_sums does (12001 x 8192 x 2048 by 16
+// groups 382 us with that, 378 so; depth 512 95 and 83); for 32 bits, whose rows of 128 bytes leave slower than longer ones,
+// it loses (16 x 8192 x 2048 of depth 768 526 and 497).  Lane (i, g) holds columns 4 g .. of each 16 columns' block of row i.
+template <class OUT> struct rows_out {
+  static constexpr int V = 16 / sizeof(OUT), COLUMNS = 8 * V, BLOCKS = COLUMNS / 16;
+  OUT* to;
+  i64 stride, m_there, n_there;  // of `to`
+  i32 wide;                      // as store_columns takes it
+
+  UNPM_DEV void put(u8* lds, int row, int column, const f32x4 (&v)[BLOCKS], int lane) const {
+    const int i = lane & 15, g = lane >> 4;
+    asm volatile("" ::: "memory");  // behind the reads of what was here
+#pragma unroll
+    for (int n = 0; n < BLOCKS; ++n) {
+      struct alignas(4 * sizeof(OUT)) quad {
+        OUT v[4];
+      } q;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) q.v[j] = (OUT)v[n][j];
+      const int c = n * 16 + g * 4;
+      *reinterpret_cast<quad*>(lds + i * 128 + straight_slot(i, c / V) * 16 + c % V * sizeof(OUT)) = q;
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const int r = k * 8 + lane / 8, n = column + lane % 8 * V;
+      const u8* from = lds + r * 128 + straight_slot(r, lane % 8) * 16;
+      const i64 there = n_there - n;
+      if (row + r >= m_there || there <= 0) continue;
+      OUT* p = to + (row + r) * stride + n;
+      if (wide && there >= V) {
+        const u32x4 q = *reinterpret_cast<const u32x4*>(from);
+        if (wide == 2)
+          __builtin_nontemporal_store(q, reinterpret_cast<u32x4*>(p));
+        else
+          *reinterpret_cast<u32x4*>(p) = q;
+      } else {
+#pragma clang loop unroll(disable)
+        for (int j = 0; j < V && j < there; ++j) p[j] = reinterpret_cast<const OUT*>(from)[j];
+      }
+    }
+  }
+};
+
 // Tiles of 256 x 256 for much work: eight waves, two on each SIMD, of which one multiplies while the other reads LDS and
-// starts loads (the second set runs one barrier behind the first).  A wave has four blocks of 64 x 32, one in each quarter of
-// the tile; the halves of the operands' tiles lie in LDS twice, and as a half has been read by every wave, the loads of
-// the same half two steps on go there: five halves are on their way at any time.
+// starts loads (the second set runs one barrier behind the first).  A wave has 128 x 64 of the tile as four blocks of 64 x 32,
+// one of each pair of halves; the halves of the operands' tiles lie in LDS twice, and as a half has been read by every wave, the
+// loads of the same half two steps on go there: five halves are on their way at any time.  (X0 is the first 128 rows; W0 the
+// first 32 of each 64, so that a wave stores whole lines, or where W lies along out the first 128, as loads take more of a row.)
 //   phase  reads     multiplies  loads
 //   0      X0 W0     X0 W0       scales and X1 of the next step
 //   1      W1        X0 W1       X0 of the one after it
@@ -633,36 +686,41 @@ UNPM_DEV void matmul_wide(const u8* xp, const u8* wp, const float* xsp, const fl
 
   // The halves of the operands: X0, X1, W0, W1.  Two loads of a wave each.
   xside xh[2];
-  wside wh[2];
+  wside w;
+  // Row i of half h of W; of one that lies along out, chunk i of 8 columns.
+  auto of_half = [](int h) {
+    return [h](int i) { return WT ? h * 16 + i : (i >> 5) * 64 + h * 32 + (i & 31); };
+  };
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
     xh[h].row = a.x_row;
     xh[h].p = XT ? o.x.p + h * 256 : o.x.p + h * 128 * a.x_row;
     xh[h].there = o.x.there - h * (XT ? 256 : 128);
-    wh[h].row = a.w_row;
-    wh[h].p = WT ? o.w.p + h * 256 : o.w.p + h * 128 * a.w_row;
-    wh[h].there = o.w.there - h * (WT ? 256 : 128);
-    xh[h].vectors = wh[h].vectors = true;
+    xh[h].vectors = true;
   }
+  w.row = a.w_row;
+  w.p = o.w.p;
+  w.there = o.w.there;
+  w.vectors = true;
   u32 offset[4][2];
 #pragma unroll
   for (int h = 0; h < 2; ++h)
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       offset[h][i] = xh[h].offset(i * 8 + wave, lane);
-      offset[2 + h][i] = wh[h].offset(i * 8 + wave, lane);
+      offset[2 + h][i] = w.offset(i * 8 + wave, lane, of_half(h));
     }
   const float* scale = nullptr;
   if constexpr (E == 1) {
-    const int f = wave * 64 + lane;
-    scale = f < 256 ? o.xs + least(f, o.xs_last) * a.xs_row : o.ws + least((f - 256) / SB, o.ws_last) * a.ws_row;
+    const int f = wave * 64 + lane, n = of_half(f >> 7 & 1)(f & 127);  // codes' rows are not turned
+    scale = f < 256 ? o.xs + least(f, o.xs_last) * a.xs_row : o.ws + least(n / SB, o.ws_last) * a.ws_row;
   }
   // What of a step has to be left for a lane's 16 bytes to exist is the same for every load of it along d.
   const i32 x_after = xside::after(wave, lane), w_after = wside::after(wave, lane);
   auto issue = [&](int half, i64 step) {
     const bool isx = half < 2;
     const i32 left = (i32)(o.end - (o.first + step) * D);
-    const u8* p = isx ? xh[half & 1].at(o.first + step) : wh[half & 1].at(o.first + step);
+    const u8* p = isx ? xh[half & 1].at(o.first + step) : w.at(o.first + step);
     const u32 to = lds0 + (u32)(step & 1) * STAGE + half * HALF + wave * 1024;
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
@@ -715,10 +773,10 @@ UNPM_DEV void matmul_wide(const u8* xp, const u8* wp, const float* xsp, const fl
           xsc[m] = scales[h * 128 + wm * 64 + m * 16 + (lane & 15)];
     };
     auto read_w_scales = [&](const float* scales, int h) {
-      const float* s = scales + 256 + h * 128;
+      const float* s = scales + 256 + h * 128 + wn * 32;
       if constexpr (E == 1 && SB == 1)
 #pragma unroll
-        for (int n = 0; n < 2; ++n) wrow[n] = *reinterpret_cast<const f32x4*>(s + wn * 32 + n * 16 + (lane >> 4) * 4);
+        for (int n = 0; n < 2; ++n) wrow[n] = *reinterpret_cast<const f32x4*>(s + n * 16 + (lane >> 4) * 4);
       if constexpr (E == 1 && SB > 1) wsc = *s;
     };
     auto read_w = [&](const u8* at, const float* scales, int h) {
@@ -825,10 +883,10 @@ UNPM_DEV void matmul_wide(const u8* xp, const u8* wp, const float* xsp, const fl
       lds_barrier();
 #pragma clang loop unroll(disable)
       for (int q = threadIdx.x; q < 1024; q += 512) {
-        xh[0].alone(lds, q, last, left);
-        xh[1].alone(lds + HALF, q, last, left);
-        wh[0].alone(lds + 2 * HALF, q, last, left);
-        wh[1].alone(lds + 3 * HALF, q, last, left);
+        xh[0].alone(lds, q, last, left, [](int i) { return i; });
+        xh[1].alone(lds + HALF, q, last, left, [](int i) { return i; });
+        w.alone(lds + 2 * HALF, q, last, left, of_half(0));
+        w.alone(lds + 3 * HALF, q, last, left, of_half(1));
       }
       if constexpr (E == 1) *reinterpret_cast<float*>(lds + 2 * STAGE + threadIdx.x * 4) = scale[last];
       lds_barrier();
@@ -844,22 +902,50 @@ UNPM_DEV void matmul_wide(const u8* xp, const u8* wp, const float* xsp, const fl
       products(0, 1);
     }
   }
-  // A half of X at a time: 128 rows of sums fill what held the steps.
-  float* sums = reinterpret_cast<float*>(lds);
+  lds_barrier();
+  if constexpr (sizeof(OUT) == 2 && !WT) {
+    const i64 n0 = o.n0 + wn * 64, m_there = o.m_there - wm * 64;
+    u8* own = lds + wave * 2048;
+    auto send = [&](auto to) {
+      constexpr int BLOCKS = decltype(to)::BLOCKS;
 #pragma unroll
-  for (int hx = 0; hx < 2; ++hx) {
-    if (hx && low) break;
-    lds_barrier();
-#pragma unroll
-    for (int hw = 0; hw < 2; ++hw)
-#pragma unroll
-      for (int n = 0; n < 2; ++n)
+      for (int hx = 0; hx < 2; ++hx) {
+        if (hx && low) break;
 #pragma unroll
         for (int m = 0; m < 4; ++m)
-          *reinterpret_cast<f32x4*>(sums + sum_at<128, 256>(0, wm * 64 + m * 16 + (lane & 15),
-                                                            hw * 128 + wn * 32 + n * 16 + (lane >> 4) * 4)) = acc[hw][hx][n][m];
-    lds_barrier();
-    store_sums<OUT, BY, 128, 256, 1, 512>(sums, out, parts, a, part, o.row0, o.m0, o.n0, o.m_there, hx * 128);
+#pragma unroll
+          for (int t = 0; t < 4 / BLOCKS; ++t) {
+            f32x4 v[BLOCKS];
+#pragma unroll
+            for (int i = 0; i < BLOCKS; ++i) v[i] = acc[BLOCKS == 4 ? i / 2 : t][hx][i % 2][m];
+            to.put(own, hx * 128 + m * 16, t * 32, v, lane);
+          }
+      }
+    };
+    if (a.parts > 1) {
+      const i64 wide = (a.n + 7) / 8 * 8;
+      send(rows_out<float>{parts + (part * a.m + o.row0 + wm * 64) * wide + n0, wide, m_there, wide - n0, 1});
+    } else {
+      send(rows_out<OUT>{out + (o.m0 + wm * 64) * a.out_row + n0, a.out_row, m_there, a.n - n0, a.wide});
+    }
+  } else {
+    // A half of X at a time: 128 rows of sums fill what held the steps, and go out as whole rows of 256.
+    float* sums = reinterpret_cast<float*>(lds);
+#pragma unroll
+    for (int hx = 0; hx < 2; ++hx) {
+      if (hx && low) break;
+      lds_barrier();
+#pragma unroll
+      for (int hw = 0; hw < 2; ++hw)
+#pragma unroll
+        for (int n = 0; n < 2; ++n)
+#pragma unroll
+          for (int m = 0; m < 4; ++m)
+            *reinterpret_cast<f32x4*>(sums + sum_at<128, 256>(0, wm * 64 + m * 16 + (lane & 15),
+                                                              (WT ? hw * 128 + wn * 32 : wn * 64 + hw * 32) + n * 16 + (lane >> 4) * 4)) = acc[hw][hx][n][m];
+      lds_barrier();
+      store_sums<OUT, BY, 128, 256, 1, 512>(sums, out, parts, a, part, o.row0, o.m0, o.n0, o.m_there, hx * 128);
+    }
   }
 }
 
