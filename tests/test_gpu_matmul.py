@@ -521,6 +521,19 @@ def test_a_split_depth_gives_the_same_whole_numbers(hip_device, workspace):
     assert all(p > 1 for p in parts) if workspace is None else parts == [1] * 4
 
 
+def test_a_split_depth_that_ends_inside_a_vector(hip_device):
+    parts = [matmul8_case(60, 200, 28001, top=1, pad=15)["chunks"], matmul8_case(33, 70, 20007, top=1, pad=9, b_rows=1)["chunks"],
+             grouped_case("forward", 60, 136, 16385, 2, way="gaps", pad=7)["chunks"],
+             grouped_case("input", 60, 16391, 136, 1, pad=8, x_pad=1)["chunks"]]
+    assert all(p > 1 for p in parts)
+
+
+def test_more_tiles_than_a_launch_has(hip_device):
+    ex, b, null = executor("lower_matmul8", a_kind="Fp8E4M3FN", b_kind="Fp8E4M3FN", out="Bf16", b_rows=128, grouped=False), u.DeviceBuffer(64), \
+        u.DeviceBuffer.held(0, 0, None)
+    invalid(ex, null, null, null, null, b, b.at(16), 1 << 28, 1 << 28, 0, 0, 0, 0, 0, 1 << 28, 0)
+
+
 @pytest.mark.parametrize("case", ["codes", "forward", "input", "weight", "weight16"])
 def test_more_wide_tiles_than_compute_units(hip_device, case):
     """Tiles of 256 x 256, of whole and half heights, at the edges of each operand."""

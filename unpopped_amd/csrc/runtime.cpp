@@ -15,6 +15,7 @@
 // decode, MFMA and prep kernels do the same over their (row tile, split of K, column tile), tile
 // and (group, column slab) items.  One entry departs from the rule: the streaming entry launches a
 // block per item (an item loop around its LDS pipeline made it spill).
+// So do the attention over a cache and the floating point products, whose lengths the device knows.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -2245,6 +2246,8 @@ EntryCost entry_cost(int tile, bool codes) {
   }
 }
 
+constexpr int64_t kMostTiles = 0x7FFFFF;  // of 512 lanes: a launch has less than 2^32
+
 // The entry and the number of parts of the depth that take the least time.  Operands that no entry loads directly, or rows of
 // other sizes than whole vectors along out, go to the last one but the join, unsplit.
 ProductPlan product_plan(const unp_exec* x, const Extents& e, bool direct, int64_t workspace_bytes) {
@@ -2267,6 +2270,7 @@ ProductPlan product_plan(const unp_exec* x, const Extents& e, bool direct, int64
       const double read = weights / c.rate;
       for (int64_t parts : {1, 2, 3, 4, 6, 8, 12, 16}) {
         if (parts > 1 && (steps < 4.0 * es[k].k * (double)parts || parts_bytes(e, parts) > workspace_bytes)) break;
+        if (row_tiles(e, es[k].vec) * ((e.n + es[k].cols - 1) / es[k].cols) * parts > kMostTiles) break;
         const double blocks = tiles * (double)parts, each = std::ceil(steps / (double)parts), rounds = std::ceil(blocks / hold);
         double t = std::max(read, blocks <= x->cu_count ? each * c.alone : rounds * each * c.full) + c.fixed + 1.5 * (rounds - 1);
         if (parts > 1) t += 4.0 + 2.0 * (double)parts_bytes(e, parts) / 3.2e6;
@@ -2287,7 +2291,7 @@ int32_t launch_product(unp_exec* x, const Extents& e, product_args_host args, co
                        bool direct, hipStream_t s, unp_error* err) {
   const ProductPlan p = product_plan(x, e, direct, workspace_bytes);
   const int64_t blocks = p.tiles_m * p.tiles_n * p.parts;
-  if (blocks > kMostBlocks) return invalid(err, "more than 2^24 - 1 tiles of the result: " + std::to_string(blocks));
+  if (blocks > kMostTiles) return invalid(err, "more than 2^23 - 1 tiles of the result: " + std::to_string(blocks));
   args.m = e.m;
   args.n = e.n;
   args.depth = e.depth;
