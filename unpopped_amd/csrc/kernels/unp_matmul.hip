@@ -660,14 +660,14 @@ template <class OUT> struct rows_out {
 // one of each pair of halves; the halves of the operands' tiles lie in LDS twice, and as a half has been read by every wave, the
 // loads of the same half two steps on go there: five halves are on their way at any time.  (X0 is the first 128 rows; W0 the
 // first 32 of each 64, so that a wave stores whole lines, or where W lies along out the first 128, as loads take more of a row.)
-//   phase  reads     multiplies  loads
-//   0      X0 W0     X0 W0       scales and X1 of the next step
-//   1      W1        X0 W1       X0 of the one after it
-//   2      X1        X1 W1       W0
-//   3                X1 W0       W1
+//   phase  reads     multiplies    loads
+//   0      X0 W0 W1  X0 W0, X0 W1  scales two steps on, X1 of the next step
+//   1      X1        X1 W1, X1 W0  X0, W0 and W1 of the one after it
 // A wave waits for its own loads of what the next phase reads before the barrier that ends its reads: all but those that it
-// has started since.  A tile of at most 128 rows, the last of a group, has the first two phases alone: they load scales two
-// steps ahead and W1 of the next, then X0 and W0 two ahead.
+// has started since.  (Four phases of half the products each took 519 us for 8192^3 codes, these
+// 482, and 399 and 387 for 12001 x 8192 x 2048 in 16 bits by 16 groups.)  A tile of at most
+// 128 rows, the last of a group, multiplies X0 W0 and X0 W1 in a phase each: the first loads scales two steps ahead and W1 of the next,
+// the second X0 and W0 two ahead.
 template <int XK, int WKIND, bool XT, bool WT, class OUT, int BY, int SB>
 UNPM_DEV void matmul_wide(const u8* xp, const u8* wp, const float* xsp, const float* wsp, const i32* starts, OUT* out, float* parts,
                           const product_args& a) {
@@ -740,22 +740,19 @@ UNPM_DEV void matmul_wide(const u8* xp, const u8* wp, const float* xsp, const fl
   const i64 steps = o.last - o.first;
   const bool low = o.m_there <= 128;
   if (steps > 0) {
+    issue_scales(0);
     issue(0, 0);
     issue(2, 0);
     issue(3, 0);
-    issue_scales(0);
-    if (low) {
-      issue_scales(1);
-      issue(0, 1);
-      issue(2, 1);
-      wait_loads<E == 1 ? 5 : 4>();
-    } else {
-      issue(1, 0);
-      issue(0, 1);
-      issue(2, 1);
-      issue(3, 1);
-      wait_loads<E == 1 ? 8 : 10>();
-    }
+    issue_scales(1);
+    if (!low) issue(1, 0);
+    issue(0, 1);
+    issue(2, 1);
+    if (!low) issue(3, 1);
+    if (low)
+      wait_loads<E == 1 ? 7 : 6>();
+    else
+      wait_loads<E == 1 ? 9 : 8>();
     lds_barrier();
     if (wm == 1) lds_barrier();
 
@@ -779,14 +776,18 @@ UNPM_DEV void matmul_wide(const u8* xp, const u8* wp, const float* xsp, const fl
         for (int n = 0; n < 2; ++n) wrow[n] = *reinterpret_cast<const f32x4*>(s + n * 16 + (lane >> 4) * 4);
       if constexpr (E == 1 && SB > 1) wsc = *s;
     };
-    auto read_w = [&](const u8* at, const float* scales, int h) {
+    auto read_w_codes = [&](const u8* at, int h) {
 #pragma unroll
       for (int n = 0; n < 2; ++n)
 #pragma unroll
         for (int k = 0; k < 2; ++k) wf[h][n][k] = wside::read(at + (2 + h) * HALF, wn * 32 + n * 16, k, lane);
+    };
+    auto read_w = [&](const u8* at, const float* scales, int h) {
+      read_w_codes(at, h);
       read_w_scales(scales, h);
     };
-    auto products = [&](int hw, int hx) {
+    // `next`: where the scales of W's other half are, read as this half's are used up.
+    auto products = [&](int hw, int hx, const float* next = nullptr) {
       __builtin_amdgcn_s_setprio(1);
       if constexpr (E == 2) {
 #pragma unroll
@@ -813,6 +814,11 @@ UNPM_DEV void matmul_wide(const u8* xp, const u8* wp, const float* xsp, const fl
               acc[hw][hx][n][m][j] =
                   __builtin_fmaf(p[(i - LATE) % (LATE + 1)][j], SB == 1 ? both[m] * wrow[n][j] : both[m], acc[hw][hx][n][m][j]);
           }
+          if constexpr (SB == 1)
+            if (next && (i == 3 + LATE || i == 7 + LATE)) {
+              const int n = (i - LATE) / 4;
+              wrow[n] = *reinterpret_cast<const f32x4*>(next + 256 + (1 - hw) * 128 + wn * 32 + n * 16 + (lane >> 4) * 4);
+            }
           __builtin_amdgcn_sched_barrier(0);
         }
       }
@@ -851,27 +857,21 @@ UNPM_DEV void matmul_wide(const u8* xp, const u8* wp, const float* xsp, const fl
       const float* sc = reinterpret_cast<const float*>(lds + 2 * STAGE + (u32)(s & 3) * SCALES);
       read_x(at, sc, 0);
       read_w(at, sc, 0);
-      issue_scales(s + 1);
+      read_w_codes(at, 1);
+      issue_scales(s + 2);
       issue(1, s + 1);
-      wait_loads<E == 1 ? 12 : 10>();
+      wait_loads<E == 1 ? 9 : 8>();
       read_done();
-      products(0, 0);
-      meet();
-      read_w(at, sc, 1);
-      issue(0, s + 2);
-      wait_loads<E == 1 ? 11 : 10>();
-      read_done();
+      products(0, 0, sc);
       products(1, 0);
       meet();
       read_x(at, sc, 1);
+      issue(0, s + 2);
       issue(2, s + 2);
-      read_done();
-      products(1, 1);
-      meet();
-      read_w_scales(sc, 0);
       issue(3, s + 2);
-      wait_loads<E == 1 ? 8 : 10>();
+      wait_loads<E == 1 ? 9 : 8>();
       read_done();
+      products(1, 1, sc);
       products(0, 1);
       meet();
     }
