@@ -478,7 +478,7 @@ def test_product_of_codes_by_kernel(hip_device, m, n, k, kw, entry):
 @pytest.mark.parametrize("m, n, k, groups, way, entry", [
     (40, 48, 256, 8, "all", "_slim"), (500, 2100, 144, 40, "gaps", "_few"), (500, 260, 640, 10, "all", "_slim"), (900, 300, 272, 6, "gaps", "_few"),
     (4000, 2300, 144, 5, "gaps", "_wide"), (3500, 2561, 272, 2, "one", "_wide"),
-    (40, 48, 1040, 8, "all", "_one"), (500, 1100, 640, 10, "all", "_few"), (900, 1300, 272, 6, "gaps", "_some"), (2000, 2100, 272, 6, "gaps", "_tile"),
+    (40, 48, 1040, 8, "all", "_slim"), (40, 48, 2064, 8, "all", "_one"), (500, 1100, 640, 10, "all", "_few"), (900, 1300, 272, 6, "gaps", "_some"), (2000, 2100, 272, 6, "gaps", "_tile"),
 ])
 def test_product_of_codes_by_group_and_kernel(hip_device, m, n, k, groups, way, entry):
     assert matmul8_case(m, n, k, groups=groups, way=way)["entry"].endswith(entry)

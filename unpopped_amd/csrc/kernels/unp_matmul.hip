@@ -658,16 +658,15 @@ template <class OUT> struct rows_out {
 // Tiles of 256 x 256 for much work: eight waves, two on each SIMD, of which one multiplies while the other reads LDS and
 // starts loads (the second set runs one barrier behind the first).  A wave has 128 x 64 of the tile as four blocks of 64 x 32,
 // one of each pair of halves; the halves of the operands' tiles lie in LDS twice, and as a half has been read by every wave, the
-// loads of the same half two steps on go there: five halves are on their way at any time.  (X0 is the first 128 rows; W0 the
+// loads of the same half two steps on go there: four halves or five are on their way at any time.  (X0 is the first 128 rows; W0 the
 // first 32 of each 64, so that a wave stores whole lines, or where W lies along out the first 128, as loads take more of a row.)
 //   phase  reads     multiplies    loads
 //   0      X0 W0 W1  X0 W0, X0 W1  scales two steps on, X1 of the next step
 //   1      X1        X1 W1, X1 W0  X0, W0 and W1 of the one after it
 // A wave waits for its own loads of what the next phase reads before the barrier that ends its reads: all but those that it
-// has started since.  (Four phases of half the products each took 519 us for 8192^3 codes, these
-// 482, and 399 and 387 for 12001 x 8192 x 2048 in 16 bits by 16 groups.)  A tile of at most
-// 128 rows, the last of a group, multiplies X0 W0 and X0 W1 in a phase each: the first loads scales two steps ahead and W1 of the next,
-// the second X0 and W0 two ahead.
+// has started since.  (Four phases of half the products each took 519 us for 8192^3 codes, these 482, and 399 and 387 for 12001 x
+// 8192 x 2048 in 16 bits by 16 groups.)  A tile of at most 128 rows, the last of a group, multiplies X0 W0 and X0 W1 in a phase
+// each: the first loads scales two steps ahead and W1 of the next, the second X0 and W0 two ahead.
 template <int XK, int WKIND, bool XT, bool WT, class OUT, int BY, int SB>
 UNPM_DEV void matmul_wide(const u8* xp, const u8* wp, const float* xsp, const float* wsp, const i32* starts, OUT* out, float* parts,
                           const product_args& a) {

@@ -2231,7 +2231,7 @@ int64_t row_tiles(const Extents& e, int64_t t) {
 // What a direct entry takes, in microseconds: to begin and end, and a step (128 bytes along the depth) of the blocks of a CU,
 // of one block and of as many as the CU holds; and the TB/s at which it reads weights that no cache holds.  Fitted to times of
 // 78 shapes of 1 to 16000 rows, 72 to 28672 columns, depths of 64 to 28672 and 1 to 64 groups, where it chooses entries and parts
-// that are 4 % slower than the best of each (geometric mean; over 12 % at 7 shapes, 43 % at the worst).
+// that are 3 % slower than the best of each (geometric mean; over 12 % at 7 shapes, 33 % at the worst).
 struct EntryCost {
   double fixed, alone, full, rate;
 };
@@ -2267,11 +2267,12 @@ ProductPlan product_plan(const unp_exec* x, const Extents& e, bool direct, int64
       const double tiles = rows * (double)((e.n + es[k].cols - 1) / es[k].cols);
       const double hold = (double)x->cu_count * std::max(1, x->resident[k]);
       const EntryCost c = entry_cost(es[k].vec * es[k].cols, codes);
-      const double read = weights / c.rate;
       for (int64_t parts : {1, 2, 3, 4, 6, 8, 12, 16}) {
         if (parts > 1 && (steps < 4.0 * es[k].k * (double)parts || parts_bytes(e, parts) > workspace_bytes)) break;
         if (row_tiles(e, es[k].vec) * ((e.n + es[k].cols - 1) / es[k].cols) * parts > kMostTiles) break;
         const double blocks = tiles * (double)parts, each = std::ceil(steps / (double)parts), rounds = std::ceil(blocks / hold);
+        // A CU reads at 1.5 times its share of the rate at most, where others read nothing.
+        const double read = weights / (c.rate * std::min(1.0, 1.5 * blocks / (double)x->cu_count));
         double t = std::max(read, blocks <= x->cu_count ? each * c.alone : rounds * each * c.full) + c.fixed + 1.5 * (rounds - 1);
         if (parts > 1) t += 4.0 + 2.0 * (double)parts_bytes(e, parts) / 3.2e6;
         if (least > 0 && t >= least) continue;
