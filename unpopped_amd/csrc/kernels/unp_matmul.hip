@@ -71,7 +71,6 @@ struct product_args {
   i64 xs_row, ws_row, ws_group;    // of the scales, in elements
   i64 out_row, out_group;          // in elements
   i32 groups, tiles_m, tiles_n, parts;
-  i32 x_vectors, w_vectors;        // rows of whole 16-byte vectors
   i32 wide;                        // out takes vectors of 16 bytes: 1, or 2 past the caches
   i32 tail;                        // bytes of a row's last 16 along d that exist, where not all do
   i32 turn, pad;                   // steps by which neighbouring columns of tiles begin apart
@@ -96,10 +95,13 @@ UNPM_DEV void load_word_to_lds(const float* p, u32 to) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" ::"s"(scalar(to)), "v"(p) : "memory");
 }
 
-// 16 bytes at p of which `there` exist (elements of E bytes), zeros for the others.
-template <int E> UNPM_DEV u32x4 fetch16(const u8* p, i64 there, bool vector) {
-  if (vector && there >= 16) return *reinterpret_cast<const u32x4*>(p);
+// 16 bytes at p, aligned or not, of which `there` exist (elements of E bytes), zeros for the others.
+template <int E> UNPM_DEV u32x4 fetch16(const u8* p, i64 there) {
   u32x4 x = {0, 0, 0, 0};
+  if (there >= 16) {
+    __builtin_memcpy(&x, p, 16);
+    return x;
+  }
 #pragma unroll
   for (int i = 0; i < 16; i += E)
     if (i < there) {
@@ -130,7 +132,6 @@ template <int KIND, bool TURNED, int T> struct side {
   const u8* p;      // the tile's first element
   i64 row;          // stride in bytes
   i64 there;        // rows of the tile that exist (TURNED: bytes of its columns)
-  bool vectors;
 
   // Lane `lane` of unit u: the row and the chunk that lie at its 16 bytes.
   static UNPM_DEV int row_of(int u, int lane) { return u * (64 / CHUNKS) + lane / CHUNKS; }
@@ -173,11 +174,11 @@ template <int KIND, bool TURNED, int T> struct side {
     const int r = q / CHUNKS, c = q % CHUNKS;
     if constexpr (TURNED) {
       const int from = map(c);
-      if (r < elements - first) v = fetch16<E>(at(step) + (first + r) * row + from * 16, there - from * 16, vectors);
+      if (r < elements - first) v = fetch16<E>(at(step) + (first + r) * row + from * 16, there - from * 16);
       *reinterpret_cast<u32x4*>(lds + r * (T * 2) + turned_slot<T>(r, c) * 16) = v;
     } else {
       const int from = map(r);
-      if (c == 0 && from < there) v = fetch16<E>(at(step) + from * row + first * E, (elements - first) * E, false);
+      if (c == 0 && from < there) v = fetch16<E>(at(step) + from * row + first * E, (elements - first) * E);
       *reinterpret_cast<u32x4*>(lds + r * 128 + straight_slot(r, c) * 16) = v;
     }
   }
@@ -185,7 +186,7 @@ template <int KIND, bool TURNED, int T> struct side {
   UNPM_DEV u32x4 fetch(int u, int lane, i64 step, i64 elements) const {
     const int r = row_of(u, lane), c = chunk_of(u, lane);
     const i64 bytes = TURNED ? (r < elements ? there - c * 16 : 0) : (r < there ? elements * E - c * 16 : 0);
-    return fetch16<E>(at(step) + r * row + c * 16, bytes, vectors);
+    return fetch16<E>(at(step) + r * row + c * 16, bytes);
   }
 
   // The 16 bytes of lane (i, g) for the matrix instruction: half h of the step of tile row first + i.
@@ -376,11 +377,9 @@ UNPM_DEV bool find_place(const u8* x, const u8* w, const float* xs, const float*
   o.x.p = XT ? x + o.m0 * 2 : x + o.m0 * a.x_row;
   o.x.row = a.x_row;
   o.x.there = XT ? o.m_there * 2 : o.m_there;
-  o.x.vectors = a.x_vectors;
   o.w.p = WT ? w + o.n0 * 2 : w + o.n0 * a.w_row;
   o.w.row = a.w_row;
   o.w.there = WT ? n_there * 2 : n_there;
-  o.w.vectors = a.w_vectors;
   if constexpr (E == 1) {
     o.xs = xs + o.m0 * a.xs_row;
     o.xs_last = o.m_there - 1;
@@ -695,12 +694,10 @@ UNPM_DEV void matmul_wide(const u8* xp, const u8* wp, const float* xsp, const fl
     xh[h].row = a.x_row;
     xh[h].p = XT ? o.x.p + h * 256 : o.x.p + h * 128 * a.x_row;
     xh[h].there = o.x.there - h * (XT ? 256 : 128);
-    xh[h].vectors = true;
   }
   w.row = a.w_row;
   w.p = o.w.p;
   w.there = o.w.there;
-  w.vectors = true;
   u32 offset[4][2];
 #pragma unroll
   for (int h = 0; h < 2; ++h)

@@ -2187,7 +2187,7 @@ int32_t run_cache4_attention(unp_exec* x, const unp_arg* a, size_t n, hipStream_
 // Host images of the kernels' argument structs (passed by value).
 struct product_args_host {
   int64_t m, n, depth, x_row, w_row, w_group, xs_row, ws_row, ws_group, out_row, out_group;
-  int32_t groups, tiles_m, tiles_n, parts, x_vectors, w_vectors, wide, tail, turn, pad;
+  int32_t groups, tiles_m, tiles_n, parts, wide, tail, turn, pad;
 };
 struct quant_args_host {
   int64_t rows, cols, x_row, code_row, scale_row;
@@ -2358,11 +2358,9 @@ int32_t run_matmul8(unp_exec* x, const unp_arg* a, size_t n, hipStream_t s, unp_
   args.ws_row = bs_row;
   args.ws_group = bs_group;
   args.out_row = out_row;
-  args.x_vectors = vectors(A.buf[0], a_row, 1);
-  args.w_vectors = vectors(A.buf[2], b_row, 1) && b_group % 16 == 0;
   args.wide = vectors(A.buf[out], out_row, size);
   args.tail = (int32_t)(e.depth % 16);
-  const bool direct = args.x_vectors && args.w_vectors && near(a_row) && near(b_row);
+  const bool direct = vectors(A.buf[0], a_row, 1) && vectors(A.buf[2], b_row, 1) && b_group % 16 == 0 && near(a_row) && near(b_row);
   const uint64_t buf[7] = {A.buf[0], A.buf[2], A.buf[1], A.buf[3], starts, A.buf[out], A.buf[out + 1]};
   return launch_product(x, e, args, buf, bytes, direct, s, err);
 }
@@ -2410,13 +2408,11 @@ int32_t run_grouped_matmul(unp_exec* x, const unp_arg* a, size_t n, hipStream_t 
   args.w_group = 2 * w_group;
   args.out_row = out_row;
   args.out_group = out_group;
-  args.x_vectors = vectors(A.buf[0], x_row, 2);
-  args.w_vectors = vectors(A.buf[1], w_row, 2) && w_group % 8 == 0;
   args.wide = vectors(A.buf[3], out_row, size) && out_group * size % 16 == 0;
   // Columns of out that lie along an operand's rows are whole vectors; a depth that does may end inside one.
   const bool whole = weight ? nn % 8 == 0 && kk % 8 == 0 : input ? kk % 8 == 0 : true;
   args.tail = weight ? 0 : (int32_t)(2 * e.depth % 16);
-  const bool direct = args.x_vectors && args.w_vectors && whole && near(2 * x_row) && near(2 * w_row);
+  const bool direct = vectors(A.buf[0], x_row, 2) && vectors(A.buf[1], w_row, 2) && w_group % 8 == 0 && whole && near(2 * x_row) && near(2 * w_row);
   const uint64_t buf[7] = {A.buf[0], A.buf[1], 0, 0, A.buf[2], A.buf[3], A.buf[4]};
   return launch_product(x, e, args, buf, bytes, direct, s, err);
 }
