@@ -434,6 +434,7 @@ typedef struct unp_quant8 {
 /* A scale for each block of block_rows rows and 128 columns of y: the largest magnitude of the block times the f32 number
  * nearest to 1 / 448 (or 1 / 57344), the largest code's inverse.  A code is its element over the scale, correctly rounded to f32
  * and from there to even.  A block of zeros has the scale 0 and codes 0; one that holds a NaN or an infinity has a NaN scale and codes 0.
+ * Quotients past the largest code, which scales below 2^-145 may leave, take that code; a block whose scale rounds to 0 has codes 0.
  * Launch: x ([rows][cols]), codes (y's shape), scales (F32 [y's rows / block_rows][y's columns / 128], both rounded up);
  * rows, cols, x_row, code_row, scale_row (strides).  Bytes of a row of codes behind its columns are not written. */
 int32_t unp_hip_lower_quant8(const unp_quant8* q, unp_generated** out, unp_error* err);

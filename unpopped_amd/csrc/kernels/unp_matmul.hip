@@ -976,6 +976,9 @@ UNPM_DEV void join(const i32* starts, OUT* out, const float* parts, const produc
 // Quantisation: codes of y = x or its transpose, and the f32 scale of each block of 128 columns and RB rows of y:
 // scale = most times the f32 nearest to 1 / largest code, code = y / scale rounded to even from the correctly rounded quotient.
 // A block of zeros has the scale 0 and divides as by 1; one that holds a NaN or an infinity has a NaN scale and codes 0.
+// Where the scale is a subnormal number of few digits, its rounding may leave quotients past what rounds to the largest code, up
+// to half as much again: they take that code (the conversions would make a NaN or an infinity of them).  A scale that rounds to
+// 0 leaves codes 0.
 //
 // Magnitudes are compared as integers (NaN above infinity above every number).  The quotient of two f32 numbers is taken
 // from the divisor's reciprocal by one correction (P. Markstein, 1990), exact while the remainder is a normal number;
@@ -987,7 +990,8 @@ struct quant_args {
   i32 x_vectors, code_vectors;
 };
 
-template <int KIND> UNPM_DEV float inverse_largest() { return KIND == E4M3 ? 1.0f / 448.0f : 1.0f / 57344.0f; }
+template <int KIND> UNPM_DEV float largest() { return KIND == E4M3 ? 448.0f : 57344.0f; }
+template <int KIND> UNPM_DEV float inverse_largest() { return 1.0f / largest<KIND>(); }
 
 struct step_of {
   float scale, unit, inverse;
@@ -1002,11 +1006,12 @@ template <int KIND> UNPM_DEV step_of block_step(u32 most) {
   s.divide = s.unit < 0x1p-90f;
   return s;
 }
-// Numbers of one block over its step; where it is none, whatever comes out.  A wave divides or multiplies as one.
-template <int N> UNPM_DEV void quotients(float (&y)[N], const step_of& s) {
+// Numbers of one block over its step; where it is none, whatever comes out.  A wave divides or multiplies as one.  Only scales
+// that divide may be subnormal.
+template <int KIND, int N> UNPM_DEV void quotients(float (&y)[N], const step_of& s) {
   if (__any(s.divide)) {
 #pragma unroll
-    for (int i = 0; i < N; ++i) y[i] = y[i] / s.unit;
+    for (int i = 0; i < N; ++i) y[i] = __builtin_amdgcn_fmed3f(y[i] / s.unit, -largest<KIND>(), largest<KIND>());
   } else {
 #pragma unroll
     for (int i = 0; i < N; ++i) {
@@ -1089,7 +1094,7 @@ template <class T, int KIND> UNPM_DEV void quantise_rows(const T* x, u8* codes, 
       most = more(most, magnitude(y[j]));
     }
     const step_of s = block_step<KIND>(most_of_8(most));
-    quotients(y, s);
+    quotients<KIND>(y, s);
 #pragma unroll
     for (int p = 0; p < PIECES; ++p) {
       u32 w[V / 4];
@@ -1160,7 +1165,7 @@ UNPM_DEV void quantise_tiles(const T* x, u8* codes, float* scales, const quant_a
       if (threadIdx.x == 0) scales[(TURNED ? tc : tr) * a.scale_row + (TURNED ? tr : tc)] = s.scale;
 #pragma unroll
       for (int c = 0; c < 8; ++c) {
-        quotients(y[c], s);
+        quotients<KIND>(y[c], s);
         none[c] = s.none;
       }
     } else {
@@ -1178,7 +1183,7 @@ UNPM_DEV void quantise_tiles(const T* x, u8* codes, float* scales, const quant_a
 #pragma unroll
       for (int c = 0; c < 8; ++c) {
         const step_of s = block_step<KIND>(tops[0][column(c)]);
-        quotients(y[c], s);
+        quotients<KIND>(y[c], s);
         none[c] = s.none;
       }
     }
