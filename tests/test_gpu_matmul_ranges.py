@@ -57,3 +57,29 @@ def test_blocks_whose_scale_is_subnormal(hip_device, dtype, kind, block_rows, tr
         y[-1, rng.integers(0, 128)] = -most
         blocks.append(y)
     quantise_blocks(dtype, kind, block_rows, transpose, np.concatenate(blocks) * UNIT)
+
+
+@pytest.mark.parametrize("block_rows, transpose", [(1, False), (1, True), (128, False)])
+@pytest.mark.parametrize("kind", ["Fp8E4M3FN", "Fp8E5M2"])
+def test_quotients_beside_the_smallest_ties(hip_device, kind, block_rows, transpose):
+    """A quotient next to a tie is on its side of it, for scales about those from which on they are not divided; the rows of one wave have
+    scales of both sorts."""
+    bits, low = ref.FIELDS[kind]
+    top, ties = np.float32(ref.LARGEST[kind]), np.ldexp(np.arange(1, 16, 2), low - bits - 1).astype(np.float32)
+    rng, rows = np.random.default_rng(3), []
+    for e in range(-96, -76):
+        for f in (1.0, 2.0 - 2.0 ** -23, 2.0 - 7 * 2.0 ** -22, *(1.0 + rng.integers(0, 1 << 23, 5) * 2.0 ** -23)):
+            most = np.float32(np.ldexp(f, e)) * top
+            unit = most * np.float32(1.0 / top)
+            y = [ties * unit]
+            for _ in range(3):
+                y = [np.nextafter(y[0], np.float32(0)), *y, np.nextafter(y[-1], top)]
+            y = np.concatenate(y)[:127]
+            rows.append(np.concatenate([[most], y, np.zeros(127 - len(y), np.float32)]))
+    for most, other in (("0x1.bffff2p-74", "0x1.fffff4p-107"), ("0x1.bffffap-73", "0x1.fffffcp-106")):
+        rows.append(np.array([float.fromhex(most), float.fromhex(other)] + [0.0] * 126))
+        rows += [np.zeros(128)] * 7  # no scale that divides beside it
+    y = np.array(rows)
+    y = np.concatenate([y, rng.permutation(y)])
+    y = np.concatenate([y, np.zeros((-len(y) % 128, 128))]) if block_rows == 1 else np.repeat(y[-60:], 128, 0) * (rng.random((60 * 128, 1)) < 0.5)
+    quantise_blocks("F32", kind, block_rows, transpose, y)

@@ -981,8 +981,9 @@ UNPM_DEV void join(const i32* starts, OUT* out, const float* parts, const produc
 // 0 leaves codes 0.
 //
 // Magnitudes are compared as integers (NaN above infinity above every number).  The quotient of two f32 numbers is taken
-// from the divisor's reciprocal by one correction (P. Markstein, 1990), exact while the remainder is a normal number;
-// the scales where it may not be divide.
+// from the divisor's reciprocal by one correction (P. Markstein, 1990), right while f32 holds the remainder; the scales where it may not
+// divide.  A code is decided at quotients from the smallest tie on, 2^-17 (e5m2; e4m3 2^-10).  Beside it a quotient has steps of
+// 2^-41, a scale of 2^e has steps of 2^(e-23), and so the remainder steps of 2^(e-64): f32's smallest, 2^-149, at e = -85.
 // ---------------------------------------------------------------------------------------
 struct quant_args {
   i64 rows, cols;  // of x
@@ -1003,7 +1004,7 @@ template <int KIND> UNPM_DEV step_of block_step(u32 most) {
   s.scale = s.none ? __builtin_nanf("") : bits<float>(most) * inverse_largest<KIND>();
   s.unit = s.scale > 0.0f ? s.scale : 1.0f;
   s.inverse = 1.0f / s.unit;
-  s.divide = s.unit < 0x1p-90f;
+  s.divide = s.unit < 0x1p-80f;
   return s;
 }
 // Numbers of one block over its step; where it is none, whatever comes out.  A wave divides or multiplies as one.  Only scales
