@@ -4,7 +4,7 @@ import pytest
 
 import unpopped_amd as u
 from tests import matmul_reference as ref
-from tests.test_gpu_matmul import dev, executor, held, run
+from tests.test_gpu_matmul import JUNK, dev, executor, held, laid, read, run, starts_of
 
 pytestmark = pytest.mark.gpu
 UNIT = 2.0 ** -149  # the smallest step of f32
@@ -83,3 +83,94 @@ def test_quotients_beside_the_smallest_ties(hip_device, kind, block_rows, transp
     y = np.concatenate([y, rng.permutation(y)])
     y = np.concatenate([y, np.zeros((-len(y) % 128, 128))]) if block_rows == 1 else np.repeat(y[-60:], 128, 0) * (rng.random((60 * 128, 1)) < 0.5)
     quantise_blocks("F32", kind, block_rows, transpose, y)
+
+
+# ---------------------------------------------------------------------------------------
+# Products of codes whose scales are far from 1
+# ---------------------------------------------------------------------------------------
+def launch_codes(a, sa, b, sb, a_kind, b_kind, out, b_rows, pad, starts, workspace=None):
+    """The product of numbers that are codes: [m][n] in 64 bits, and the launch."""
+    (m, k), (g, n, _) = a.shape, b.shape
+    aa, a_row, _ = laid(ref.encoded(a, a_kind), pad, 0, JUNK[a_kind])
+    ba, b_row, b_group = laid(ref.encoded(b, b_kind), pad, 0, JUNK[b_kind])
+    sab, as_row, _ = laid(sa, 0, 0, np.float32(np.nan))
+    sbb, bs_row, bs_group = laid(sb, 0, 0, np.float32(np.nan))
+    ex = executor("lower_matmul8", a_kind=a_kind, b_kind=b_kind, out=out, b_rows=b_rows, grouped=starts is not None)
+    shape = (m, n, k) if starts is None else (m, n, k, g)
+    ws = ex.workspace_bytes(*shape) if workspace is None else workspace
+    ob = dev(held(np.full((m, n), 9.0), out))
+    run(ex, dev(aa), dev(sab), dev(ba), dev(sbb), *([] if starts is None else [dev(starts.astype(np.int32))]), ob,
+        dev(np.full(ws + 16, 0xFF, np.uint8)), *shape, a_row, as_row, b_row, bs_row, *([] if starts is None else [b_group, bs_group]), n, ws)
+    return read(ob, m * n, out).reshape(m, n), ex.last_launch()
+
+
+FAR = [
+    (16, 33, 1040, dict(), "_one"), (16, 33, 1040, dict(b_rows=1), "_one"), (1, 300, 2048, dict(b_kind="Fp8E5M2"), "_one"),
+    (32, 2100, 272, dict(), "_slim"), (65, 4100, 272, dict(b_rows=1), "_few"), (600, 2100, 272, dict(b_rows=1), "_some"),
+    (1000, 2100, 16, dict(), "_tile"), (2817, 2561, 143, dict(b_rows=1, pad=1), "_tile"), (130, 300, 200, dict(pad=1), "_any"),
+    (70, 300, 200, dict(pad=1, b_rows=1), "_any"), (4000, 2561, 272, dict(), "_wide"), (4000, 2561, 272, dict(a_kind="Fp8E5M2"), "_wide"),
+    (4000, 2100, 143, dict(pad=1, b_rows=1), "_wide"), (2817, 4100, 257, dict(pad=15), "_wide"), (2817, 2820, 400, dict(b_rows=1), "_wide"),
+    (60, 300, 28000, dict(), "_join"), (3500, 2561, 272, dict(groups=2), "_wide"), (900, 1300, 272, dict(groups=6), "_some"),
+]
+
+
+def far_inputs(m, n, k, a_kind, b_kind, b_rows, groups):
+    rng = np.random.default_rng(6)
+    nb, nr, g = -(-k // 128), -(-n // b_rows), max(1, groups)
+    a, b = (ref.decoded(ref.encoded(32 + 64 * np.minimum(np.abs(rng.normal(size=s)), 4), kind), kind) for s, kind in (((m, k), a_kind), ((g, n, k), b_kind)))
+    sa, sb = (np.exp(rng.normal(size=s) / 2) for s in ((m, nb), (g, nr, nb)))
+    starts = starts_of(rng, m, groups, "all") if groups else None
+    return rng, a, sa, b, sb, starts
+
+
+@pytest.mark.parametrize("m, n, k, kw, entry", FAR)
+def test_scales_whose_product_is_no_number(hip_device, m, n, k, kw, entry):
+    """Products of scales far below f32 and past its end, whose products with the sums of codes are ordinary numbers or 0."""
+    kinds = [kw.get(s, "Fp8E4M3FN") for s in ("a_kind", "b_kind")]
+    b_rows, groups = kw.get("b_rows", 128), kw.get("groups", 0)
+    rng, a, sa, b, sb, starts = far_inputs(m, n, k, *kinds, b_rows, groups)
+    nb, nr = sa.shape[1], sb.shape[1]
+    some = rng.permutation(m)
+    # Columns of 2^-60, of 2^-110 and, in one block, of 2^40.
+    sb[:, 0] *= 2.0 ** -60
+    if nr > 2:
+        sb[:, nr // 2] *= 2.0 ** -110
+        sb[:, -1, nb - 1] *= 2.0 ** 40
+    # Rows of 2^-84, of subnormal scales, of 2^120, and of 2^100 where all codes are 0.
+    sa[some[:2]] *= 2.0 ** -84
+    if m > 6:
+        sa[some[2:3]] *= 2.0 ** -143
+        sa[some[3:4]] *= 2.0 ** 120
+        sa[some[4:5], nb - 1], a[some[4], 128 * (nb - 1):] = 2.0 ** 100, 0
+    sa, sb = sa.astype(np.float32), sb.astype(np.float32)
+    got, launch = launch_codes(a, sa, b, sb, *kinds, "Bf16", b_rows, kw.get("pad", 0), starts)
+    assert launch["entry"].endswith(entry), launch
+    assert not np.isnan(got).any()
+    for i in {*some[:5], *some[-20:], 0, m - 1}:
+        w = 0 if starts is None else int(np.searchsorted(starts, i, "right")) - 1
+        want, size, tops = (v[0] for v in ref.product8(a[i:i + 1], sa[i:i + 1], b[w], sb[w], b_rows))
+        # As for scales near 1: the matrix unit's 2^-13 of the largest of 16 products, 2^-23 of the magnitudes for each sum and product.
+        # A sum that takes exponents below f32's keeps steps of 2^-149 times 4 of the fractions.  Then the type's rounding.
+        tol = tops * 15 * 2.0 ** -13 + size * (8 + 3 * nb) * 2.0 ** -23 + nb * 2.0 ** -147
+        tol += (np.abs(want) + tol) * 2.0 ** -8 + 2.0 ** -134
+        over = want > 2.0 ** 130
+        assert (over | (want < 2.0 ** 127)).all()
+        with np.errstate(invalid="ignore"):
+            bad = np.where(over, got[i] != np.inf, ~(np.abs(got[i] - want) <= tol))
+        assert not bad.any(), (launch, i, np.flatnonzero(bad)[:5], got[i][bad][:5], want[bad][:5])
+
+
+@pytest.mark.parametrize("m, n, k, kw, entry", [c for c in FAR if c[0] > 6])
+def test_far_scales_leave_other_rows_as_they_were(hip_device, m, n, k, kw, entry):
+    """Bit for bit: rows beside one of a tiny scale, columns beside some of a large one."""
+    kinds = [kw.get(s, "Fp8E4M3FN") for s in ("a_kind", "b_kind")]
+    b_rows, groups = kw.get("b_rows", 128), kw.get("groups", 0)
+    _, a, sa, b, sb, starts = far_inputs(m, n, k, *kinds, b_rows, groups)
+    args = (b, sb.astype(np.float32), *kinds, "F16", b_rows, kw.get("pad", 0), starts)
+    sa /= 2.0 ** 20
+    plain, _ = launch_codes(a, sa.astype(np.float32), *args)
+    sa[m // 2] *= 2.0 ** -90
+    got, launch = launch_codes(a, sa.astype(np.float32), *args)
+    assert launch["entry"].endswith(entry) and np.isfinite(plain).all()
+    keep = np.arange(m) != m // 2
+    assert np.array_equal(got[keep], plain[keep]) and (got[m // 2] == 0).all()

@@ -45,6 +45,7 @@ template <int N> UNPM_DEV void wait_loads() { asm volatile("s_waitcnt vmcnt(%0)"
 UNPM_DEV void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 UNPM_DEV u32 lds_address(const void* p) { return (u32)(size_t)(lds_void*)p; }
 UNPM_DEV i64 least(i64 a, i64 b) { return a < b ? a : b; }
+UNPM_DEV u32 more(u32 a, u32 b) { return a > b ? a : b; }
 // What every lane of a wave has, in scalar registers.
 UNPM_DEV u32 scalar(u32 x) { return __builtin_amdgcn_readfirstlane(x); }
 UNPM_DEV i64 uniform(i64 x) {
@@ -224,6 +225,35 @@ template <int KA, int KB> UNPM_DEV f32x4 multiply8(const u32x4 (&a)[2], const u3
   const i32x8 x = bits<i32x8>(both{{a[0], a[1]}}), y = bits<i32x8>(both{{b[0], b[1]}});
   return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(x, y, f32x4{0, 0, 0, 0}, KA - E4M3, KB - E4M3, 0, 0, 0, 0);
 }
+
+// A block's sum of codes times both scales, added to the sum of blocks.  One multiply-add with the product of the scales serves
+// where that is a normal number, as that of scales from 2^-63 up to 2^64 is, and for zeros, infinities and NaN.  Scales beyond
+// are rare, but their product may be outside f32 where its product with a sum of up to 2^39 is not: add_far gives the sum their
+// exponents and multiplies by the product of their fractions.  The waves of a tile look at the scales that they loaded, and
+// a tile with one beyond is made again with add_far once its sums are there.  That gives the same bits where one multiply-add serves
+// (and the result is above 2^-124), so a row's do not go by its neighbours' scales.  Looking takes up to 3 % of a launch of
+// a few hundred rows (1024 x 4096 x 4096 32.8 us, 31.8 without) and nothing that shows of 8192^3; a choice inside the loop took
+// 36 registers more than there are.
+UNPM_DEV u32 reach(float scale) { return (u32)(__builtin_amdgcn_frexp_expf(scale) + 62); }  // above 126: beyond
+struct parts_of {
+  float fraction;  // 1 to 2
+  i32 exponent;
+};
+UNPM_DEV parts_of taken_apart(float scale) {  // of 0 an exponent that no other's makes up for
+  return {2.0f * __builtin_amdgcn_frexp_mantf(scale), scale == 0.0f ? -1000 : __builtin_amdgcn_frexp_expf(scale) - 1};
+}
+UNPM_DEV void add_far(f32x4& sum, const f32x4& p, float a, const f32x4& b) {
+  const parts_of x = taken_apart(a);
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const parts_of y = taken_apart(b[j]);
+    sum[j] = __builtin_fmaf(__builtin_amdgcn_ldexpf(p[j], x.exponent + y.exponent), x.fraction * y.fraction, sum[j]);
+  }
+  __builtin_amdgcn_sched_barrier(0);  // in fewer registers
+}
+template <bool B> struct choice {
+  static constexpr bool value = B;
+};
 
 // Blocks are dealt to the 8 XCDs in turn.  Each takes a run of as many neighbouring tiles as its CUs hold at once, so that
 // its L2 holds what they share; the runs of the XCDs lie side by side, so that groups of any size load them alike.
@@ -450,6 +480,7 @@ UNPM_DEV void matmul(const u8* xp, const u8* wp, const float* xsp, const float* 
   static_assert(E == 2 || TM + TN <= SET * 64, "a scale a lane");
   static_assert(SPLIT * TM * TN * 4 <= STAGES * STAGE, "the sums of split steps");
   __shared__ __attribute__((aligned(1024))) u8 lds[STAGES * STAGE];
+  __shared__ u32 farthest[WAVES];
 
   place<XK, WKIND, XT, WT, BY, TM, TN> o;
   int part;
@@ -519,7 +550,8 @@ UNPM_DEV void matmul(const u8* xp, const u8* wp, const float* xsp, const float* 
         *reinterpret_cast<float*>(lds + to + lane * 4) = *p;
     }
   };
-  auto compute = [&](int slot) {
+  u32 far = 0;  // the farthest of the scales that this wave loaded
+  auto compute = [&](int slot, auto again) {
     const u8* xl = lds + slot * STAGE + own * STEP;
     const u8* wl = xl + xside::BYTES;
     if constexpr (E == 2) {
@@ -537,6 +569,7 @@ UNPM_DEV void matmul(const u8* xp, const u8* wp, const float* xsp, const float* 
       }
     } else {
       const float* sl = reinterpret_cast<const float*>(lds + slot * STAGE + SPLIT * STEP) + own * SET * 64;
+      const float mine = sl[in_set * 64 + lane];
       u32x4 xf[MT][2];
       float xsc[MT];
 #pragma unroll
@@ -559,16 +592,22 @@ UNPM_DEV void matmul(const u8* xp, const u8* wp, const float* xsp, const float* 
 #pragma unroll
         for (int m = 0; m < MT; ++m) {
           const f32x4 p = multiply8<WKIND, XK>(wf, xf[m]);
+          if constexpr (decltype(again)::value) {
+            add_far(acc[n][m], p, xsc[m], SB == 1 ? wsc : f32x4{wsc[0], wsc[0], wsc[0], wsc[0]});
+          } else {
 #pragma unroll
-          for (int j = 0; j < 4; ++j)
-            acc[n][m][j] = __builtin_fmaf(p[j], xsc[m] * (SB == 1 ? wsc[j] : wsc[0]), acc[n][m][j]);
+            for (int j = 0; j < 4; ++j)
+              acc[n][m][j] = __builtin_fmaf(p[j], xsc[m] * (SB == 1 ? wsc[j] : wsc[0]), acc[n][m][j]);
+          }
         }
       }
+      if constexpr (!decltype(again)::value) far = more(far, reach(mine));
     }
   };
 
   const i32 stages = (steps + SPLIT - 1) / SPLIT;
-  if (stages > 0) {
+  auto walk = [&](auto again) {
+    if (stages == 0) return;
     constexpr int LOADS = EACH + (E == 1);  // of a wave and stage
     // The stage that holds a step whose last 16 bytes do not all exist, which no load to LDS took.
     const i32 cut = DIRECT && a.tail && o.end == o.depth ? (turn > 0 ? steps - 1 - turn : steps - 1) : -1;
@@ -590,13 +629,28 @@ UNPM_DEV void matmul(const u8* xp, const u8* wp, const float* xsp, const float* 
         }
         lds_barrier();
       }
-      compute(slot);
+      compute(slot, again);
       slot = slot == STAGES - 1 ? 0 : slot + 1;
     }
     if constexpr (DIRECT) wait_loads<0>();  // LDS is not written after the block's end
+  };
+  walk(choice<false>{});
+  if constexpr (E == 1) {
+    if (__any(far > 126)) far = 127;
+    if (lane == 0) farthest[wave] = far;
+    lds_barrier();
+    if (__any(farthest[lane % WAVES] > 126)) {
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int m = 0; m < MT; ++m) acc[n][m] = f32x4{0, 0, 0, 0};
+      walk(choice<true>{});
+      lds_barrier();
+    }
+  } else {
+    lds_barrier();
   }
 
-  lds_barrier();
   float* sums = reinterpret_cast<float*>(lds);
 #pragma unroll
   for (int n = 0; n < NT; ++n)
@@ -674,6 +728,7 @@ UNPM_DEV void matmul_wide(const u8* xp, const u8* wp, const float* xsp, const fl
   typedef side<WKIND, WT, 128> wside;
   constexpr int HALF = 16384, STAGE = 4 * HALF, SCALES = E == 1 ? 2048 : 0;
   __shared__ __attribute__((aligned(1024))) u8 lds[2 * STAGE + 4 * SCALES];  // the scales of four steps
+  __shared__ u32 farthest[8];
 
   place<XK, WKIND, XT, WT, BY, 256, 256> o;
   int part;
@@ -731,8 +786,16 @@ UNPM_DEV void matmul_wide(const u8* xp, const u8* wp, const float* xsp, const fl
   };
 
   f32x4 acc[2][2][2][4];  // of W half, X half, tile of W, tile of X
+  auto clear = [&] {
 #pragma unroll
-  for (int i = 0; i < 32; ++i) (&acc[0][0][0][0])[i] = f32x4{0, 0, 0, 0};
+    for (int i = 0; i < 32; ++i) (&acc[0][0][0][0])[i] = f32x4{0, 0, 0, 0};
+  };
+  clear();
+  u32 far = 0;  // the farthest of the scales that this wave loaded
+  auto look = [&](i64 step) {
+    if constexpr (E == 1)
+      far = more(far, reach(*reinterpret_cast<const float*>(lds + 2 * STAGE + (u32)(step & 3) * SCALES + wave * 256 + lane * 4)));
+  };
   const i64 steps = o.last - o.first;
   const bool low = o.m_there <= 128;
   if (steps > 0) {
@@ -783,7 +846,7 @@ UNPM_DEV void matmul_wide(const u8* xp, const u8* wp, const float* xsp, const fl
       read_w_scales(scales, h);
     };
     // `next`: where the scales of W's other half are, read as this half's are used up.
-    auto products = [&](int hw, int hx, const float* next = nullptr) {
+    auto products = [&](auto again, int hw, int hx, const float* next = nullptr) {
       __builtin_amdgcn_s_setprio(1);
       if constexpr (E == 2) {
 #pragma unroll
@@ -805,10 +868,14 @@ UNPM_DEV void matmul_wide(const u8* xp, const u8* wp, const float* xsp, const fl
           __builtin_amdgcn_sched_barrier(0);
           if (i >= LATE) {
             const int n = (i - LATE) / 4, m = (i - LATE) % 4;
+            if constexpr (decltype(again)::value) {
+              add_far(acc[hw][hx][n][m], p[(i - LATE) % (LATE + 1)], xsc[m], SB == 1 ? wrow[n] : f32x4{wsc, wsc, wsc, wsc});
+            } else {
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-              acc[hw][hx][n][m][j] =
-                  __builtin_fmaf(p[(i - LATE) % (LATE + 1)][j], SB == 1 ? both[m] * wrow[n][j] : both[m], acc[hw][hx][n][m][j]);
+              for (int j = 0; j < 4; ++j)
+                acc[hw][hx][n][m][j] =
+                    __builtin_fmaf(p[(i - LATE) % (LATE + 1)][j], SB == 1 ? both[m] * wrow[n][j] : both[m], acc[hw][hx][n][m][j]);
+            }
           }
           if constexpr (SB == 1)
             if (next && (i == 3 + LATE || i == 7 + LATE)) {
@@ -829,6 +896,20 @@ UNPM_DEV void matmul_wide(const u8* xp, const u8* wp, const float* xsp, const fl
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
       meet();
     };
+    // A step that lies in LDS for every wave, whatever its scales are.
+    auto single = [&](const u8* at, const float* sc) {
+      constexpr choice<E == 1> again{};
+      read_x(at, sc, 0);
+      read_w(at, sc, 0);
+      products(again, 0, 0);
+      read_w(at, sc, 1);
+      products(again, 1, 0);
+      read_x(at, sc, 1);
+      products(again, 1, 1);
+      read_w(at, sc, 0);
+      products(again, 0, 1);
+    };
+    constexpr choice<false> once{};
     for (i64 s = 0; low && s < steps; ++s) {
       const u8* at = lds + (u32)(s & 1) * STAGE;
       const float* sc = reinterpret_cast<const float*>(lds + 2 * STAGE + (u32)(s & 3) * SCALES);
@@ -838,14 +919,15 @@ UNPM_DEV void matmul_wide(const u8* xp, const u8* wp, const float* xsp, const fl
       issue(3, s + 1);
       wait_loads<E == 1 ? 7 : 6>();
       read_done();
-      products(0, 0);
+      products(once, 0, 0);
       meet();
       read_w(at, sc, 1);
+      look(s);
       issue(0, s + 2);
       issue(2, s + 2);
       wait_loads<E == 1 ? 7 : 6>();
       read_done();
-      products(1, 0);
+      products(once, 1, 0);
       meet();
     }
     for (i64 s = 0; !low && s < steps; ++s) {
@@ -858,21 +940,42 @@ UNPM_DEV void matmul_wide(const u8* xp, const u8* wp, const float* xsp, const fl
       issue(1, s + 1);
       wait_loads<E == 1 ? 9 : 8>();
       read_done();
-      products(0, 0, sc);
-      products(1, 0);
+      products(once, 0, 0, sc);
+      products(once, 1, 0);
       meet();
       read_x(at, sc, 1);
+      look(s);
       issue(0, s + 2);
       issue(2, s + 2);
       issue(3, s + 2);
       wait_loads<E == 1 ? 9 : 8>();
       read_done();
-      products(1, 1, sc);
-      products(0, 1);
+      products(once, 1, 1, sc);
+      products(once, 0, 1);
       meet();
+    }
+    if constexpr (E == 1) {
+      if (__any(far > 126)) far = 127;
+      if (lane == 0) farthest[wave] = far;
     }
     if (wm == 0) lds_barrier();
     wait_loads<0>();
+    if constexpr (E == 1) {
+      lds_barrier();
+      if (__any(farthest[lane & 7] > 126)) {
+        clear();
+        for (i64 s = 0; s < steps; ++s) {
+          const u32 at = (u32)(s & 1) * STAGE;
+          issue_scales(s);
+#pragma unroll
+          for (int h = 0; h < 4; ++h) issue(h, s);
+          wait_loads<0>();
+          lds_barrier();
+          single(lds + at, reinterpret_cast<const float*>(lds + 2 * STAGE + (u32)(s & 3) * SCALES));
+          lds_barrier();
+        }
+      }
+    }
     if (a.tail && o.end == o.depth) {
       // The bytes of the last 16 that exist, which the last step had as zeros: one more step of them alone.
       const i64 last = o.last - 1, left = o.end - last * D;
@@ -887,15 +990,7 @@ UNPM_DEV void matmul_wide(const u8* xp, const u8* wp, const float* xsp, const fl
       if constexpr (E == 1) *reinterpret_cast<float*>(lds + 2 * STAGE + threadIdx.x * 4) = scale[last];
       lds_barrier();
       const float* sc = reinterpret_cast<const float*>(lds + 2 * STAGE);
-      read_x(lds, sc, 0);
-      read_w(lds, sc, 0);
-      products(0, 0);
-      read_w(lds, sc, 1);
-      products(1, 0);
-      read_x(lds, sc, 1);
-      products(1, 1);
-      read_w_scales(sc, 0);
-      products(0, 1);
+      single(lds, sc);
     }
   }
   lds_barrier();
@@ -1029,7 +1124,6 @@ template <int KIND> UNPM_DEV u32 codes4(float a, float b, float c, float d) {
     return __builtin_amdgcn_cvt_pk_bf8_f32(c, d, __builtin_amdgcn_cvt_pk_bf8_f32(a, b, 0, false), true);
 }
 UNPM_DEV u32 magnitude(float x) { return bits<u32>(x) & 0x7FFFFFFFu; }
-UNPM_DEV u32 more(u32 a, u32 b) { return a > b ? a : b; }
 
 // 16 bytes of a row from column c on, zeros past the last one (whole: known to be there and aligned).
 template <class T> struct alignas(16) vec_of {
