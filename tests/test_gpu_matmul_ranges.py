@@ -174,3 +174,31 @@ def test_far_scales_leave_other_rows_as_they_were(hip_device, m, n, k, kw, entry
     assert launch["entry"].endswith(entry) and np.isfinite(plain).all()
     keep = np.arange(m) != m // 2
     assert np.array_equal(got[keep], plain[keep]) and (got[m // 2] == 0).all()
+
+
+# ---------------------------------------------------------------------------------------
+# 16-bit products
+# ---------------------------------------------------------------------------------------
+@pytest.mark.parametrize("direction, rows, n, k, entry", [
+    ("input", 4000, 129, 2304, "_wide"), ("input", 4000, 143, 2304, "_wide"), ("input", 900, 71, 304, "_few"), ("input", 40, 257, 48, "_slim"),
+    ("input", 2000, 71, 2104, "_tile"), ("input", 33, 17, 64, "_slim"), ("input", 40, 1041, 48, "_one"), ("forward", 4000, 2304, 129, "_wide"), ("forward", 900, 304, 71, "_few"),
+    ("forward", 40, 48, 1041, "_one"),
+])
+def test_infinities_in_a_depths_last_elements(hip_device, direction, rows, n, k, entry):
+    """A weight that is infinite makes infinities of the sums that it is in, also where a depth ends inside 16 bytes, and nothing else."""
+    rng = np.random.default_rng(9)
+    forward, groups = direction == "forward", 3
+    depth, wide = (k, n) if forward else (n, k)
+    x = rng.integers(1, 4, (rows, depth)).astype(float)
+    w = rng.integers(-3, 4, (groups, wide, depth)).astype(float)  # of each column of out
+    w[0, 3, depth - 1], w[1, wide - 1, depth // 8 * 8], w[2, 5, 0], w[2, 8, depth - 1] = np.inf, -np.inf, np.inf, -np.inf
+    starts = np.array([0, rows // 3, rows // 2, rows])
+    want = np.concatenate([x[r0:r1] @ w[g].T for g, (r0, r1) in enumerate(ref.bounds(starts, rows))])
+    xa, x_row, _ = laid(held(x, "Bf16"), -depth % 8, 0, held(np.array([np.nan]), "Bf16")[0])
+    wa = held(w if forward else w.transpose(0, 2, 1), "Bf16")
+    wa, w_row, w_group = laid(np.ascontiguousarray(wa), -wa.shape[-1] % 8, 0, held(np.array([np.nan]), "Bf16")[0])
+    ex, ob = executor("lower_grouped_matmul", dtype="Bf16", out="F32", direction=direction), u.DeviceBuffer(4 * want.size)
+    run(ex, dev(xa), dev(wa), dev(starts.astype(np.int32)), ob, u.DeviceBuffer(16), rows, n, k, groups, x_row, w_group, w_row, wide, 0)
+    assert ex.last_launch()["entry"].endswith(entry), ex.last_launch()
+    got = ob.download(np.float32, want.size).reshape(want.shape)
+    assert np.array_equal(got, want), (np.argwhere(got != want)[:5], got[got != want][:5], want[got != want][:5])

@@ -770,7 +770,8 @@ UNPM_DEV void matmul_wide(const u8* xp, const u8* wp, const float* xsp, const fl
   const i32 x_after = xside::after(wave, lane), w_after = wside::after(wave, lane);
   auto issue = [&](int half, i64 step) {
     const bool isx = half < 2;
-    const i32 left = (i32)(o.end - (o.first + step) * D);
+    // Of W that lies along out only the rows that meet whole 16 bytes of X: the others meet zeros, which times infinity are NaN.
+    const i32 there = (i32)(o.end - (o.first + step) * D), left = !isx && WT && !XT ? there & ~(16 / E - 1) : there;
     const u8* p = isx ? xh[half & 1].at(o.first + step) : w.at(o.first + step);
     const u32 to = lds0 + (u32)(step & 1) * STAGE + half * HALF + wave * 1024;
 #pragma unroll
