@@ -447,8 +447,8 @@ typedef struct unp_matmul8 {
 } unp_matmul8;
 /* out[i][j] = sum over blocks c of 128 columns of a_scales[i][c] * b_scales[j / b_rows][c] * (the sum over the block of
  * a[i][l] * b[j][l]).  Row i's product is with its group's b where they are grouped: group g's rows are starts[g] ..
- * starts[g + 1] - 1, and rows that no group names are left as they were.  starts do not decrease; in a list that does,
- * which group takes a row, if any, is not said.
+ * starts[g + 1] - 1, and rows that no group names are left as they were.  starts do not decrease; one below
+ * an earlier one counts as that one.
  * Launch: a ([m][k]), a_scales (F32 [m][k / 128, rounded up]), b ([groups][n][k]), b_scales (F32 [groups][n / b_rows][k / 128],
  * rounded up), grouped: starts (I32 [groups + 1]), out ([m][n]), workspace; m, n, k, grouped: groups, a_row, a_scale_row, b_row,
  * b_scale_row, grouped: b_group, b_scale_group, out_row (strides), workspace_bytes.
@@ -472,7 +472,7 @@ typedef struct unp_grouped_matmul {
   int32_t out;       /* dtype or F32 */
   int32_t direction; /* unp_grouped_direction */
 } unp_grouped_matmul;
-/* Groups and starts, limits and the workspace as above (rows for m); products and sums in f32, each output rounded once.
+/* Groups and starts, limits and the workspace as above (rows for m; WEIGHT takes starts[g] .. starts[g + 1] - 1 as they are); products and sums in f32, each output rounded once.
  * Launch: x, w ([groups][n][k]; WEIGHT: y, [rows][k]), starts (I32 [groups + 1]), out, workspace; rows, n, k, groups, x_row,
  * then w_group, w_row, out_row (WEIGHT: y_row, out_group, out_row), workspace_bytes.  The fast launches need 16-byte aligned
  * operands with strides of whole 16 bytes, at most 4 MiB (that of a group aside), and what lies along out in them to be a

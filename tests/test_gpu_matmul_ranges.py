@@ -202,3 +202,45 @@ def test_infinities_in_a_depths_last_elements(hip_device, direction, rows, n, k,
     assert ex.last_launch()["entry"].endswith(entry), ex.last_launch()
     got = ob.download(np.float32, want.size).reshape(want.shape)
     assert np.array_equal(got, want), (np.argwhere(got != want)[:5], got[got != want][:5], want[got != want][:5])
+
+
+@pytest.mark.parametrize("how", ["forward", "input", "codes"])
+@pytest.mark.parametrize("rows, groups, depth, lists", [
+    (40, 5, 96, [[0, 39, 0, 39, 0, 40], [40, 0, 40, 0, 40, 0], [5, 3, 1, 0, 2, 4], [2 ** 31 - 1, -2 ** 31, 5, 2 ** 31 - 1, 0, -1], [3, -7, 20, 10, 30, 25]]),
+    (60, 5, 16384, [[0, 39, 0, 39, 0, 40], [0, 59, 0, 59, 0, 60], [50, 10, 55, 20, 57, 3], [40, 0, 0, 0, 0, 0], [-4, 20, 19, 70, 0, 1]]),
+    (500, 200, 128, ["steps", "drop", "any"]),
+])
+def test_a_start_below_an_earlier_one_counts_as_that_one(hip_device, how, rows, groups, depth, lists):
+    """Every row from the first start to the largest is one group's, whatever the workspace held before; the others stay."""
+    rng = np.random.default_rng(11)
+    wide = 136
+    x, w = rng.integers(-1, 2, (rows, depth)).astype(float), rng.integers(-1, 2, (groups, wide, depth)).astype(float)
+    blocks = -(-depth // 128)
+    if how == "codes":
+        ex = executor("lower_matmul8", a_kind="Fp8E4M3FN", b_kind="Fp8E4M3FN", out="F16", b_rows=128, grouped=True)
+        ones = dev(np.ones(max(rows, groups * 2) * blocks, np.float32))
+        ins = [dev(ref.encoded(x, "Fp8E4M3FN")), ones, dev(ref.encoded(w, "Fp8E4M3FN")), ones]
+        shape, strides = (rows, wide, depth, groups), (depth, blocks, depth, blocks, wide * depth, 2 * blocks, wide)
+    else:
+        ex = executor("lower_grouped_matmul", dtype="F16", out="F16", direction=how)
+        n, k = (wide, depth) if how == "forward" else (depth, wide)
+        ins = [dev(held(x, "F16")), dev(held(w if how == "forward" else np.ascontiguousarray(w.transpose(0, 2, 1)), "F16"))]
+        shape, strides = (rows, n, k, groups), (depth, n * k, k, wide)
+    need = ex.workspace_bytes(*shape)
+    for starts in lists:
+        if starts == "steps":
+            starts = np.arange(groups + 1) * 2 + rng.integers(-9, 10, groups + 1)
+        elif starts == "drop":  # a large start in the first 64 groups, ones below it in the others
+            starts = np.sort(rng.integers(0, rows, groups + 1))
+            starts[30] = starts[-1] - 20
+        elif starts == "any":
+            starts = rng.integers(-50, rows + 50, groups + 1)
+        want = np.full((rows, wide), 9.0)
+        for g, (r0, r1) in enumerate(ref.bounds(np.maximum.accumulate(np.clip(starts, 0, rows)), rows)):
+            want[r0:r1] = x[r0:r1] @ w[g].T
+        for junk in (0xFF, 0x3F):
+            ob = dev(held(np.full((rows, wide), 9.0), "F16"))
+            run(ex, *ins, dev(np.array(starts, np.int32)), ob, dev(np.full(need + 16, junk, np.uint8)), *shape, *strides, need)
+            got = read(ob, rows * wide, "F16").reshape(rows, wide)
+            assert np.array_equal(got, want), (list(starts), junk, np.argwhere(got != want)[:5])
+    assert depth < 1000 or ex.last_launch()["chunks"] > 1

@@ -286,15 +286,28 @@ UNPM_DEV void group_rows(const i32* starts, int g, i64 rows, i64& r0, i64& r1) {
   r0 = least(starts[g] < 0 ? 0 : starts[g], rows);
   r1 = least(starts[g + 1] < 0 ? 0 : starts[g + 1], rows);
 }
-// How many tiles of T rows this lane's group has, of the 64 groups from `first` on, and how many those up to it have.
+// How many tiles of T rows this lane's group has, of the 64 groups from `first` on, and how many those up to it have.  A start
+// below an earlier one, of which `floor` is the largest before these, counts as that one: so no row is two groups', each from the
+// first start to the largest is one's, and there are no more tiles than the launch has.
 struct tiles_upto {
   i32 own, upto;
   i64 r0, r1;
 };
-template <int T> UNPM_DEV tiles_upto group_tiles(const i32* starts, int groups, i64 rows, int first) {
+template <int T> UNPM_DEV tiles_upto group_tiles(const i32* starts, int groups, i64 rows, int first, i32 floor) {
   const int lane = threadIdx.x & 63;
+  const bool in = first + lane < groups;
   tiles_upto t{0, 0, 0, 0};
-  if (first + lane < groups) group_rows(starts, first + lane, rows, t.r0, t.r1);
+  if (in) group_rows(starts, first + lane, rows, t.r0, t.r1);
+  if (__any(in && (t.r1 < t.r0 || t.r0 < floor))) {
+    i32 top = t.r0 < floor ? floor : (i32)t.r0;
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) {
+      const i32 v = __shfl_up(top, d);
+      if (lane >= d && v > top) top = v;
+    }
+    t.r0 = top;
+    if (t.r1 < top) t.r1 = top;
+  }
   t.own = t.r1 > t.r0 ? (i32)((t.r1 - t.r0 + T - 1) / T) : 0;
   t.upto = t.own;
 #pragma unroll
@@ -307,14 +320,18 @@ template <int T> UNPM_DEV tiles_upto group_tiles(const i32* starts, int groups, 
 // This block's tile of T rows of the groups that have rows: its place, group and rows, or none.  Every wave finds it alike.
 template <int T, u32 RUN>
 UNPM_DEV bool find_group(const i32* starts, const product_args& a, tile_at& at, int& group, i64& r0, i64& r1) {
-  tiles_upto t = group_tiles<T>(starts, a.groups, a.m, 0);
+  tiles_upto t = group_tiles<T>(starts, a.groups, a.m, 0, 0);
+  const tiles_upto low = t;
   i64 all = __shfl(t.upto, 63);
-  for (int first = 64; first < a.groups; first += 64) all += __shfl(group_tiles<T>(starts, a.groups, a.m, first).upto, 63);
-  // Starts that decrease may name more tiles than there are blocks.
-  if (!tile_of<RUN>(a, (u32)__builtin_amdgcn_readfirstlane((i32)least(all, a.tiles_m)), at)) return false;
+  for (int first = 64; first < a.groups; first += 64) {
+    t = group_tiles<T>(starts, a.groups, a.m, first, __shfl((i32)t.r1, 63));
+    all += __shfl(t.upto, 63);
+  }
+  if (!tile_of<RUN>(a, scalar((u32)all), at)) return false;
   i64 past = 0;
+  t = low;
   for (int first = 0;; first += 64) {
-    if (first > 0) t = group_tiles<T>(starts, a.groups, a.m, first);
+    if (first > 0) t = group_tiles<T>(starts, a.groups, a.m, first, __shfl((i32)t.r1, 63));
     const u64 has = __ballot(past + t.upto > at.m);
     if (has) {
       const int l = __builtin_ctzll(has);
@@ -1046,10 +1063,16 @@ template <class OUT, int BY>
 UNPM_DEV void join(const i32* starts, OUT* out, const float* parts, const product_args& a) {
   const i64 rows = BY == DEPTH ? a.groups * a.m : a.m, units = (a.n + 7) / 8;
   i64 r0 = 0, r1 = rows;
-  if constexpr (BY == ROWS) {
-    i64 skip;
-    group_rows(starts, 0, rows, r0, skip);
-    group_rows(starts, a.groups - 1, rows, skip, r1);
+  if constexpr (BY == ROWS) {  // from the first start to the largest
+    i32 top = 0;
+    for (int i = threadIdx.x & 63; i <= a.groups; i += 64) top = starts[i] > top ? starts[i] : top;
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) {
+      const i32 v = __shfl_xor(top, d);
+      top = v > top ? v : top;
+    }
+    r0 = least(starts[0] < 0 ? 0 : starts[0], rows);
+    r1 = least(top, rows);
   }
   for (i64 i = r0 * units + (i64)blockIdx.x * 256 + threadIdx.x; i < r1 * units; i += (i64)gridDim.x * 256) {
     const i64 r = i / units, n = i % units * 8;
