@@ -4,7 +4,7 @@ import pytest
 
 import unpopped_amd as u
 from tests import matmul_reference as ref
-from tests.test_gpu_matmul import JUNK, dev, executor, held, laid, read, run, starts_of
+from tests.test_gpu_matmul import JUNK, dev, executor, grouped_case, held, laid, matmul8_case, read, run, starts_of
 
 pytestmark = pytest.mark.gpu
 UNIT = 2.0 ** -149  # the smallest step of f32
@@ -244,3 +244,45 @@ def test_a_start_below_an_earlier_one_counts_as_that_one(hip_device, how, rows, 
             got = read(ob, rows * wide, "F16").reshape(rows, wide)
             assert np.array_equal(got, want), (list(starts), junk, np.argwhere(got != want)[:5])
     assert depth < 1000 or ex.last_launch()["chunks"] > 1
+
+
+# ---------------------------------------------------------------------------------------
+# Split depths of every kernel, and long ones of the largest
+# ---------------------------------------------------------------------------------------
+@pytest.mark.parametrize("kind, m, n, k, groups, kw, parts", [
+    ("codes", 300, 264, 12297, 0, dict(pad=7), 12),                # 64 x 128
+    ("codes", 1030, 2056, 12297, 0, dict(pad=7), 4),               # 256 x 256
+    ("codes", 1030, 2056, 12297, 0, dict(pad=7, b_rows=1), 4),     # 256 x 256
+    ("codes", 1030, 520, 32777, 2, dict(pad=7, way="gaps"), 16),   # 256 x 256
+    ("codes", 1500, 520, 12304, 5, dict(way="gaps"), 3),           # 128 x 128
+    ("codes", 260, 264, 12297, 3, dict(pad=7, out_pad=1), 12),     # 64 x 128
+    ("codes", 24, 72, 12304, 2, dict(b_rows=1), 12),               # 32 x 64
+    ("forward", 1500, 520, 8201, 5, dict(pad=7, way="gaps"), 8),   # 256 x 256
+    ("forward", 1500, 520, 8201, 5, dict(pad=7, out="F32"), 8),    # 256 x 256
+    ("forward", 520, 1544, 8200, 5, dict(way="gaps"), 3),          # 128 x 128
+    ("forward", 260, 264, 8201, 3, dict(pad=7), 12),               # 64 x 128
+    ("forward", 24, 136, 12296, 5, dict(way="gaps"), 16),          # 32 x 64
+    ("input", 1500, 8201, 520, 5, dict(pad=8, x_pad=7, way="gaps"), 8),
+    ("input", 520, 8200, 1544, 5, dict(way="gaps"), 3),
+    ("input", 260, 8201, 264, 3, dict(pad=8, x_pad=7, out_pad=1), 12),
+    ("input", 24, 12296, 136, 5, dict(way="gaps"), 16),
+    ("weight", 24584, 264, 1032, 5, dict(way="gaps"), 4),          # 256 x 256
+    ("weight", 24584, 264, 1032, 5, dict(out="F32", out_pad=4), 4),
+    ("weight", 2320, 104, 264, 2, dict(way="gaps"), 4),            # 128 x 128
+])
+def test_a_split_depth_of_each_kernel(hip_device, kind, m, n, k, groups, kw, parts):
+    """Whole numbers, exactly, by each shape of tile; lengths that end inside 16 bytes, which the last part alone takes up."""
+    if kind == "codes":
+        launch = matmul8_case(m, n, k, groups=groups, top=1, **kw)
+    else:
+        launch = grouped_case(kind, m, n, k, groups, **kw)
+    assert launch["chunks"] == parts, launch
+
+
+@pytest.mark.parametrize("kw", [
+    dict(m=4000, n=2561, k=1175, pad=9), dict(m=4000, n=2561, k=1175, pad=9, b_rows=1), dict(m=4000, n=2561, k=2208, b_rows=1, a_kind="Fp8E5M2", top=2),
+    dict(m=3500, n=2561, k=1303, pad=9, groups=2, starts=[0, 1100, 3500]), dict(m=3500, n=2561, k=1312, groups=2, starts=[0, 1100, 3500], b_rows=1),
+])
+def test_codes_of_more_steps_than_their_scales_have_places(hip_device, kw):
+    """256 x 256 tiles of whole and half height, from 10 steps on."""
+    assert matmul8_case(**kw)["entry"].endswith("_wide")
