@@ -1231,11 +1231,11 @@ template <class T, int KIND> UNPM_DEV void quantise_rows(const T* x, u8* codes, 
 // The other forms: a block takes 128 x 128 elements of x; thread (i, j) R rows from R i on and 8 columns, 16 bytes of each run
 // of 16 lanes.  One scale for all of them, or (TURNED) one for each column, whose 128 rows lie along y's row.
 // 34.5 microseconds for 8192 x 4096 of 32 bits (4.9 TB/s), 30 for a copy; threads of 8 rows each, half as many, took 35.4.
-template <class T, int KIND, int RB, bool TURNED, int THREADS = 512>
+template <class T, int KIND, int RB, bool TURNED>
 UNPM_DEV void quantise_tiles(const T* x, u8* codes, float* scales, const quant_args& a) {
   static_assert(RB == 128 || TURNED, "scales of rows are quantise_rows's");
   constexpr int ROW = 128 + 16;  // of a transposed tile in LDS
-  constexpr int V = 16 / sizeof(T), PIECES = 8 / V, R = 2048 / THREADS, TEAMS = 128 / R;
+  constexpr int THREADS = 512, V = 16 / sizeof(T), PIECES = 8 / V, R = 2048 / THREADS, TEAMS = 128 / R;
   __shared__ u32 tops[TEAMS][128];
   __shared__ __attribute__((aligned(16))) u8 turned[TURNED ? 128 * ROW : 16];
   const i64 across = (a.cols + 127) / 128, all = (a.rows + 127) / 128 * across;
