@@ -2230,8 +2230,8 @@ int64_t row_tiles(const Extents& e, int64_t t) {
 
 // What a direct entry takes, in microseconds: to begin and end, and a step (128 bytes along the depth) of the blocks of a CU,
 // of one block and of as many as the CU holds; and the TB/s at which it reads weights that no cache holds.  Fitted to times of
-// 78 shapes of 1 to 16000 rows, 72 to 28672 columns, depths of 64 to 28672 and 1 to 64 groups, where it chooses entries and parts
-// that are 3 % slower than the best of each (geometric mean; over 12 % at 7 shapes, 33 % at the worst).
+// 78 shapes of 1 to 16000 rows, 72 to 28672 columns, depths of 64 to 28672 and 1 to 100 groups; measured again on 76 of them it
+// chooses entries and parts that are 3 % slower than the best of each (geometric mean; over 12 % at 6 shapes, 38 % at the worst).
 struct EntryCost {
   double fixed, alone, full, rate;
 };
